@@ -1,5 +1,13 @@
 """PyTorch operators ``torch.ops.mhcpre.mhc_pre`` and
-``torch.ops.mhcpre.mhc_pre_with_h_pre``.
+``torch.ops.mhcpre.mhc_pre_with_h_pre``, and the serving operators
+``qk_norm_rope``, ``qk_norm_rope_append``, ``paged_attention``,
+``cache_update``, ``cache_compact`` and ``cache_copy_pages`` (native too, from
+``csrc/mhc_serve_torch.cpp`` over ``include/mhc_serve.h``, which says what each
+computes).
+
+The serving operators take x-like tensors as ``[..., heads, d]`` with any
+leading dimensions; inputs that are not laid out as the C ABI wants them are
+copied first, caches never are.
 
 The operators are native: ``libmhcpre_torch.so`` (built from
 ``csrc/mhc_pre_torch.cpp``) registers them with PyTorch's dispatcher and calls
@@ -105,3 +113,38 @@ def _(x, phi, alpha, bias, gamma=None, norm_eps=1e-6, hc_eps=1e-6):
 @torch.library.register_fake(f"{_LIB_NAME}::mhc_pre_with_h_pre")
 def _(x, phi, alpha, bias, gamma=None, norm_eps=1e-6, hc_eps=1e-6):
     return _fake_outputs(x)
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::qk_norm_rope")
+def _(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, amplitude=1.0):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::qk_norm_rope_append")
+def _(q, k, v, positions, inv_freq, slots, k_cache, v_cache, q_weight=None, k_weight=None, eps=1e-6,
+      interleaved=False, amplitude=1.0):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::paged_attention")
+def _(q, k_cache, v_cache, page_table, lengths, scale=None, window=0):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::cache_update")
+def _(page_table, lengths, parents, counts, pages, page_size, tokens=1):
+    rows = page_table.shape[0]
+    row = [page_table.new_empty((rows,)) for _ in range(4)]
+    slots = page_table.new_empty((rows, tokens), dtype=torch.int64)
+    return page_table.new_empty(page_table.shape), row[0], slots, row[1], row[2], row[3]
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::cache_compact")
+def _(page_table, lengths, pages, page_size):
+    return (page_table.new_empty(page_table.shape), page_table.new_empty((pages // 2,)),
+            page_table.new_empty((pages // 2,)), page_table.new_empty((1,)))
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::cache_copy_pages")
+def _(k_cache, v_cache, src, dst):
+    return None
