@@ -146,7 +146,9 @@ MHC_API int mhcRotaryFrequencies(int32_t rot, double base, int32_t kind, double 
  *
  * d is one of 32, 64, 80, 96, 112, 128, 160, 192, 256; q, the caches and out
  * are 16-byte aligned with strides (other than the last) of multiples of 8
- * elements; heads is a multiple of kvHeads.  The results do not depend on other
+ * elements; heads is a multiple of kvHeads; B * kvHeads * (width * pageSize / 128
+ * + 2) is below 2^31, with kvHeads counted ceil(heads / kvHeads / 32) times where
+ * more than 16 query heads share one.  The results do not depend on other
  * rows of the batch or on timing.
  */
 MHC_API int mhcPagedAttentionGetWorkspaceSize(

@@ -1,0 +1,524 @@
+// Attention of one new token per sequence over a paged cache
+// (mhcPagedAttention): the kernels, instantiated per element type.
+//
+// The keys of a row are cut into units of 128 (aligned to multiples of 128, so
+// a unit never changes with the row's length).  All units of all (row, kv head,
+// group of query heads) in that order form one line, which is shared out evenly
+// to a fixed grid: the lengths are on the device, and so is this arithmetic.  A
+// workgroup walks its stretch; a (row, kv head, group) that lies in one
+// stretch is finished there, the others leave their maximum, sum and output per
+// stretch in the workspace and a second launch joins them, in the order of the
+// keys.
+//
+// In a unit each of the 4 waves has 32 keys of its own.  The scores are S^T =
+// K Q^T, 16 keys by 16 query heads (a wave's K rows go straight from memory to
+// the operand's registers), so a lane has the scores of one head, and the
+// probabilities are, as they lie in its registers, the operand of O^T = V^T
+// P^T: the order of the keys within a product is free.  V goes through LDS,
+// rows as they come, and is read transposed (ds_read_b64_tr_b16); the region is
+// the wave's own, so the loop has no barrier.  The probabilities are split into
+// hi + lo of the 16-bit type: a weight in 8 bits alone would add an error as
+// large as the output's own rounding, and the matrix cores have time.
+//
+// Bound: the cache is read once, 4 bytes a value pair for at most 4 * 16
+// flops, so the memory's rate decides.
+#pragma once
+
+#include "mhc_pre_device.h"
+#include "mhc_serve_internal.h"
+
+namespace mhc {
+namespace attention {
+
+using dev::f32x4_t;
+using dev::kWave;
+using dev::u32x4_t;
+
+constexpr int kWaves = 4;
+constexpr int kTile = 32;               // keys of a wave at a time
+constexpr int kUnit = kWaves * kTile;   // keys of a unit
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8v_t __attribute__((ext_vector_type(8)));
+
+// How the units are shared out: the same arithmetic in both launches.
+struct Shares {
+    int units, grid;  // all units; workgroups that have some (each has at least one)
+
+    __device__ Shares(int units_, int most) : units(units_), grid(units_ < most ? units_ : most) {}
+    __device__ int start(int w) const
+    {
+        const int q = units / grid, r = units % grid;
+        return w * q + (w < r ? w : r);
+    }
+    __device__ int owner(int u) const
+    {
+        const int q = units / grid, r = units % grid;
+        return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q;
+    }
+};
+
+struct Args {
+    PagedAttentionArgs a;
+    int group;    // query heads of a kv head
+    int blocks;   // blocks of 16 * RT query heads in a group
+    int most;     // workgroups of the first launch
+    float *parts; // [2 * most][16 * RT rows][D], then [2 * most][16 * RT][2] maxima (base 2) and sums
+};
+
+// The keys of row b: [low, high), and its units' number (one at least).
+struct Keys {
+    int low, high, first, units;
+
+    __device__ Keys(const PagedAttentionArgs &a, int b)
+    {
+        const int most = a.width * a.pageSize;
+        int L = a.lengths[b];
+        L = L < 0 ? 0 : L > most ? most : L;
+        low = a.window > 0 && L > a.window ? L - (int)a.window : 0;
+        high = L;
+        first = low / kUnit;
+        units = high > low ? (high + kUnit - 1) / kUnit - first : 1;
+    }
+};
+
+__device__ __forceinline__ int wave_sum_int(int v)
+{
+#pragma unroll
+    for (int m = 1; m < kWave; m *= 2) {
+        v += __shfl_xor(v, m);
+    }
+    return v;
+}
+
+__device__ __forceinline__ int64_t shfl64(int64_t v, int lane)
+{
+    const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)v, lane), hi = (uint32_t)__shfl((int)(v >> 32), lane);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// LDS bytes between two rows of V: 8 banks off a multiple of 16 or 32, so that
+// the four rows that 16 lanes read together lie in different banks.
+template <int D>
+constexpr int pitch()
+{
+    return 2 * D + (D == 112 ? 0 : 32);
+}
+
+// Bytes of a wave's LDS: V's tile, then the wave's output for the join.
+template <int D>
+constexpr int region()
+{
+    constexpr int v = kTile * pitch<D>(), o = 16 * (D + 4) * 4;
+    return v > o ? v : o;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ f32x4_t mfma32(u32x4_t a, u32x4_t b, f32x4_t c)
+{
+    if constexpr (kBf16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v_t, a),
+                                                       __builtin_bit_cast(bf16x8v_t, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b),
+                                                      c, 0, 0, 0);
+    }
+}
+
+// 4 values at the same column of 4 rows of LDS (the lane's column of 16).
+__device__ __forceinline__ u32x2_t read_transposed(const char *p)
+{
+    return __builtin_bit_cast(
+        u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t *)p));
+}
+
+template <int D>
+struct Shape {
+    static constexpr int kSteps = (D + 31) / 32;     // of 32 values in a product over d
+    static constexpr int kChunks = D / 8;            // 16-byte chunks of a row
+    static constexpr int kLoads = kTile * kChunks / kWave;  // of V, by a wave
+    static constexpr int kDims = D / 16;
+};
+
+// 16 rows of K or Q: lane l has row l % 16, values 32 s + 8 (l / 16) .. + 7.
+// Where D % 32 == 16 the last step's upper half is zero in both.  (A 16x16x16
+// product in its place, added to the sum of the 16x16x32 ones, came out wrong.)
+template <int D>
+struct Fragment {
+    u32x4_t step[Shape<D>::kSteps];
+
+    __device__ void load(const uint16_t *row, int lane)
+    {
+        const int c = lane / 16;
+#pragma unroll
+        for (int s = 0; s < Shape<D>::kSteps; ++s) {
+            const bool half = 32 * s + 32 > D;
+            step[s] = *reinterpret_cast<const u32x4_t *>(row + 32 * s + 8 * (half ? c % 2 : c));
+            if (half && c >= 2) {
+                step[s] = u32x4_t{0, 0, 0, 0};
+            }
+        }
+    }
+    __device__ void clear()
+    {
+#pragma unroll
+        for (int s = 0; s < Shape<D>::kSteps; ++s) {
+            step[s] = u32x4_t{0, 0, 0, 0};
+        }
+    }
+};
+
+template <bool kBf16, int D, int RT>
+__global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attention_units(Args args)
+{
+    using S = Shape<D>;
+    constexpr int P = pitch<D>();
+    __shared__ __align__(16) char lds[kWaves][region<D>()];
+    __shared__ float tops[kWaves][16 * RT], sums[kWaves][16 * RT];
+    const PagedAttentionArgs &a = args.a;
+    const int lane = (int)threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int c = lane / 16, col = lane % 16;
+    const int perRow = a.kvHeads * args.blocks;
+
+    // The workgroup's stretch and the row it begins in.
+    int count = 0;
+    for (int b = lane; b < a.B; b += kWave) {
+        count += Keys(a, b).units;
+    }
+    const Shares shares(wave_sum_int(count) * perRow, args.most);
+    const int w = (int)blockIdx.x;
+    if (w >= shares.grid) {
+        return;
+    }
+    const int begin = shares.start(w), end = shares.start(w + 1);
+    int b = 0, base = 0;  // base: the row's first unit
+    for (int b0 = 0;; b0 += kWave) {
+        const int mine = b0 + lane < a.B ? Keys(a, b0 + lane).units * perRow : 0;
+        int upto = mine;
+#pragma unroll
+        for (int m = 1; m < kWave; m *= 2) {
+            const int u = __shfl_up(upto, m);
+            upto += lane >= m ? u : 0;
+        }
+        const uint64_t past = __ballot(base + upto > begin);
+        if (past != 0) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            b = b0 + at;
+            base += __shfl(upto - mine, at);
+            break;
+        }
+        base += __shfl(upto, kWave - 1);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    base = __builtin_amdgcn_readfirstlane(base);
+
+    for (int u = begin; u < end;) {
+        const Keys keys(a, b);
+        const int inRow = u - base, hg = inRow / keys.units, tile0 = inRow % keys.units;
+        const int stop = base + (hg + 1) * keys.units < end ? base + (hg + 1) * keys.units : end;
+        const int tile1 = tile0 + stop - u;
+        const int kvHead = hg / args.blocks, block = hg % args.blocks;
+        const int head0 = block * 16 * RT;  // in the group
+
+        Fragment<D> q[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int h = head0 + rt * 16 + col;
+            q[rt].clear();
+            if (h < args.group) {
+                q[rt].load(static_cast<const uint16_t *>(a.q.data) + b * a.q.row +
+                               (int64_t)(kvHead * args.group + h) * a.q.head,
+                           lane);
+            }
+        }
+        f32x4_t o[RT][S::kDims];
+        float top[RT], sum[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            top[rt] = -INFINITY;
+            sum[rt] = 0.f;
+#pragma unroll
+            for (int j = 0; j < S::kDims; ++j) {
+                o[rt][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+
+        const uint16_t *kBase = static_cast<const uint16_t *>(a.kCache.data) + kvHead * a.kCache.head;
+        const uint16_t *vBase = static_cast<const uint16_t *>(a.vCache.data) + kvHead * a.vCache.head;
+        const int32_t *table = a.table + (int64_t)b * a.width;
+
+        // The wave's tiles: tile i has the keys from (first unit + i) * kUnit + wave * kTile.
+        const int offset = wave * kTile;
+        const auto key0 = [&](int i) { return (keys.first + i) * kUnit + offset; };
+        // The page of key key0(i) + lane % 32, -1 where the row has no such key.
+        const auto find_page = [&](int i) {
+            const int t = key0(i) + lane % kTile;
+            return i < tile1 && t >= keys.low && t < keys.high ? table[t / a.pageSize] : -1;
+        };
+        Fragment<D> k[2];
+        u32x4_t v[S::kLoads];
+        uint32_t mask = 0;  // keys of the loaded tile that the row sees
+        const auto load = [&](int i, int page) {
+            const bool seen = page >= 0 && page < a.pages;
+            const int slot = (key0(i) + lane % kTile) % a.pageSize;
+            mask = (uint32_t)__ballot(seen);
+            // Where there is no key the first row of the cache is read instead, and not used.
+            const int64_t kAt = seen ? page * a.kCache.page + slot * a.kCache.slot : 0;
+            const int64_t vAt = seen ? page * a.vCache.page + slot * a.vCache.slot : 0;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                k[kt].load(kBase + shfl64(kAt, kt * 16 + col), lane);
+            }
+#pragma unroll
+            for (int n = 0; n < S::kLoads; ++n) {
+                const int at = n * kWave + lane;
+                v[n] = *reinterpret_cast<const u32x4_t *>(vBase + shfl64(vAt, at / S::kChunks) + at % S::kChunks * 8);
+            }
+        };
+
+        load(tile0, find_page(tile0));
+        int page = find_page(tile0 + 1);
+        for (int i = tile0; i < tile1; ++i) {
+            char *mine = lds[wave];
+            const uint32_t now = mask;
+            // V to LDS; what the row does not see is zero there, whatever the cache holds.
+#pragma unroll
+            for (int n = 0; n < S::kLoads; ++n) {
+                const int at = n * kWave + lane, row = at / S::kChunks;
+                if (now != 0xFFFFFFFFu && (now >> row & 1u) == 0u) {
+                    v[n] = u32x4_t{0, 0, 0, 0};
+                }
+                *reinterpret_cast<u32x4_t *>(mine + row * P + at % S::kChunks * 16) = v[n];
+            }
+            f32x4_t s[RT][2];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    s[rt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int x = 0; x < S::kSteps; ++x) {
+                        s[rt][kt] = mfma32<kBf16>(k[kt].step[x], q[rt].step[x], s[rt][kt]);
+                    }
+                }
+            }
+            if (i + 1 < tile1) {
+                load(i + 1, page);
+                page = find_page(i + 2);
+            }
+            if (now == 0u) {
+                continue;
+            }
+            u32x4_t hi[RT], lo[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float x[8], most = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int key = e / 4 * 16 + 4 * c + e % 4;
+                    x[e] = (now >> key & 1u) != 0u ? s[rt][e / 4][e % 4] * (a.scale * kLog2e) : -INFINITY;
+                    most = fmaxf(most, x[e]);
+                }
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                const float next = fmaxf(top[rt], most);
+                const float zero = next == -INFINITY ? 0.f : next;
+                const float keep = __builtin_amdgcn_exp2f(top[rt] - zero);
+                top[rt] = next;
+                float part = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(x[e] - zero);
+                    part += x[e];
+                }
+                sum[rt] = sum[rt] * keep + part;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p0 = x[2 * e], p1 = x[2 * e + 1];
+                    const uint32_t h = dev::pack2_x<kBf16>(p0, p1);
+                    hi[rt][e] = h;
+                    lo[rt][e] = dev::pack2_x<kBf16>(p0 - dev::x_to_f32<kBf16>(h & 0xFFFFu),
+                                                    p1 - dev::x_to_f32<kBf16>(h >> 16));
+                }
+#pragma unroll
+                for (int j = 0; j < S::kDims; ++j) {
+                    o[rt][j] *= keep;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < S::kDims; ++j) {
+                const char *at = mine + (4 * c + col / 4) * P + (16 * j + col % 4 * 4) * 2;
+                const u32x2_t v0 = read_transposed(at), v1 = read_transposed(at + 16 * P);
+                const u32x4_t vt = {v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    o[rt][j] = mfma32<kBf16>(vt, hi[rt], o[rt][j]);
+                    o[rt][j] = mfma32<kBf16>(vt, lo[rt], o[rt][j]);
+                }
+            }
+        }
+
+        // The waves' results together, 16 query heads at a time.
+        const bool whole = tile0 == 0 && tile1 == keys.units;
+        const int slot = 2 * w + (u == begin ? 0 : 1);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            sum[rt] += __shfl_xor(sum[rt], 16);
+            sum[rt] += __shfl_xor(sum[rt], 32);
+            if (c == 0) {
+                tops[wave][rt * 16 + col] = top[rt];
+                sums[wave][rt * 16 + col] = sum[rt];
+            }
+            float *mine = reinterpret_cast<float *>(lds[wave]) + col * (D + 4);
+#pragma unroll
+            for (int j = 0; j < S::kDims; ++j) {
+                *reinterpret_cast<f32x4_t *>(mine + 16 * j + 4 * c) = o[rt][j];
+            }
+            __syncthreads();
+            for (int at = (int)threadIdx.x; at < 16 * D / 4; at += 64 * kWaves) {
+                const int row = at / (D / 4), e = at % (D / 4) * 4;
+                float most = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < kWaves; ++x) {
+                    most = fmaxf(most, tops[x][rt * 16 + row]);
+                }
+                const float zero = most == -INFINITY ? 0.f : most;
+                float total = 0.f;
+                f32x4_t all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < kWaves; ++x) {
+                    const float f = __builtin_amdgcn_exp2f(tops[x][rt * 16 + row] - zero);
+                    total += f * sums[x][rt * 16 + row];
+                    all += f * *reinterpret_cast<const f32x4_t *>(reinterpret_cast<const float *>(lds[x]) +
+                                                                  row * (D + 4) + e);
+                }
+                const int h = head0 + rt * 16 + row;
+                if (!whole) {
+                    const int64_t line = (int64_t)slot * 16 * RT + rt * 16 + row;
+                    *reinterpret_cast<f32x4_t *>(args.parts + line * D + e) = all;
+                    if (e == 0) {
+                        float *ends = args.parts + (int64_t)2 * args.most * 16 * RT * D + 2 * line;
+                        ends[0] = most;
+                        ends[1] = total;
+                    }
+                } else if (h < args.group) {
+                    const int64_t head = kvHead * args.group + h;
+                    const float inv = total == 0.f ? 0.f : 1.f / total;
+                    uint16_t *out = static_cast<uint16_t *>(a.out.data) + b * a.out.row + head * a.out.head + e;
+                    *reinterpret_cast<u32x2_t *>(out) = u32x2_t{dev::pack2_x<kBf16>(all[0] * inv, all[1] * inv),
+                                                                dev::pack2_x<kBf16>(all[2] * inv, all[3] * inv)};
+                    if (e == 0 && a.lse != nullptr) {
+                        a.lse[(int64_t)b * a.heads + head] = (zero + __builtin_amdgcn_logf(total)) * kLn2;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        u = stop;
+        if (u == base + perRow * keys.units) {
+            base = u;
+            ++b;
+        }
+    }
+}
+
+// One workgroup per (row, kv head, block of query heads): joins its stretches'
+// parts, where it has more than one.
+template <bool kBf16, int D, int RT>
+__global__ __launch_bounds__(256) void attention_join(Args args)
+{
+    __shared__ int counts[kWaves], befores[kWaves];
+    const PagedAttentionArgs &a = args.a;
+    const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
+    const int perRow = a.kvHeads * args.blocks;
+    const int b = (int)blockIdx.x / perRow, hg = (int)blockIdx.x % perRow;
+    int count = 0, before = 0;
+    for (int x = (int)threadIdx.x; x < a.B; x += 256) {
+        const int n = Keys(a, x).units;
+        count += n;
+        before += x < b ? n : 0;
+    }
+    count = wave_sum_int(count);
+    before = wave_sum_int(before);
+    if (lane == 0) {
+        counts[wave] = count;
+        befores[wave] = before;
+    }
+    __syncthreads();
+    count = counts[0] + counts[1] + counts[2] + counts[3];
+    before = befores[0] + befores[1] + befores[2] + befores[3];
+    const Shares shares(count * perRow, args.most);
+    const Keys keys(a, b);
+    const int u0 = before * perRow + hg * keys.units;
+    const int first = shares.owner(u0), last = shares.owner(u0 + keys.units - 1);
+    if (first == last) {
+        return;
+    }
+    const float *ends = args.parts + (int64_t)2 * args.most * 16 * RT * D;
+    const int head0 = hg % args.blocks * 16 * RT;
+    const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
+    const int firstSlot = 2 * first + (shares.start(first) == u0 ? 0 : 1);
+    for (int at = (int)threadIdx.x; at < rows * (D / 4); at += 256) {
+        const int row = at / (D / 4), e = at % (D / 4) * 4;
+        float most = -INFINITY;
+        for (int x = first; x <= last; ++x) {
+            most = fmaxf(most, ends[2 * ((int64_t)(x == first ? firstSlot : 2 * x) * 16 * RT + row)]);
+        }
+        const float zero = most == -INFINITY ? 0.f : most;
+        float total = 0.f;
+        f32x4_t all = {0.f, 0.f, 0.f, 0.f};
+        for (int x = first; x <= last; ++x) {
+            const int64_t line = (int64_t)(x == first ? firstSlot : 2 * x) * 16 * RT + row;
+            const float f = __builtin_amdgcn_exp2f(ends[2 * line] - zero);
+            total += f * ends[2 * line + 1];
+            all += f * *reinterpret_cast<const f32x4_t *>(args.parts + line * D + e);
+        }
+        const int64_t head = hg / args.blocks * args.group + head0 + row;
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        uint16_t *out = static_cast<uint16_t *>(a.out.data) + b * a.out.row + head * a.out.head + e;
+        *reinterpret_cast<u32x2_t *>(out) = u32x2_t{dev::pack2_x<kBf16>(all[0] * inv, all[1] * inv),
+                                                    dev::pack2_x<kBf16>(all[2] * inv, all[3] * inv)};
+        if (e == 0 && a.lse != nullptr) {
+            a.lse[(int64_t)b * a.heads + head] = (zero + __builtin_amdgcn_logf(total)) * kLn2;
+        }
+    }
+}
+
+template <bool kBf16, int D, int RT>
+hipError_t launch_size(const Args &args, hipStream_t stream)
+{
+    hipLaunchKernelGGL((attention_units<kBf16, D, RT>), dim3((unsigned)args.most), dim3(64 * kWaves), 0, stream, args);
+    if (const hipError_t err = hipGetLastError(); err != hipSuccess) {
+        return err;
+    }
+    hipLaunchKernelGGL((attention_join<kBf16, D, RT>), dim3((unsigned)(args.a.B * args.a.kvHeads * args.blocks)),
+                       dim3(256), 0, stream, args);
+    return hipGetLastError();
+}
+
+template <bool kBf16, int RT>
+hipError_t launch_heads(const Args &args, hipStream_t stream)
+{
+    switch (args.a.d) {
+    case 32: return launch_size<kBf16, 32, RT>(args, stream);
+    case 64: return launch_size<kBf16, 64, RT>(args, stream);
+    case 80: return launch_size<kBf16, 80, RT>(args, stream);
+    case 96: return launch_size<kBf16, 96, RT>(args, stream);
+    case 112: return launch_size<kBf16, 112, RT>(args, stream);
+    case 128: return launch_size<kBf16, 128, RT>(args, stream);
+    case 160: return launch_size<kBf16, 160, RT>(args, stream);
+    case 192: return launch_size<kBf16, 192, RT>(args, stream);
+    case 256: return launch_size<kBf16, 256, RT>(args, stream);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+// One file per instance: mhc_paged_attention_{bf16,f16}.hip, RT 1 and 2.
+hipError_t launch_bf16(const Args &args, bool wide, hipStream_t stream);
+hipError_t launch_f16(const Args &args, bool wide, hipStream_t stream);
+
+}  // namespace attention
+}  // namespace mhc

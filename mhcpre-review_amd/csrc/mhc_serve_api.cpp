@@ -482,7 +482,7 @@ int mhcPagedAttentionGetWorkspaceSize(const mhcStridedTensor *q, const mhcStride
     if (pageTable->dims[0] != B) {
         return MHC_STATUS_INVALID_SHAPE;
     }
-    if (!mhc::paged_attention_head_size(static_cast<int>(d)) || heads > 65536 || B > (1 << 20)) {
+    if (!mhc::paged_attention_head_size(d) || heads > 65536 || B > (1 << 20)) {
         return MHC_STATUS_UNSUPPORTED_SHAPE;
     }
     st = first_of({check_strided(q, q->dtype, {B, heads, d}, 16), check_strided(out, q->dtype, {B, heads, d}, 16),
@@ -517,6 +517,10 @@ int mhcPagedAttentionGetWorkspaceSize(const mhcStridedTensor *q, const mhcStride
     a.scale = scale;
     a.window = window;
     a.lse = lse != nullptr ? static_cast<float *>(lse->data) : nullptr;
+    if (!mhc::paged_attention_units_fit(a)) {
+        delete ex;
+        return MHC_STATUS_UNSUPPORTED_SHAPE;
+    }
     return finish(ex, q->data, workspaceSize, executor);
 }
 
