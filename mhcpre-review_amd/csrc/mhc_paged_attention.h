@@ -7,8 +7,11 @@
 // to a fixed grid: the lengths are on the device, and so is this arithmetic.  A
 // workgroup walks its stretch; a (row, kv head, group) that lies in one
 // stretch is finished there, the others leave their maximum, sum and output per
-// stretch in the workspace and a second launch joins them, in the order of the
-// keys.
+// stretch in the workspace, and the workgroup that finds all of them there joins
+// them, in the order of the keys.  Nobody waits: every workgroup that leaves a
+// part then looks whether the others' are there, so the last one finds them (two
+// may, and then write the same bits).  What tells this launch's parts from what
+// the workspace held before is the launch's tag (LaunchTag).
 //
 // In a unit each of the 4 waves has 32 keys of its own.  The scores are S^T =
 // K Q^T, 16 keys by 16 query heads (a wave's K rows go straight from memory to
@@ -65,9 +68,53 @@ struct Args {
     PagedAttentionArgs a;
     int group;    // query heads of a kv head
     int blocks;   // blocks of 16 * RT query heads in a group
-    int most;     // workgroups of the first launch
-    float *parts; // [2 * most][16 * RT rows][D], then [2 * most][16 * RT][2] maxima (base 2) and sums
+    int most;     // workgroups of the launch
+    char *parts;  // see Parts
+    LaunchTag tag;
 };
+
+// A stretch leaves at most two parts in the workspace, of the (row, kv head,
+// group) that it begins in and of the one that it ends in: [2 * most] outputs [16
+// RT][D], maxima (base 2) and sums [16 RT][2], and 8-byte words that say that
+// the part is there.  All of it is stored through to memory and read from there:
+// the reader may be on another XCD.
+template <int D, int RT>
+struct Parts {
+    static constexpr int kRows = 16 * RT;
+    __amdgpu_buffer_rsrc_t outs, ends;
+    uint64_t *words;
+
+    static constexpr size_t bytes(int most) { return (size_t)2 * most * (kRows * (D + 2) * 4 + 8); }
+    __device__ Parts(char *base, int most)
+        : outs(dev::make_rsrc(base, 2 * most * kRows * D * 4)),
+          ends(dev::make_rsrc(base + (size_t)2 * most * kRows * D * 4, 2 * most * kRows * 8)),
+          words(reinterpret_cast<uint64_t *>(base + (size_t)2 * most * kRows * (D + 2) * 4))
+    {
+    }
+    __device__ static uint64_t word(uint32_t tag, int slot)
+    {
+        return (uint64_t)mix32(tag ^ (2u * (uint32_t)slot + 1u)) << 32 | tag;
+    }
+    __device__ void put(int slot, int row, int e, f32x4_t out) const
+    {
+        dev::store16<dev::kCpolDev>(__builtin_bit_cast(u32x4_t, out), outs, ((slot * kRows + row) * D + e) * 4);
+    }
+    __device__ void put_ends(int slot, int row, float top, float sum) const
+    {
+        const u32x2_t v = {__float_as_uint(top), __float_as_uint(sum)};
+        __builtin_amdgcn_raw_buffer_store_b64(v, ends, (slot * kRows + row) * 8, 0, dev::kCpolDev);
+    }
+    __device__ f32x4_t out(int slot, int row, int e) const
+    {
+        return __builtin_bit_cast(f32x4_t, dev::load16<dev::kCpolDev>(outs, ((slot * kRows + row) * D + e) * 4));
+    }
+    __device__ u32x2_t end(int slot, int row) const
+    {
+        return __builtin_bit_cast(
+            u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(ends, (slot * kRows + row) * 8, 0, dev::kCpolDev));
+    }
+};
+
 
 // The keys of row b: [low, high), and its units' number (one at least).
 struct Keys {
@@ -171,17 +218,38 @@ struct Fragment {
     }
 };
 
+// 4 values of the output from their sum, its weights' sum and their maximum; the
+// first ones' thread also writes the head's lse.
+template <bool kBf16>
+__device__ __forceinline__ void finish(const PagedAttentionArgs &a, int b, int head, int e, f32x4_t all, float top,
+                                       float total)
+{
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    uint16_t *out = static_cast<uint16_t *>(a.out.data) + b * a.out.row + head * a.out.head + e;
+    *reinterpret_cast<u32x2_t *>(out) =
+        u32x2_t{dev::pack2_x<kBf16>(all[0] * inv, all[1] * inv), dev::pack2_x<kBf16>(all[2] * inv, all[3] * inv)};
+    if (e == 0 && a.lse != nullptr) {
+        a.lse[(int64_t)b * a.heads + head] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+    }
+}
+
 template <bool kBf16, int D, int RT>
 __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attention_units(Args args)
 {
     using S = Shape<D>;
+    using Left = Parts<D, RT>;
     constexpr int P = pitch<D>();
     __shared__ __align__(16) char lds[kWaves][region<D>()];
     __shared__ float tops[kWaves][16 * RT], sums[kWaves][16 * RT];
+    __shared__ uint32_t tag;
+    __shared__ bool complete;
     const PagedAttentionArgs &a = args.a;
+    const int w = (int)blockIdx.x;
+    const uint32_t replay = threadIdx.x == 0 ? dev::replay_load(args.tag.words, w) : 0u;
     const int lane = (int)threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int c = lane / 16, col = lane % 16;
     const int perRow = a.kvHeads * args.blocks;
+    const Left parts(args.parts, args.most);
 
     // The workgroup's stretch and the row it begins in.
     int count = 0;
@@ -189,7 +257,9 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
         count += Keys(a, b).units;
     }
     const Shares shares(wave_sum_int(count) * perRow, args.most);
-    const int w = (int)blockIdx.x;
+    if (threadIdx.x == 0) {
+        tag = dev::launch_epoch<Args>(w, replay);
+    }
     if (w >= shares.grid) {
         return;
     }
@@ -397,23 +467,61 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
                 }
                 const int h = head0 + rt * 16 + row;
                 if (!whole) {
-                    const int64_t line = (int64_t)slot * 16 * RT + rt * 16 + row;
-                    *reinterpret_cast<f32x4_t *>(args.parts + line * D + e) = all;
+                    parts.put(slot, rt * 16 + row, e, all);
                     if (e == 0) {
-                        float *ends = args.parts + (int64_t)2 * args.most * 16 * RT * D + 2 * line;
-                        ends[0] = most;
-                        ends[1] = total;
+                        parts.put_ends(slot, rt * 16 + row, most, total);
                     }
                 } else if (h < args.group) {
-                    const int64_t head = kvHead * args.group + h;
-                    const float inv = total == 0.f ? 0.f : 1.f / total;
-                    uint16_t *out = static_cast<uint16_t *>(a.out.data) + b * a.out.row + head * a.out.head + e;
-                    *reinterpret_cast<u32x2_t *>(out) = u32x2_t{dev::pack2_x<kBf16>(all[0] * inv, all[1] * inv),
-                                                                dev::pack2_x<kBf16>(all[2] * inv, all[3] * inv)};
-                    if (e == 0 && a.lse != nullptr) {
-                        a.lse[(int64_t)b * a.heads + head] = (zero + __builtin_amdgcn_logf(total)) * kLn2;
-                    }
+                    finish<kBf16>(a, b, kvHead * args.group + h, e, all, zero, total);
                 }
+            }
+            __syncthreads();
+        }
+        if (!whole) {
+            // The part is there once its stores have ended; then the word that says so, and
+            // after that a look at the others' words.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const int u0 = u - tile0, first = shares.owner(u0), last = shares.owner(u0 + keys.units - 1);
+            const int firstSlot = 2 * first + (shares.start(first) == u0 ? 0 : 1);
+            if (wave == 0) {
+                if (lane == 0) {
+                    (void)__hip_atomic_exchange(parts.words + slot, Left::word(tag, slot), __ATOMIC_RELAXED,
+                                                __HIP_MEMORY_SCOPE_AGENT);
+                }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                bool all = true;
+                for (int x = first + lane; x <= last; x += kWave) {
+                    const int at = x == first ? firstSlot : 2 * x;
+                    all = all && __hip_atomic_load(parts.words + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                                     Left::word(tag, at);
+                }
+                all = __all(all);
+                if (lane == 0) {
+                    complete = all;
+                }
+            }
+            __syncthreads();
+            const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
+            for (int at = complete ? (int)threadIdx.x : rows * (D / 4); at < rows * (D / 4); at += 64 * kWaves) {
+                const int row = at / (D / 4), e = at % (D / 4) * 4;
+                float most = -INFINITY;
+#pragma unroll 4
+                for (int x = first; x <= last; ++x) {
+                    most = fmaxf(most, __uint_as_float(parts.end(x == first ? firstSlot : 2 * x, row)[0]));
+                }
+                const float zero = most == -INFINITY ? 0.f : most;
+                float total = 0.f;
+                f32x4_t all = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                for (int x = first; x <= last; ++x) {
+                    const int at = x == first ? firstSlot : 2 * x;
+                    const u32x2_t end = parts.end(at, row);
+                    const float f = __builtin_amdgcn_exp2f(__uint_as_float(end[0]) - zero);
+                    total += f * __uint_as_float(end[1]);
+                    all += f * parts.out(at, row, e);
+                }
+                finish<kBf16>(a, b, kvHead * args.group + head0 + row, e, all, zero, total);
             }
             __syncthreads();
         }
@@ -425,77 +533,10 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
     }
 }
 
-// One workgroup per (row, kv head, block of query heads): joins its stretches'
-// parts, where it has more than one.
-template <bool kBf16, int D, int RT>
-__global__ __launch_bounds__(256) void attention_join(Args args)
-{
-    __shared__ int counts[kWaves], befores[kWaves];
-    const PagedAttentionArgs &a = args.a;
-    const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
-    const int perRow = a.kvHeads * args.blocks;
-    const int b = (int)blockIdx.x / perRow, hg = (int)blockIdx.x % perRow;
-    int count = 0, before = 0;
-    for (int x = (int)threadIdx.x; x < a.B; x += 256) {
-        const int n = Keys(a, x).units;
-        count += n;
-        before += x < b ? n : 0;
-    }
-    count = wave_sum_int(count);
-    before = wave_sum_int(before);
-    if (lane == 0) {
-        counts[wave] = count;
-        befores[wave] = before;
-    }
-    __syncthreads();
-    count = counts[0] + counts[1] + counts[2] + counts[3];
-    before = befores[0] + befores[1] + befores[2] + befores[3];
-    const Shares shares(count * perRow, args.most);
-    const Keys keys(a, b);
-    const int u0 = before * perRow + hg * keys.units;
-    const int first = shares.owner(u0), last = shares.owner(u0 + keys.units - 1);
-    if (first == last) {
-        return;
-    }
-    const float *ends = args.parts + (int64_t)2 * args.most * 16 * RT * D;
-    const int head0 = hg % args.blocks * 16 * RT;
-    const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
-    const int firstSlot = 2 * first + (shares.start(first) == u0 ? 0 : 1);
-    for (int at = (int)threadIdx.x; at < rows * (D / 4); at += 256) {
-        const int row = at / (D / 4), e = at % (D / 4) * 4;
-        float most = -INFINITY;
-        for (int x = first; x <= last; ++x) {
-            most = fmaxf(most, ends[2 * ((int64_t)(x == first ? firstSlot : 2 * x) * 16 * RT + row)]);
-        }
-        const float zero = most == -INFINITY ? 0.f : most;
-        float total = 0.f;
-        f32x4_t all = {0.f, 0.f, 0.f, 0.f};
-        for (int x = first; x <= last; ++x) {
-            const int64_t line = (int64_t)(x == first ? firstSlot : 2 * x) * 16 * RT + row;
-            const float f = __builtin_amdgcn_exp2f(ends[2 * line] - zero);
-            total += f * ends[2 * line + 1];
-            all += f * *reinterpret_cast<const f32x4_t *>(args.parts + line * D + e);
-        }
-        const int64_t head = hg / args.blocks * args.group + head0 + row;
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-        uint16_t *out = static_cast<uint16_t *>(a.out.data) + b * a.out.row + head * a.out.head + e;
-        *reinterpret_cast<u32x2_t *>(out) = u32x2_t{dev::pack2_x<kBf16>(all[0] * inv, all[1] * inv),
-                                                    dev::pack2_x<kBf16>(all[2] * inv, all[3] * inv)};
-        if (e == 0 && a.lse != nullptr) {
-            a.lse[(int64_t)b * a.heads + head] = (zero + __builtin_amdgcn_logf(total)) * kLn2;
-        }
-    }
-}
-
 template <bool kBf16, int D, int RT>
 hipError_t launch_size(const Args &args, hipStream_t stream)
 {
     hipLaunchKernelGGL((attention_units<kBf16, D, RT>), dim3((unsigned)args.most), dim3(64 * kWaves), 0, stream, args);
-    if (const hipError_t err = hipGetLastError(); err != hipSuccess) {
-        return err;
-    }
-    hipLaunchKernelGGL((attention_join<kBf16, D, RT>), dim3((unsigned)(args.a.B * args.a.kvHeads * args.blocks)),
-                       dim3(256), 0, stream, args);
     return hipGetLastError();
 }
 

@@ -20,6 +20,7 @@ Args plan(const PagedAttentionArgs &a, int cus, bool &wide)
     wide = p.group > 16;
     p.blocks = (p.group + (wide ? 31 : 15)) / (wide ? 32 : 16);
     p.most = cus * (a.d > 128 || wide ? 1 : 2);
+    p.most = p.most < kMaxExchangeGrid ? p.most : kMaxExchangeGrid;
     return p;
 }
 
@@ -44,14 +45,19 @@ size_t paged_attention_workspace(const PagedAttentionArgs &a, int cus)
 {
     bool wide;
     const attention::Args p = attention::plan(a, cus, wide);
-    return (size_t)2 * p.most * (wide ? 32 : 16) * (a.d + 2) * 4;
+    return kWsHeaderBytes + (size_t)2 * p.most * ((wide ? 32 : 16) * (a.d + 2) * 4 + 8);
 }
 
-hipError_t launch_paged_attention(const PagedAttentionArgs &a, void *workspace, int cus, hipStream_t stream)
+hipError_t launch_paged_attention(const PagedAttentionArgs &a, void *workspace, int device, int cus,
+                                  hipStream_t stream)
 {
     bool wide;
     attention::Args p = attention::plan(a, cus, wide);
-    p.parts = static_cast<float *>(workspace);
+    p.parts = static_cast<char *>(workspace) + kWsHeaderBytes;
+    const hipError_t err = make_launch_tag(next_launch_id(), device, p.most, workspace, stream, p.tag);
+    if (err != hipSuccess) {
+        return err;
+    }
     return a.isBf16 ? attention::launch_bf16(p, wide, stream) : attention::launch_f16(p, wide, stream);
 }
 

@@ -78,6 +78,30 @@ void buffer_release(const void *buffer)
 
 }  // namespace
 
+namespace mhc {
+
+// Launch ids (hashed into every exchange tag, and written into the status word
+// with a timeout): process-wide, strictly increasing from a start that differs
+// between processes (time and address mixed), skipping 0 and ~0.
+uint32_t next_launch_id()
+{
+    static std::atomic<uint32_t> counter{[] {
+        const uint64_t t = static_cast<uint64_t>(
+            std::chrono::high_resolution_clock::now().time_since_epoch().count());
+        const uint64_t a = reinterpret_cast<uintptr_t>(&counter);
+        uint64_t h = (t ^ (a << 17)) * 0x9E3779B97F4A7C15ull;
+        return static_cast<uint32_t>(h >> 32);
+    }()};
+    for (;;) {
+        const uint32_t e = counter.fetch_add(1u, std::memory_order_relaxed);
+        if (e != 0u && e != 0xFFFFFFFFu) {
+            return e;
+        }
+    }
+}
+
+}  // namespace mhc
+
 struct mhcPreExecutor {
     mhc::Plan plan;
     // Device that holds x (-1: the runtime could not tell, e.g. no device is
@@ -391,26 +415,6 @@ int device_of(const void *p)
         return -1;
     }
     return attr.type == hipMemoryTypeDevice ? attr.device : -1;
-}
-
-// Launch ids (hashed into every exchange tag, and written into the status word
-// with a timeout): process-wide, strictly increasing from a start that differs
-// between processes (time and address mixed), skipping 0 and ~0.
-uint32_t next_launch_id()
-{
-    static std::atomic<uint32_t> counter{[] {
-        const uint64_t t = static_cast<uint64_t>(
-            std::chrono::high_resolution_clock::now().time_since_epoch().count());
-        const uint64_t a = reinterpret_cast<uintptr_t>(&counter);
-        uint64_t h = (t ^ (a << 17)) * 0x9E3779B97F4A7C15ull;
-        return static_cast<uint32_t>(h >> 32);
-    }()};
-    for (;;) {
-        const uint32_t e = counter.fetch_add(1u, std::memory_order_relaxed);
-        if (e != 0u && e != 0xFFFFFFFFu) {
-            return e;
-        }
-    }
 }
 
 // Trailing dims of `t` must be `tail` and its element count `count`.
@@ -1140,7 +1144,7 @@ int launch_on(void *workspace, mhcPreExecutor *executor, hipStream_t stream)
         !device_shape(device, shape)) {
         return MHC_STATUS_HIP_ERROR;
     }
-    const uint32_t launchId = next_launch_id();
+    const uint32_t launchId = mhc::next_launch_id();
     executor->lastLaunchId.store(launchId, std::memory_order_relaxed);
     mhc::LaunchTag tag;
     const char *kernel = "split";

@@ -63,6 +63,8 @@ __host__ __device__ inline uint32_t mix32(uint32_t v)
     return v ^ (v >> 16);
 }
 
+// A number for a launch that no other launch of the process has (mhc_pre_api.cpp).
+uint32_t next_launch_id();
 // The tag of launch `launchId` with `grid` workgroups, on the current device
 // `device` (mhc_pre_replay.hip).
 hipError_t make_launch_tag(uint32_t launchId, int device, int grid, void *workspace, hipStream_t stream,

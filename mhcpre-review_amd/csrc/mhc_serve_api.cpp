@@ -2,6 +2,7 @@
 // executors, workspace sizes and launches.
 
 #include "mhc_serve.h"
+#include "mhc_pre_internal.h"
 #include "mhc_serve_internal.h"
 
 #include <hip/hip_runtime.h>
@@ -183,6 +184,18 @@ mhc::CacheRows cache_rows(const mhcStridedTensor *t)
     return {t->data, stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)};
 }
 
+// Looks the device's replay words up (once per device), so that a launch under
+// stream capture does not have to.
+void prime_replay_words(const mhcServeExecutor &ex)
+{
+    int current = -1;
+    uint32_t *words = nullptr;
+    if (ex.device >= 0 && hipGetDevice(&current) == hipSuccess && current == ex.device) {
+        (void)mhc::replay_words_address(current, &words);
+    }
+    (void)hipGetLastError();
+}
+
 // Hands a filled executor out.
 int finish(mhcServeExecutor *ex, const void *someTensor, uint64_t *workspaceSize, mhcServeExecutor **executor)
 {
@@ -192,6 +205,7 @@ int finish(mhcServeExecutor *ex, const void *someTensor, uint64_t *workspaceSize
     switch (ex->op) {
     case Op::kAttention:
         ex->workspace = ex->empty ? 0 : mhc::paged_attention_workspace(ex->attention, ex->cus);
+        prime_replay_words(*ex);
         break;
     case Op::kUpdate:
         ex->workspace = ex->empty ? 0 : mhc::cache_update_workspace(ex->update);
@@ -222,15 +236,13 @@ int launch(Op op, void *workspace, uint64_t workspaceSize, mhcServeExecutor *ex,
     if (ex->empty) {
         return MHC_STATUS_SUCCESS;
     }
-    if (ex->device >= 0) {
-        int current = -1;
-        if (hipGetDevice(&current) != hipSuccess) {
-            (void)hipGetLastError();
-            return MHC_STATUS_HIP_ERROR;
-        }
-        if (current != ex->device) {
-            return MHC_STATUS_DEVICE_MISMATCH;
-        }
+    int current = -1;
+    if (hipGetDevice(&current) != hipSuccess) {
+        (void)hipGetLastError();
+        return MHC_STATUS_HIP_ERROR;
+    }
+    if (ex->device >= 0 && current != ex->device) {
+        return MHC_STATUS_DEVICE_MISMATCH;
     }
     (void)hipGetLastError();  // an earlier call's error is not this launch's
     hipError_t err = hipSuccess;
@@ -239,7 +251,7 @@ int launch(Op op, void *workspace, uint64_t workspaceSize, mhcServeExecutor *ex,
         err = mhc::launch_norm_rope(ex->rope, ex->cus, stream);
         break;
     case Op::kAttention:
-        err = mhc::launch_paged_attention(ex->attention, workspace, ex->cus, stream);
+        err = mhc::launch_paged_attention(ex->attention, workspace, current, ex->cus, stream);
         break;
     case Op::kUpdate:
         err = mhc::launch_cache_update(ex->update, workspace, ex->cus, stream);

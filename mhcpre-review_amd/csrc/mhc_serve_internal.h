@@ -83,7 +83,8 @@ size_t paged_attention_workspace(const PagedAttentionArgs &a, int cus);
 bool paged_attention_head_size(int64_t d);
 // Whether the kernels' counts of work fit 31 bits.
 bool paged_attention_units_fit(const PagedAttentionArgs &a);
-hipError_t launch_paged_attention(const PagedAttentionArgs &a, void *workspace, int cus, hipStream_t stream);
+hipError_t launch_paged_attention(const PagedAttentionArgs &a, void *workspace, int device, int cus,
+                                  hipStream_t stream);
 size_t cache_update_workspace(const CacheUpdateArgs &a);
 hipError_t launch_cache_update(const CacheUpdateArgs &a, void *workspace, int cus, hipStream_t stream);
 size_t cache_compact_workspace(const CacheCompactArgs &a);
