@@ -90,13 +90,14 @@ __global__ __launch_bounds__(256) void update_rows(CacheUpdateArgs a, uint32_t *
 }
 
 // Inclusive scan of v over the workgroup of 1024; *total gets the sum.
-__device__ int64_t scan_1024(int64_t v, int64_t *total)
+template <typename Int>
+__device__ Int scan_1024(Int v, Int *total)
 {
-    __shared__ int64_t sums[16];
+    __shared__ Int sums[16];
     const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
 #pragma unroll
     for (int m = 1; m < kWave; m *= 2) {
-        const int64_t u = __shfl_up(v, m);
+        const Int u = __shfl_up(v, m);
         v += lane >= m ? u : 0;
     }
     __syncthreads();
@@ -104,7 +105,8 @@ __device__ int64_t scan_1024(int64_t v, int64_t *total)
         sums[wave] = v;
     }
     __syncthreads();
-    int64_t all = 0;
+    Int all = 0;
+#pragma unroll
     for (int w = 0; w < 16; ++w) {
         v += w < wave ? sums[w] : 0;
         all += sums[w];
@@ -113,58 +115,73 @@ __device__ int64_t scan_1024(int64_t v, int64_t *total)
     return v;
 }
 
-// The held pages before each group of words, in LDS.
+// The held pages before each group of words, in LDS: kGroups + 1 counts, the
+// groups as many words each as it takes.
 struct Counts {
     const uint32_t *used;
-    int64_t pages, words, span;  // span: words of a group
-    const int32_t *before;       // [kGroups + 1]
+    int64_t pages, words;
+    int span, groups;  // words of a group; groups that have words
+    const int32_t *before;
 
-    // Called by all 1024 threads.
+    // Called by all 1024 threads; each counts neighbouring groups.
     __device__ Counts(const uint32_t *used_, int64_t pages_, int32_t *lds) : used(used_), pages(pages_), before(lds)
     {
+        constexpr int kEach = kGroups / 1024;
         words = words_of(pages);
-        span = (words + kGroups - 1) / kGroups;
-        int64_t base = 0;
-        for (int g = 0; g < kGroups; g += 1024) {
-            const int64_t first = (g + (int64_t)threadIdx.x) * span;
-            int n = 0;
-            for (int64_t w = first; w < first + span && w < words; ++w) {
-                n += __popc(used[w]);
+        span = (int)((words + kGroups - 1) / kGroups);
+        groups = (int)((words + span - 1) / span);
+        int n[kEach], mine = 0;
+        const int64_t first = (int64_t)threadIdx.x * kEach * span;
+#pragma unroll
+        for (int g = 0; g < kEach; ++g) {
+            n[g] = 0;
+            if (span == 1) {
+                n[g] = first + g < words ? __popc(used[first + g]) : 0;
+            } else {
+                for (int64_t w = first + g * span; w < first + (g + 1) * span && w < words; ++w) {
+                    n[g] += __popc(used[w]);
+                }
             }
-            int64_t total;
-            lds[g + threadIdx.x + 1] = (int32_t)(base + scan_1024(n, &total));
-            base += total;
-            if (g == 0 && threadIdx.x == 0) {
-                lds[0] = 0;
-            }
+            mine += n[g];
+        }
+        int total;
+        int base = scan_1024(mine, &total) - mine;
+#pragma unroll
+        for (int g = 0; g < kEach; ++g) {
+            lds[threadIdx.x * kEach + g] = base;
+            base += n[g];
+        }
+        if (threadIdx.x == 1023) {
+            lds[kGroups] = total;
         }
         __syncthreads();
     }
-    __device__ int64_t held() const { return before[kGroups]; }
+    __device__ int held() const { return before[kGroups]; }
     // Held pages before `page`.
-    __device__ int64_t rank(int64_t page) const
+    __device__ int rank(int64_t page) const
     {
         const int64_t word = page / 32, g = word / span;
-        int64_t n = before[g];
+        int n = before[g];
         for (int64_t w = g * span; w < word; ++w) {
             n += __popc(used[w]);
         }
         return word < words ? n + __popc(used[word] & ((1u << (page % 32)) - 1u)) : n;
     }
+    __device__ int free_before(int g) const { return (int)((int64_t)g * span * 32 - before[g]); }
     // The k-th free page (there is one).
-    __device__ int64_t free_page(int64_t k) const
+    __device__ int free_page(int k) const
     {
-        int low = 0, high = kGroups;  // free pages before group low <= k < before group high
+        int low = 0, high = groups;  // free pages before group low <= k < before group high
         while (high - low > 1) {
             const int mid = (low + high) / 2;
-            if ((int64_t)mid * span * 32 - before[mid] <= k) {
+            if (free_before(mid) <= k) {
                 low = mid;
             } else {
                 high = mid;
             }
         }
-        k -= (int64_t)low * span * 32 - before[low];
-        for (int64_t w = low * span;; ++w) {
+        k -= free_before(low);
+        for (int64_t w = (int64_t)low * span;; ++w) {
             uint32_t f = ~used[w];
             const int n = __popc(f);
             if (k >= n) {
@@ -174,7 +191,7 @@ struct Counts {
             for (; k > 0; --k) {
                 f &= f - 1u;
             }
-            return w * 32 + __ffs(f) - 1;
+            return (int)(w * 32) + __ffs(f) - 1;
         }
     }
 };
@@ -210,7 +227,7 @@ __global__ __launch_bounds__(1024) void update_grants(CacheUpdateArgs a, const u
             any = row.add > 0;
         }
         int64_t total;
-        const int64_t upto = asked + scan_1024(need, &total);
+        const int64_t upto = asked + scan_1024<int64_t>(need, &total);
         asked += total;
         if (r < a.rows) {
             const bool served = any && (need == 0 || upto <= free);
@@ -218,9 +235,10 @@ __global__ __launch_bounds__(1024) void update_grants(CacheUpdateArgs a, const u
         }
     }
     const int64_t given = asked < free ? asked : free;
-    for (int g = (int)threadIdx.x; g < kGroups; g += 1024) {
-        int64_t k = (int64_t)g * counts.span * 32 - lds[g];
-        for (int64_t w = g * counts.span; w < (g + 1) * counts.span && w < counts.words && k < given; ++w) {
+    for (int g = (int)threadIdx.x; g < counts.groups; g += 1024) {
+        int64_t k = counts.free_before(g);
+        for (int64_t w = (int64_t)g * counts.span; w < (int64_t)(g + 1) * counts.span && w < counts.words && k < given;
+             ++w) {
             for (uint32_t f = ~used[w]; f != 0u && k < given; f &= f - 1u) {
                 const int64_t page = w * 32 + __ffs(f) - 1;
                 if (page < a.pages) {
@@ -298,16 +316,16 @@ __global__ __launch_bounds__(1024) void compact_apply(CacheCompactArgs a, const 
 {
     __shared__ int32_t lds[kGroups + 1];
     const Counts counts(used, a.pages, lds);
-    const int64_t U = counts.held(), stay = counts.rank(U), moves = U - stay;
+    const int U = counts.held(), stay = counts.rank(U), moves = U - stay;
     const int64_t at = (int64_t)blockIdx.x * 1024 + threadIdx.x, all = (int64_t)gridDim.x * 1024;
     if (at == 0) {
         a.used[0] = (int32_t)U;
     }
     for (int64_t page = U + at; page < a.pages; page += all) {
         if ((used[page / 32] >> (page % 32) & 1u) != 0u) {
-            const int64_t k = counts.rank(page) - stay;
+            const int k = counts.rank(page) - stay;
             a.src[k] = (int32_t)page;
-            a.dst[k] = (int32_t)counts.free_page(k);
+            a.dst[k] = counts.free_page(k);
         }
     }
     for (int64_t k = moves + at; k < a.pages / 2; k += all) {
@@ -317,31 +335,104 @@ __global__ __launch_bounds__(1024) void compact_apply(CacheCompactArgs a, const 
         for (int64_t j = threadIdx.x; j < a.width; j += 1024) {
             int page = held_entry(a, r, j);
             if (page >= U) {
-                page = (int)counts.free_page(counts.rank(page) - stay);
+                page = counts.free_page(counts.rank(page) - stay);
             }
             a.newTable[r * a.width + j] = page;
         }
     }
 }
 
-// One workgroup per pair and cache.
-__global__ __launch_bounds__(256) void copy_rows(CopyPagesArgs a)
+// A page as n0 x n1 runs of `run` bytes, s0 and s1 bytes apart.
+struct Runs {
+    char *base;
+    int64_t page;  // bytes
+    int n0, n1;
+    int64_t s0, s1, run;
+};
+
+// Vec-sized pieces of the pages, kPer a thread: a workgroup has 256 * kPer pieces of
+// one pair's page in one cache.
+constexpr int kPer = 4;
+
+template <typename Vec>
+__global__ __launch_bounds__(256) void copy_pieces(Runs k, Runs v, const int32_t *srcs, const int32_t *dsts, int64_t n,
+                                                   int64_t pages, int64_t pieces, int64_t blocksPerPage)
 {
-    const CacheRows &c = blockIdx.y == 0 ? a.k : a.v;
-    const int rows = a.kvHeads * a.pageSize;
-    for (int64_t i = blockIdx.x; i < a.n; i += gridDim.x) {
-        const int64_t src = a.src[i], dst = a.dst[i];
-        if (src < 0 || src >= a.pages || dst < 0 || dst >= a.pages) {
+    for (int64_t block = blockIdx.x; block < 2 * n * blocksPerPage; block += gridDim.x) {
+        const int64_t pair = block / blocksPerPage, i = pair / 2;
+        const int64_t src = srcs[i], dst = dsts[i];
+        if (src < 0 || src >= pages || dst < 0 || dst >= pages) {
             continue;
         }
-        char *base = static_cast<char *>(c.data);
-        for (int64_t e = threadIdx.x; e < (int64_t)rows * (a.rowBytes / 2); e += 256) {
-            const int64_t row = e / (a.rowBytes / 2), at = e % (a.rowBytes / 2) * 2;
-            const int64_t inside = (row / a.kvHeads * c.slot + row % a.kvHeads * c.head) * a.elemBytes + at;
-            *reinterpret_cast<uint16_t *>(base + dst * c.page * a.elemBytes + inside) =
-                *reinterpret_cast<const uint16_t *>(base + src * c.page * a.elemBytes + inside);
+        const Runs &c = pair % 2 == 0 ? k : v;
+        const int64_t first = block % blocksPerPage * (256 * kPer) + threadIdx.x;
+        const int64_t inRun = c.run / (int64_t)sizeof(Vec);
+        Vec held[kPer];
+        int64_t at[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int64_t e = first + 256 * j;
+            at[j] = -1;
+            if (e < pieces) {
+                int64_t inside = e * (int64_t)sizeof(Vec);
+                if (c.n0 * (int64_t)c.n1 > 1) {
+                    const int64_t row = e / inRun;
+                    inside = row / c.n1 * c.s0 + row % c.n1 * c.s1 + e % inRun * (int64_t)sizeof(Vec);
+                }
+                at[j] = inside;
+                held[j] = *reinterpret_cast<const Vec *>(c.base + src * c.page + inside);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if (at[j] >= 0) {
+                *reinterpret_cast<Vec *>(c.base + dst * c.page + at[j]) = held[j];
+            }
         }
     }
+}
+
+// The runs of a cache's pages, as long as they come.
+Runs runs_of(const CacheRows &c, const CopyPagesArgs &a)
+{
+    Runs r;
+    r.base = static_cast<char *>(c.data);
+    r.page = c.page * a.elemBytes;
+    int64_t slot = c.slot * a.elemBytes, head = c.head * a.elemBytes;
+    r.run = a.rowBytes;
+    int slots = a.pageSize, heads = a.kvHeads;
+    for (int again = 0; again < 2; ++again) {
+        if (heads > 1 && head == r.run) {
+            r.run *= heads;
+            heads = 1;
+        }
+        if (slots > 1 && slot == r.run) {
+            r.run *= slots;
+            slots = 1;
+        }
+    }
+    r.n0 = slots;
+    r.s0 = slots > 1 ? slot : 0;
+    r.n1 = heads;
+    r.s1 = heads > 1 ? head : 0;
+    return r;
+}
+
+bool whole_pieces(const Runs &r, int64_t size)
+{
+    return reinterpret_cast<uintptr_t>(r.base) % size == 0 && r.page % size == 0 && r.s0 % size == 0 &&
+           r.s1 % size == 0 && r.run % size == 0;
+}
+
+template <typename Vec>
+hipError_t launch_pieces(const CopyPagesArgs &a, const Runs &k, const Runs &v, int cus, hipStream_t stream)
+{
+    const int64_t pieces = (int64_t)a.pageSize * a.kvHeads * a.rowBytes / (int64_t)sizeof(Vec);
+    const int64_t perPage = (pieces + 256 * kPer - 1) / (256 * kPer);
+    const int64_t blocks = 2 * a.n * perPage, most = (int64_t)cus * 1024;
+    hipLaunchKernelGGL((copy_pieces<Vec>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, k, v,
+                       a.src, a.dst, a.n, a.pages, pieces, perPage);
+    return hipGetLastError();
 }
 
 size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
@@ -405,9 +496,14 @@ hipError_t launch_cache_compact(const CacheCompactArgs &a, void *workspace, int 
 
 hipError_t launch_copy_pages(const CopyPagesArgs &a, int cus, hipStream_t stream)
 {
-    const int64_t blocks = a.n < 8 * (int64_t)cus ? a.n : 8 * (int64_t)cus;
-    hipLaunchKernelGGL(copy_rows, dim3((unsigned)blocks, 2), dim3(256), 0, stream, a);
-    return hipGetLastError();
+    const Runs k = runs_of(a.k, a), v = runs_of(a.v, a);
+    if (whole_pieces(k, 16) && whole_pieces(v, 16)) {
+        return launch_pieces<dev::u32x4_t>(a, k, v, cus, stream);
+    }
+    if (whole_pieces(k, 4) && whole_pieces(v, 4)) {
+        return launch_pieces<uint32_t>(a, k, v, cus, stream);
+    }
+    return launch_pieces<uint16_t>(a, k, v, cus, stream);
 }
 
 }  // namespace mhc

@@ -30,7 +30,8 @@ __device__ __forceinline__ uint16_t *cache_at(const CacheRows &c, const NormRope
     return static_cast<uint16_t *>(c.data) + slot / a.pageSize * c.page + slot % a.pageSize * c.slot + h * c.head;
 }
 
-// Row `row` of the tokens' heads of q, k and v, one wave.
+// Row `row` of the tokens' heads of q, k and v, one wave: any size, stride and
+// alignment.
 template <bool kBf16>
 __device__ void one_row(const NormRopeArgs &a, int64_t row, int perToken, int lane)
 {
@@ -116,11 +117,202 @@ __global__ __launch_bounds__(256) void norm_rope_rows(NormRopeArgs a, int64_t ro
     }
 }
 
+// Sum over the aligned group of L lanes that the lane is in.
+template <int L>
+__device__ __forceinline__ float group_sum(float v)
+{
+    const auto add = [&](auto ctrl) {
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xF, 0xF, true));
+    };
+    if constexpr (L >= 2) {
+        add(std::integral_constant<int, 0xB1>{});  // quad_perm [1, 0, 3, 2]
+    }
+    if constexpr (L >= 4) {
+        add(std::integral_constant<int, 0x4E>{});  // quad_perm [2, 3, 0, 1]
+    }
+    if constexpr (L >= 8) {
+        add(std::integral_constant<int, 0x141>{});  // row_half_mirror: the other quad, all alike
+    }
+    if constexpr (L >= 16) {
+        add(std::integral_constant<int, 0x140>{});  // row_mirror
+    }
+    if constexpr (L >= 32) {
+        v += __shfl_xor(v, 16);
+    }
+    if constexpr (L >= 64) {
+        v += __shfl_xor(v, 32);
+    }
+    return v;
+}
+
+struct Split {
+    int parts;       // of a token's rows, each a wave's
+    int q, k, all;   // steps of 64 / L rows: of q, of k, with v's
+};
+
+// Rows whose 16-byte pieces are aligned: L lanes to a row (d / 16 of them with
+// work), each with 8 pairs: the pieces at 8 c and rot / 2 + 8 c, or the two at 16
+// c (interleaved; and the rest of a head beyond rot).  A wave has some of a token's
+// rows, 64 / L at a time, and computes the token's 8 angles per lane once for all of
+// them.
+template <bool kBf16, int L, bool kInterleaved>
+__global__ __launch_bounds__(256) void norm_rope_pieces(NormRopeArgs a, Split split)
+{
+    constexpr int kRows = kWave / L;
+    const int lane = (int)threadIdx.x % kWave, c = lane % L, sub = lane / L;
+    const int half = a.rot / 2;
+    const bool on = 16 * c < a.d;
+    const bool turned = 8 * c < half;  // (whole pieces, or interleaved)
+    const int at0 = kInterleaved ? 16 * c : turned ? 8 * c : a.rot + 2 * (8 * c - half);
+    const int at1 = kInterleaved || !turned ? at0 + 8 : half + 8 * c;
+    double freq[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int p = 8 * c + j;
+        freq[j] = p < half ? a.invFreq[p] * 0.15915494309189533577 : 0.0;
+    }
+    const int64_t items = a.T * split.parts, step = (int64_t)gridDim.x * 4;
+    for (int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave); item < items;
+         item += step) {
+        const int64_t t = split.parts == 1 ? item : item / split.parts;
+        const int part = split.parts == 1 ? 0 : (int)(item - t * split.parts);
+        const int begin = part * split.all / split.parts, end = (part + 1) * split.all / split.parts;
+        float cosine[8], sine[8];
+        const double pos = a.positions64 ? (double)static_cast<const int64_t *>(a.positions)[t]
+                                         : (double)static_cast<const int32_t *>(a.positions)[t];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double turns = pos * freq[j];
+            const float f = (float)(turns - __builtin_rint(turns));
+            cosine[j] = __builtin_amdgcn_cosf(f) * a.amplitude;
+            sine[j] = __builtin_amdgcn_sinf(f) * a.amplitude;
+        }
+        for (int i = begin; i < end; ++i) {
+            const bool isQ = i < split.q, isV = i >= split.q + split.k;
+            const int h = (isQ ? i : isV ? i - split.q - split.k : i - split.q) * kRows + sub;
+            if (h >= (isQ ? a.heads : a.kvHeads)) {
+                continue;  // (a row's lanes leave together)
+            }
+            const HeadRows &in = isQ ? a.q : isV ? a.v : a.k;
+            const uint16_t *x = static_cast<const uint16_t *>(in.data) + t * in.row + h * in.head;
+            uint16_t *y;
+            if (isQ) {
+                y = static_cast<uint16_t *>(a.qOut.data) + t * a.qOut.row + h * a.qOut.head;
+            } else if (a.kOut.data != nullptr) {
+                y = static_cast<uint16_t *>(a.kOut.data) + t * a.kOut.row + h * a.kOut.head;
+            } else {
+                y = cache_at(isV ? a.vCache : a.kCache, a, t, h);
+                if (y == nullptr) {
+                    break;  // no slot: neither k nor v of this token goes anywhere
+                }
+            }
+            // (Lanes without values stay: their row's sum goes through them.)
+            dev::u32x4_t r0 = {0, 0, 0, 0}, r1 = {0, 0, 0, 0};
+            if (on) {
+                r0 = *reinterpret_cast<const dev::u32x4_t *>(x + at0);
+                r1 = *reinterpret_cast<const dev::u32x4_t *>(x + at1);
+            }
+            if (!isV) {
+                float u[8], v[8];
+                dev::unpack8<kBf16>(r0, u);
+                dev::unpack8<kBf16>(r1, v);
+                const float *w = isQ ? a.qWeight : a.kWeight;
+                if (w != nullptr) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        sum = __builtin_fmaf(u[j], u[j], sum);
+                        sum = __builtin_fmaf(v[j], v[j], sum);
+                    }
+                    sum = group_sum<L>(sum);
+                    const float inv = 1.f / __builtin_sqrtf(sum / (float)a.d + a.eps);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        u[j] *= inv * (on ? w[at0 + j] : 0.f);
+                        v[j] *= inv * (on ? w[at1 + j] : 0.f);
+                    }
+                }
+                if constexpr (kInterleaved) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float &first = j < 4 ? u[2 * j] : v[2 * j - 8], &second = j < 4 ? u[2 * j + 1] : v[2 * j - 7];
+                        const float u0 = first, v0 = second;
+                        const bool turn = 8 * c + j < half;
+                        first = turn ? u0 * cosine[j] - v0 * sine[j] : u0;
+                        second = turn ? u0 * sine[j] + v0 * cosine[j] : v0;
+                    }
+                } else if (turned) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float u0 = u[j];
+                        u[j] = u0 * cosine[j] - v[j] * sine[j];
+                        v[j] = u0 * sine[j] + v[j] * cosine[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    r0[j] = dev::pack2_x<kBf16>(u[2 * j], u[2 * j + 1]);
+                    r1[j] = dev::pack2_x<kBf16>(v[2 * j], v[2 * j + 1]);
+                }
+            }
+            if (on) {
+                *reinterpret_cast<dev::u32x4_t *>(y + at0) = r0;
+                *reinterpret_cast<dev::u32x4_t *>(y + at1) = r1;
+            }
+        }
+    }
+}
+
+bool even_rows(const HeadRows &r)
+{
+    return (reinterpret_cast<uintptr_t>(r.data) % 16 | r.row % 8 | r.head % 8) == 0;
+}
+
+bool even_cache(const CacheRows &r)
+{
+    return (reinterpret_cast<uintptr_t>(r.data) % 16 | r.page % 8 | r.slot % 8 | r.head % 8) == 0;
+}
+
+template <bool kBf16, int L>
+hipError_t launch_pieces(const NormRopeArgs &a, int cus, hipStream_t stream)
+{
+    constexpr int kRows = kWave / L;
+    Split s;
+    s.q = (a.heads + kRows - 1) / kRows;
+    s.k = (a.kvHeads + kRows - 1) / kRows;
+    s.all = s.q + s.k * (a.kOut.data != nullptr ? 1 : 2);
+    // A token's rows are shared out while that gives the waves that fill the CUs something to do.
+    const int64_t fill = (int64_t)cus * 16;
+    const int64_t want = a.T < fill ? (fill + a.T - 1) / a.T : 1;
+    s.parts = want < s.all ? (int)want : s.all;
+    const int64_t blocks = (a.T * s.parts + 3) / 4, most = (int64_t)cus * 8;
+    const auto kernel = a.interleaved ? norm_rope_pieces<kBf16, L, true> : norm_rope_pieces<kBf16, L, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, a, s);
+    return hipGetLastError();
+}
+
+template <bool kBf16>
+hipError_t launch_pieces_of(const NormRopeArgs &a, int cus, hipStream_t stream)
+{
+    const int lanes = a.d / 16;
+    return lanes <= 1    ? launch_pieces<kBf16, 1>(a, cus, stream)
+           : lanes <= 2  ? launch_pieces<kBf16, 2>(a, cus, stream)
+           : lanes <= 4  ? launch_pieces<kBf16, 4>(a, cus, stream)
+           : lanes <= 8  ? launch_pieces<kBf16, 8>(a, cus, stream)
+           : lanes <= 16 ? launch_pieces<kBf16, 16>(a, cus, stream)
+           : lanes <= 32 ? launch_pieces<kBf16, 32>(a, cus, stream)
+                         : launch_pieces<kBf16, 64>(a, cus, stream);
+}
+
 }  // namespace
 
 hipError_t launch_norm_rope(const NormRopeArgs &a, int cus, hipStream_t stream)
 {
-    (void)cus;
+    const bool append = a.kOut.data == nullptr;
+    if (a.d % 16 == 0 && (a.interleaved || a.rot % 16 == 0) && even_rows(a.q) && even_rows(a.k) && even_rows(a.qOut) &&
+        (append ? even_rows(a.v) && even_cache(a.kCache) && even_cache(a.vCache) : even_rows(a.kOut))) {
+        return a.isBf16 ? launch_pieces_of<true>(a, cus, stream) : launch_pieces_of<false>(a, cus, stream);
+    }
     const int perToken = a.heads + a.kvHeads * (a.kOut.data != nullptr ? 1 : 2);
     const int64_t rows = a.T * perToken;
     const int64_t most = int64_t{1} << 22, blocks = (rows + 3) / 4 < most ? (rows + 3) / 4 : most;
