@@ -145,16 +145,19 @@ __device__ __forceinline__ float group_sum(float v)
     return v;
 }
 
+constexpr int kSteps = 4;
+
 struct Split {
     int parts;       // of a token's rows, each a wave's
     int q, k, all;   // steps of 64 / L rows: of q, of k, with v's
 };
 
 // Rows whose 16-byte pieces are aligned: L lanes to a row (d / 16 of them with
-// work), each with 8 pairs: the pieces at 8 c and rot / 2 + 8 c, or the two at 16
-// c (interleaved; and the rest of a head beyond rot).  A wave has some of a token's
-// rows, 64 / L at a time, and computes the token's 8 angles per lane once for all of
-// them.
+// work), each with 8 pairs in two pieces: at 8 c and rot / 2 + 8 c (the half layout;
+// beyond rot likewise, half of the rest apart), or at 8 c and d / 2 + 8 c
+// (interleaved), so that neighbouring lanes have neighbouring pieces.  A wave has
+// some of a token's rows, 64 / L at a time, and computes the token's 8 angles per
+// lane once for all of them.
 template <bool kBf16, int L, bool kInterleaved>
 __global__ __launch_bounds__(256) void norm_rope_pieces(NormRopeArgs a, Split split)
 {
@@ -162,13 +165,15 @@ __global__ __launch_bounds__(256) void norm_rope_pieces(NormRopeArgs a, Split sp
     const int lane = (int)threadIdx.x % kWave, c = lane % L, sub = lane / L;
     const int half = a.rot / 2;
     const bool on = 16 * c < a.d;
-    const bool turned = 8 * c < half;  // (whole pieces, or interleaved)
-    const int at0 = kInterleaved ? 16 * c : turned ? 8 * c : a.rot + 2 * (8 * c - half);
-    const int at1 = kInterleaved || !turned ? at0 + 8 : half + 8 * c;
+    const bool turned = 8 * c < half;  // (the half layout: a lane's pairs all are or none is)
+    const int at0 = kInterleaved || turned ? 8 * c : half + 8 * c;
+    const int at1 = kInterleaved ? a.d / 2 + 8 * c : turned ? half + 8 * c : a.d / 2 + 8 * c;
+    const float perValue = 1.f / (float)a.d;
+    const auto pair = [&](int j) { return !kInterleaved ? 8 * c + j : j < 4 ? 4 * c + j : a.d / 4 + 4 * c + j - 4; };
     double freq[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const int p = 8 * c + j;
+        const int p = pair(j);
         freq[j] = p < half ? a.invFreq[p] * 0.15915494309189533577 : 0.0;
     }
     const int64_t items = a.T * split.parts, step = (int64_t)gridDim.x * 4;
@@ -187,77 +192,108 @@ __global__ __launch_bounds__(256) void norm_rope_pieces(NormRopeArgs a, Split sp
             cosine[j] = __builtin_amdgcn_cosf(f) * a.amplitude;
             sine[j] = __builtin_amdgcn_sinf(f) * a.amplitude;
         }
-        for (int i = begin; i < end; ++i) {
-            const bool isQ = i < split.q, isV = i >= split.q + split.k;
-            const int h = (isQ ? i : isV ? i - split.q - split.k : i - split.q) * kRows + sub;
-            if (h >= (isQ ? a.heads : a.kvHeads)) {
-                continue;  // (a row's lanes leave together)
-            }
-            const HeadRows &in = isQ ? a.q : isV ? a.v : a.k;
-            const uint16_t *x = static_cast<const uint16_t *>(in.data) + t * in.row + h * in.head;
-            uint16_t *y;
-            if (isQ) {
-                y = static_cast<uint16_t *>(a.qOut.data) + t * a.qOut.row + h * a.qOut.head;
-            } else if (a.kOut.data != nullptr) {
-                y = static_cast<uint16_t *>(a.kOut.data) + t * a.kOut.row + h * a.kOut.head;
-            } else {
-                y = cache_at(isV ? a.vCache : a.kCache, a, t, h);
-                if (y == nullptr) {
-                    break;  // no slot: neither k nor v of this token goes anywhere
+        // Norm and rotation of the lane's two pieces.
+        const auto turn_row = [&](dev::u32x4_t &r0, dev::u32x4_t &r1, bool norm, const float (&w)[16]) {
+            float u[8], v[8];
+            dev::unpack8<kBf16>(r0, u);
+            dev::unpack8<kBf16>(r1, v);
+            if (norm) {
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    sum = __builtin_fmaf(u[j], u[j], sum);
+                    sum = __builtin_fmaf(v[j], v[j], sum);
+                }
+                const float inv = __builtin_amdgcn_rsqf(group_sum<L>(sum) * perValue + a.eps);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    u[j] *= inv * w[j];
+                    v[j] *= inv * w[8 + j];
                 }
             }
-            // (Lanes without values stay: their row's sum goes through them.)
-            dev::u32x4_t r0 = {0, 0, 0, 0}, r1 = {0, 0, 0, 0};
-            if (on) {
-                r0 = *reinterpret_cast<const dev::u32x4_t *>(x + at0);
-                r1 = *reinterpret_cast<const dev::u32x4_t *>(x + at1);
-            }
-            if (!isV) {
-                float u[8], v[8];
-                dev::unpack8<kBf16>(r0, u);
-                dev::unpack8<kBf16>(r1, v);
-                const float *w = isQ ? a.qWeight : a.kWeight;
-                if (w != nullptr) {
-                    float sum = 0.f;
+            if constexpr (kInterleaved) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        sum = __builtin_fmaf(u[j], u[j], sum);
-                        sum = __builtin_fmaf(v[j], v[j], sum);
-                    }
-                    sum = group_sum<L>(sum);
-                    const float inv = 1.f / __builtin_sqrtf(sum / (float)a.d + a.eps);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        u[j] *= inv * (on ? w[at0 + j] : 0.f);
-                        v[j] *= inv * (on ? w[at1 + j] : 0.f);
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    float &first = j < 4 ? u[2 * j] : v[2 * j - 8], &second = j < 4 ? u[2 * j + 1] : v[2 * j - 7];
+                    const float u0 = first, v0 = second;
+                    const bool turn = pair(j) < half;
+                    first = turn ? u0 * cosine[j] - v0 * sine[j] : u0;
+                    second = turn ? u0 * sine[j] + v0 * cosine[j] : v0;
                 }
-                if constexpr (kInterleaved) {
+            } else if (turned) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float &first = j < 4 ? u[2 * j] : v[2 * j - 8], &second = j < 4 ? u[2 * j + 1] : v[2 * j - 7];
-                        const float u0 = first, v0 = second;
-                        const bool turn = 8 * c + j < half;
-                        first = turn ? u0 * cosine[j] - v0 * sine[j] : u0;
-                        second = turn ? u0 * sine[j] + v0 * cosine[j] : v0;
-                    }
-                } else if (turned) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float u0 = u[j];
-                        u[j] = u0 * cosine[j] - v[j] * sine[j];
-                        v[j] = u0 * sine[j] + v[j] * cosine[j];
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    r0[j] = dev::pack2_x<kBf16>(u[2 * j], u[2 * j + 1]);
-                    r1[j] = dev::pack2_x<kBf16>(v[2 * j], v[2 * j + 1]);
+                for (int j = 0; j < 8; ++j) {
+                    const float u0 = u[j];
+                    u[j] = u0 * cosine[j] - v[j] * sine[j];
+                    v[j] = u0 * sine[j] + v[j] * cosine[j];
                 }
             }
-            if (on) {
-                *reinterpret_cast<dev::u32x4_t *>(y + at0) = r0;
-                *reinterpret_cast<dev::u32x4_t *>(y + at1) = r1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                r0[j] = dev::pack2_x<kBf16>(u[2 * j], u[2 * j + 1]);
+                r1[j] = dev::pack2_x<kBf16>(v[2 * j], v[2 * j + 1]);
+            }
+        };
+        // kSteps steps' rows are on their way at once.
+        const auto rows = [&](auto kind, const HeadRows &in, const HeadRows &out, int heads, const float *w, int first,
+                              int last) {
+            constexpr bool isV = decltype(kind)::value == 2;
+            float weights[16];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                weights[j] = !isV && w != nullptr && on ? w[at0 + j] : 0.f;
+                weights[8 + j] = !isV && w != nullptr && on ? w[at1 + j] : 0.f;
+            }
+            for (int i = first; i < last; i += kSteps) {
+                dev::u32x4_t r0[kSteps], r1[kSteps];
+#pragma unroll
+                for (int n = 0; n < kSteps; ++n) {
+                    const int h = (i + n) * kRows + sub;
+                    // (Lanes without values stay: their row's sum goes through them.)
+                    r0[n] = r1[n] = dev::u32x4_t{0, 0, 0, 0};
+                    if (on && i + n < last && h < heads) {
+                        const uint16_t *x = static_cast<const uint16_t *>(in.data) + t * in.row + h * in.head;
+                        r0[n] = *reinterpret_cast<const dev::u32x4_t *>(x + at0);
+                        r1[n] = *reinterpret_cast<const dev::u32x4_t *>(x + at1);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < kSteps; ++n) {
+                    if (i + n >= last) {
+                        break;
+                    }
+                    const int h = (i + n) * kRows + sub;
+                    if constexpr (!isV) {
+                        turn_row(r0[n], r1[n], w != nullptr, weights);
+                    }
+                    if (on && h < heads) {
+                        uint16_t *y = static_cast<uint16_t *>(out.data) + h * out.head;
+                        *reinterpret_cast<dev::u32x4_t *>(y + at0) = r0[n];
+                        *reinterpret_cast<dev::u32x4_t *>(y + at1) = r1[n];
+                    }
+                }
+            }
+        };
+        const auto clip = [](int v, int low, int high) { return v < low ? low : v > high ? high : v; };
+        const int q0 = clip(begin, 0, split.q), q1 = clip(end, 0, split.q);
+        if (q0 < q1) {
+            HeadRows out = a.qOut;
+            out.data = static_cast<uint16_t *>(out.data) + t * out.row;
+            rows(std::integral_constant<int, 0>{}, a.q, out, a.heads, a.qWeight, q0, q1);
+        }
+        const int k0 = clip(begin - split.q, 0, split.k), k1 = clip(end - split.q, 0, split.k);
+        const int v0 = clip(begin - split.q - split.k, 0, split.k), v1 = clip(end - split.q - split.k, 0, split.k);
+        if (a.kOut.data != nullptr) {
+            HeadRows out = a.kOut;
+            out.data = static_cast<uint16_t *>(out.data) + t * out.row;
+            rows(std::integral_constant<int, 1>{}, a.k, out, a.kvHeads, a.kWeight, k0, k1);
+        } else if (k0 < k1 || v0 < v1) {
+            // No slot: neither k nor v of this token goes anywhere.
+            uint16_t *y = cache_at(a.kCache, a, t, 0);
+            if (y != nullptr) {
+                rows(std::integral_constant<int, 1>{}, a.k, HeadRows{y, 0, a.kCache.head}, a.kvHeads, a.kWeight, k0, k1);
+                rows(std::integral_constant<int, 2>{}, a.v, HeadRows{cache_at(a.vCache, a, t, 0), 0, a.vCache.head},
+                     a.kvHeads, nullptr, v0, v1);
             }
         }
     }
