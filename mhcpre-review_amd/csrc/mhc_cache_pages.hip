@@ -15,40 +15,51 @@ namespace {
 
 using dev::kWave;
 
+// What one workgroup does alone.
+constexpr int kSmallPages = 1 << 16, kSmallWords = kSmallPages / 32, kSmallRows = 1024;
+constexpr int64_t kSmallEntries = 1 << 15;
+constexpr int kSmallBatch = 8;
+
 constexpr int kGroups = 8192;  // of words whose counts LDS holds (32 KB)
 
 __host__ __device__ __forceinline__ int64_t words_of(int64_t pages) { return (pages + 31) / 32; }
 
-__device__ __forceinline__ int64_t clamped(int64_t v, int64_t most) { return v < 0 ? 0 : v > most ? most : v; }
+__device__ __forceinline__ int clamped(int v, int most) { return v < 0 ? 0 : v > most ? most : v; }
+
+// Pages of `tokens` tokens (below 2^32).
+__device__ __forceinline__ int pages_for(uint32_t tokens, int pageSize)
+{
+    return tokens == 0 ? 0 : (int)((tokens - 1) / (uint32_t)pageSize) + 1;
+}
 
 // Row r of mhcCacheUpdate: what it goes on from and what it asks for.
 struct Row {
-    const int32_t *base;  // its parent's entries, or null
-    int64_t length, held, grown;
+    int parent;  // row of the old table, or -1
+    int length, held, grown;
     int add;  // tokens, 0 where they cannot fit the table's width
 
+    Row() = default;
     __device__ Row(const CacheUpdateArgs &a, int64_t r)
     {
-        const int64_t p = a.parents[r];
-        const bool alive = p >= 0 && p < a.rows;
-        length = alive ? clamped(a.lengths[p], (int64_t)a.width * a.pageSize) : 0;
-        base = alive ? a.table + p * a.width : nullptr;
-        held = (length + a.pageSize - 1) / a.pageSize;
-        add = (int)clamped(a.counts[r], a.tokens);
-        grown = (length + add + a.pageSize - 1) / a.pageSize;
+        parent = a.parents[r];
+        parent = parent >= 0 && parent < a.rows ? parent : -1;
+        length = parent >= 0 ? clamped(a.lengths[parent], a.width * a.pageSize) : 0;
+        held = pages_for((uint32_t)length, a.pageSize);
+        add = clamped(a.counts[r], a.tokens);
+        grown = pages_for((uint32_t)length + (uint32_t)add, a.pageSize);
         if (grown > a.width) {
             add = 0;
             grown = held;
         }
     }
     // The entry at column j < held, -1 for a hole.
-    __device__ int entry(const CacheUpdateArgs &a, int64_t j) const
+    __device__ int entry(const CacheUpdateArgs &a, int j) const
     {
-        const int page = base[j];
+        const int page = a.table[(int64_t)parent * a.width + j];
         return page >= 0 && page < a.pages ? page : -1;
     }
     // The first column that the new tokens may change.
-    __device__ int64_t open(const CacheUpdateArgs &a) const
+    __device__ int open(const CacheUpdateArgs &a) const
     {
         return add > 0 && length % a.pageSize != 0 ? held - 1 : held;
     }
@@ -61,30 +72,53 @@ __global__ __launch_bounds__(256) void clear_words(uint32_t *words, int64_t n)
     }
 }
 
-__device__ __forceinline__ void mark(int page, uint32_t *used, uint32_t *many)
+// Marks pages (-1: none), all of them on their way at once.
+template <int N>
+__device__ __forceinline__ void mark_all(const int (&page)[N], uint32_t *used, uint32_t *many)
 {
-    const uint32_t bit = 1u << (page % 32);
-    const uint32_t before = __hip_atomic_fetch_or(used + page / 32, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (many != nullptr && (before & bit) != 0u) {
-        (void)__hip_atomic_fetch_or(many + page / 32, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    uint32_t before[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        before[n] = page[n] >= 0 ? __hip_atomic_fetch_or(used + page[n] / 32, 1u << (page[n] % 32), __ATOMIC_RELAXED,
+                                                         __HIP_MEMORY_SCOPE_AGENT)
+                                 : 0u;
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        if (many != nullptr && page[n] >= 0 && (before[n] >> (page[n] % 32) & 1u) != 0u) {
+            (void)__hip_atomic_fetch_or(many + page[n] / 32, 1u << (page[n] % 32), __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT);
+        }
     }
 }
 
-// Marks a row's pages and writes the columns of its new row that the new
-// tokens leave alone.
+// One workgroup per row: marks its pages and writes the columns of its new row
+// that the new tokens leave alone.  The entries are loaded kBatch at a time
+// before the first is marked, for a mark waits for the word that was there.
+constexpr int kBatch = 4;
+
 __global__ __launch_bounds__(256) void update_rows(CacheUpdateArgs a, uint32_t *used, uint32_t *many)
 {
     const int64_t r = blockIdx.x;
     const Row row(a, r);
-    const int64_t open = row.open(a), end = row.add > 0 ? row.grown : open;
+    const int open = row.open(a), end = row.add > 0 ? row.grown : open;
     int32_t *out = a.newTable + r * a.width;
-    for (int64_t j = threadIdx.x; j < a.width; j += 256) {
-        const int page = j < row.held ? row.entry(a, j) : -1;
-        if (page >= 0) {
-            mark(page, used, many);
+    for (int j0 = (int)threadIdx.x; j0 < a.width; j0 += 256 * kBatch) {
+        int page[kBatch];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            const int j = j0 + 256 * n;
+            page[n] = j < row.held ? row.entry(a, j) : -1;
         }
-        if (j < open || j >= end) {
-            out[j] = page;
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            const int j = j0 + 256 * n;
+            if (j < a.width && (j < open || j >= end)) {
+                out[j] = page[n];
+            }
+        }
+        if (j0 - (int)threadIdx.x < row.held) {
+            mark_all(page, used, many);
         }
     }
 }
@@ -115,31 +149,39 @@ __device__ Int scan_1024(Int v, Int *total)
     return v;
 }
 
-// The held pages before each group of words, in LDS: kGroups + 1 counts, the
-// groups as many words each as it takes.
+// The held pages before each group of words, in LDS: kMost + 1 counts, with
+// kOne a word to a group and the words in LDS too (a copy, or there already), else
+// as many words to a group as it takes.
+template <int kMost, bool kOne>
 struct Counts {
     const uint32_t *used;
-    int64_t pages, words;
+    int pages, words;
     int span, groups;  // words of a group; groups that have words
     const int32_t *before;
 
-    // Called by all 1024 threads; each counts neighbouring groups.
-    __device__ Counts(const uint32_t *used_, int64_t pages_, int32_t *lds) : used(used_), pages(pages_), before(lds)
+    // Called by all 1024 threads; each counts neighbouring groups.  copy: LDS for
+    // the words, or null.
+    __device__ Counts(const uint32_t *from, int64_t pages_, int32_t *lds, uint32_t *copy)
+        : used(kOne && copy != nullptr ? copy : from), pages((int)pages_), before(lds)
     {
-        constexpr int kEach = kGroups / 1024;
-        words = words_of(pages);
-        span = (int)((words + kGroups - 1) / kGroups);
-        groups = (int)((words + span - 1) / span);
+        constexpr int kEach = kMost / 1024;
+        words = (int)words_of(pages);
+        span = kOne ? 1 : (words + kMost - 1) / kMost;
+        groups = kOne ? words : (words + span - 1) / span;
         int n[kEach], mine = 0;
         const int64_t first = (int64_t)threadIdx.x * kEach * span;
 #pragma unroll
         for (int g = 0; g < kEach; ++g) {
             n[g] = 0;
-            if (span == 1) {
-                n[g] = first + g < words ? __popc(used[first + g]) : 0;
+            if constexpr (kOne) {
+                const uint32_t word = first + g < words ? from[first + g] : 0u;
+                n[g] = __popc(word);
+                if (copy != nullptr && first + g < words) {
+                    copy[first + g] = word;
+                }
             } else {
                 for (int64_t w = first + g * span; w < first + (g + 1) * span && w < words; ++w) {
-                    n[g] += __popc(used[w]);
+                    n[g] += __popc(from[w]);
                 }
             }
             mine += n[g];
@@ -152,20 +194,22 @@ struct Counts {
             base += n[g];
         }
         if (threadIdx.x == 1023) {
-            lds[kGroups] = total;
+            lds[kMost] = total;
         }
         __syncthreads();
     }
-    __device__ int held() const { return before[kGroups]; }
-    // Held pages before `page`.
-    __device__ int rank(int64_t page) const
+    __device__ int held() const { return before[kMost]; }
+    // Held pages before `page` (at most `pages`).
+    __device__ int rank(int page) const
     {
-        const int64_t word = page / 32, g = word / span;
+        const int word = page / 32, g = kOne ? word : word / span;
         int n = before[g];
-        for (int64_t w = g * span; w < word; ++w) {
-            n += __popc(used[w]);
+        if constexpr (!kOne) {
+            for (int w = g * span; w < word; ++w) {
+                n += __popc(used[w]);
+            }
         }
-        return word < words ? n + __popc(used[word] & ((1u << (page % 32)) - 1u)) : n;
+        return page < pages ? n + __popc(used[word] & ((1u << (page % 32)) - 1u)) : held();
     }
     __device__ int free_before(int g) const { return (int)((int64_t)g * span * 32 - before[g]); }
     // The k-th free page (there is one).
@@ -181,18 +225,25 @@ struct Counts {
             }
         }
         k -= free_before(low);
-        for (int64_t w = (int64_t)low * span;; ++w) {
-            uint32_t f = ~used[w];
-            const int n = __popc(f);
+        int w = low * span;
+        uint32_t f = ~used[w];
+        if constexpr (!kOne) {
+            for (int n = __popc(f); k >= n; n = __popc(f)) {
+                k -= n;
+                f = ~used[++w];
+            }
+        }
+        int bit = 0;  // the k-th set bit of f
+#pragma unroll
+        for (int half = 16; half > 0; half /= 2) {
+            const int n = __popc(f & ((1u << half) - 1u));
             if (k >= n) {
                 k -= n;
-                continue;
+                f >>= half;
+                bit += half;
             }
-            for (; k > 0; --k) {
-                f &= f - 1u;
-            }
-            return (int)(w * 32) + __ffs(f) - 1;
         }
+        return w * 32 + bit;
     }
 };
 
@@ -209,11 +260,13 @@ __device__ __forceinline__ bool wants_copy(const CacheUpdateArgs &a, const Row &
 
 // One workgroup: which rows get their pages, first[r] = rank of the row's
 // first free page or -1, and the list of the free pages given out.
+template <bool kOne>
 __global__ __launch_bounds__(1024) void update_grants(CacheUpdateArgs a, const uint32_t *used, const uint32_t *many,
                                                       int32_t *first, int32_t *list)
 {
     __shared__ int32_t lds[kGroups + 1];
-    const Counts counts(used, a.pages, lds);
+    __shared__ uint32_t copy[kOne ? kGroups : 1];
+    const Counts<kGroups, kOne> counts(used, a.pages, lds, copy);
     const int64_t free = a.pages - counts.held();
     int64_t asked = 0;
     for (int64_t r0 = 0; r0 < a.rows; r0 += 1024) {
@@ -236,21 +289,17 @@ __global__ __launch_bounds__(1024) void update_grants(CacheUpdateArgs a, const u
     }
     const int64_t given = asked < free ? asked : free;
     for (int g = (int)threadIdx.x; g < counts.groups; g += 1024) {
-        int64_t k = counts.free_before(g);
-        for (int64_t w = (int64_t)g * counts.span; w < (int64_t)(g + 1) * counts.span && w < counts.words && k < given;
-             ++w) {
-            for (uint32_t f = ~used[w]; f != 0u && k < given; f &= f - 1u) {
-                const int64_t page = w * 32 + __ffs(f) - 1;
-                if (page < a.pages) {
-                    list[k++] = (int32_t)page;
-                }
+        int k = counts.free_before(g);
+        for (int w = g * counts.span; w < (g + 1) * counts.span && w < counts.words && k < given; ++w) {
+            for (uint32_t f = ~counts.used[w]; f != 0u && k < given; f &= f - 1u) {
+                list[k++] = w * 32 + __ffs(f) - 1;
             }
         }
     }
 }
 
-// One wave per row: the columns that its new tokens change, its slots and
-// the rest of its state.
+// One wave per row: the columns that its new tokens change, its slots and the
+// rest of its state.
 __global__ __launch_bounds__(256) void update_finish(CacheUpdateArgs a, const uint32_t *many, const int32_t *first,
                                                      const int32_t *list)
 {
@@ -259,42 +308,148 @@ __global__ __launch_bounds__(256) void update_finish(CacheUpdateArgs a, const ui
     if (r >= a.rows) {
         return;
     }
+    const int from = first[r];
     const Row row(a, r);
     int last;
     const bool copy = wants_copy(a, row, many, &last);
-    const bool served = first[r] >= 0;
-    const int32_t *mine = list + (served ? first[r] : 0);
-    const auto column = [&](int64_t j) -> int {  // of the new row, j in [open, grown)
+    const bool served = from >= 0;
+    const int32_t *mine = list + (served ? from : 0);
+    const auto column = [&](int j) -> int {  // of the new row, j in [open, grown)
         if (j >= row.held) {
             return served ? mine[copy + j - row.held] : -1;
         }
         return served && copy ? mine[0] : last;
     };
-    const int64_t open = row.open(a), end = row.add > 0 ? row.grown : open;
-    for (int64_t j = open + lane; j < end; j += kWave) {
+    const int open = row.open(a), end = row.add > 0 ? row.grown : open;
+    for (int j = open + lane; j < end; j += kWave) {
         a.newTable[r * a.width + j] = column(j);
     }
     const int granted = served ? row.add : 0;
-    for (int64_t i = lane; i < a.tokens; i += kWave) {
-        const int64_t t = row.length + i;
-        const int page = i < granted ? column(t / a.pageSize) : -1;
-        a.slots[r * a.tokens + i] = page >= 0 ? (int64_t)page * a.pageSize + t % a.pageSize : -1;
+    for (int i = lane; i < a.tokens; i += kWave) {
+        const uint32_t t = (uint32_t)row.length + (uint32_t)i;
+        const int page = i < granted ? column((int)(t / (uint32_t)a.pageSize)) : -1;
+        a.slots[r * a.tokens + i] = page >= 0 ? (int64_t)page * a.pageSize + t % (uint32_t)a.pageSize : -1;
     }
     if (lane == 0) {
-        a.newLengths[r] = (int32_t)(row.length + granted);
+        a.newLengths[r] = row.length + granted;
         a.granted[r] = granted;
         a.src[r] = served && copy ? last : -1;
         a.dst[r] = served && copy ? mine[0] : -1;
     }
 }
 
-// Column j of row r as mhcCacheCompact sees it.
-__device__ __forceinline__ int held_entry(const CacheCompactArgs &a, int64_t r, int64_t j)
-{
-    const int64_t length = clamped(a.lengths[r], (int64_t)a.width * a.pageSize);
-    if (j >= (length + a.pageSize - 1) / a.pageSize) {
-        return -1;
+// The cells of a table as 1024 threads take them: in a pass each thread has one,
+// at the same column every time (wide tables: columns 1024 apart).
+struct Cells {
+    int rows, width, row0, column0, step, pieces, passes;
+
+    __device__ Cells(int rows_, int width_) : rows(rows_), width(width_)
+    {
+        const int me = (int)threadIdx.x;
+        pieces = (width + 1023) / 1024;
+        step = width < 1024 ? 1024 / width : 1;  // rows of a pass
+        row0 = pieces > 1 ? 0 : me / width;
+        column0 = me - row0 * width;
+        if (row0 >= step) {
+            row0 = rows;  // (more threads than cells)
+        }
+        passes = (rows + step - 1) / step * pieces;
     }
+    __device__ int row(int p) const { return row0 + (pieces > 1 ? p / pieces : p * step); }
+    __device__ int column(int p) const { return column0 + (pieces > 1 ? p % pieces * 1024 : 0); }
+    __device__ bool has(int r, int j) const { return r < rows && j < width; }
+};
+
+// All of it by one workgroup, the bitmaps and the rows in its LDS.  `lanes`
+// threads share a row's columns and slots.
+__global__ __launch_bounds__(1024) void update_small(CacheUpdateArgs a, int lanes)
+{
+    __shared__ uint32_t used[kSmallWords], many[kSmallWords];
+    __shared__ int32_t lds[kSmallWords + 1];
+    __shared__ Row rows[kSmallRows];
+    __shared__ int32_t lasts[kSmallRows], first[kSmallRows];
+    const int me = (int)threadIdx.x;
+    for (int w = me; w < words_of(a.pages); w += 1024) {
+        used[w] = many[w] = 0u;
+    }
+    if (me < a.rows) {
+        rows[me] = Row(a, me);
+        lasts[me] = -1;
+    }
+    __syncthreads();
+    const Cells cells(a.rows, a.width);
+    for (int p = 0; p < cells.passes; p += kSmallBatch) {
+        int page[kSmallBatch];
+#pragma unroll
+        for (int n = 0; n < kSmallBatch; ++n) {
+            const int r = cells.row(p + n), j = cells.column(p + n);
+            page[n] = cells.has(r, j) && j < rows[r].held ? rows[r].entry(a, j) : -1;
+        }
+#pragma unroll
+        for (int n = 0; n < kSmallBatch; ++n) {
+            const int r = cells.row(p + n), j = cells.column(p + n);
+            if (cells.has(r, j)) {
+                const Row &row = rows[r];
+                const int open = row.open(a);
+                if (j < open || j >= (row.add > 0 ? row.grown : open)) {
+                    a.newTable[r * a.width + j] = page[n];
+                } else if (j < row.held) {
+                    lasts[r] = page[n];  // the partly filled page
+                }
+            }
+        }
+        mark_all(page, used, many);
+    }
+    __syncthreads();
+    const Counts<kSmallWords, true> counts(used, a.pages, lds, nullptr);
+    const auto wants = [&](int r) { return lasts[r] >= 0 && (many[lasts[r] / 32] >> (lasts[r] % 32) & 1u) != 0u; };
+    {
+        const int need = me < a.rows ? wants(me) + rows[me].grown - rows[me].held : 0;
+        int total;
+        const int upto = scan_1024(need, &total);
+        if (me < a.rows) {
+            const bool served = rows[me].add > 0 && (need == 0 || upto <= a.pages - counts.held());
+            first[me] = served ? upto - need : -1;
+        }
+    }
+    __syncthreads();
+    const int lane = me % lanes;
+    for (int r = me / lanes; r < a.rows; r += 1024 / lanes) {
+        const Row row = rows[r];
+        const int from = first[r], last = lasts[r];
+        const bool served = from >= 0, copy = served && wants(r);
+        const int own = copy ? counts.free_page(from) : last;  // the page of the column before held
+        const auto column = [&](int j) {
+            return j < row.held ? own : served ? counts.free_page(from + copy + j - row.held) : -1;
+        };
+        const int open = row.open(a), end = row.add > 0 ? row.grown : open;
+        for (int j = open + lane; j < end; j += lanes) {
+            a.newTable[r * a.width + j] = column(j);
+        }
+        const int granted = served ? row.add : 0;
+        for (int i = lane; i < a.tokens; i += lanes) {
+            const uint32_t t = (uint32_t)row.length + (uint32_t)i;
+            const int page = i < granted ? column((int)(t / (uint32_t)a.pageSize)) : -1;
+            a.slots[(int64_t)r * a.tokens + i] =
+                page >= 0 ? (int64_t)page * a.pageSize + t % (uint32_t)a.pageSize : -1;
+        }
+        if (lane == 0) {
+            a.newLengths[r] = row.length + granted;
+            a.granted[r] = granted;
+            a.src[r] = copy ? last : -1;
+            a.dst[r] = copy ? own : -1;
+        }
+    }
+}
+
+// Pages that row r holds as mhcCacheCompact sees it, and its column j < that.
+__device__ __forceinline__ int held_pages(const CacheCompactArgs &a, int64_t r)
+{
+    return pages_for((uint32_t)clamped(a.lengths[r], a.width * a.pageSize), a.pageSize);
+}
+
+__device__ __forceinline__ int held_entry(const CacheCompactArgs &a, int64_t r, int j)
+{
     const int page = a.table[r * a.width + j];
     return page >= 0 && page < a.pages ? page : -1;
 }
@@ -302,42 +457,124 @@ __device__ __forceinline__ int held_entry(const CacheCompactArgs &a, int64_t r, 
 __global__ __launch_bounds__(256) void compact_mark(CacheCompactArgs a, uint32_t *used)
 {
     const int64_t r = blockIdx.x;
-    for (int64_t j = threadIdx.x; j < a.width; j += 256) {
-        const int page = held_entry(a, r, j);
-        if (page >= 0) {
-            mark(page, used, nullptr);
+    const int held = held_pages(a, r);
+    for (int j0 = (int)threadIdx.x; j0 < held; j0 += 256 * kBatch) {
+        int page[kBatch];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            page[n] = j0 + 256 * n < held ? held_entry(a, r, j0 + 256 * n) : -1;
         }
+        mark_all(page, used, nullptr);
     }
 }
 
-// Every workgroup counts for itself, then writes its part of the moves and of
-// the table.
+// Every workgroup counts for itself, then does its part: of the moves, and of
+// the table, cut into pieces of 64 * kBatch columns of a row, a wave's each.
+template <bool kOne>
 __global__ __launch_bounds__(1024) void compact_apply(CacheCompactArgs a, const uint32_t *used)
 {
     __shared__ int32_t lds[kGroups + 1];
-    const Counts counts(used, a.pages, lds);
-    const int U = counts.held(), stay = counts.rank(U), moves = U - stay;
+    __shared__ uint32_t copy[kOne ? kGroups : 1];
+    const Counts<kGroups, kOne> counts(used, a.pages, lds, copy);
+    const int U = counts.held(), stay = counts.rank(U);
     const int64_t at = (int64_t)blockIdx.x * 1024 + threadIdx.x, all = (int64_t)gridDim.x * 1024;
     if (at == 0) {
-        a.used[0] = (int32_t)U;
+        a.used[0] = U;
     }
     for (int64_t page = U + at; page < a.pages; page += all) {
-        if ((used[page / 32] >> (page % 32) & 1u) != 0u) {
-            const int k = counts.rank(page) - stay;
+        if ((counts.used[page / 32] >> (page % 32) & 1u) != 0u) {
+            const int k = counts.rank((int)page) - stay;
             a.src[k] = (int32_t)page;
             a.dst[k] = counts.free_page(k);
         }
     }
-    for (int64_t k = moves + at; k < a.pages / 2; k += all) {
+    for (int64_t k = U - stay + at; k < a.pages / 2; k += all) {
         a.src[k] = a.dst[k] = -1;
     }
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        for (int64_t j = threadIdx.x; j < a.width; j += 1024) {
-            int page = held_entry(a, r, j);
-            if (page >= U) {
-                page = counts.free_page(counts.rank(page) - stay);
+    constexpr int kColumns = kWave * kBatch;
+    const int pieces = (a.width + kColumns - 1) / kColumns;
+    const int64_t waves = 16 * (int64_t)gridDim.x;
+    for (int64_t n = (int64_t)blockIdx.x * 16 + threadIdx.x / kWave; n < (int64_t)a.rows * pieces; n += waves) {
+        const int64_t r = n / pieces;
+        const int j0 = (int)(n - r * pieces) * kColumns + (int)threadIdx.x % kWave, held = held_pages(a, r);
+        int page[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            page[i] = j0 + i * kWave < held ? held_entry(a, r, j0 + i * kWave) : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (page[i] >= U) {
+                page[i] = counts.free_page(counts.rank(page[i]) - stay);
             }
-            a.newTable[r * a.width + j] = page;
+            if (j0 + i * kWave < a.width) {
+                a.newTable[r * a.width + j0 + i * kWave] = page[i];
+            }
+        }
+    }
+}
+
+// All of it by one workgroup, the bitmap, the rows' pages and the moves'
+// destinations in its LDS.
+__global__ __launch_bounds__(1024) void compact_small(CacheCompactArgs a)
+{
+    __shared__ uint32_t used[kSmallWords];
+    __shared__ int32_t lds[kSmallWords + 1], held[kSmallRows];
+    __shared__ uint16_t to[kSmallPages / 2];
+    const int me = (int)threadIdx.x;
+    for (int w = me; w < words_of(a.pages); w += 1024) {
+        used[w] = 0u;
+    }
+    if (me < a.rows) {
+        held[me] = held_pages(a, me);
+    }
+    __syncthreads();
+    const Cells cells(a.rows, a.width);
+    const auto load = [&](int p, int (&page)[kSmallBatch]) {
+#pragma unroll
+        for (int n = 0; n < kSmallBatch; ++n) {
+            const int r = cells.row(p + n), j = cells.column(p + n);
+            page[n] = cells.has(r, j) && j < held[r] ? held_entry(a, r, j) : -1;
+        }
+    };
+    for (int p = 0; p < cells.passes; p += kSmallBatch) {
+        int page[kSmallBatch];
+        load(p, page);
+        mark_all(page, used, nullptr);
+    }
+    __syncthreads();
+    const Counts<kSmallWords, true> counts(used, a.pages, lds, nullptr);
+    const int U = counts.held(), stay = counts.rank(U), moves = U - stay;
+    if (me == 0) {
+        a.used[0] = U;
+    }
+    for (int w = me; w < counts.words; w += 1024) {
+        // The free pages below U and the held ones from U on, in order.
+        const int below = U - w * 32;  // the word's pages that are
+        const uint32_t low = below >= 32 ? 0xFFFFFFFFu : below <= 0 ? 0u : (1u << below) - 1u;
+        int k = counts.free_before(w);
+        for (uint32_t f = ~used[w] & low; f != 0u; f &= f - 1u, ++k) {
+            to[k] = (uint16_t)(w * 32 + __ffs(f) - 1);
+            a.dst[k] = w * 32 + __ffs(f) - 1;
+        }
+        k = counts.rank(w * 32 < U ? U : w * 32) - stay;
+        for (uint32_t f = used[w] & ~low; f != 0u; f &= f - 1u, ++k) {
+            a.src[k] = w * 32 + __ffs(f) - 1;
+        }
+    }
+    for (int k = moves + me; k < a.pages / 2; k += 1024) {
+        a.src[k] = a.dst[k] = -1;
+    }
+    __syncthreads();
+    for (int p = 0; p < cells.passes; p += kSmallBatch) {
+        int page[kSmallBatch];
+        load(p, page);
+#pragma unroll
+        for (int n = 0; n < kSmallBatch; ++n) {
+            const int r = cells.row(p + n), j = cells.column(p + n);
+            if (cells.has(r, j)) {
+                a.newTable[r * a.width + j] = page[n] >= U ? to[counts.rank(page[n]) - stay] : page[n];
+            }
         }
     }
 }
@@ -437,6 +674,12 @@ hipError_t launch_pieces(const CopyPagesArgs &a, const Runs &k, const Runs &v, i
 
 size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 
+template <typename Args>
+bool small(const Args &a)
+{
+    return a.rows <= kSmallRows && a.pages <= kSmallPages && (int64_t)a.rows * a.width <= kSmallEntries;
+}
+
 hipError_t clear(uint32_t *words, int64_t n, hipStream_t stream)
 {
     const int64_t blocks = (n + 1023) / 1024;
@@ -455,6 +698,14 @@ size_t cache_update_workspace(const CacheUpdateArgs &a)
 hipError_t launch_cache_update(const CacheUpdateArgs &a, void *workspace, int, hipStream_t stream)
 {
     char *ws = static_cast<char *>(workspace);
+    if (small(a)) {
+        int lanes = 1;
+        while (lanes < kWave && lanes * 4 < a.tokens) {
+            lanes *= 2;
+        }
+        hipLaunchKernelGGL(update_small, dim3(1), dim3(1024), 0, stream, a, lanes);
+        return hipGetLastError();
+    }
     const size_t bits = align_up(words_of(a.pages) * 4);
     uint32_t *used = reinterpret_cast<uint32_t *>(ws), *many = reinterpret_cast<uint32_t *>(ws + bits);
     int32_t *first = reinterpret_cast<int32_t *>(ws + 2 * bits);
@@ -467,7 +718,8 @@ hipError_t launch_cache_update(const CacheUpdateArgs &a, void *workspace, int, h
     if ((err = hipGetLastError()) != hipSuccess) {
         return err;
     }
-    hipLaunchKernelGGL(update_grants, dim3(1), dim3(1024), 0, stream, a, used, many, first, list);
+    const auto grants = words_of(a.pages) <= kGroups ? update_grants<true> : update_grants<false>;
+    hipLaunchKernelGGL(grants, dim3(1), dim3(1024), 0, stream, a, used, many, first, list);
     if ((err = hipGetLastError()) != hipSuccess) {
         return err;
     }
@@ -479,6 +731,10 @@ size_t cache_compact_workspace(const CacheCompactArgs &a) { return align_up(word
 
 hipError_t launch_cache_compact(const CacheCompactArgs &a, void *workspace, int cus, hipStream_t stream)
 {
+    if (small(a)) {
+        hipLaunchKernelGGL(compact_small, dim3(1), dim3(1024), 0, stream, a);
+        return hipGetLastError();
+    }
     uint32_t *used = static_cast<uint32_t *>(workspace);
     hipError_t err = clear(used, words_of(a.pages), stream);
     if (err != hipSuccess) {
@@ -490,7 +746,8 @@ hipError_t launch_cache_compact(const CacheCompactArgs &a, void *workspace, int 
             return err;
         }
     }
-    hipLaunchKernelGGL(compact_apply, dim3((unsigned)cus), dim3(1024), 0, stream, a, used);
+    const auto apply = words_of(a.pages) <= kGroups ? compact_apply<true> : compact_apply<false>;
+    hipLaunchKernelGGL(apply, dim3((unsigned)cus), dim3(1024), 0, stream, a, used);
     return hipGetLastError();
 }
 
