@@ -34,9 +34,12 @@ __device__ __forceinline__ int pages_for(uint32_t tokens, int pageSize)
 
 // Row r of mhcCacheUpdate: what it goes on from and what it asks for.
 struct Row {
-    int parent;  // row of the old table, or -1
+    int parent;       // row of the old table, or -1
     int length, held, grown;
-    int add;  // tokens, 0 where they cannot fit the table's width
+    int full;         // pages that are filled; the next one holds `rest` tokens
+    int rest;
+    int add;          // tokens, 0 where they cannot fit the table's width
+    int open, end;    // the columns that the new tokens may change
 
     Row() = default;
     __device__ Row(const CacheUpdateArgs &a, int64_t r)
@@ -44,13 +47,17 @@ struct Row {
         parent = a.parents[r];
         parent = parent >= 0 && parent < a.rows ? parent : -1;
         length = parent >= 0 ? clamped(a.lengths[parent], a.width * a.pageSize) : 0;
-        held = pages_for((uint32_t)length, a.pageSize);
+        full = (int)((uint32_t)length / (uint32_t)a.pageSize);
+        rest = length - full * a.pageSize;
+        held = full + (rest > 0 ? 1 : 0);
         add = clamped(a.counts[r], a.tokens);
-        grown = pages_for((uint32_t)length + (uint32_t)add, a.pageSize);
+        grown = full + pages_for((uint32_t)rest + (uint32_t)add, a.pageSize);
         if (grown > a.width) {
             add = 0;
             grown = held;
         }
+        open = add > 0 ? full : held;
+        end = add > 0 ? grown : held;
     }
     // The entry at column j < held, -1 for a hole.
     __device__ int entry(const CacheUpdateArgs &a, int j) const
@@ -58,10 +65,12 @@ struct Row {
         const int page = a.table[(int64_t)parent * a.width + j];
         return page >= 0 && page < a.pages ? page : -1;
     }
-    // The first column that the new tokens may change.
-    __device__ int open(const CacheUpdateArgs &a) const
+    // The same where `on`, else -1: a load in any case (of the table's first entry), so that
+    // a batch of them has no branches and all are on their way before the first is used.
+    __device__ int entry_if(const CacheUpdateArgs &a, int j, bool on) const
     {
-        return add > 0 && length % a.pageSize != 0 ? held - 1 : held;
+        const int page = a.table[on ? (int64_t)parent * a.width + j : 0];
+        return on && page >= 0 && page < a.pages ? page : -1;
     }
 };
 
@@ -101,19 +110,18 @@ __global__ __launch_bounds__(256) void update_rows(CacheUpdateArgs a, uint32_t *
 {
     const int64_t r = blockIdx.x;
     const Row row(a, r);
-    const int open = row.open(a), end = row.add > 0 ? row.grown : open;
     int32_t *out = a.newTable + r * a.width;
     for (int j0 = (int)threadIdx.x; j0 < a.width; j0 += 256 * kBatch) {
         int page[kBatch];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
             const int j = j0 + 256 * n;
-            page[n] = j < row.held ? row.entry(a, j) : -1;
+            page[n] = row.entry_if(a, j, j < row.held);
         }
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
             const int j = j0 + 256 * n;
-            if (j < a.width && (j < open || j >= end)) {
+            if (j < a.width && (j < row.open || j >= row.end)) {
                 out[j] = page[n];
             }
         }
@@ -251,7 +259,7 @@ struct Counts {
 __device__ __forceinline__ bool wants_copy(const CacheUpdateArgs &a, const Row &row, const uint32_t *many, int *last)
 {
     *last = -1;
-    if (row.add == 0 || row.length % a.pageSize == 0) {
+    if (row.add == 0 || row.rest == 0) {
         return false;
     }
     *last = row.entry(a, row.held - 1);
@@ -320,15 +328,14 @@ __global__ __launch_bounds__(256) void update_finish(CacheUpdateArgs a, const ui
         }
         return served && copy ? mine[0] : last;
     };
-    const int open = row.open(a), end = row.add > 0 ? row.grown : open;
-    for (int j = open + lane; j < end; j += kWave) {
+    for (int j = row.open + lane; j < row.end; j += kWave) {
         a.newTable[r * a.width + j] = column(j);
     }
     const int granted = served ? row.add : 0;
     for (int i = lane; i < a.tokens; i += kWave) {
-        const uint32_t t = (uint32_t)row.length + (uint32_t)i;
-        const int page = i < granted ? column((int)(t / (uint32_t)a.pageSize)) : -1;
-        a.slots[r * a.tokens + i] = page >= 0 ? (int64_t)page * a.pageSize + t % (uint32_t)a.pageSize : -1;
+        const uint32_t t = (uint32_t)row.rest + (uint32_t)i, past = t / (uint32_t)a.pageSize;
+        const int page = i < granted ? column(row.full + (int)past) : -1;
+        a.slots[r * a.tokens + i] = page >= 0 ? (int64_t)page * a.pageSize + (t - past * (uint32_t)a.pageSize) : -1;
     }
     if (lane == 0) {
         a.newLengths[r] = row.length + granted;
@@ -338,27 +345,20 @@ __global__ __launch_bounds__(256) void update_finish(CacheUpdateArgs a, const ui
     }
 }
 
-// The cells of a table as 1024 threads take them: in a pass each thread has one,
-// at the same column every time (wide tables: columns 1024 apart).
-struct Cells {
-    int rows, width, row0, column0, step, pieces, passes;
-
-    __device__ Cells(int rows_, int width_) : rows(rows_), width(width_)
-    {
-        const int me = (int)threadIdx.x;
-        pieces = (width + 1023) / 1024;
-        step = width < 1024 ? 1024 / width : 1;  // rows of a pass
-        row0 = pieces > 1 ? 0 : me / width;
-        column0 = me - row0 * width;
-        if (row0 >= step) {
-            row0 = rows;  // (more threads than cells)
+// The cells of a table as 1024 threads take them: narrow tables several rows at a
+// time, wide ones 1024 columns.  f(j, r, step): the thread's cells at column j in rows
+// r, r + step, ..., kSmallBatch of them (those below `rows`).
+template <typename F>
+__device__ __forceinline__ void each_cells(int rows, int width, F f)
+{
+    const int step = width < 1024 ? 1024 / width : 1;
+    const int row0 = width < 1024 ? (int)threadIdx.x / width : 0;
+    for (int j = (int)threadIdx.x - row0 * width; j < width; j += 1024) {
+        for (int r = row0 < step ? row0 : rows; r < rows; r += step * kSmallBatch) {
+            f(j, r, step);
         }
-        passes = (rows + step - 1) / step * pieces;
     }
-    __device__ int row(int p) const { return row0 + (pieces > 1 ? p / pieces : p * step); }
-    __device__ int column(int p) const { return column0 + (pieces > 1 ? p % pieces * 1024 : 0); }
-    __device__ bool has(int r, int j) const { return r < rows && j < width; }
-};
+}
 
 // All of it by one workgroup, the bitmaps and the rows in its LDS.  `lanes`
 // threads share a row's columns and slots.
@@ -377,29 +377,27 @@ __global__ __launch_bounds__(1024) void update_small(CacheUpdateArgs a, int lane
         lasts[me] = -1;
     }
     __syncthreads();
-    const Cells cells(a.rows, a.width);
-    for (int p = 0; p < cells.passes; p += kSmallBatch) {
+    each_cells(a.rows, a.width, [&](int j, int r0, int step) {
         int page[kSmallBatch];
 #pragma unroll
         for (int n = 0; n < kSmallBatch; ++n) {
-            const int r = cells.row(p + n), j = cells.column(p + n);
-            page[n] = cells.has(r, j) && j < rows[r].held ? rows[r].entry(a, j) : -1;
+            const int r = r0 + n * step;
+            const Row &row = rows[r < a.rows ? r : 0];
+            page[n] = row.entry_if(a, j, r < a.rows && j < row.held);
         }
 #pragma unroll
         for (int n = 0; n < kSmallBatch; ++n) {
-            const int r = cells.row(p + n), j = cells.column(p + n);
-            if (cells.has(r, j)) {
-                const Row &row = rows[r];
-                const int open = row.open(a);
-                if (j < open || j >= (row.add > 0 ? row.grown : open)) {
+            const int r = r0 + n * step;
+            if (r < a.rows) {
+                if (j < rows[r].open || j >= rows[r].end) {
                     a.newTable[r * a.width + j] = page[n];
-                } else if (j < row.held) {
+                } else if (j < rows[r].held) {
                     lasts[r] = page[n];  // the partly filled page
                 }
             }
         }
         mark_all(page, used, many);
-    }
+    });
     __syncthreads();
     const Counts<kSmallWords, true> counts(used, a.pages, lds, nullptr);
     const auto wants = [&](int r) { return lasts[r] >= 0 && (many[lasts[r] / 32] >> (lasts[r] % 32) & 1u) != 0u; };
@@ -422,16 +420,15 @@ __global__ __launch_bounds__(1024) void update_small(CacheUpdateArgs a, int lane
         const auto column = [&](int j) {
             return j < row.held ? own : served ? counts.free_page(from + copy + j - row.held) : -1;
         };
-        const int open = row.open(a), end = row.add > 0 ? row.grown : open;
-        for (int j = open + lane; j < end; j += lanes) {
+        for (int j = row.open + lane; j < row.end; j += lanes) {
             a.newTable[r * a.width + j] = column(j);
         }
         const int granted = served ? row.add : 0;
         for (int i = lane; i < a.tokens; i += lanes) {
-            const uint32_t t = (uint32_t)row.length + (uint32_t)i;
-            const int page = i < granted ? column((int)(t / (uint32_t)a.pageSize)) : -1;
+            const uint32_t t = (uint32_t)row.rest + (uint32_t)i, past = t / (uint32_t)a.pageSize;
+            const int page = i < granted ? column(row.full + (int)past) : -1;
             a.slots[(int64_t)r * a.tokens + i] =
-                page >= 0 ? (int64_t)page * a.pageSize + t % (uint32_t)a.pageSize : -1;
+                page >= 0 ? (int64_t)page * a.pageSize + (t - past * (uint32_t)a.pageSize) : -1;
         }
         if (lane == 0) {
             a.newLengths[r] = row.length + granted;
@@ -448,10 +445,11 @@ __device__ __forceinline__ int held_pages(const CacheCompactArgs &a, int64_t r)
     return pages_for((uint32_t)clamped(a.lengths[r], a.width * a.pageSize), a.pageSize);
 }
 
-__device__ __forceinline__ int held_entry(const CacheCompactArgs &a, int64_t r, int j)
+// (A load in any case, as Row::entry_if's.)
+__device__ __forceinline__ int held_entry(const CacheCompactArgs &a, int64_t r, int j, bool on)
 {
-    const int page = a.table[r * a.width + j];
-    return page >= 0 && page < a.pages ? page : -1;
+    const int page = a.table[on ? r * a.width + j : 0];
+    return on && page >= 0 && page < a.pages ? page : -1;
 }
 
 __global__ __launch_bounds__(256) void compact_mark(CacheCompactArgs a, uint32_t *used)
@@ -462,7 +460,7 @@ __global__ __launch_bounds__(256) void compact_mark(CacheCompactArgs a, uint32_t
         int page[kBatch];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
-            page[n] = j0 + 256 * n < held ? held_entry(a, r, j0 + 256 * n) : -1;
+            page[n] = held_entry(a, r, j0 + 256 * n, j0 + 256 * n < held);
         }
         mark_all(page, used, nullptr);
     }
@@ -500,7 +498,7 @@ __global__ __launch_bounds__(1024) void compact_apply(CacheCompactArgs a, const 
         int page[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            page[i] = j0 + i * kWave < held ? held_entry(a, r, j0 + i * kWave) : -1;
+            page[i] = held_entry(a, r, j0 + i * kWave, j0 + i * kWave < held);
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
@@ -529,19 +527,18 @@ __global__ __launch_bounds__(1024) void compact_small(CacheCompactArgs a)
         held[me] = held_pages(a, me);
     }
     __syncthreads();
-    const Cells cells(a.rows, a.width);
-    const auto load = [&](int p, int (&page)[kSmallBatch]) {
+    const auto load = [&](int j, int r0, int step, int (&page)[kSmallBatch]) {
 #pragma unroll
         for (int n = 0; n < kSmallBatch; ++n) {
-            const int r = cells.row(p + n), j = cells.column(p + n);
-            page[n] = cells.has(r, j) && j < held[r] ? held_entry(a, r, j) : -1;
+            const int r = r0 + n * step;
+            page[n] = held_entry(a, r, j, r < a.rows && j < held[r < a.rows ? r : 0]);
         }
     };
-    for (int p = 0; p < cells.passes; p += kSmallBatch) {
+    each_cells(a.rows, a.width, [&](int j, int r, int step) {
         int page[kSmallBatch];
-        load(p, page);
+        load(j, r, step, page);
         mark_all(page, used, nullptr);
-    }
+    });
     __syncthreads();
     const Counts<kSmallWords, true> counts(used, a.pages, lds, nullptr);
     const int U = counts.held(), stay = counts.rank(U), moves = U - stay;
@@ -566,17 +563,17 @@ __global__ __launch_bounds__(1024) void compact_small(CacheCompactArgs a)
         a.src[k] = a.dst[k] = -1;
     }
     __syncthreads();
-    for (int p = 0; p < cells.passes; p += kSmallBatch) {
+    each_cells(a.rows, a.width, [&](int j, int r0, int step) {
         int page[kSmallBatch];
-        load(p, page);
+        load(j, r0, step, page);
 #pragma unroll
         for (int n = 0; n < kSmallBatch; ++n) {
-            const int r = cells.row(p + n), j = cells.column(p + n);
-            if (cells.has(r, j)) {
-                a.newTable[r * a.width + j] = page[n] >= U ? to[counts.rank(page[n]) - stay] : page[n];
+            if (r0 + n * step < a.rows) {
+                a.newTable[(r0 + n * step) * a.width + j] =
+                    page[n] >= U ? to[counts.rank(page[n]) - stay] : page[n];
             }
         }
-    }
+    });
 }
 
 // A page as n0 x n1 runs of `run` bytes, s0 and s1 bytes apart.
