@@ -116,14 +116,13 @@ struct Parts {
 };
 
 
-// The keys of row b: [low, high), and its units' number (one at least).
+// The keys of a row of length L: [low, high), and its units' number (one at least).
 struct Keys {
     int low, high, first, units;
 
-    __device__ Keys(const PagedAttentionArgs &a, int b)
+    __device__ Keys(const PagedAttentionArgs &a, int L)
     {
         const int most = a.width * a.pageSize;
-        int L = a.lengths[b];
         L = L < 0 ? 0 : L > most ? most : L;
         low = a.window > 0 && L > a.window ? L - (int)a.window : 0;
         high = L;
@@ -253,10 +252,10 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
 
     // The workgroup's stretch and the row it begins in.
     int count = 0;
-    for (int b = lane; b < a.B; b += kWave) {
-        count += Keys(a, b).units;
+    for (int x = lane; x < a.B; x += kWave) {
+        count += Keys(a, a.lengths[x]).units;
     }
-    const Shares shares(wave_sum_int(count) * perRow, args.most);
+    const Shares shares(__builtin_amdgcn_readfirstlane(wave_sum_int(count)) * perRow, args.most);
     if (threadIdx.x == 0) {
         tag = dev::launch_epoch<Args>(w, replay);
     }
@@ -266,7 +265,7 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
     const int begin = shares.start(w), end = shares.start(w + 1);
     int b = 0, base = 0;  // base: the row's first unit
     for (int b0 = 0;; b0 += kWave) {
-        const int mine = b0 + lane < a.B ? Keys(a, b0 + lane).units * perRow : 0;
+        const int mine = b0 + lane < a.B ? Keys(a, a.lengths[b0 + lane]).units * perRow : 0;
         int upto = mine;
 #pragma unroll
         for (int m = 1; m < kWave; m *= 2) {
@@ -286,7 +285,7 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
     base = __builtin_amdgcn_readfirstlane(base);
 
     for (int u = begin; u < end;) {
-        const Keys keys(a, b);
+        const Keys keys(a, __builtin_amdgcn_readfirstlane(a.lengths[b]));
         const int inRow = u - base, hg = inRow / keys.units, tile0 = inRow % keys.units;
         const int stop = base + (hg + 1) * keys.units < end ? base + (hg + 1) * keys.units : end;
         const int tile1 = tile0 + stop - u;
@@ -330,38 +329,57 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
         };
         Fragment<D> k[2];
         u32x4_t v[S::kLoads];
-        uint32_t mask = 0;  // keys of the loaded tile that the row sees
-        const auto load = [&](int i, int page) {
+        const uint16_t *kFrom[2], *vFrom[S::kLoads];  // the next tile's rows
+        uint32_t mask = 0;                            // its keys that the row sees
+        // (Found a tile ahead, so that the loads can leave as soon as their registers are free.)
+        const auto find_rows = [&](int i, int page) {
             const bool seen = page >= 0 && page < a.pages;
-            const int slot = (key0(i) + lane % kTile) % a.pageSize;
-            mask = (uint32_t)__ballot(seen);
+            const int slot = (int)((uint32_t)(key0(i) + lane % kTile) % (uint32_t)a.pageSize);
+            mask = __builtin_amdgcn_readfirstlane((int)(uint32_t)__ballot(seen));
             // Where there is no key the first row of the cache is read instead, and not used.
             const int64_t kAt = seen ? page * a.kCache.page + slot * a.kCache.slot : 0;
             const int64_t vAt = seen ? page * a.vCache.page + slot * a.vCache.slot : 0;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
-                k[kt].load(kBase + shfl64(kAt, kt * 16 + col), lane);
+                kFrom[kt] = kBase + shfl64(kAt, kt * 16 + col);
             }
 #pragma unroll
             for (int n = 0; n < S::kLoads; ++n) {
                 const int at = n * kWave + lane;
-                v[n] = *reinterpret_cast<const u32x4_t *>(vBase + shfl64(vAt, at / S::kChunks) + at % S::kChunks * 8);
+                vFrom[n] = vBase + shfl64(vAt, at / S::kChunks) + at % S::kChunks * 8;
+            }
+        };
+        const auto load = [&]() {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                k[kt].load(kFrom[kt], lane);
+            }
+#pragma unroll
+            for (int n = 0; n < S::kLoads; ++n) {
+                v[n] = *reinterpret_cast<const u32x4_t *>(vFrom[n]);
             }
         };
 
-        load(tile0, find_page(tile0));
-        int page = find_page(tile0 + 1);
+        find_rows(tile0, find_page(tile0));
+        load();
+        uint32_t now = mask;
+        int page = find_page(tile0 + 2);
+        find_rows(tile0 + 1, find_page(tile0 + 1));
         for (int i = tile0; i < tile1; ++i) {
             char *mine = lds[wave];
-            const uint32_t now = mask;
             // V to LDS; what the row does not see is zero there, whatever the cache holds.
+            if (now != 0xFFFFFFFFu) {
+#pragma unroll
+                for (int n = 0; n < S::kLoads; ++n) {
+                    if ((now >> ((n * kWave + lane) / S::kChunks) & 1u) == 0u) {
+                        v[n] = u32x4_t{0, 0, 0, 0};
+                    }
+                }
+            }
 #pragma unroll
             for (int n = 0; n < S::kLoads; ++n) {
-                const int at = n * kWave + lane, row = at / S::kChunks;
-                if (now != 0xFFFFFFFFu && (now >> row & 1u) == 0u) {
-                    v[n] = u32x4_t{0, 0, 0, 0};
-                }
-                *reinterpret_cast<u32x4_t *>(mine + row * P + at % S::kChunks * 16) = v[n];
+                const int at = n * kWave + lane;
+                *reinterpret_cast<u32x4_t *>(mine + at / S::kChunks * P + at % S::kChunks * 16) = v[n];
             }
             f32x4_t s[RT][2];
 #pragma unroll
@@ -375,11 +393,14 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
                     }
                 }
             }
+            const uint32_t seen = now;
             if (i + 1 < tile1) {
-                load(i + 1, page);
-                page = find_page(i + 2);
+                load();
+                now = mask;
+                find_rows(i + 2, page);
+                page = find_page(i + 3);
             }
-            if (now == 0u) {
+            if (seen == 0u) {
                 continue;
             }
             u32x4_t hi[RT], lo[RT];
@@ -388,23 +409,38 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
                 float x[8], most = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int key = e / 4 * 16 + 4 * c + e % 4;
-                    x[e] = (now >> key & 1u) != 0u ? s[rt][e / 4][e % 4] * (a.scale * kLog2e) : -INFINITY;
+                    x[e] = s[rt][e / 4][e % 4] * (a.scale * kLog2e);
+                }
+                if (seen != 0xFFFFFFFFu) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = (seen >> (e / 4 * 16 + 4 * c + e % 4) & 1u) != 0u ? x[e] : -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
                     most = fmaxf(most, x[e]);
                 }
                 most = fmaxf(most, __shfl_xor(most, 16));
                 most = fmaxf(most, __shfl_xor(most, 32));
                 const float next = fmaxf(top[rt], most);
                 const float zero = next == -INFINITY ? 0.f : next;
-                const float keep = __builtin_amdgcn_exp2f(top[rt] - zero);
-                top[rt] = next;
+                if (__any(next > top[rt])) {  // (else the sums are on the right scale)
+                    const float keep = __builtin_amdgcn_exp2f(top[rt] - zero);
+                    top[rt] = next;
+                    sum[rt] *= keep;
+#pragma unroll
+                    for (int j = 0; j < S::kDims; ++j) {
+                        o[rt][j] *= keep;
+                    }
+                }
                 float part = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     x[e] = __builtin_amdgcn_exp2f(x[e] - zero);
                     part += x[e];
                 }
-                sum[rt] = sum[rt] * keep + part;
+                sum[rt] += part;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float p0 = x[2 * e], p1 = x[2 * e + 1];
@@ -412,10 +448,6 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
                     hi[rt][e] = h;
                     lo[rt][e] = dev::pack2_x<kBf16>(p0 - dev::x_to_f32<kBf16>(h & 0xFFFFu),
                                                     p1 - dev::x_to_f32<kBf16>(h >> 16));
-                }
-#pragma unroll
-                for (int j = 0; j < S::kDims; ++j) {
-                    o[rt][j] *= keep;
                 }
             }
 #pragma unroll
@@ -505,21 +537,36 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
             const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
             for (int at = complete ? (int)threadIdx.x : rows * (D / 4); at < rows * (D / 4); at += 64 * kWaves) {
                 const int row = at / (D / 4), e = at % (D / 4) * 4;
-                float most = -INFINITY;
-#pragma unroll 4
-                for (int x = first; x <= last; ++x) {
-                    most = fmaxf(most, __uint_as_float(parts.end(x == first ? firstSlot : 2 * x, row)[0]));
-                }
-                const float zero = most == -INFINITY ? 0.f : most;
-                float total = 0.f;
+                float most = -INFINITY, zero = 0.f, total = 0.f;
                 f32x4_t all = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-                for (int x = first; x <= last; ++x) {
-                    const int at = x == first ? firstSlot : 2 * x;
-                    const u32x2_t end = parts.end(at, row);
-                    const float f = __builtin_amdgcn_exp2f(__uint_as_float(end[0]) - zero);
-                    total += f * __uint_as_float(end[1]);
-                    all += f * parts.out(at, row, e);
+                constexpr int kBlock = 8;  // parts on their way at once
+                for (int x0 = first; x0 <= last; x0 += kBlock) {
+                    u32x2_t ends[kBlock];
+                    f32x4_t outs[kBlock];
+                    float next = most;
+#pragma unroll
+                    for (int n = 0; n < kBlock; ++n) {
+                        const int x = x0 + n < last ? x0 + n : last, from = x == first ? firstSlot : 2 * x;
+                        ends[n] = parts.end(from, row);
+                        outs[n] = parts.out(from, row, e);
+                    }
+#pragma unroll
+                    for (int n = 0; n < kBlock; ++n) {
+                        next = fmaxf(next, __uint_as_float(ends[n][0]));
+                    }
+                    zero = next == -INFINITY ? 0.f : next;
+                    const float keep = __builtin_amdgcn_exp2f(most - zero);
+                    most = next;
+                    total *= keep;
+                    all *= keep;
+#pragma unroll
+                    for (int n = 0; n < kBlock; ++n) {
+                        if (x0 + n <= last) {
+                            const float f = __builtin_amdgcn_exp2f(__uint_as_float(ends[n][0]) - zero);
+                            total += f * __uint_as_float(ends[n][1]);
+                            all += f * outs[n];
+                        }
+                    }
                 }
                 finish<kBf16>(a, b, kvHead * args.group + head0 + row, e, all, zero, total);
             }
