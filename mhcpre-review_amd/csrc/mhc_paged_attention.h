@@ -284,27 +284,99 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
     b = __builtin_amdgcn_readfirstlane(b);
     base = __builtin_amdgcn_readfirstlane(base);
 
-    for (int u = begin; u < end;) {
-        const Keys keys(a, __builtin_amdgcn_readfirstlane(a.lengths[b]));
-        const int inRow = u - base, hg = inRow / keys.units, tile0 = inRow % keys.units;
-        const int stop = base + (hg + 1) * keys.units < end ? base + (hg + 1) * keys.units : end;
-        const int tile1 = tile0 + stop - u;
-        const int kvHead = hg / args.blocks, block = hg % args.blocks;
-        const int head0 = block * 16 * RT;  // in the group
+    // A place in the line: unit `tile` of (row b, its hg-th kv head and block).
+    struct Place {
+        int b, hg, tile;
+        Keys keys;
+    };
+    const auto row_keys = [&](int x) { return Keys(a, __builtin_amdgcn_readfirstlane(a.lengths[x])); };
+    const auto advance = [&](Place &x) {
+        if (++x.tile < x.keys.units) {
+            return;
+        }
+        x.tile = 0;
+        if (++x.hg == perRow) {
+            x.hg = 0;
+            if (++x.b < a.B) {
+                x.keys = row_keys(x.b);
+            }
+        }
+    };
+    Place place{b, 0, 0, row_keys(b)};
+    place.hg = (begin - base) / place.keys.units;
+    place.tile = (begin - base) % place.keys.units;
 
-        Fragment<D> q[RT];
+    // The loads run ahead of the products, over the ends of rows: a unit's pages are
+    // looked up three units ahead, its rows' addresses found two ahead, and its
+    // keys and values leave memory one ahead.
+    Place ahead = place;
+    int unit = begin;  // the unit at `ahead`
+    struct Found {     // lane's key (lane % 32) of a unit
+        int page, slot, kvHead;
+    };
+    const auto find_page = [&]() {
+        Found f{-1, 0, 0};
+        if (unit < end) {
+            const int t = (ahead.keys.first + ahead.tile) * kUnit + wave * kTile + lane % kTile;
+            f.kvHead = ahead.hg / args.blocks;
+            if (t >= ahead.keys.low && t < ahead.keys.high) {
+                const uint32_t at = (uint32_t)t / (uint32_t)a.pageSize;
+                f.page = a.table[(int64_t)ahead.b * a.width + at];
+                f.slot = t - (int)(at * (uint32_t)a.pageSize);
+            }
+            ++unit;
+            advance(ahead);
+        }
+        return f;
+    };
+    Fragment<D> k[2];
+    u32x4_t v[S::kLoads];
+    const uint16_t *kFrom[2], *vFrom[S::kLoads];
+    uint32_t mask = 0;  // keys at kFrom and vFrom that the row sees
+    const auto find_rows = [&](const Found &f) {
+        const bool seen = f.page >= 0 && f.page < a.pages;
+        mask = __builtin_amdgcn_readfirstlane((int)(uint32_t)__ballot(seen));
+        // Where there is no key the first row of the cache is read instead, and not used.
+        const int64_t kAt = seen ? f.page * a.kCache.page + f.slot * a.kCache.slot : 0;
+        const int64_t vAt = seen ? f.page * a.vCache.page + f.slot * a.vCache.slot : 0;
+        const uint16_t *kBase = static_cast<const uint16_t *>(a.kCache.data) + f.kvHead * a.kCache.head;
+        const uint16_t *vBase = static_cast<const uint16_t *>(a.vCache.data) + f.kvHead * a.vCache.head;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            kFrom[kt] = kBase + shfl64(kAt, kt * 16 + col);
+        }
+#pragma unroll
+        for (int n = 0; n < S::kLoads; ++n) {
+            const int at = n * kWave + lane;
+            vFrom[n] = vBase + shfl64(vAt, at / S::kChunks) + at % S::kChunks * 8;
+        }
+    };
+    const auto load = [&]() {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            k[kt].load(kFrom[kt], lane);
+        }
+#pragma unroll
+        for (int n = 0; n < S::kLoads; ++n) {
+            v[n] = *reinterpret_cast<const u32x4_t *>(vFrom[n]);
+        }
+    };
+    Fragment<D> q[RT];
+    const auto load_q = [&](const Place &x) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int h = head0 + rt * 16 + col;
+            const int h = x.hg % args.blocks * 16 * RT + rt * 16 + col;
             q[rt].clear();
             if (h < args.group) {
-                q[rt].load(static_cast<const uint16_t *>(a.q.data) + b * a.q.row +
-                               (int64_t)(kvHead * args.group + h) * a.q.head,
+                q[rt].load(static_cast<const uint16_t *>(a.q.data) + x.b * a.q.row +
+                               (int64_t)(x.hg / args.blocks * args.group + h) * a.q.head,
                            lane);
             }
         }
-        f32x4_t o[RT][S::kDims];
-        float top[RT], sum[RT];
+    };
+    f32x4_t o[RT][S::kDims];
+    float top[RT], sum[RT];
+    const auto clear = [&]() {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             top[rt] = -INFINITY;
@@ -314,95 +386,60 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
                 o[rt][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
             }
         }
+    };
 
-        const uint16_t *kBase = static_cast<const uint16_t *>(a.kCache.data) + kvHead * a.kCache.head;
-        const uint16_t *vBase = static_cast<const uint16_t *>(a.vCache.data) + kvHead * a.vCache.head;
-        const int32_t *table = a.table + (int64_t)b * a.width;
-
-        // The wave's tiles: tile i has the keys from (first unit + i) * kUnit + wave * kTile.
-        const int offset = wave * kTile;
-        const auto key0 = [&](int i) { return (keys.first + i) * kUnit + offset; };
-        // The page of key key0(i) + lane % 32, -1 where the row has no such key.
-        const auto find_page = [&](int i) {
-            const int t = key0(i) + lane % kTile;
-            return i < tile1 && t >= keys.low && t < keys.high ? table[t / a.pageSize] : -1;
-        };
-        Fragment<D> k[2];
-        u32x4_t v[S::kLoads];
-        const uint16_t *kFrom[2], *vFrom[S::kLoads];  // the next tile's rows
-        uint32_t mask = 0;                            // its keys that the row sees
-        // (Found a tile ahead, so that the loads can leave as soon as their registers are free.)
-        const auto find_rows = [&](int i, int page) {
-            const bool seen = page >= 0 && page < a.pages;
-            const int slot = (int)((uint32_t)(key0(i) + lane % kTile) % (uint32_t)a.pageSize);
-            mask = __builtin_amdgcn_readfirstlane((int)(uint32_t)__ballot(seen));
-            // Where there is no key the first row of the cache is read instead, and not used.
-            const int64_t kAt = seen ? page * a.kCache.page + slot * a.kCache.slot : 0;
-            const int64_t vAt = seen ? page * a.vCache.page + slot * a.vCache.slot : 0;
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                kFrom[kt] = kBase + shfl64(kAt, kt * 16 + col);
-            }
+    Found found = find_page();
+    Found second = find_page(), third = find_page();
+    find_rows(found);
+    load();
+    load_q(place);
+    uint32_t now = mask;
+    find_rows(second);
+    found = third;
+    clear();
+    int from = begin;  // the first unit of the (row, kv head, block) in this stretch
+    char *mine = lds[wave];
+    for (int u = begin; u < end; ++u) {
+        // V to LDS; what the row does not see is zero there, whatever the cache holds.
+        if (now != 0xFFFFFFFFu) {
 #pragma unroll
             for (int n = 0; n < S::kLoads; ++n) {
-                const int at = n * kWave + lane;
-                vFrom[n] = vBase + shfl64(vAt, at / S::kChunks) + at % S::kChunks * 8;
-            }
-        };
-        const auto load = [&]() {
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                k[kt].load(kFrom[kt], lane);
-            }
-#pragma unroll
-            for (int n = 0; n < S::kLoads; ++n) {
-                v[n] = *reinterpret_cast<const u32x4_t *>(vFrom[n]);
-            }
-        };
-
-        find_rows(tile0, find_page(tile0));
-        load();
-        uint32_t now = mask;
-        int page = find_page(tile0 + 2);
-        find_rows(tile0 + 1, find_page(tile0 + 1));
-        for (int i = tile0; i < tile1; ++i) {
-            char *mine = lds[wave];
-            // V to LDS; what the row does not see is zero there, whatever the cache holds.
-            if (now != 0xFFFFFFFFu) {
-#pragma unroll
-                for (int n = 0; n < S::kLoads; ++n) {
-                    if ((now >> ((n * kWave + lane) / S::kChunks) & 1u) == 0u) {
-                        v[n] = u32x4_t{0, 0, 0, 0};
-                    }
+                if ((now >> ((n * kWave + lane) / S::kChunks) & 1u) == 0u) {
+                    v[n] = u32x4_t{0, 0, 0, 0};
                 }
             }
+        }
 #pragma unroll
-            for (int n = 0; n < S::kLoads; ++n) {
-                const int at = n * kWave + lane;
-                *reinterpret_cast<u32x4_t *>(mine + at / S::kChunks * P + at % S::kChunks * 16) = v[n];
-            }
-            f32x4_t s[RT][2];
+        for (int n = 0; n < S::kLoads; ++n) {
+            const int at = n * kWave + lane;
+            *reinterpret_cast<u32x4_t *>(mine + at / S::kChunks * P + at % S::kChunks * 16) = v[n];
+        }
+        f32x4_t s[RT][2];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
+        for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-                    s[rt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (int kt = 0; kt < 2; ++kt) {
+                s[rt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int x = 0; x < S::kSteps; ++x) {
-                        s[rt][kt] = mfma32<kBf16>(k[kt].step[x], q[rt].step[x], s[rt][kt]);
-                    }
+                for (int x = 0; x < S::kSteps; ++x) {
+                    s[rt][kt] = mfma32<kBf16>(k[kt].step[x], q[rt].step[x], s[rt][kt]);
                 }
             }
-            const uint32_t seen = now;
-            if (i + 1 < tile1) {
-                load();
-                now = mask;
-                find_rows(i + 2, page);
-                page = find_page(i + 3);
+        }
+        const uint32_t seen = now;
+        const Place here = place;
+        const bool ends = place.tile + 1 == place.keys.units || u + 1 == end;
+        advance(place);
+        if (u + 1 < end) {
+            load();
+            if (ends) {
+                load_q(place);
             }
-            if (seen == 0u) {
-                continue;
-            }
+            now = mask;
+            find_rows(found);
+            found = find_page();
+        }
+        if (seen != 0u) {
             u32x4_t hi[RT], lo[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
@@ -462,10 +499,15 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
                 }
             }
         }
+        if (!ends) {
+            continue;
+        }
 
         // The waves' results together, 16 query heads at a time.
-        const bool whole = tile0 == 0 && tile1 == keys.units;
-        const int slot = 2 * w + (u == begin ? 0 : 1);
+        const int kvHead = here.hg / args.blocks, head0 = here.hg % args.blocks * 16 * RT;
+        const int u0 = u - here.tile;  // where it begins, in this stretch or before
+        const bool whole = from == u0 && here.tile + 1 == here.keys.units;
+        const int slot = 2 * w + (from == begin ? 0 : 1);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             sum[rt] += __shfl_xor(sum[rt], 16);
@@ -474,10 +516,10 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
                 tops[wave][rt * 16 + col] = top[rt];
                 sums[wave][rt * 16 + col] = sum[rt];
             }
-            float *mine = reinterpret_cast<float *>(lds[wave]) + col * (D + 4);
+            float *row = reinterpret_cast<float *>(mine) + col * (D + 4);
 #pragma unroll
             for (int j = 0; j < S::kDims; ++j) {
-                *reinterpret_cast<f32x4_t *>(mine + 16 * j + 4 * c) = o[rt][j];
+                *reinterpret_cast<f32x4_t *>(row + 16 * j + 4 * c) = o[rt][j];
             }
             __syncthreads();
             for (int at = (int)threadIdx.x; at < 16 * D / 4; at += 64 * kWaves) {
@@ -504,7 +546,7 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
                         parts.put_ends(slot, rt * 16 + row, most, total);
                     }
                 } else if (h < args.group) {
-                    finish<kBf16>(a, b, kvHead * args.group + h, e, all, zero, total);
+                    finish<kBf16>(a, here.b, kvHead * args.group + h, e, all, zero, total);
                 }
             }
             __syncthreads();
@@ -514,7 +556,7 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
             // after that a look at the others' words.
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            const int u0 = u - tile0, first = shares.owner(u0), last = shares.owner(u0 + keys.units - 1);
+            const int first = shares.owner(u0), last = shares.owner(u0 + here.keys.units - 1);
             const int firstSlot = 2 * first + (shares.start(first) == u0 ? 0 : 1);
             if (wave == 0) {
                 if (lane == 0) {
@@ -568,15 +610,12 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
                         }
                     }
                 }
-                finish<kBf16>(a, b, kvHead * args.group + head0 + row, e, all, zero, total);
+                finish<kBf16>(a, here.b, kvHead * args.group + head0 + row, e, all, zero, total);
             }
             __syncthreads();
         }
-        u = stop;
-        if (u == base + perRow * keys.units) {
-            base = u;
-            ++b;
-        }
+        from = u + 1;
+        clear();
     }
 }
 
