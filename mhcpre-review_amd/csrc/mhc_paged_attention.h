@@ -7,11 +7,10 @@
 // to a fixed grid: the lengths are on the device, and so is this arithmetic.  A
 // workgroup walks its stretch; a (row, kv head, group) that lies in one
 // stretch is finished there, the others leave their maximum, sum and output per
-// stretch in the workspace, and the workgroup that finds all of them there joins
-// them, in the order of the keys.  Nobody waits: every workgroup that leaves a
-// part then looks whether the others' are there, so the last one finds them (two
-// may, and then write the same bits).  What tells this launch's parts from what
-// the workspace held before is the launch's tag (LaunchTag).
+// stretch in the workspace and count them, and the workgroup that counts the last
+// one joins them, in the order of the keys.  Nobody waits.  What tells this
+// launch's counts from what the workspace held before is the launch's tag
+// (LaunchTag).
 //
 // In a unit each of the 4 waves has 32 keys of its own.  The scores are S^T =
 // K Q^T, 16 keys by 16 query heads (a wave's K rows go straight from memory to
@@ -75,9 +74,11 @@ struct Args {
 
 // A stretch leaves at most two parts in the workspace, of the (row, kv head,
 // group) that it begins in and of the one that it ends in: [2 * most] outputs [16
-// RT][D], maxima (base 2) and sums [16 RT][2], and 8-byte words that say that
-// the part is there.  All of it is stored through to memory and read from there:
-// the reader may be on another XCD.
+// RT][D], maxima (base 2) and sums [16 RT][2]; and an 8-byte word, of those of a
+// (row, kv head, group) its first part's, that counts the parts that are there:
+// its upper 52 bits are the launch's and the place's, so that the first to come
+// sees that the word is not yet this launch's and sets it to none.  All of it is
+// stored through to memory and read from there: the reader may be on another XCD.
 template <int D, int RT>
 struct Parts {
     static constexpr int kRows = 16 * RT;
@@ -91,9 +92,11 @@ struct Parts {
           words(reinterpret_cast<uint64_t *>(base + (size_t)2 * most * kRows * (D + 2) * 4))
     {
     }
-    __device__ static uint64_t word(uint32_t tag, int slot)
+    static constexpr uint64_t kCount = 0xFFF;
+    // A word of this launch before the first part is counted.
+    __device__ static uint64_t sign(uint32_t tag, int slot)
     {
-        return (uint64_t)mix32(tag ^ (2u * (uint32_t)slot + 1u)) << 32 | tag;
+        return ((uint64_t)mix32(tag ^ (2u * (uint32_t)slot + 1u)) << 32 | tag) & ~kCount;
     }
     __device__ void put(int slot, int row, int e, f32x4_t out) const
     {
@@ -232,6 +235,14 @@ __device__ __forceinline__ void finish(const PagedAttentionArgs &a, int b, int h
     }
 }
 
+// What a stretch leaves of the (row, kv head, block) that it begins in, or of
+// the one that it ends in, whose parts are those of workgroups first to last.
+struct Part {
+    bool on;
+    int b, hg, first, last, firstSlot;
+    __device__ int slot(int x) const { return x == first ? firstSlot : 2 * x; }
+};
+
 template <bool kBf16, int D, int RT>
 __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attention_units(Args args)
 {
@@ -241,7 +252,8 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
     __shared__ __align__(16) char lds[kWaves][region<D>()];
     __shared__ float tops[kWaves][16 * RT], sums[kWaves][16 * RT];
     __shared__ uint32_t tag;
-    __shared__ bool complete;
+    __shared__ bool complete[2];
+    __shared__ Part left[2];
     const PagedAttentionArgs &a = args.a;
     const int w = (int)blockIdx.x;
     const uint32_t replay = threadIdx.x == 0 ? dev::replay_load(args.tag.words, w) : 0u;
@@ -258,6 +270,7 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
     const Shares shares(__builtin_amdgcn_readfirstlane(wave_sum_int(count)) * perRow, args.most);
     if (threadIdx.x == 0) {
         tag = dev::launch_epoch<Args>(w, replay);
+        left[0].on = left[1].on = false;
     }
     if (w >= shares.grid) {
         return;
@@ -397,6 +410,7 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
     find_rows(second);
     found = third;
     clear();
+    bool partial = false;
     int from = begin;  // the first unit of the (row, kv head, block) in this stretch
     char *mine = lds[wave];
     for (int u = begin; u < end; ++u) {
@@ -552,70 +566,84 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
             __syncthreads();
         }
         if (!whole) {
-            // The part is there once its stores have ended; then the word that says so, and
-            // after that a look at the others' words.
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            const int first = shares.owner(u0), last = shares.owner(u0 + here.keys.units - 1);
-            const int firstSlot = 2 * first + (shares.start(first) == u0 ? 0 : 1);
-            if (wave == 0) {
-                if (lane == 0) {
-                    (void)__hip_atomic_exchange(parts.words + slot, Left::word(tag, slot), __ATOMIC_RELAXED,
-                                                __HIP_MEMORY_SCOPE_AGENT);
-                }
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                bool all = true;
-                for (int x = first + lane; x <= last; x += kWave) {
-                    const int at = x == first ? firstSlot : 2 * x;
-                    all = all && __hip_atomic_load(parts.words + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                                     Left::word(tag, at);
-                }
-                all = __all(all);
-                if (lane == 0) {
-                    complete = all;
-                }
+            partial = true;
+            if (threadIdx.x == 0) {
+                const int first = shares.owner(u0), last = shares.owner(u0 + here.keys.units - 1);
+                left[from == begin ? 0 : 1] =
+                    Part{true, here.b, here.hg, first, last, 2 * first + (shares.start(first) == u0 ? 0 : 1)};
             }
-            __syncthreads();
-            const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
-            for (int at = complete ? (int)threadIdx.x : rows * (D / 4); at < rows * (D / 4); at += 64 * kWaves) {
-                const int row = at / (D / 4), e = at % (D / 4) * 4;
-                float most = -INFINITY, zero = 0.f, total = 0.f;
-                f32x4_t all = {0.f, 0.f, 0.f, 0.f};
-                constexpr int kBlock = 8;  // parts on their way at once
-                for (int x0 = first; x0 <= last; x0 += kBlock) {
-                    u32x2_t ends[kBlock];
-                    f32x4_t outs[kBlock];
-                    float next = most;
-#pragma unroll
-                    for (int n = 0; n < kBlock; ++n) {
-                        const int x = x0 + n < last ? x0 + n : last, from = x == first ? firstSlot : 2 * x;
-                        ends[n] = parts.end(from, row);
-                        outs[n] = parts.out(from, row, e);
-                    }
-#pragma unroll
-                    for (int n = 0; n < kBlock; ++n) {
-                        next = fmaxf(next, __uint_as_float(ends[n][0]));
-                    }
-                    zero = next == -INFINITY ? 0.f : next;
-                    const float keep = __builtin_amdgcn_exp2f(most - zero);
-                    most = next;
-                    total *= keep;
-                    all *= keep;
-#pragma unroll
-                    for (int n = 0; n < kBlock; ++n) {
-                        if (x0 + n <= last) {
-                            const float f = __builtin_amdgcn_exp2f(__uint_as_float(ends[n][0]) - zero);
-                            total += f * __uint_as_float(ends[n][1]);
-                            all += f * outs[n];
-                        }
-                    }
-                }
-                finish<kBf16>(a, here.b, kvHead * args.group + head0 + row, e, all, zero, total);
-            }
-            __syncthreads();
         }
         from = u + 1;
         clear();
+    }
+    if (!partial) {
+        return;
+    }
+
+    // The parts are there once their stores have ended; then they are counted.
+    uint64_t found_word = 0;
+    if (wave == 0 && lane < 2 && left[lane].on) {
+        found_word = __hip_atomic_load(parts.words + left[lane].firstSlot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (wave == 0 && lane < 2) {
+        bool all = false;
+        if (left[lane].on) {
+            uint64_t *word = parts.words + left[lane].firstSlot;
+            const uint64_t zero = Left::sign(tag, left[lane].firstSlot);
+            if ((found_word & ~Left::kCount) != zero) {  // (fails where another workgroup was first)
+                (void)__hip_atomic_compare_exchange_strong(word, &found_word, zero, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                                           __HIP_MEMORY_SCOPE_AGENT);
+            }
+            const uint64_t before = __hip_atomic_fetch_add(word, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            all = (int)(before & Left::kCount) == left[lane].last - left[lane].first;
+        }
+        complete[lane] = all;
+    }
+    __syncthreads();
+    for (int n = 0; n < 2; ++n) {
+        if (!complete[n]) {
+            continue;
+        }
+        const Part part = left[n];
+        const int head0 = part.hg % args.blocks * 16 * RT;
+        const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
+        for (int at = (int)threadIdx.x; at < rows * (D / 4); at += 64 * kWaves) {
+            const int row = at / (D / 4), e = at % (D / 4) * 4;
+            float most = -INFINITY, zero = 0.f, total = 0.f;
+            f32x4_t all = {0.f, 0.f, 0.f, 0.f};
+            constexpr int kBlock = 16;  // parts on their way at once
+            for (int x0 = part.first; x0 <= part.last; x0 += kBlock) {
+                u32x2_t ends[kBlock];
+                f32x4_t outs[kBlock];
+                float next = most;
+#pragma unroll
+                for (int m = 0; m < kBlock; ++m) {
+                    const int slot = part.slot(x0 + m < part.last ? x0 + m : part.last);
+                    ends[m] = parts.end(slot, row);
+                    outs[m] = parts.out(slot, row, e);
+                }
+#pragma unroll
+                for (int m = 0; m < kBlock; ++m) {
+                    next = fmaxf(next, __uint_as_float(ends[m][0]));
+                }
+                zero = next == -INFINITY ? 0.f : next;
+                const float keep = __builtin_amdgcn_exp2f(most - zero);
+                most = next;
+                total *= keep;
+                all *= keep;
+#pragma unroll
+                for (int m = 0; m < kBlock; ++m) {
+                    if (x0 + m <= part.last) {
+                        const float f = __builtin_amdgcn_exp2f(__uint_as_float(ends[m][0]) - zero);
+                        total += f * __uint_as_float(ends[m][1]);
+                        all += f * outs[m];
+                    }
+                }
+            }
+            finish<kBf16>(a, part.b, part.hg / args.blocks * args.group + head0 + row, e, all, zero, total);
+        }
     }
 }
 
