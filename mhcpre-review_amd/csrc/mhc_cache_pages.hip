@@ -106,10 +106,25 @@ __device__ __forceinline__ void mark_all(const int (&page)[N], uint32_t *used, u
 // before the first is marked, for a mark waits for the word that was there.
 constexpr int kBatch = 4;
 
-__global__ __launch_bounds__(256) void update_rows(CacheUpdateArgs a, uint32_t *used, uint32_t *many)
+// What update_rows finds out about a row, for the launches after it.
+struct Found {
+    Row row;
+    int last;  // the partly filled page that the row appends to, or -1
+};
+
+// ... and what update_grants decides: the rank of the row's first free page (-1: it
+// gets nothing), and whether that takes the place of `last`.
+struct Grant {
+    int32_t first, copy;
+};
+
+__global__ __launch_bounds__(256) void update_rows(CacheUpdateArgs a, uint32_t *used, uint32_t *many, Found *found)
 {
     const int64_t r = blockIdx.x;
     const Row row(a, r);
+    if (threadIdx.x == 0) {
+        found[r] = Found{row, row.add > 0 && row.rest > 0 ? row.entry(a, row.held - 1) : -1};
+    }
     int32_t *out = a.newTable + r * a.width;
     for (int j0 = (int)threadIdx.x; j0 < a.width; j0 += 256 * kBatch) {
         int page[kBatch];
@@ -182,9 +197,10 @@ struct Counts {
         for (int g = 0; g < kEach; ++g) {
             n[g] = 0;
             if constexpr (kOne) {
-                const uint32_t word = first + g < words ? from[first + g] : 0u;
-                n[g] = __popc(word);
-                if (copy != nullptr && first + g < words) {
+                const bool on = first + g < words;
+                const uint32_t word = from[on ? first + g : 0];  // (a load in any case)
+                n[g] = on ? __popc(word) : 0;
+                if (copy != nullptr && on) {
                     copy[first + g] = word;
                 }
             } else {
@@ -220,6 +236,27 @@ struct Counts {
         return page < pages ? n + __popc(used[word] & ((1u << (page % 32)) - 1u)) : held();
     }
     __device__ int free_before(int g) const { return (int)((int64_t)g * span * 32 - before[g]); }
+    // LDS for `words` places; starts[k / 32] becomes the word of free page 32 (k / 32), from
+    // where a search for the k-th has a word or two to go.  All 1024 threads.
+    __device__ void index(uint16_t *starts) const
+    {
+        static_assert(kOne, "a word to a group");
+        for (int w = (int)threadIdx.x; w < words; w += 1024) {
+            const int low = free_before(w), at = (low + 31) / 32;
+            if (at * 32 < low + 32 - (int)__popc(used[w])) {
+                starts[at] = (uint16_t)w;
+            }
+        }
+        __syncthreads();
+    }
+    __device__ int free_page(int k, const uint16_t *starts) const
+    {
+        int w = starts[k / 32];
+        while (w + 1 < words && free_before(w + 1) <= k) {
+            ++w;
+        }
+        return free_in(w, k);
+    }
     // The k-th free page (there is one).
     __device__ int free_page(int k) const
     {
@@ -232,6 +269,11 @@ struct Counts {
                 high = mid;
             }
         }
+        return free_in(low, k);
+    }
+    // ... which is in group low.
+    __device__ int free_in(int low, int k) const
+    {
         k -= free_before(low);
         int w = low * span;
         uint32_t f = ~used[w];
@@ -255,48 +297,52 @@ struct Counts {
     }
 };
 
-// Whether the row's partly filled page, which it would append to, is shared.
-__device__ __forceinline__ bool wants_copy(const CacheUpdateArgs &a, const Row &row, const uint32_t *many, int *last)
-{
-    *last = -1;
-    if (row.add == 0 || row.rest == 0) {
-        return false;
-    }
-    *last = row.entry(a, row.held - 1);
-    return *last >= 0 && (many[*last / 32] >> (*last % 32) & 1u) != 0u;
-}
-
-// One workgroup: which rows get their pages, first[r] = rank of the row's
-// first free page or -1, and the list of the free pages given out.
+// One workgroup: which rows get their pages, and the list of the free pages
+// given out.
 template <bool kOne>
 __global__ __launch_bounds__(1024) void update_grants(CacheUpdateArgs a, const uint32_t *used, const uint32_t *many,
-                                                      int32_t *first, int32_t *list)
+                                                      const Found *found, Grant *grants, int32_t *list)
 {
     __shared__ int32_t lds[kGroups + 1];
-    __shared__ uint32_t copy[kOne ? kGroups : 1];
+    __shared__ uint32_t copy[kOne ? kGroups : 1], shared[kOne ? kGroups : 1];
+    const int me = (int)threadIdx.x;
+    const auto load = [&](int64_t r) {
+        Found f{};
+        f.last = -1;
+        if (r < a.rows) {
+            f.row.add = found[r].row.add;
+            f.row.held = found[r].row.held;
+            f.row.grown = found[r].row.grown;
+            f.last = found[r].last;
+        }
+        return f;
+    };
+    Found next = load(me);  // (on its way while the words are counted)
+    if constexpr (kOne) {
+        for (int w = me; w < words_of(a.pages); w += 1024) {
+            shared[w] = many[w];
+        }
+        many = shared;
+    }
     const Counts<kGroups, kOne> counts(used, a.pages, lds, copy);
     const int64_t free = a.pages - counts.held();
     int64_t asked = 0;
     for (int64_t r0 = 0; r0 < a.rows; r0 += 1024) {
-        const int64_t r = r0 + threadIdx.x;
-        int64_t need = 0;
-        bool any = false;
-        if (r < a.rows) {
-            const Row row(a, r);
-            int last;
-            need = wants_copy(a, row, many, &last) + row.grown - row.held;
-            any = row.add > 0;
-        }
+        const int64_t r = r0 + me;
+        const Found f = next;
+        next = load(r + 1024);
+        const int swap = f.last >= 0 ? (int)(many[f.last / 32] >> (f.last % 32) & 1u) : 0;
+        const int64_t need = swap + f.row.grown - f.row.held;
         int64_t total;
         const int64_t upto = asked + scan_1024<int64_t>(need, &total);
         asked += total;
         if (r < a.rows) {
-            const bool served = any && (need == 0 || upto <= free);
-            first[r] = served ? (int32_t)(need == 0 ? 0 : upto - need) : -1;
+            const bool served = f.row.add > 0 && (need == 0 || upto <= free);
+            grants[r] = Grant{served ? (int32_t)(need == 0 ? 0 : upto - need) : -1, served ? swap : 0};
         }
     }
     const int64_t given = asked < free ? asked : free;
-    for (int g = (int)threadIdx.x; g < counts.groups; g += 1024) {
+    for (int g = me; g < counts.groups; g += 1024) {
         int k = counts.free_before(g);
         for (int w = g * counts.span; w < (g + 1) * counts.span && w < counts.words && k < given; ++w) {
             for (uint32_t f = ~counts.used[w]; f != 0u && k < given; f &= f - 1u) {
@@ -308,7 +354,7 @@ __global__ __launch_bounds__(1024) void update_grants(CacheUpdateArgs a, const u
 
 // One wave per row: the columns that its new tokens change, its slots and the
 // rest of its state.
-__global__ __launch_bounds__(256) void update_finish(CacheUpdateArgs a, const uint32_t *many, const int32_t *first,
+__global__ __launch_bounds__(256) void update_finish(CacheUpdateArgs a, const Found *found, const Grant *grants,
                                                      const int32_t *list)
 {
     const int lane = (int)threadIdx.x % kWave;
@@ -316,17 +362,16 @@ __global__ __launch_bounds__(256) void update_finish(CacheUpdateArgs a, const ui
     if (r >= a.rows) {
         return;
     }
-    const int from = first[r];
-    const Row row(a, r);
-    int last;
-    const bool copy = wants_copy(a, row, many, &last);
-    const bool served = from >= 0;
-    const int32_t *mine = list + (served ? from : 0);
-    const auto column = [&](int j) -> int {  // of the new row, j in [open, grown)
+    const Row row = found[r].row;
+    const int last = found[r].last;
+    const Grant grant = grants[r];
+    const bool served = grant.first >= 0, copy = grant.copy != 0;
+    const int32_t *mine = list + (served ? grant.first : 0);
+    const auto column = [&](int j) -> int {  // of the new row, j in [open, end)
         if (j >= row.held) {
             return served ? mine[copy + j - row.held] : -1;
         }
-        return served && copy ? mine[0] : last;
+        return copy ? mine[0] : last;
     };
     for (int j = row.open + lane; j < row.end; j += kWave) {
         a.newTable[r * a.width + j] = column(j);
@@ -340,8 +385,8 @@ __global__ __launch_bounds__(256) void update_finish(CacheUpdateArgs a, const ui
     if (lane == 0) {
         a.newLengths[r] = row.length + granted;
         a.granted[r] = granted;
-        a.src[r] = served && copy ? last : -1;
-        a.dst[r] = served && copy ? mine[0] : -1;
+        a.src[r] = copy ? last : -1;
+        a.dst[r] = copy ? mine[0] : -1;
     }
 }
 
@@ -467,48 +512,69 @@ __global__ __launch_bounds__(256) void compact_mark(CacheCompactArgs a, uint32_t
 }
 
 // Every workgroup counts for itself, then does its part: of the moves, and of
-// the table, cut into pieces of 64 * kBatch columns of a row, a wave's each.
+// the table, cut into pieces of 512 columns of a row, a wave's each.
 template <bool kOne>
 __global__ __launch_bounds__(1024) void compact_apply(CacheCompactArgs a, const uint32_t *used)
 {
     __shared__ int32_t lds[kGroups + 1];
     __shared__ uint32_t copy[kOne ? kGroups : 1];
+    __shared__ uint16_t starts[kOne ? kGroups : 1];
+    constexpr int kPieces = 8, kColumns = kWave * kPieces;
+    const int pieces = (a.width + kColumns - 1) / kColumns;
+    const int64_t waves = 16 * (int64_t)gridDim.x;
+    int64_t n = (int64_t)blockIdx.x * 16 + threadIdx.x / kWave, r = 0;
+    int j0 = 0, page[kPieces];
+    const auto load = [&]() {
+        r = n / pieces;
+        j0 = (int)(n - r * pieces) * kColumns + (int)threadIdx.x % kWave;
+        const int held = r < a.rows ? held_pages(a, r) : 0;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            page[i] = held > 0 ? held_entry(a, r, j0 + i * kWave, j0 + i * kWave < held) : -1;
+        }
+    };
+    load();  // (on its way while the words are counted)
     const Counts<kGroups, kOne> counts(used, a.pages, lds, copy);
+    if constexpr (kOne) {
+        counts.index(starts);
+    }
+    const auto to = [&](int k) {  // the k-th free page
+        if constexpr (kOne) {
+            return counts.free_page(k, starts);
+        } else {
+            return counts.free_page(k);
+        }
+    };
     const int U = counts.held(), stay = counts.rank(U);
+    for (;;) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            if (page[i] >= U) {
+                page[i] = to(counts.rank(page[i]) - stay);
+            }
+            if (r < a.rows && j0 + i * kWave < a.width) {
+                a.newTable[r * a.width + j0 + i * kWave] = page[i];
+            }
+        }
+        n += waves;
+        if (n >= (int64_t)a.rows * pieces) {
+            break;
+        }
+        load();
+    }
     const int64_t at = (int64_t)blockIdx.x * 1024 + threadIdx.x, all = (int64_t)gridDim.x * 1024;
     if (at == 0) {
         a.used[0] = U;
     }
-    for (int64_t page = U + at; page < a.pages; page += all) {
-        if ((counts.used[page / 32] >> (page % 32) & 1u) != 0u) {
-            const int k = counts.rank((int)page) - stay;
-            a.src[k] = (int32_t)page;
-            a.dst[k] = counts.free_page(k);
+    for (int64_t x = U + at; x < a.pages; x += all) {
+        if ((counts.used[x / 32] >> (x % 32) & 1u) != 0u) {
+            const int k = counts.rank((int)x) - stay;
+            a.src[k] = (int32_t)x;
+            a.dst[k] = to(k);
         }
     }
     for (int64_t k = U - stay + at; k < a.pages / 2; k += all) {
         a.src[k] = a.dst[k] = -1;
-    }
-    constexpr int kColumns = kWave * kBatch;
-    const int pieces = (a.width + kColumns - 1) / kColumns;
-    const int64_t waves = 16 * (int64_t)gridDim.x;
-    for (int64_t n = (int64_t)blockIdx.x * 16 + threadIdx.x / kWave; n < (int64_t)a.rows * pieces; n += waves) {
-        const int64_t r = n / pieces;
-        const int j0 = (int)(n - r * pieces) * kColumns + (int)threadIdx.x % kWave, held = held_pages(a, r);
-        int page[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            page[i] = held_entry(a, r, j0 + i * kWave, j0 + i * kWave < held);
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            if (page[i] >= U) {
-                page[i] = counts.free_page(counts.rank(page[i]) - stay);
-            }
-            if (j0 + i * kWave < a.width) {
-                a.newTable[r * a.width + j0 + i * kWave] = page[i];
-            }
-        }
     }
 }
 
@@ -686,10 +752,11 @@ hipError_t clear(uint32_t *words, int64_t n, hipStream_t stream)
 
 }  // namespace
 
-// [used bits][many bits][first: rows][list: pages]
+// [used bits][many bits][Found: rows][Grant: rows][list: pages]
 size_t cache_update_workspace(const CacheUpdateArgs &a)
 {
-    return 2 * align_up(words_of(a.pages) * 4) + align_up((size_t)a.rows * 4) + align_up((size_t)a.pages * 4);
+    return 2 * align_up(words_of(a.pages) * 4) + align_up((size_t)a.rows * sizeof(Found)) +
+           align_up((size_t)a.rows * sizeof(Grant)) + align_up((size_t)a.pages * 4);
 }
 
 hipError_t launch_cache_update(const CacheUpdateArgs &a, void *workspace, int, hipStream_t stream)
@@ -705,22 +772,25 @@ hipError_t launch_cache_update(const CacheUpdateArgs &a, void *workspace, int, h
     }
     const size_t bits = align_up(words_of(a.pages) * 4);
     uint32_t *used = reinterpret_cast<uint32_t *>(ws), *many = reinterpret_cast<uint32_t *>(ws + bits);
-    int32_t *first = reinterpret_cast<int32_t *>(ws + 2 * bits);
-    int32_t *list = reinterpret_cast<int32_t *>(ws + 2 * bits + align_up((size_t)a.rows * 4));
+    ws += 2 * bits;
+    Found *found = reinterpret_cast<Found *>(ws);
+    ws += align_up((size_t)a.rows * sizeof(Found));
+    Grant *grant = reinterpret_cast<Grant *>(ws);
+    int32_t *list = reinterpret_cast<int32_t *>(ws + align_up((size_t)a.rows * sizeof(Grant)));
     hipError_t err = clear(used, (int64_t)(2 * bits / 4), stream);
     if (err != hipSuccess) {
         return err;
     }
-    hipLaunchKernelGGL(update_rows, dim3((unsigned)a.rows), dim3(256), 0, stream, a, used, many);
+    hipLaunchKernelGGL(update_rows, dim3((unsigned)a.rows), dim3(256), 0, stream, a, used, many, found);
     if ((err = hipGetLastError()) != hipSuccess) {
         return err;
     }
     const auto grants = words_of(a.pages) <= kGroups ? update_grants<true> : update_grants<false>;
-    hipLaunchKernelGGL(grants, dim3(1), dim3(1024), 0, stream, a, used, many, first, list);
+    hipLaunchKernelGGL(grants, dim3(1), dim3(1024), 0, stream, a, used, many, found, grant, list);
     if ((err = hipGetLastError()) != hipSuccess) {
         return err;
     }
-    hipLaunchKernelGGL(update_finish, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, stream, a, many, first, list);
+    hipLaunchKernelGGL(update_finish, dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, stream, a, found, grant, list);
     return hipGetLastError();
 }
 
