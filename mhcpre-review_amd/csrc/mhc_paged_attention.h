@@ -263,8 +263,9 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
     const Left parts(args.parts, args.most);
 
     // The workgroup's stretch and the row it begins in.
-    int count = 0;
-    for (int x = lane; x < a.B; x += kWave) {
+    const int firstLength = a.lengths[lane < a.B ? lane : 0];
+    int count = lane < a.B ? Keys(a, firstLength).units : 0;
+    for (int x = lane + kWave; x < a.B; x += kWave) {
         count += Keys(a, a.lengths[x]).units;
     }
     const Shares shares(__builtin_amdgcn_readfirstlane(wave_sum_int(count)) * perRow, args.most);
@@ -276,9 +277,10 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
         return;
     }
     const int begin = shares.start(w), end = shares.start(w + 1);
-    int b = 0, base = 0;  // base: the row's first unit
+    int b = 0, base = 0, length = 0;  // base: the row's first unit
     for (int b0 = 0;; b0 += kWave) {
-        const int mine = b0 + lane < a.B ? Keys(a, a.lengths[b0 + lane]).units * perRow : 0;
+        const int L = b0 == 0 ? firstLength : a.lengths[b0 + lane < a.B ? b0 + lane : 0];
+        const int mine = b0 + lane < a.B ? Keys(a, L).units * perRow : 0;
         int upto = mine;
 #pragma unroll
         for (int m = 1; m < kWave; m *= 2) {
@@ -290,12 +292,14 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
             const int at = __ffsll((unsigned long long)past) - 1;
             b = b0 + at;
             base += __shfl(upto - mine, at);
+            length = __shfl(L, at);
             break;
         }
         base += __shfl(upto, kWave - 1);
     }
     b = __builtin_amdgcn_readfirstlane(b);
     base = __builtin_amdgcn_readfirstlane(base);
+    length = __builtin_amdgcn_readfirstlane(length);
 
     // A place in the line: unit `tile` of (row b, its hg-th kv head and block).
     struct Place {
@@ -315,7 +319,7 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
             }
         }
     };
-    Place place{b, 0, 0, row_keys(b)};
+    Place place{b, 0, 0, Keys(a, length)};
     place.hg = (begin - base) / place.keys.units;
     place.tile = (begin - base) % place.keys.units;
 
@@ -609,40 +613,62 @@ __global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attent
         const Part part = left[n];
         const int head0 = part.hg % args.blocks * 16 * RT;
         const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
-        for (int at = (int)threadIdx.x; at < rows * (D / 4); at += 64 * kWaves) {
-            const int row = at / (D / 4), e = at % (D / 4) * 4;
-            float most = -INFINITY, zero = 0.f, total = 0.f;
-            f32x4_t all = {0.f, 0.f, 0.f, 0.f};
-            constexpr int kBlock = 16;  // parts on their way at once
+        // A thread's kTasks times kBlock parts are on their way at once.
+        constexpr int kTasks = D > 128 ? 4 : D > 64 ? 2 : 1, kBlock = kTasks > 1 ? 32 / kTasks : 16;
+        for (int at0 = (int)threadIdx.x; at0 < rows * (D / 4); at0 += 64 * kWaves * kTasks) {
+            int row[kTasks], e[kTasks];
+            float most[kTasks], zero[kTasks], total[kTasks];
+            f32x4_t all[kTasks];
+#pragma unroll
+            for (int t = 0; t < kTasks; ++t) {
+                const int at = at0 + t * 64 * kWaves < rows * (D / 4) ? at0 + t * 64 * kWaves : at0;
+                row[t] = at / (D / 4);
+                e[t] = at % (D / 4) * 4;
+                most[t] = -INFINITY;
+                zero[t] = total[t] = 0.f;
+                all[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            }
             for (int x0 = part.first; x0 <= part.last; x0 += kBlock) {
-                u32x2_t ends[kBlock];
-                f32x4_t outs[kBlock];
-                float next = most;
+                u32x2_t ends[kTasks][kBlock];
+                f32x4_t outs[kTasks][kBlock];
 #pragma unroll
                 for (int m = 0; m < kBlock; ++m) {
                     const int slot = part.slot(x0 + m < part.last ? x0 + m : part.last);
-                    ends[m] = parts.end(slot, row);
-                    outs[m] = parts.out(slot, row, e);
+#pragma unroll
+                    for (int t = 0; t < kTasks; ++t) {
+                        ends[t][m] = parts.end(slot, row[t]);
+                        outs[t][m] = parts.out(slot, row[t], e[t]);
+                    }
                 }
 #pragma unroll
-                for (int m = 0; m < kBlock; ++m) {
-                    next = fmaxf(next, __uint_as_float(ends[m][0]));
-                }
-                zero = next == -INFINITY ? 0.f : next;
-                const float keep = __builtin_amdgcn_exp2f(most - zero);
-                most = next;
-                total *= keep;
-                all *= keep;
+                for (int t = 0; t < kTasks; ++t) {
+                    float next = most[t];
 #pragma unroll
-                for (int m = 0; m < kBlock; ++m) {
-                    if (x0 + m <= part.last) {
-                        const float f = __builtin_amdgcn_exp2f(__uint_as_float(ends[m][0]) - zero);
-                        total += f * __uint_as_float(ends[m][1]);
-                        all += f * outs[m];
+                    for (int m = 0; m < kBlock; ++m) {
+                        next = fmaxf(next, __uint_as_float(ends[t][m][0]));
+                    }
+                    zero[t] = next == -INFINITY ? 0.f : next;
+                    const float keep = __builtin_amdgcn_exp2f(most[t] - zero[t]);
+                    most[t] = next;
+                    total[t] *= keep;
+                    all[t] *= keep;
+#pragma unroll
+                    for (int m = 0; m < kBlock; ++m) {
+                        if (x0 + m <= part.last) {
+                            const float f = __builtin_amdgcn_exp2f(__uint_as_float(ends[t][m][0]) - zero[t]);
+                            total[t] += f * __uint_as_float(ends[t][m][1]);
+                            all[t] += f * outs[t][m];
+                        }
                     }
                 }
             }
-            finish<kBf16>(a, part.b, part.hg / args.blocks * args.group + head0 + row, e, all, zero, total);
+#pragma unroll
+            for (int t = 0; t < kTasks; ++t) {
+                if (at0 + t * 64 * kWaves < rows * (D / 4)) {
+                    finish<kBf16>(a, part.b, part.hg / args.blocks * args.group + head0 + row[t], e[t], all[t], zero[t],
+                                  total[t]);
+                }
+            }
         }
     }
 }
