@@ -755,8 +755,9 @@ hipError_t clear(uint32_t *words, int64_t n, hipStream_t stream)
 // [used bits][many bits][Found: rows][Grant: rows][list: pages]
 size_t cache_update_workspace(const CacheUpdateArgs &a)
 {
-    return 2 * align_up(words_of(a.pages) * 4) + align_up((size_t)a.rows * sizeof(Found)) +
-           align_up((size_t)a.rows * sizeof(Grant)) + align_up((size_t)a.pages * 4);
+    return small(a) ? 0
+                    : 2 * align_up(words_of(a.pages) * 4) + align_up((size_t)a.rows * sizeof(Found)) +
+                          align_up((size_t)a.rows * sizeof(Grant)) + align_up((size_t)a.pages * 4);
 }
 
 hipError_t launch_cache_update(const CacheUpdateArgs &a, void *workspace, int, hipStream_t stream)
@@ -794,7 +795,7 @@ hipError_t launch_cache_update(const CacheUpdateArgs &a, void *workspace, int, h
     return hipGetLastError();
 }
 
-size_t cache_compact_workspace(const CacheCompactArgs &a) { return align_up(words_of(a.pages) * 4); }
+size_t cache_compact_workspace(const CacheCompactArgs &a) { return small(a) ? 0 : align_up(words_of(a.pages) * 4); }
 
 hipError_t launch_cache_compact(const CacheCompactArgs &a, void *workspace, int cus, hipStream_t stream)
 {
