@@ -146,6 +146,29 @@ __global__ __launch_bounds__(256) void update_rows(CacheUpdateArgs a, uint32_t *
     }
 }
 
+// The bitmap's words into registers, neighbouring threads' neighbouring ones, and
+// from there into LDS; words beyond it are 0.
+struct Words {
+    uint32_t held[kGroups / 1024];
+
+    __device__ Words(const uint32_t *from, int words)
+    {
+#pragma unroll
+        for (int n = 0; n < kGroups / 1024; ++n) {
+            const int w = (int)threadIdx.x + 1024 * n;
+            held[n] = from[w < words ? w : 0];  // (a load in any case)
+            held[n] = w < words ? held[n] : 0u;
+        }
+    }
+    __device__ void put(uint32_t *lds) const
+    {
+#pragma unroll
+        for (int n = 0; n < kGroups / 1024; ++n) {
+            lds[threadIdx.x + 1024 * n] = held[n];
+        }
+    }
+};
+
 // Inclusive scan of v over the workgroup of 1024; *total gets the sum.
 template <typename Int>
 __device__ Int scan_1024(Int v, Int *total)
@@ -182,29 +205,23 @@ struct Counts {
     int span, groups;  // words of a group; groups that have words
     const int32_t *before;
 
-    // Called by all 1024 threads; each counts neighbouring groups.  copy: LDS for
-    // the words, or null.
-    __device__ Counts(const uint32_t *from, int64_t pages_, int32_t *lds, uint32_t *copy)
-        : used(kOne && copy != nullptr ? copy : from), pages((int)pages_), before(lds)
+    // Called by all 1024 threads; each counts neighbouring groups.  With kOne `from` is
+    // in LDS, kMost words of which those beyond the pages are 0.
+    __device__ Counts(const uint32_t *from, int64_t pages_, int32_t *lds) : used(from), pages((int)pages_), before(lds)
     {
         constexpr int kEach = kMost / 1024;
         words = (int)words_of(pages);
         span = kOne ? 1 : (words + kMost - 1) / kMost;
         groups = kOne ? words : (words + span - 1) / span;
         int n[kEach], mine = 0;
-        const int64_t first = (int64_t)threadIdx.x * kEach * span;
 #pragma unroll
         for (int g = 0; g < kEach; ++g) {
             n[g] = 0;
             if constexpr (kOne) {
-                const bool on = first + g < words;
-                const uint32_t word = from[on ? first + g : 0];  // (a load in any case)
-                n[g] = on ? __popc(word) : 0;
-                if (copy != nullptr && on) {
-                    copy[first + g] = word;
-                }
+                n[g] = __popc(from[threadIdx.x * kEach + g]);
             } else {
-                for (int64_t w = first + g * span; w < first + (g + 1) * span && w < words; ++w) {
+                const int64_t first = ((int64_t)threadIdx.x * kEach + g) * span;
+                for (int64_t w = first; w < first + span && w < words; ++w) {
                     n[g] += __popc(from[w]);
                 }
             }
@@ -303,8 +320,8 @@ template <bool kOne>
 __global__ __launch_bounds__(1024) void update_grants(CacheUpdateArgs a, const uint32_t *used, const uint32_t *many,
                                                       const Found *found, Grant *grants, int32_t *list)
 {
-    __shared__ int32_t lds[kGroups + 1];
-    __shared__ uint32_t copy[kOne ? kGroups : 1], shared[kOne ? kGroups : 1];
+    __shared__ __align__(16) int32_t lds[kGroups + 1];
+    __shared__ __align__(16) uint32_t copy[kOne ? kGroups : 4], shared[kOne ? kGroups : 4];
     const int me = (int)threadIdx.x;
     const auto load = [&](int64_t r) {
         Found f{};
@@ -319,19 +336,20 @@ __global__ __launch_bounds__(1024) void update_grants(CacheUpdateArgs a, const u
     };
     Found next = load(me);  // (on its way while the words are counted)
     if constexpr (kOne) {
-        for (int w = me; w < words_of(a.pages); w += 1024) {
-            shared[w] = many[w];
-        }
-        many = shared;
+        const Words one(used, (int)words_of(a.pages)), two(many, (int)words_of(a.pages));
+        one.put(copy);
+        two.put(shared);
+        __syncthreads();
     }
-    const Counts<kGroups, kOne> counts(used, a.pages, lds, copy);
+    const uint32_t *twice = kOne ? shared : many;
+    const Counts<kGroups, kOne> counts(kOne ? copy : used, a.pages, lds);
     const int64_t free = a.pages - counts.held();
     int64_t asked = 0;
     for (int64_t r0 = 0; r0 < a.rows; r0 += 1024) {
         const int64_t r = r0 + me;
         const Found f = next;
         next = load(r + 1024);
-        const int swap = f.last >= 0 ? (int)(many[f.last / 32] >> (f.last % 32) & 1u) : 0;
+        const int swap = f.last >= 0 ? (int)(twice[f.last / 32] >> (f.last % 32) & 1u) : 0;
         const int64_t need = swap + f.row.grown - f.row.held;
         int64_t total;
         const int64_t upto = asked + scan_1024<int64_t>(need, &total);
@@ -409,12 +427,12 @@ __device__ __forceinline__ void each_cells(int rows, int width, F f)
 // threads share a row's columns and slots.
 __global__ __launch_bounds__(1024) void update_small(CacheUpdateArgs a, int lanes)
 {
-    __shared__ uint32_t used[kSmallWords], many[kSmallWords];
-    __shared__ int32_t lds[kSmallWords + 1];
+    __shared__ __align__(16) uint32_t used[kSmallWords], many[kSmallWords];
+    __shared__ __align__(16) int32_t lds[kSmallWords + 1];
     __shared__ Row rows[kSmallRows];
     __shared__ int32_t lasts[kSmallRows], first[kSmallRows];
     const int me = (int)threadIdx.x;
-    for (int w = me; w < words_of(a.pages); w += 1024) {
+    for (int w = me; w < kSmallWords; w += 1024) {
         used[w] = many[w] = 0u;
     }
     if (me < a.rows) {
@@ -444,7 +462,7 @@ __global__ __launch_bounds__(1024) void update_small(CacheUpdateArgs a, int lane
         mark_all(page, used, many);
     });
     __syncthreads();
-    const Counts<kSmallWords, true> counts(used, a.pages, lds, nullptr);
+    const Counts<kSmallWords, true> counts(used, a.pages, lds);
     const auto wants = [&](int r) { return lasts[r] >= 0 && (many[lasts[r] / 32] >> (lasts[r] % 32) & 1u) != 0u; };
     {
         const int need = me < a.rows ? wants(me) + rows[me].grown - rows[me].held : 0;
@@ -516,8 +534,8 @@ __global__ __launch_bounds__(256) void compact_mark(CacheCompactArgs a, uint32_t
 template <bool kOne>
 __global__ __launch_bounds__(1024) void compact_apply(CacheCompactArgs a, const uint32_t *used)
 {
-    __shared__ int32_t lds[kGroups + 1];
-    __shared__ uint32_t copy[kOne ? kGroups : 1];
+    __shared__ __align__(16) int32_t lds[kGroups + 1];
+    __shared__ __align__(16) uint32_t copy[kOne ? kGroups : 4];
     __shared__ uint16_t starts[kOne ? kGroups : 1];
     constexpr int kPieces = 8, kColumns = kWave * kPieces;
     const int pieces = (a.width + kColumns - 1) / kColumns;
@@ -534,7 +552,12 @@ __global__ __launch_bounds__(1024) void compact_apply(CacheCompactArgs a, const 
         }
     };
     load();  // (on its way while the words are counted)
-    const Counts<kGroups, kOne> counts(used, a.pages, lds, copy);
+    if constexpr (kOne) {
+        const Words words(used, (int)words_of(a.pages));
+        words.put(copy);
+        __syncthreads();
+    }
+    const Counts<kGroups, kOne> counts(kOne ? copy : used, a.pages, lds);
     if constexpr (kOne) {
         counts.index(starts);
     }
@@ -586,7 +609,7 @@ __global__ __launch_bounds__(1024) void compact_small(CacheCompactArgs a)
     __shared__ int32_t lds[kSmallWords + 1], held[kSmallRows];
     __shared__ uint16_t to[kSmallPages / 2];
     const int me = (int)threadIdx.x;
-    for (int w = me; w < words_of(a.pages); w += 1024) {
+    for (int w = me; w < kSmallWords; w += 1024) {
         used[w] = 0u;
     }
     if (me < a.rows) {
@@ -606,7 +629,7 @@ __global__ __launch_bounds__(1024) void compact_small(CacheCompactArgs a)
         mark_all(page, used, nullptr);
     });
     __syncthreads();
-    const Counts<kSmallWords, true> counts(used, a.pages, lds, nullptr);
+    const Counts<kSmallWords, true> counts(used, a.pages, lds);
     const int U = counts.held(), stay = counts.rank(U), moves = U - stay;
     if (me == 0) {
         a.used[0] = U;
