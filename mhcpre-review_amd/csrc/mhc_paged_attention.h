@@ -41,6 +41,10 @@ constexpr int kTile = 32;               // keys of a wave at a time
 constexpr int kUnit = kWaves * kTile;   // keys of a unit
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
+// Workgroups that a CU's registers hold.
+constexpr int workgroups_per_cu(int d, bool wide) { return d <= (wide ? 64 : 128) ? 2 : 1; }
+constexpr int kWideMost = 192;  // the largest d with 32 query heads at a time
+
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -244,7 +248,7 @@ struct Part {
 };
 
 template <bool kBf16, int D, int RT>
-__global__ __launch_bounds__(64 * kWaves, D > 128 || RT > 1 ? 1 : 2) void attention_units(Args args)
+__global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void attention_units(Args args)
 {
     using S = Shape<D>;
     using Left = Parts<D, RT>;
@@ -692,7 +696,11 @@ hipError_t launch_heads(const Args &args, hipStream_t stream)
     case 128: return launch_size<kBf16, 128, RT>(args, stream);
     case 160: return launch_size<kBf16, 160, RT>(args, stream);
     case 192: return launch_size<kBf16, 192, RT>(args, stream);
-    case 256: return launch_size<kBf16, 256, RT>(args, stream);
+    case 256:
+        if constexpr (RT == 1) {
+            return launch_size<kBf16, 256, RT>(args, stream);
+        }
+        return hipErrorInvalidValue;
     default: return hipErrorInvalidValue;
     }
 }
