@@ -72,7 +72,7 @@ struct Args {
     int group;    // query heads of a kv head
     int blocks;   // blocks of 16 * RT query heads in a group
     int most;     // workgroups of the launch
-    char *parts;  // see Parts
+    char *parts;  // see Parts; null: the kernel of short rows
     LaunchTag tag;
 };
 
@@ -127,14 +127,16 @@ struct Parts {
 struct Keys {
     int low, high, first, units;
 
-    __device__ Keys(const PagedAttentionArgs &a, int L)
+    Keys() = default;
+    // unit: keys of a unit.
+    __device__ Keys(const PagedAttentionArgs &a, int L, int unit)
     {
         const int most = a.width * a.pageSize;
         L = L < 0 ? 0 : L > most ? most : L;
         low = a.window > 0 && L > a.window ? L - (int)a.window : 0;
         high = L;
-        first = low / kUnit;
-        units = high > low ? (high + kUnit - 1) / kUnit - first : 1;
+        first = low / unit;
+        units = high > low ? (high + unit - 1) / unit - first : 1;
     }
 };
 
@@ -247,7 +249,11 @@ struct Part {
     __device__ int slot(int x) const { return x == first ? firstSlot : 2 * x; }
 };
 
-template <bool kBf16, int D, int RT>
+// kShort: rows of few keys (by the table's width or the window) in large batches.  Each
+// wave is on its own: a share of the (row, kv head, block)s, each of which it does
+// alone, 32 keys at a time, with no join and no workspace.  (Otherwise a row of up
+// to 32 keys leaves three waves of its workgroup without any.)
+template <bool kBf16, int D, int RT, bool kShort>
 __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void attention_units(Args args)
 {
     using S = Shape<D>;
@@ -260,57 +266,78 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
     __shared__ Part left[2];
     const PagedAttentionArgs &a = args.a;
     const int w = (int)blockIdx.x;
-    const uint32_t replay = threadIdx.x == 0 ? dev::replay_load(args.tag.words, w) : 0u;
     const int lane = (int)threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int c = lane / 16, col = lane % 16;
     const int perRow = a.kvHeads * args.blocks;
+    constexpr int kPer = kShort ? kTile : kUnit;  // keys of a unit
     const Left parts(args.parts, args.most);
-
-    // The workgroup's stretch and the row it begins in.
-    const int firstLength = a.lengths[lane < a.B ? lane : 0];
-    int count = lane < a.B ? Keys(a, firstLength).units : 0;
-    for (int x = lane + kWave; x < a.B; x += kWave) {
-        count += Keys(a, a.lengths[x]).units;
-    }
-    const Shares shares(__builtin_amdgcn_readfirstlane(wave_sum_int(count)) * perRow, args.most);
-    if (threadIdx.x == 0) {
-        tag = dev::launch_epoch<Args>(w, replay);
-        left[0].on = left[1].on = false;
-    }
-    if (w >= shares.grid) {
-        return;
-    }
-    const int begin = shares.start(w), end = shares.start(w + 1);
-    int b = 0, base = 0, length = 0;  // base: the row's first unit
-    for (int b0 = 0;; b0 += kWave) {
-        const int L = b0 == 0 ? firstLength : a.lengths[b0 + lane < a.B ? b0 + lane : 0];
-        const int mine = b0 + lane < a.B ? Keys(a, L).units * perRow : 0;
-        int upto = mine;
-#pragma unroll
-        for (int m = 1; m < kWave; m *= 2) {
-            const int u = __shfl_up(upto, m);
-            upto += lane >= m ? u : 0;
-        }
-        const uint64_t past = __ballot(base + upto > begin);
-        if (past != 0) {
-            const int at = __ffsll((unsigned long long)past) - 1;
-            b = b0 + at;
-            base += __shfl(upto - mine, at);
-            length = __shfl(L, at);
-            break;
-        }
-        base += __shfl(upto, kWave - 1);
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
-    base = __builtin_amdgcn_readfirstlane(base);
-    length = __builtin_amdgcn_readfirstlane(length);
 
     // A place in the line: unit `tile` of (row b, its hg-th kv head and block).
     struct Place {
         int b, hg, tile;
         Keys keys;
     };
-    const auto row_keys = [&](int x) { return Keys(a, __builtin_amdgcn_readfirstlane(a.lengths[x])); };
+    const auto row_keys = [&](int x) { return Keys(a, __builtin_amdgcn_readfirstlane(a.lengths[x]), kPer); };
+
+    // The workgroup's stretch of units (the wave's, of (row, kv head, block)s) and where it
+    // begins.
+    Shares shares(1, 1);
+    int begin, end;
+    Place first{};
+    if constexpr (kShort) {
+        shares = Shares(a.B * perRow, args.most * kWaves);
+        const int worker = w * kWaves + wave;
+        if (worker >= shares.grid) {
+            return;
+        }
+        begin = shares.start(worker);
+        end = shares.start(worker + 1);
+        first.b = begin / perRow;
+        first.hg = begin % perRow;
+        first.keys = row_keys(first.b);
+    } else {
+        const uint32_t replay = threadIdx.x == 0 ? dev::replay_load(args.tag.words, w) : 0u;
+        const int firstLength = a.lengths[lane < a.B ? lane : 0];
+        int count = lane < a.B ? Keys(a, firstLength, kPer).units : 0;
+        for (int x = lane + kWave; x < a.B; x += kWave) {
+            count += Keys(a, a.lengths[x], kPer).units;
+        }
+        shares = Shares(__builtin_amdgcn_readfirstlane(wave_sum_int(count)) * perRow, args.most);
+        if (threadIdx.x == 0) {
+            tag = dev::launch_epoch<Args>(w, replay);
+            left[0].on = left[1].on = false;
+        }
+        if (w >= shares.grid) {
+            return;
+        }
+        begin = shares.start(w);
+        end = shares.start(w + 1);
+        int b = 0, base = 0, length = 0;  // base: the row's first unit
+        for (int b0 = 0;; b0 += kWave) {
+            const int L = b0 == 0 ? firstLength : a.lengths[b0 + lane < a.B ? b0 + lane : 0];
+            const int mine = b0 + lane < a.B ? Keys(a, L, kPer).units * perRow : 0;
+            int upto = mine;
+#pragma unroll
+            for (int m = 1; m < kWave; m *= 2) {
+                const int u = __shfl_up(upto, m);
+                upto += lane >= m ? u : 0;
+            }
+            const uint64_t past = __ballot(base + upto > begin);
+            if (past != 0) {
+                const int at = __ffsll((unsigned long long)past) - 1;
+                b = b0 + at;
+                base += __shfl(upto - mine, at);
+                length = __shfl(L, at);
+                break;
+            }
+            base += __shfl(upto, kWave - 1);
+        }
+        first.b = __builtin_amdgcn_readfirstlane(b);
+        first.keys = Keys(a, __builtin_amdgcn_readfirstlane(length), kPer);
+        base = __builtin_amdgcn_readfirstlane(base);
+        first.hg = (begin - base) / first.keys.units;
+        first.tile = (begin - base) % first.keys.units;
+    }
     const auto advance = [&](Place &x) {
         if (++x.tile < x.keys.units) {
             return;
@@ -323,9 +350,8 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
             }
         }
     };
-    Place place{b, 0, 0, Keys(a, length)};
-    place.hg = (begin - base) / place.keys.units;
-    place.tile = (begin - base) % place.keys.units;
+    const auto inside = [&](const Place &x, int unit) { return kShort ? x.b * perRow + x.hg < end : unit < end; };
+    Place place = first;
 
     // The loads run ahead of the products, over the ends of rows: a unit's pages are
     // looked up three units ahead, its rows' addresses found two ahead, and its
@@ -337,8 +363,8 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
     };
     const auto find_page = [&]() {
         Found f{-1, 0, 0};
-        if (unit < end) {
-            const int t = (ahead.keys.first + ahead.tile) * kUnit + wave * kTile + lane % kTile;
+        if (inside(ahead, unit)) {
+            const int t = (ahead.keys.first + ahead.tile) * kPer + (kShort ? 0 : wave * kTile) + lane % kTile;
             f.kvHead = ahead.hg / args.blocks;
             if (t >= ahead.keys.low && t < ahead.keys.high) {
                 const uint32_t at = (uint32_t)t / (uint32_t)a.pageSize;
@@ -421,7 +447,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
     bool partial = false;
     int from = begin;  // the first unit of the (row, kv head, block) in this stretch
     char *mine = lds[wave];
-    for (int u = begin; u < end; ++u) {
+    for (int u = begin; inside(place, u); ++u) {
         // V to LDS; what the row does not see is zero there, whatever the cache holds.
         if (now != 0xFFFFFFFFu) {
 #pragma unroll
@@ -450,9 +476,10 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         }
         const uint32_t seen = now;
         const Place here = place;
-        const bool ends = place.tile + 1 == place.keys.units || u + 1 == end;
         advance(place);
-        if (u + 1 < end) {
+        const bool more = inside(place, u + 1);
+        const bool ends = here.tile + 1 == here.keys.units || !more;
+        if (more) {
             load();
             if (ends) {
                 load_q(place);
@@ -525,6 +552,24 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
             continue;
         }
 
+        if constexpr (kShort) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                sum[rt] += __shfl_xor(sum[rt], 16);
+                sum[rt] += __shfl_xor(sum[rt], 32);
+                const int h = here.hg % args.blocks * 16 * RT + rt * 16 + col;
+                if (h < args.group) {
+#pragma unroll
+                    for (int j = 0; j < S::kDims; ++j) {
+                        finish<kBf16>(a, here.b, here.hg / args.blocks * args.group + h, 16 * j + 4 * c, o[rt][j],
+                                      top[rt] == -INFINITY ? 0.f : top[rt], sum[rt]);
+                    }
+                }
+            }
+            clear();
+            continue;
+        }
+
         // The waves' results together, 16 query heads at a time.
         const int kvHead = here.hg / args.blocks, head0 = here.hg % args.blocks * 16 * RT;
         const int u0 = u - here.tile;  // where it begins, in this stretch or before
@@ -584,7 +629,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         from = u + 1;
         clear();
     }
-    if (!partial) {
+    if (kShort || !partial) {
         return;
     }
 
@@ -680,7 +725,16 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
 template <bool kBf16, int D, int RT>
 hipError_t launch_size(const Args &args, hipStream_t stream)
 {
-    hipLaunchKernelGGL((attention_units<kBf16, D, RT>), dim3((unsigned)args.most), dim3(64 * kWaves), 0, stream, args);
+    int grid = args.most;
+    auto kernel = attention_units<kBf16, D, RT, false>;
+    if constexpr (RT == 1) {
+        if (args.parts == nullptr) {
+            kernel = attention_units<kBf16, D, RT, true>;
+            const int items = args.a.B * args.a.kvHeads * args.blocks;
+            grid = (items + kWaves - 1) / kWaves < grid ? (items + kWaves - 1) / kWaves : grid;
+        }
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * kWaves), 0, stream, args);
     return hipGetLastError();
 }
 

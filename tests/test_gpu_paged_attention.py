@@ -91,6 +91,18 @@ def test_long_few_rows(ops, device, dtype, slot_major):
     _run(ops, _state(device, 2, 4, 2, 128, 16, [9000, 3], dtype, seed=1, slot_major=slot_major))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,heads,kv_heads,d,page,most,window", [
+    (300, 8, 8, 32, 16, 90, 0), (1100, 3, 1, 64, 7, 40, 0), (150, 16, 8, 128, 64, 300, 0), (260, 20, 4, 80, 1, 65, 0),
+    (280, 4, 2, 256, 16, 48, 0), (270, 4, 4, 96, 16, 3000, 37), (2100, 1, 1, 112, 32, 33, 1)])
+def test_many_short_rows(ops, device, B, heads, kv_heads, d, page, most, window, dtype):
+    """Large batches of rows that the table's width or the window keeps short: empty ones and holes among them."""
+    lengths = [(i * i * 37) % (most + 1) for i in range(B)]
+    state = _state(device, B, heads, kv_heads, d, page, lengths, dtype, seed=B)
+    state[3][::11, 0] = -1
+    _run(ops, state, window=window)
+
+
 def test_large_ragged_batch(ops, device):
     lengths = [(i * i * 37) % 701 for i in range(300)]
     _run(ops, _state(device, 300, 6, 2, 32, 16, lengths, torch.float16))
