@@ -24,10 +24,15 @@ __device__ __forceinline__ float wave_sum(float v)
 __device__ __forceinline__ uint16_t *cache_at(const CacheRows &c, const NormRopeArgs &a, int64_t t, int h)
 {
     const int64_t slot = a.slots[t];
-    if (slot < 0 || slot / a.pageSize >= a.pages) {
+    if (slot < 0) {
         return nullptr;
     }
-    return static_cast<uint16_t *>(c.data) + slot / a.pageSize * c.page + slot % a.pageSize * c.slot + h * c.head;
+    // (A 64-bit division takes ten times as long.)
+    const int64_t page = slot >> 32 == 0 ? (uint32_t)slot / (uint32_t)a.pageSize : slot / a.pageSize;
+    if (page >= a.pages) {
+        return nullptr;
+    }
+    return static_cast<uint16_t *>(c.data) + page * c.page + (slot - page * a.pageSize) * c.slot + h * c.head;
 }
 
 // Row `row` of the tokens' heads of q, k and v, one wave: any size, stride and
@@ -330,8 +335,10 @@ hipError_t launch_pieces(const NormRopeArgs &a, int cus, hipStream_t stream)
     s.q = (a.heads + kRows - 1) / kRows;
     s.k = (a.kvHeads + kRows - 1) / kRows;
     s.all = s.q + s.k * (a.kOut.data != nullptr ? 1 : 2);
-    // A token's rows are shared out while that gives the waves that fill the CUs something to do.
-    const int64_t fill = (int64_t)cus * 16;
+    // A token's rows are shared out until each SIMD has a wave; more waves would each compute
+    // the token's angles again (1024 tokens of 40 heads of 128, us: 16 waves a CU 13.1, 4 9.0;
+    // 2048 tokens into the cache 13.8 / 12.7).
+    const int64_t fill = (int64_t)cus * 4;
     const int64_t want = a.T < fill ? (fill + a.T - 1) / a.T : 1;
     s.parts = want < s.all ? (int)want : s.all;
     const int64_t blocks = (a.T * s.parts + 3) / 4, most = (int64_t)cus * 8;
