@@ -148,8 +148,9 @@ MHC_API int mhcRotaryFrequencies(int32_t rot, double base, int32_t kind, double 
  * are 16-byte aligned with strides (other than the last) of multiples of 8
  * elements; heads is a multiple of kvHeads; B * kvHeads * (width * pageSize / 128
  * + 2) is below 2^31, with kvHeads counted ceil(heads / kvHeads / 32) times where
- * more than 16 query heads share one.  The results do not depend on other
- * rows of the batch or on timing.
+ * more than 16 query heads share one.  The same call gives the same bits again;
+ * how a row's sums are cut depends on the batch's lengths, so that in another batch
+ * they may differ in their last bits, by roundings in fp32.
  */
 MHC_API int mhcPagedAttentionGetWorkspaceSize(
     const mhcStridedTensor *q, const mhcStridedTensor *kCache, const mhcStridedTensor *vCache,

@@ -6,6 +6,14 @@
 // pages that two rows or more hold), from which ranks (how many held pages lie
 // before this one) and selections (the k-th free page) follow by counting
 // bits.  The counts up to every group of words are kept in LDS.
+//
+// Bound: latencies.  Up to some entries one workgroup does all of it (64 rows of 128
+// entries, us: 9.3, compaction 8.6); above, each launch waits for the one before.
+// 1000 rows of up to 2048 entries, 200001 pages, us: clearing the bitmaps 2.0, marking
+// and the columns that stay 11.1 (about 6 of it the atomics, which go past the L2s, for
+// every XCD marks), who gets pages 6.2, the columns that change 3.4; compaction 2.0,
+// 7.8 and 12.0.  What they read and write is 9 MB, 1.6 us.  Copies are bound by the memory:
+// 2000 pages of 128 KB twice, read and written, 198 us (5.3 TB/s).
 
 #include "mhc_pre_device.h"
 #include "mhc_serve_internal.h"
@@ -200,7 +208,8 @@ __device__ Int scan_1024(Int v, Int *total)
 
 // The held pages before each group of words, in LDS: kMost + 1 counts, with
 // kOne a word to a group and the words in LDS too (a copy, or there already), else
-// as many words to a group as it takes.
+// as many words to a group as it takes (262144 pages, 512 rows of 1024, us, words in
+// LDS / in memory: update 22.0 / 24.7, compaction 22.9 / 33.5).
 template <int kMost, bool kOne>
 struct Counts {
     const uint32_t *used;
@@ -762,8 +771,9 @@ hipError_t launch_pieces(const CopyPagesArgs &a, const Runs &k, const Runs &v, i
     const int64_t perPage = (pieces + 256 * kPer - 1) / (256 * kPer);
     const int64_t blocks = 2 * a.n * perPage, most = (int64_t)cus * 1024;
     const bool stream_by = 2 * a.n * pieces * (int64_t)sizeof(Vec) > kCacheBytes;
-    hipLaunchKernelGGL((stream_by ? copy_pieces<Vec, true> : copy_pieces<Vec, false>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, k, v,
-                       a.src, a.dst, a.n, a.pages, pieces, perPage);
+    hipLaunchKernelGGL((stream_by ? copy_pieces<Vec, true> : copy_pieces<Vec, false>),
+                       dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, k, v, a.src, a.dst, a.n,
+                       a.pages, pieces, perPage);
     return hipGetLastError();
 }
 

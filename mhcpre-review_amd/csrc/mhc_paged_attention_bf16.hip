@@ -17,9 +17,7 @@ Args plan(const PagedAttentionArgs &a, int cus, bool &wide)
     Args p{};
     p.a = a;
     p.group = a.heads / a.kvHeads;
-    // 32 query heads at a time where the registers hold them: d = 256 spills, and reading the
-    // cache once for each 16 heads is faster (64 rows of 8192, 32 heads to one: 285 us
-    // against 166).
+    // 32 query heads at a time where there are as many and the registers hold them.
     wide = p.group > 16 && a.d <= kWideMost;
     p.blocks = (p.group + (wide ? 31 : 15)) / (wide ? 32 : 16);
     p.most = cus * workgroups_per_cu(a.d, wide);

@@ -33,8 +33,8 @@ constexpr size_t kWsReplayOff = 256;  // uint32 [kMaxExchangeGrid]
 constexpr int kMaxExchangeGrid = 2048;  // largest grid of a kernel whose workgroups exchange words
 constexpr size_t kWsHeaderBytes = kWsReplayOff + 4 * kMaxExchangeGrid;
 
-// What the kernels whose workgroups exchange words (cell, slab, strip, fused)
-// mix into every tag, so that no word of another launch is taken for one of
+// What the kernels whose workgroups exchange words (cell, slab, strip, fused,
+// and paged attention, which counts) mix into every tag, so that no word of another launch is taken for one of
 // this launch's, whatever the workspace held before: the hash (mix32, a
 // bijection) of a number that no other launch of the process has.  An eager
 // launch: its own number, 31 bits of it (`seed`, hashed; `words` null).  The

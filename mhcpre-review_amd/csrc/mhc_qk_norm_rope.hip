@@ -1,5 +1,18 @@
 // Norms of queries and keys per head, rotary positions and the cache write
-// (mhcQkNormRope).
+// (mhcQkNormRope): y = x w / sqrt(mean(x^2) + eps), each pair of y's first rot
+// values turned by its angle.
+//
+// A row is read once, into the registers of the lanes that write it, for its sum of
+// squares and the products; sums, angles' sines and products are fp32, each output is
+// rounded once.  An angle is position * frequency / (2 pi) in 64 bits, of which the
+// nearest whole number is taken away before it is rounded to fp32 (in 32 bits a
+// position of 10^6 would have lost the phase: 2^-4 of a radian); the hardware's sine and
+// cosine take turns, and are within 1.3e-7 there.
+//
+// Bound: the memory (2 bytes in, 2 out a value, and 6 flops).  Measured: 8192 tokens, 64 + 8
+// heads of 128, 302 MB, 58 us (5.2 TB/s; a copy of 2 GiB reaches 4.8); one
+// token each for 64 rows, 32 + 8 + 8 heads of 128 into the cache 5.6 us, which is a
+// launch and two latencies.
 
 #include "mhc_pre_device.h"
 #include "mhc_serve_internal.h"
@@ -157,7 +170,8 @@ struct Split {
     int q, k, all;   // steps of 64 / L rows: of q, of k, with v's
 };
 
-// Rows whose 16-byte pieces are aligned: L lanes to a row (d / 16 of them with
+// Rows whose 16-byte pieces are aligned (a value at a time as above, 8192 tokens of 72 heads
+// of 128 take 345 us, so 60.6): L lanes to a row (d / 16 of them with
 // work), each with 8 pairs in two pieces: at 8 c and rot / 2 + 8 c (the half layout;
 // beyond rot likewise, half of the rest apart), or at 8 c and d / 2 + 8 c
 // (interleaved), so that neighbouring lanes have neighbouring pieces.  A wave has
