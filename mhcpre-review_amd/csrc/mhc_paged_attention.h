@@ -149,12 +149,15 @@ struct Keys {
     }
 };
 
-__device__ __forceinline__ int wave_sum_int(int v)
+// Inclusive scan over the wave, all lanes active.
+__device__ __forceinline__ int wave_scan(int v)
 {
-#pragma unroll
-    for (int m = 1; m < kWave; m *= 2) {
-        v += __shfl_xor(v, m);
-    }
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15: rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast 31: rows 2 and 3
     return v;
 }
 
@@ -307,11 +310,13 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
     } else {
         const uint32_t replay = threadIdx.x == 0 ? dev::replay_load(args.tag.words, w) : 0u;
         const int firstLength = a.lengths[lane < a.B ? lane : 0];
-        int count = lane < a.B ? Keys(a, firstLength, kPer).units : 0;
-        for (int x = lane + kWave; x < a.B; x += kWave) {
-            count += Keys(a, a.lengths[x], kPer).units;
+        const int firstUnits = lane < a.B ? Keys(a, firstLength, kPer).units : 0, firstUpto = wave_scan(firstUnits);
+        int all = __builtin_amdgcn_readlane(firstUpto, kWave - 1);
+        for (int b0 = kWave; b0 < a.B; b0 += kWave) {
+            const int x = b0 + lane, L = a.lengths[x < a.B ? x : 0];
+            all += __builtin_amdgcn_readlane(wave_scan(x < a.B ? Keys(a, L, kPer).units : 0), kWave - 1);
         }
-        shares = Shares(__builtin_amdgcn_readfirstlane(wave_sum_int(count)) * perRow, args.most);
+        shares = Shares(all * perRow, args.most);
         if (threadIdx.x == 0) {
             tag = dev::launch_epoch<Args>(w, replay);
             left[0].on = left[1].on = false;
@@ -322,28 +327,24 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         begin = shares.start(w);
         end = shares.start(w + 1);
         int b = 0, base = 0, length = 0;  // base: the row's first unit
-        for (int b0 = 0;; b0 += kWave) {
-            const int L = b0 == 0 ? firstLength : a.lengths[b0 + lane < a.B ? b0 + lane : 0];
-            const int mine = b0 + lane < a.B ? Keys(a, L, kPer).units * perRow : 0;
-            int upto = mine;
-#pragma unroll
-            for (int m = 1; m < kWave; m *= 2) {
-                const int u = __shfl_up(upto, m);
-                upto += lane >= m ? u : 0;
-            }
-            const uint64_t past = __ballot(base + upto > begin);
+        int L = firstLength, units = firstUnits, upto = firstUpto;
+        for (int b0 = 0;;) {
+            const uint64_t past = __ballot(base + upto * perRow > begin);
             if (past != 0) {
                 const int at = __ffsll((unsigned long long)past) - 1;
                 b = b0 + at;
-                base += __shfl(upto - mine, at);
-                length = __shfl(L, at);
+                base += __builtin_amdgcn_readlane(upto - units, at) * perRow;
+                length = __builtin_amdgcn_readlane(L, at);
                 break;
             }
-            base += __shfl(upto, kWave - 1);
+            base += __builtin_amdgcn_readlane(upto, kWave - 1) * perRow;
+            b0 += kWave;
+            L = a.lengths[b0 + lane < a.B ? b0 + lane : 0];
+            units = b0 + lane < a.B ? Keys(a, L, kPer).units : 0;
+            upto = wave_scan(units);
         }
-        first.b = __builtin_amdgcn_readfirstlane(b);
-        first.keys = Keys(a, __builtin_amdgcn_readfirstlane(length), kPer);
-        base = __builtin_amdgcn_readfirstlane(base);
+        first.b = b;
+        first.keys = Keys(a, length, kPer);
         first.hg = (begin - base) / first.keys.units;
         first.tile = (begin - base) % first.keys.units;
     }
