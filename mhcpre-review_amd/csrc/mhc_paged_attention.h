@@ -665,15 +665,9 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         complete[lane] = all;
     }
     __syncthreads();
-    for (int n = 0; n < 2; ++n) {
-        if (!complete[n]) {
-            continue;
-        }
-        const Part part = left[n];
-        const int head0 = part.hg % args.blocks * 16 * RT;
-        const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
-        // A thread's kTasks times kBlock parts are on their way at once.
-        constexpr int kTasks = D > 128 ? 4 : D > 64 ? 2 : 1, kBlock = kTasks > 1 ? 32 / kTasks : 16;
+    // A thread's tasks (4 values of a head each) times 32 / tasks parts are on their way at once.
+    const auto join = [&](const Part &part, int head0, int rows, auto tasks) {
+        constexpr int kTasks = decltype(tasks)::value, kBlock = 32 / kTasks;
         for (int at0 = (int)threadIdx.x; at0 < rows * (D / 4); at0 += 64 * kWaves * kTasks) {
             int row[kTasks], e[kTasks];
             float most[kTasks], zero[kTasks], total[kTasks];
@@ -728,6 +722,19 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                                   total[t]);
                 }
             }
+        }
+    };
+    for (int n = 0; n < 2; ++n) {
+        if (!complete[n]) {
+            continue;
+        }
+        const Part part = left[n];
+        const int head0 = part.hg % args.blocks * 16 * RT;
+        const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
+        if (rows * (D / 4) <= 64 * kWaves) {
+            join(part, head0, rows, std::integral_constant<int, 1>{});
+        } else {
+            join(part, head0, rows, std::integral_constant<int, (D > 128 ? 4 : 2)>{});
         }
     }
 }
