@@ -665,9 +665,10 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         complete[lane] = all;
     }
     __syncthreads();
-    // A thread's tasks (4 values of a head each) times 32 / tasks parts are on their way at once.
+    // A thread's tasks (4 values of a head each) times 32 / tasks parts are on their way at once,
+    // in groups: those beyond the last part are left out.
     const auto join = [&](const Part &part, int head0, int rows, auto tasks) {
-        constexpr int kTasks = decltype(tasks)::value, kBlock = 32 / kTasks;
+        constexpr int kTasks = decltype(tasks)::value, kBlock = 32 / kTasks, kGroup = kBlock / 4;
         for (int at0 = (int)threadIdx.x; at0 < rows * (D / 4); at0 += 64 * kWaves * kTasks) {
             int row[kTasks], e[kTasks];
             float most[kTasks], zero[kTasks], total[kTasks];
@@ -685,12 +686,26 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                 u32x2_t ends[kTasks][kBlock];
                 f32x4_t outs[kTasks][kBlock];
 #pragma unroll
-                for (int m = 0; m < kBlock; ++m) {
-                    const int slot = part.slot(x0 + m < part.last ? x0 + m : part.last);
+                for (int m0 = 0; m0 < kBlock; m0 += kGroup) {
+                    if (x0 + m0 <= part.last) {
 #pragma unroll
-                    for (int t = 0; t < kTasks; ++t) {
-                        ends[t][m] = parts.end(slot, row[t]);
-                        outs[t][m] = parts.out(slot, row[t], e[t]);
+                        for (int m = m0; m < m0 + kGroup; ++m) {
+                            const int slot = part.slot(x0 + m < part.last ? x0 + m : part.last);
+#pragma unroll
+                            for (int t = 0; t < kTasks; ++t) {
+                                ends[t][m] = parts.end(slot, row[t]);
+                                outs[t][m] = parts.out(slot, row[t], e[t]);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int m = m0; m < m0 + kGroup; ++m) {
+#pragma unroll
+                            for (int t = 0; t < kTasks; ++t) {
+                                ends[t][m] = u32x2_t{0xFF800000u, 0u};  // (-inf: weight 0)
+                                outs[t][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                            }
+                        }
                     }
                 }
 #pragma unroll
