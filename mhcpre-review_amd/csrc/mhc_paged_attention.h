@@ -87,25 +87,40 @@ struct Args {
 
 // A stretch leaves at most two parts in the workspace, of the (row, kv head,
 // group) that it begins in and of the one that it ends in: [2 * most] outputs [16
-// RT][D], maxima (base 2) and sums [16 RT][2]; and an 8-byte word, of those of a
-// (row, kv head, group) its first part's, that counts the parts that are there:
-// its upper 52 bits are the launch's and the place's, so that the first to come
-// sees that the word is not yet this launch's and sets it to none.  All of it is
-// stored through to memory and read from there: the reader may be on another XCD.
+// RT][D], maxima (base 2) and sums [16 RT][2]; and an 8-byte word, of those of
+// the parts that are joined together the first one's, that counts the parts that are
+// there: its upper 52 bits are the launch's and the place's, so that the first to come
+// sees that the word is not yet this launch's and sets it to none.  Many parts are
+// joined in spans: a span's result takes the place of its first output, its maxima,
+// sums and word are a second [2 * most] ones.  All of it is stored through to memory
+// and read from there: the reader may be on another XCD.
 template <int D, int RT>
 struct Parts {
     static constexpr int kRows = 16 * RT;
     __amdgpu_buffer_rsrc_t outs, ends;
     uint64_t *words;
 
-    static constexpr size_t bytes(int most) { return (size_t)2 * most * (kRows * (D + 2) * 4 + 8); }
     __device__ Parts(char *base, int most)
         : outs(dev::make_rsrc(base, 2 * most * kRows * D * 4)),
-          ends(dev::make_rsrc(base + (size_t)2 * most * kRows * D * 4, 2 * most * kRows * 8)),
-          words(reinterpret_cast<uint64_t *>(base + (size_t)2 * most * kRows * (D + 2) * 4))
+          ends(dev::make_rsrc(base + (size_t)2 * most * kRows * D * 4, 4 * most * kRows * 8)),
+          words(reinterpret_cast<uint64_t *>(base + (size_t)2 * most * kRows * (D + 4) * 4))
     {
     }
     static constexpr uint64_t kCount = 0xFFF;
+    // Counts a part at the word, which was found as `found`; how many were there.
+    __device__ int count(uint32_t tag, int slot, uint64_t found) const
+    {
+        const uint64_t none = sign(tag, slot);
+        if ((found & ~kCount) != none) {  // (fails where another workgroup was first)
+            (void)__hip_atomic_compare_exchange_strong(words + slot, &found, none, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT);
+        }
+        return (int)(__hip_atomic_fetch_add(words + slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & kCount);
+    }
+    __device__ uint64_t word(int slot) const
+    {
+        return __hip_atomic_load(words + slot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     // A word of this launch before the first part is counted.
     __device__ static uint64_t sign(uint32_t tag, int slot)
     {
@@ -259,7 +274,26 @@ struct Part {
     bool on;
     int b, hg, first, last, firstSlot;
     __device__ int slot(int x) const { return x == first ? firstSlot : 2 * x; }
+    // Parts that are joined together (2 to this power): all of them where one round of loads
+    // takes them, or spans of about the root of their number, whose results are joined then.
+    int spanBits;
+    __device__ int span_first(int w) const { return first + (((w - first) >> spanBits) << spanBits); }
+    __device__ int span_last(int w) const
+    {
+        const int after = (last - span_first(w)) >> spanBits;
+        return after == 0 ? last : span_first(w) + (1 << spanBits) - 1;
+    }
+    __device__ int spans() const { return ((last - first) >> spanBits) + 1; }
 };
+
+// us, all at once / in spans: 64 parts of 16 heads of 128 47.4 / 36.8, of 256 74.4 / 46.8; 32 parts of 4
+// heads of 128 (one round) 11.8 / 13.2.
+constexpr int kAllBits = 30;  // (parts are at most 2048)
+__device__ __forceinline__ int span_bits(int parts, int round)
+{
+    return parts <= round ? kAllBits : parts <= 64 ? 3 : parts <= 256 ? 4 : 5;
+}
+
 
 // kShort: rows of few keys (by the table's width or the window) in large batches.  Each
 // wave is on its own: a share of the (row, kv head, block)s, each of which it does
@@ -274,7 +308,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
     __shared__ __align__(16) char lds[kWaves][region<D>()];
     __shared__ float tops[kWaves][16 * RT], sums[kWaves][16 * RT];
     __shared__ uint32_t tag;
-    __shared__ bool complete[2];
+    __shared__ bool complete[2], spansComplete;
     __shared__ Part left[2];
     const PagedAttentionArgs &a = args.a;
     const int w = (int)blockIdx.x;
@@ -289,6 +323,12 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         int b, hg, tile;
         Keys keys;
     };
+    // Heads of a block; parts that a round of loads takes in a join of more than one task a thread.
+    const auto heads_of = [&](int hg) {
+        const int h = args.group - hg % args.blocks * 16 * RT;
+        return h < 16 * RT ? h : 16 * RT;
+    };
+    constexpr int kManyTasks = D > 128 ? 4 : 2, kRound = 32 / kManyTasks;
     const auto row_keys = [&](int x) { return Keys(a, __builtin_amdgcn_readfirstlane(a.lengths[x]), kPer); };
 
     // The workgroup's stretch of units (the wave's, of (row, kv head, block)s) and where it
@@ -617,12 +657,13 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                                                                   row * (D + 4) + e);
                 }
                 const int h = head0 + rt * 16 + row;
-                if (!whole) {
+                if (h >= args.group) {
+                } else if (!whole) {
                     parts.put(slot, rt * 16 + row, e, all);
                     if (e == 0) {
                         parts.put_ends(slot, rt * 16 + row, most, total);
                     }
-                } else if (h < args.group) {
+                } else {
                     finish<kBf16>(a, here.b, kvHead * args.group + h, e, all, zero, total);
                 }
             }
@@ -633,7 +674,8 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
             if (threadIdx.x == 0) {
                 const int first = shares.owner(u0), last = shares.owner(u0 + here.keys.units - 1);
                 left[from == begin ? 0 : 1] =
-                    Part{true, here.b, here.hg, first, last, 2 * first + (shares.start(first) == u0 ? 0 : 1)};
+                    Part{true, here.b, here.hg, first, last, 2 * first + (shares.start(first) == u0 ? 0 : 1),
+                         span_bits(last - first + 1, heads_of(here.hg) * (D / 4) <= 64 * kWaves ? 32 : kRound)};
             }
         }
         from = u + 1;
@@ -645,29 +687,27 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
 
     // The parts are there once their stores have ended; then they are counted.
     uint64_t found_word = 0;
+    int wordSlot = 0;
     if (wave == 0 && lane < 2 && left[lane].on) {
-        found_word = __hip_atomic_load(parts.words + left[lane].firstSlot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        wordSlot = left[lane].slot(left[lane].span_first(w));
+        found_word = parts.word(wordSlot);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (wave == 0 && lane < 2) {
         bool all = false;
         if (left[lane].on) {
-            uint64_t *word = parts.words + left[lane].firstSlot;
-            const uint64_t zero = Left::sign(tag, left[lane].firstSlot);
-            if ((found_word & ~Left::kCount) != zero) {  // (fails where another workgroup was first)
-                (void)__hip_atomic_compare_exchange_strong(word, &found_word, zero, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                                                           __HIP_MEMORY_SCOPE_AGENT);
-            }
-            const uint64_t before = __hip_atomic_fetch_add(word, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            all = (int)(before & Left::kCount) == left[lane].last - left[lane].first;
+            all = parts.count(tag, wordSlot, found_word) == left[lane].span_last(w) - left[lane].span_first(w);
         }
         complete[lane] = all;
     }
     __syncthreads();
     // A thread's tasks (4 values of a head each) times 32 / tasks parts are on their way at once,
     // in groups: those beyond the last part are left out.
-    const auto join = [&](const Part &part, int head0, int rows, auto tasks) {
+    // `spans`: the parts are the results of the spans; `whole`: what comes out is the output.
+    const auto join = [&](const Part &part, int head0, int rows, int first, int last, int step, bool spans, bool whole,
+                          auto tasks) {
+        const int second = spans ? 2 * args.most : 0;
         constexpr int kTasks = decltype(tasks)::value, kBlock = 32 / kTasks, kGroup = kBlock / 4;
         for (int at0 = (int)threadIdx.x; at0 < rows * (D / 4); at0 += 64 * kWaves * kTasks) {
             int row[kTasks], e[kTasks];
@@ -682,18 +722,18 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                 zero[t] = total[t] = 0.f;
                 all[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
             }
-            for (int x0 = part.first; x0 <= part.last; x0 += kBlock) {
+            for (int x0 = first; x0 <= last; x0 += kBlock * step) {
                 u32x2_t ends[kTasks][kBlock];
                 f32x4_t outs[kTasks][kBlock];
 #pragma unroll
                 for (int m0 = 0; m0 < kBlock; m0 += kGroup) {
-                    if (x0 + m0 <= part.last) {
+                    if (x0 + m0 * step <= last) {
 #pragma unroll
                         for (int m = m0; m < m0 + kGroup; ++m) {
-                            const int slot = part.slot(x0 + m < part.last ? x0 + m : part.last);
+                            const int slot = part.slot(x0 + m * step <= last ? x0 + m * step : x0 + m0 * step);
 #pragma unroll
                             for (int t = 0; t < kTasks; ++t) {
-                                ends[t][m] = parts.end(slot, row[t]);
+                                ends[t][m] = parts.end(slot + second, row[t]);
                                 outs[t][m] = parts.out(slot, row[t], e[t]);
                             }
                         }
@@ -722,7 +762,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                     all[t] *= keep;
 #pragma unroll
                     for (int m = 0; m < kBlock; ++m) {
-                        if (x0 + m <= part.last) {
+                        if (x0 + m * step <= last) {
                             const float f = __builtin_amdgcn_exp2f(__uint_as_float(ends[t][m][0]) - zero[t]);
                             total[t] += f * __uint_as_float(ends[t][m][1]);
                             all[t] += f * outs[t][m];
@@ -732,9 +772,15 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
             }
 #pragma unroll
             for (int t = 0; t < kTasks; ++t) {
-                if (at0 + t * 64 * kWaves < rows * (D / 4)) {
+                if (at0 + t * 64 * kWaves >= rows * (D / 4)) {
+                } else if (whole) {
                     finish<kBf16>(a, part.b, part.hg / args.blocks * args.group + head0 + row[t], e[t], all[t], zero[t],
                                   total[t]);
+                } else {
+                    parts.put(part.slot(first), row[t], e[t], all[t]);
+                    if (e[t] == 0) {
+                        parts.put_ends(part.slot(first) + 2 * args.most, row[t], most[t], total[t]);
+                    }
                 }
             }
         }
@@ -745,12 +791,34 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         }
         const Part part = left[n];
         const int head0 = part.hg % args.blocks * 16 * RT;
-        const int rows = args.group - head0 < 16 * RT ? args.group - head0 : 16 * RT;
-        if (rows * (D / 4) <= 64 * kWaves) {
-            join(part, head0, rows, std::integral_constant<int, 1>{});
-        } else {
-            join(part, head0, rows, std::integral_constant<int, (D > 128 ? 4 : 2)>{});
+        const int rows = heads_of(part.hg);
+        const auto join_all = [&](int first, int last, int step, bool spans, bool whole) {
+            if (rows * (D / 4) <= 64 * kWaves) {
+                join(part, head0, rows, first, last, step, spans, whole, std::integral_constant<int, 1>{});
+            } else {
+                join(part, head0, rows, first, last, step, spans, whole, std::integral_constant<int, kManyTasks>{});
+            }
+        };
+        const bool one = part.spans() == 1;
+        join_all(part.span_first(w), part.span_last(w), 1, false, one);
+        if (one) {
+            continue;
         }
+        const int slot = part.firstSlot + 2 * args.most;
+        uint64_t found = 0;
+        if (threadIdx.x == 0) {
+            found = parts.word(slot);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            spansComplete = parts.count(tag, slot, found) == part.spans() - 1;
+        }
+        __syncthreads();
+        if (spansComplete) {
+            join_all(part.first, part.last, 1 << part.spanBits, true, true);
+        }
+        __syncthreads();
     }
 }
 

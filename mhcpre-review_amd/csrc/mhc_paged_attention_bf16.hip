@@ -63,7 +63,7 @@ size_t paged_attention_workspace(const PagedAttentionArgs &a, int cus)
     if (attention::short_rows(a, p, wide)) {
         return 0;
     }
-    return kWsHeaderBytes + (size_t)2 * p.most * ((wide ? 32 : 16) * (a.d + 2) * 4 + 8);
+    return kWsHeaderBytes + (size_t)2 * p.most * ((wide ? 32 : 16) * (a.d + 4) * 4 + 16);
 }
 
 hipError_t launch_paged_attention(const PagedAttentionArgs &a, void *workspace, int device, int cus,

@@ -91,6 +91,22 @@ def test_long_few_rows(ops, device, dtype, slot_major):
     _run(ops, _state(device, 2, 4, 2, 128, 16, [9000, 3], dtype, seed=1, slot_major=slot_major))
 
 
+@pytest.mark.parametrize("heads,kv_heads,d,lengths,window", [
+    (1, 1, 32, [66000], 0), (16, 1, 64, [70000], 0), (40, 1, 192, [33000], 0), (24, 4, 128, [20000], 0),
+    (32, 2, 256, [10000, 7001], 0), (17, 1, 80, [40000, 5], 30000), (12, 1, 112, [300, 24000, 0, 26000], 0)])
+def test_rows_of_many_parts(pkg, ops, device, heads, kv_heads, d, lengths, window):
+    """So many workgroups at a row that their parts are joined in spans first; again on a workspace that holds anything."""
+    state = _state(device, len(lengths), heads, kv_heads, d, 64, lengths, torch.bfloat16, seed=d)
+    out, lse = _run(ops, state, window=window)
+    op = pkg.PagedAttentionOp(*state, window=window)
+    for fill in (0, 255, 7):
+        op.workspace.fill_(fill)
+        for _ in range(2):
+            op.out.fill_(3.0)
+            op.launch()
+            assert torch.equal(op.out, out) and torch.equal(op.lse, lse)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("B,heads,kv_heads,d,page,most,window", [
     (300, 8, 8, 32, 16, 90, 0), (1100, 3, 1, 64, 7, 40, 0), (150, 16, 8, 128, 64, 300, 0), (260, 20, 4, 80, 1, 65, 0),
