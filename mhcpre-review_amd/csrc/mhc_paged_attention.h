@@ -627,6 +627,10 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         const int slot = 2 * w + (from == begin ? 0 : 1);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+            const int rows = heads_of(here.hg) - rt * 16 < 16 ? heads_of(here.hg) - rt * 16 : 16;
+            if (rows <= 0) {
+                break;
+            }
             sum[rt] += __shfl_xor(sum[rt], 16);
             sum[rt] += __shfl_xor(sum[rt], 32);
             if (c == 0) {
@@ -634,12 +638,14 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                 sums[wave][rt * 16 + col] = sum[rt];
             }
             float *row = reinterpret_cast<float *>(mine) + col * (D + 4);
+            if (col < rows) {
 #pragma unroll
-            for (int j = 0; j < S::kDims; ++j) {
-                *reinterpret_cast<f32x4_t *>(row + 16 * j + 4 * c) = o[rt][j];
+                for (int j = 0; j < S::kDims; ++j) {
+                    *reinterpret_cast<f32x4_t *>(row + 16 * j + 4 * c) = o[rt][j];
+                }
             }
             __syncthreads();
-            for (int at = (int)threadIdx.x; at < 16 * D / 4; at += 64 * kWaves) {
+            for (int at = (int)threadIdx.x; at < rows * (D / 4); at += 64 * kWaves) {
                 const int row = at / (D / 4), e = at % (D / 4) * 4;
                 float most = -INFINITY;
 #pragma unroll
@@ -657,8 +663,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                                                                   row * (D + 4) + e);
                 }
                 const int h = head0 + rt * 16 + row;
-                if (h >= args.group) {
-                } else if (!whole) {
+                if (!whole) {
                     parts.put(slot, rt * 16 + row, e, all);
                     if (e == 0) {
                         parts.put_ends(slot, rt * 16 + row, most, total);
