@@ -8,7 +8,8 @@
 // workgroup walks its stretch; a (row, kv head, group) that lies in one
 // stretch is finished there, the others leave their maximum, sum and output per
 // stretch in the workspace and count them, and the workgroup that counts the last
-// one joins them, in the order of the keys.  Nobody waits.  What tells this
+// one joins them, in the order of the keys (many of them in spans first, each
+// joined by its own last workgroup).  Nobody waits.  What tells this
 // launch's counts from what the workspace held before is the launch's tag
 // (LaunchTag).
 //
@@ -25,11 +26,11 @@
 // Bound: the cache is read once, 4 bytes a value pair for at most 4 * 16
 // flops, so the memory's rate decides (6.05 TB/s for a cold read of two
 // tensors of 0.5 GB in the same pieces).  Measured: 64 rows of 1 to 8192 keys,
-// 32 heads to 8 of 128, 734 MB, 144 us (5.1 TB/s); 4 rows up to 131072 keys, 1007 MB,
-// 188 us (5.35 TB/s; 174.5 in a copy that leaves the join out).  The rest is the
+// 32 heads to 8 of 128, 734 MB, 137 us (5.35 TB/s); 4 rows up to 131072 keys, 1007 MB,
+// 184 us (5.5 TB/s; 174.5 in a copy that leaves the join out).  The rest is the
 // start (the first pages' addresses and translations, about 8 us) and the join's
-// chain of store, count and load, about 6 us at the end; a row of few keys is
-// nothing but these (one row of 1000 keys, 10 us).
+// chain of store, count and load, about 3 us at the end; a row of few keys is
+// nothing but these (one row of 1000 keys, 9 us).
 #pragma once
 
 #include "mhc_pre_device.h"
@@ -49,7 +50,7 @@ constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 // Workgroups that a CU's registers hold.  A product with 32 query heads reads the cache once
 // where two with 16 read it twice: 64 rows of 8192 keys, 32 heads to one, us, 32 at a
-// time / 16: d = 64 32.5 / 46.1, 128 54.1 / 86.1, 192 88.6 / 126.3.  At d = 256 its
+// time / 16: d = 64 31.4 / 45.2, 128 51.9 / 84.5, 192 88.6 / 121.0.  At d = 256 its
 // registers spill (285 / 166).
 constexpr int workgroups_per_cu(int d, bool wide) { return d <= (wide ? 64 : 128) ? 2 : 1; }
 constexpr int kWideMost = 192;  // the largest d with 32 query heads at a time

@@ -27,10 +27,10 @@ Args plan(const PagedAttentionArgs &a, int cus, bool &wide)
 
 // Whether no row has more than kShortKeys keys and there are enough (row, kv head,
 // block)s for half of the waves: then each wave does its own.  us, workgroups / waves
-// (8 kv heads of 128): 256 rows of 16 keys 22.7 / 9.1, 64 23.1 / 14.8, 256 57.7 / 51.9,
-// 512 102 / 97, of 1 to 256 37.3 / 34.6, with a window of 128 34.1 / 27.6; 1024 rows of
-// 32 77.2 / 35.5; but 64 rows (512 of them, a quarter of the waves) of 128 11.3 / 11.9,
-// of 512 28.5 / 41.8.
+// (8 kv heads of 128): 256 rows of 16 keys 20.9 / 8.7, 64 22.1 / 14.7, 256 57.2 / 51.6,
+// 512 101.5 / 97.2, of 1 to 256 36.2 / 34.9, with a window of 128 32.1 / 27.9; 1024 rows
+// of 32 72.3 / 34.5; but 64 rows (512 of them, a quarter of the waves) of 128 10.6 / 11.7,
+// of 512 27.8 / 41.8.
 constexpr int64_t kShortKeys = 512;
 bool short_rows(const PagedAttentionArgs &a, const Args &p, bool wide)
 {
