@@ -8,7 +8,7 @@
 // bits.  The counts up to every group of words are kept in LDS.
 //
 // Bound: latencies.  Up to some entries one workgroup does all of it (64 rows of 128
-// entries, us: 9.3, compaction 8.6); above, each launch waits for the one before.
+// entries, us: 9.4, compaction 8.1); above, each launch waits for the one before.
 // 1000 rows of up to 2048 entries, 200001 pages, us: clearing the bitmaps 2.0, marking
 // and the columns that stay 11.1 (about 6 of it the atomics, which go past the L2s, for
 // every XCD marks), who gets pages 6.2, the columns that change 3.4; compaction 2.0,
@@ -25,7 +25,7 @@ using dev::kWave;
 
 // What one workgroup does alone.  The rows, the bitmaps and a compaction's moves are held in its
 // LDS; and the rest of the CUs pays for its launches above some entries (us of a call alone / by
-// all CUs: 4 rows of 64 entries, update 8.7 / 19.1, compaction 8.1 / 13.9; 128 of 128 13.2 / 17.2,
+// all CUs: 4 rows of 64 entries, update 8.6 / 19.1, compaction 8.1 / 13.9; 128 of 128 12.6 / 17.2,
 // 12.6 / 14.0; 256 of 128 19.9 / 17.1, 20.9 / 14.8; 512 of 128 31.8 / 18.0, 37.0 / 15.7).
 constexpr int kSmallPages = 1 << 16, kSmallWords = kSmallPages / 32, kSmallRows = 1024;
 constexpr int64_t kSmallEntries = 1 << 14;
@@ -186,10 +186,14 @@ __device__ Int scan_1024(Int v, Int *total)
 {
     __shared__ Int sums[16];
     const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
+    if constexpr (sizeof(Int) == 4) {
+        v = dev::wave_scan(v);
+    } else {
 #pragma unroll
-    for (int m = 1; m < kWave; m *= 2) {
-        const Int u = __shfl_up(v, m);
-        v += lane >= m ? u : 0;
+        for (int m = 1; m < kWave; m *= 2) {
+            const Int u = __shfl_up(v, m);
+            v += lane >= m ? u : 0;
+        }
     }
     __syncthreads();
     if (lane == kWave - 1) {
@@ -628,7 +632,14 @@ __global__ __launch_bounds__(1024) void compact_small(CacheCompactArgs a)
         held[me] = held_pages(a, me);
     }
     __syncthreads();
-    const auto load = [&](int j, int r0, int step, int (&page)[kSmallBatch]) {
+    int page[kSmallBatch];
+    int pageColumn = -1, pageRow = -1;  // the cells of `page`: the last ones marked, for most the only ones
+    const auto load = [&](int j, int r0, int step) {
+        if (j == pageColumn && r0 == pageRow) {
+            return;
+        }
+        pageColumn = j;
+        pageRow = r0;
 #pragma unroll
         for (int n = 0; n < kSmallBatch; ++n) {
             const int r = r0 + n * step;
@@ -636,8 +647,7 @@ __global__ __launch_bounds__(1024) void compact_small(CacheCompactArgs a)
         }
     };
     each_cells(a.rows, a.width, [&](int j, int r, int step) {
-        int page[kSmallBatch];
-        load(j, r, step, page);
+        load(j, r, step);
         mark_all(page, used, nullptr);
     });
     __syncthreads();
@@ -665,8 +675,7 @@ __global__ __launch_bounds__(1024) void compact_small(CacheCompactArgs a)
     }
     __syncthreads();
     each_cells(a.rows, a.width, [&](int j, int r0, int step) {
-        int page[kSmallBatch];
-        load(j, r0, step, page);
+        load(j, r0, step);
 #pragma unroll
         for (int n = 0; n < kSmallBatch; ++n) {
             if (r0 + n * step < a.rows) {

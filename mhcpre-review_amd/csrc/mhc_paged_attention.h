@@ -165,18 +165,6 @@ struct Keys {
     }
 };
 
-// Inclusive scan over the wave, all lanes active.
-__device__ __forceinline__ int wave_scan(int v)
-{
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15: rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast 31: rows 2 and 3
-    return v;
-}
-
 __device__ __forceinline__ int64_t shfl64(int64_t v, int lane)
 {
     const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)v, lane), hi = (uint32_t)__shfl((int)(v >> 32), lane);
@@ -351,11 +339,11 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
     } else {
         const uint32_t replay = threadIdx.x == 0 ? dev::replay_load(args.tag.words, w) : 0u;
         const int firstLength = a.lengths[lane < a.B ? lane : 0];
-        const int firstUnits = lane < a.B ? Keys(a, firstLength, kPer).units : 0, firstUpto = wave_scan(firstUnits);
+        const int firstUnits = lane < a.B ? Keys(a, firstLength, kPer).units : 0, firstUpto = dev::wave_scan(firstUnits);
         int all = __builtin_amdgcn_readlane(firstUpto, kWave - 1);
         for (int b0 = kWave; b0 < a.B; b0 += kWave) {
             const int x = b0 + lane, L = a.lengths[x < a.B ? x : 0];
-            all += __builtin_amdgcn_readlane(wave_scan(x < a.B ? Keys(a, L, kPer).units : 0), kWave - 1);
+            all += __builtin_amdgcn_readlane(dev::wave_scan(x < a.B ? Keys(a, L, kPer).units : 0), kWave - 1);
         }
         shares = Shares(all * perRow, args.most);
         if (threadIdx.x == 0) {
@@ -382,7 +370,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
             b0 += kWave;
             L = a.lengths[b0 + lane < a.B ? b0 + lane : 0];
             units = b0 + lane < a.B ? Keys(a, L, kPer).units : 0;
-            upto = wave_scan(units);
+            upto = dev::wave_scan(units);
         }
         first.b = b;
         first.keys = Keys(a, length, kPer);
