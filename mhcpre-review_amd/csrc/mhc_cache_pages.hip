@@ -8,12 +8,12 @@
 // bits.  The counts up to every group of words are kept in LDS.
 //
 // Bound: latencies.  Up to some entries one workgroup does all of it (64 rows of 128
-// entries, us: 9.4, compaction 8.1); above, each launch waits for the one before.
+// entries, us: 8.7, compaction 7.7); above, each launch waits for the one before.
 // 1000 rows of up to 2048 entries, 200001 pages, us: clearing the bitmaps 2.0, marking
 // and the columns that stay 11.1 (about 6 of it the atomics, which go past the L2s, for
-// every XCD marks), who gets pages 6.2, the columns that change 3.4; compaction 2.0,
-// 7.8 and 12.0.  What they read and write is 9 MB, 1.6 us.  Copies are bound by the memory:
-// 2000 pages of 128 KB twice, read and written, 198 us (5.3 TB/s).
+// every XCD marks), who gets pages 6.0, the columns that change 3.3; compaction 1.9,
+// 7.6 and 12.0.  What they read and write is 9 MB, 1.6 us.  Copies are bound by the memory:
+// 2000 pages of 128 KB twice, read and written, 194 us (5.4 TB/s).
 
 #include "mhc_pre_device.h"
 #include "mhc_serve_internal.h"
