@@ -11,7 +11,7 @@
 // one joins them, in the order of the keys (many of them in spans first, each
 // joined by its own last workgroup).  Nobody waits.  What tells this
 // launch's counts from what the workspace held before is the launch's tag
-// (LaunchTag).
+// (LaunchTag); a count that is complete is taken away.
 //
 // In a unit each of the 4 waves has 32 keys of its own.  The scores are S^T =
 // K Q^T, 16 keys by 16 query heads (a wave's K rows go straight from memory to
@@ -91,7 +91,10 @@ struct Args {
 // RT][D], maxima (base 2) and sums [16 RT][2]; and an 8-byte word, of those of
 // the parts that are joined together the first one's, that counts the parts that are
 // there: its upper 52 bits are the launch's and the place's, so that the first to come
-// sees that the word is not yet this launch's and sets it to none.  Many parts are
+// sees that the word is not yet this launch's and sets it to none.  The last to come
+// sets it to 0: a captured launch's tag returns after 2048 replays, and which words a
+// replay uses goes by its lengths, so one that still held an old count under the same
+// tag would be taken for this replay's.  Many parts are
 // joined in spans: a span's result takes the place of its first output, its maxima,
 // sums and word are a second [2 * most] ones.  All of it is stored through to memory
 // and read from there: the reader may be on another XCD.
@@ -108,15 +111,21 @@ struct Parts {
     {
     }
     static constexpr uint64_t kCount = 0xFFF;
-    // Counts a part at the word, which was found as `found`; how many were there.
-    __device__ int count(uint32_t tag, int slot, uint64_t found) const
+    // Counts one of `all` parts at the word, which was found as `found`; whether it is the
+    // last.
+    __device__ bool count(uint32_t tag, int slot, uint64_t found, int all) const
     {
         const uint64_t none = sign(tag, slot);
         if ((found & ~kCount) != none) {  // (fails where another workgroup was first)
             (void)__hip_atomic_compare_exchange_strong(words + slot, &found, none, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
                                                        __HIP_MEMORY_SCOPE_AGENT);
         }
-        return (int)(__hip_atomic_fetch_add(words + slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) & kCount);
+        const uint64_t before = __hip_atomic_fetch_add(words + slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = (int)(before & kCount) == all - 1;
+        if (last) {
+            __hip_atomic_store(words + slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        return last;
     }
     __device__ uint64_t word(int slot) const
     {
@@ -691,7 +700,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
     if (wave == 0 && lane < 2) {
         bool all = false;
         if (left[lane].on) {
-            all = parts.count(tag, wordSlot, found_word) == left[lane].span_last(w) - left[lane].span_first(w);
+            all = parts.count(tag, wordSlot, found_word, left[lane].span_last(w) - left[lane].span_first(w) + 1);
         }
         complete[lane] = all;
     }
@@ -806,7 +815,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (threadIdx.x == 0) {
-            spansComplete = parts.count(tag, slot, found) == part.spans() - 1;
+            spansComplete = parts.count(tag, slot, found, part.spans());
         }
         __syncthreads();
         if (spansComplete) {

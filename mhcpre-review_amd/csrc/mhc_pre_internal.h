@@ -42,8 +42,10 @@ constexpr size_t kWsHeaderBytes = kWsReplayOff + 4 * kMaxExchangeGrid;
 // captured ones (`seed`, its upper 21 bits, 10 the highest two) and one word per
 // workgroup, equal in all of them, to which each replay adds one; the lower 11
 // bits are that count's, for a replay finds at its own places what the one
-// before it left there.  Without such words of its own, a node before the
-// launch sets words of the workspace to a whole number (11 the highest bits).
+// before it left there (a kernel that does not write the same places in every
+// replay has to leave none of its tags there).  Without such words of its own, a
+// node before the launch sets words of the workspace to a whole number (11 the
+// highest bits).
 struct LaunchTag {
     uint32_t seed = 0;
     uint32_t *words = nullptr;
