@@ -20,8 +20,11 @@
 // P^T: the order of the keys within a product is free.  V goes through LDS,
 // rows as they come, and is read transposed (ds_read_b64_tr_b16); the region is
 // the wave's own, so the loop has no barrier.  The probabilities are split into
-// hi + lo of the 16-bit type: a weight in 8 bits alone would add an error as
-// large as the output's own rounding, and the matrix cores have time.
+// hi + lo of the 16-bit type, 16 bits in bf16 and 22 in fp16: a weight in 8 bits
+// alone would add an error as large as the output's own rounding, and the matrix
+// cores have time.  fp16 ends at 2^-24, so there they are lifted by 2^15 (at most
+// 32768): a weight keeps 16 bits down to 2^-24 of the largest and is lost below
+// 2^-40, where 131072 keys in all are 2^-23 of it.
 //
 // Bound: the cache is read once, 4 bytes a value pair for at most 4 * 16
 // flops, so the memory's rate decides (6.05 TB/s for a cold read of two
@@ -47,6 +50,11 @@ constexpr int kWaves = 4;
 constexpr int kTile = 32;               // keys of a wave at a time
 constexpr int kUnit = kWaves * kTile;   // keys of a unit
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+
+// What the probabilities, and with them the outputs' sums (not the weights' sums), are
+// multiplied by until they are put out.
+template <bool kBf16>
+constexpr float kLift = kBf16 ? 1.f : 32768.f;
 
 // Workgroups that a CU's registers hold.  A product with 32 query heads reads the cache once
 // where two with 16 read it twice: 64 rows of 8192 keys, 32 heads to one, us, 32 at a
@@ -257,7 +265,7 @@ template <bool kBf16>
 __device__ __forceinline__ void finish(const PagedAttentionArgs &a, int b, int head, int e, f32x4_t all, float top,
                                        float total)
 {
-    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const float inv = total == 0.f ? 0.f : 1.f / kLift<kBf16> / total;
     uint16_t *out = static_cast<uint16_t *>(a.out.data) + b * a.out.row + head * a.out.head + e;
     *reinterpret_cast<u32x2_t *>(out) =
         u32x2_t{dev::pack2_x<kBf16>(all[0] * inv, all[1] * inv), dev::pack2_x<kBf16>(all[2] * inv, all[3] * inv)};
@@ -577,7 +585,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                 sum[rt] += part;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float p0 = x[2 * e], p1 = x[2 * e + 1];
+                    const float p0 = x[2 * e] * kLift<kBf16>, p1 = x[2 * e + 1] * kLift<kBf16>;
                     const uint32_t h = dev::pack2_x<kBf16>(p0, p1);
                     hi[rt][e] = h;
                     lo[rt][e] = dev::pack2_x<kBf16>(p0 - dev::x_to_f32<kBf16>(h & 0xFFFFu),

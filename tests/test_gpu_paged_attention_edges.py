@@ -4,6 +4,8 @@ from __future__ import annotations
 import pytest
 import torch
 
+import serve_ref as ref
+
 pytestmark = pytest.mark.gpu
 
 
@@ -39,3 +41,54 @@ def test_counts_of_old_replays_are_gone(pkg, ops, device, heads, kv_heads, first
         torch.cuda.synchronize()
         want = ops.paged_attention(q, k, v, table, lengths)
         assert torch.equal(op.out, want[0]) and torch.equal(op.lse, want[1]), n
+
+
+def _near(out, lse, want):
+    w_out, w_lse, b_out, b_lse = want
+    off, l_off = (out.cpu().double() - w_out).abs(), (lse.cpu().double() - w_lse).abs()
+    assert (off <= b_out).all(), f"out: {(off / b_out).max():.3g} of its bound"
+    assert (l_off <= b_lse).all(), f"lse: {(l_off / b_lse).max():.3g} of its bound"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gap", [8, 12, 14, 15, 16, 17, 18, 24])
+@pytest.mark.parametrize("B,heads,kv_heads,d,n", [
+    (600, 2, 1, 64, 512),  # each wave alone
+    (1, 2, 1, 64, 8192), (1, 4, 4, 96, 700), (2, 32, 1, 128, 8192), (1, 16, 1, 256, 4000)])
+def test_one_key_far_above_the_others(ops, device, B, heads, kv_heads, d, n, gap, dtype):
+    """A key whose score is `gap` above the others' and whose value is 0: the output is the sum of many small weights.
+    The bound is serve_ref's: a weight's error is 2^-16 of it where it is at least 2^-24 of the largest; below that
+    8192 keys' errors of 2^-40 and values up to 4 are less than half of the type's smallest spacing."""
+    g = torch.Generator().manual_seed(gap * n + d)
+    page = 16
+    pages = -(-n // page)
+    q = 0.02 * torch.randn(1, heads, d, generator=g)
+    k, v = torch.randn(pages, page, kv_heads, d, generator=g), torch.randn(pages, page, kv_heads, d, generator=g)
+    v.clamp_(-4, 4)
+    q[..., 0] = 1
+    k[..., 0] = 0
+    at = n // 3
+    k[at // page, at % page] = 0
+    k[at // page, at % page, :, 0] = gap
+    v[at // page, at % page] = 0
+    q, k, v = (x.to(dtype).to(device) for x in (q, k, v))
+    table = torch.arange(pages, dtype=torch.int32, device=device).view(1, -1)
+    lengths = torch.tensor([n], dtype=torch.int32, device=device)
+    out, lse = ops.paged_attention(q.expand(B, -1, -1).contiguous(), k, v, table.expand(B, -1).contiguous(),
+                                   lengths.expand(B).contiguous(), 1.0)
+    _near(out[-1:], lse[-1:], ref.attention(q, k, v, table, lengths, 1.0))
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.0, -0.125])
+@pytest.mark.parametrize("B", [1, 300])
+def test_extreme_scores_in_fp16(ops, device, B, scale):
+    """Scores hundreds apart, equal ones, and the order turned round."""
+    g = torch.Generator().manual_seed(B)
+    q = 30 * torch.randn(1, 4, 64, generator=g)
+    k, v = torch.randn(33, 16, 2, 64, generator=g), 100 * torch.randn(33, 16, 2, 64, generator=g)
+    q, k, v = (x.half().to(device) for x in (q, k, v))
+    table = torch.arange(32, dtype=torch.int32, device=device).view(1, -1)
+    lengths = torch.tensor([509], dtype=torch.int32, device=device)
+    out, lse = ops.paged_attention(q.expand(B, -1, -1).contiguous(), k, v, table.expand(B, -1).contiguous(),
+                                   lengths.expand(B).contiguous(), scale)
+    _near(out[-1:], lse[-1:], ref.attention(q, k, v, table, lengths, scale))
