@@ -178,7 +178,7 @@ struct Keys {
         low = a.window > 0 && L > a.window ? L - (int)a.window : 0;
         high = L;
         first = low / unit;
-        units = high > low ? (high + unit - 1) / unit - first : 1;
+        units = high > low ? (high - 1) / unit + 1 - first : 1;  // (high may be 2^31 - 1)
     }
 };
 

@@ -1,6 +1,8 @@
 """paged_attention where it could go wrong unseen: long-lived graphs, scores and values at the ends of their types."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -92,3 +94,25 @@ def test_extreme_scores_in_fp16(ops, device, B, scale):
     out, lse = ops.paged_attention(q.expand(B, -1, -1).contiguous(), k, v, table.expand(B, -1).contiguous(),
                                    lengths.expand(B).contiguous(), scale)
     _near(out[-1:], lse[-1:], ref.attention(q, k, v, table, lengths, scale))
+
+
+def test_the_longest_rows_there_may_be(ops, device):
+    """2^31 - 2 keys in two pages whose slots are one and the same memory.  The window's keys are equal but for the
+    last case's 50 from the page before (weights of e^-9 beside 2^30 of 1); lse is off by at most eight roundings."""
+    page = 2 ** 30 - 1
+    rows = torch.zeros(2, 2, 1, 1, 32)
+    rows[0, 1, ..., 0], rows[0, 0, ..., 0] = 16, -2  # scores 8 and -1
+    rows[1] = torch.arange(64).view(2, 1, 1, 32)
+    k, v = (r.to(torch.bfloat16).to(device).expand(2, page, 1, 32) for r in rows)
+    q = torch.zeros(1, 1, 32, dtype=torch.bfloat16, device=device)
+    q[..., 0] = 1
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device=device)
+    for length, window, keys in ((2 * page, 100, 100), (2 * page, 1, 1), (2 ** 31 - 1, 1000, 1000),
+                                 (2 * page, page + 50, page)):
+        lengths = torch.tensor([length], dtype=torch.int32, device=device)
+        out, lse = ops.paged_attention(q, k, v, table, lengths, 0.5, window)
+        assert torch.equal(out[0, 0], v[1, 0, 0])
+        want = 8 + math.log(keys)
+        assert abs(float(lse) - want) <= 8 * 2.0 ** -24 * (1 + want)
+    out, lse = ops.paged_attention(q, k, v, torch.full_like(table, -1), lengths, 0.5)  # holes only
+    assert (out == 0).all() and torch.isneginf(lse).all()
