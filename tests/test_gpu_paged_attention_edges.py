@@ -116,3 +116,54 @@ def test_the_longest_rows_there_may_be(ops, device):
         assert abs(float(lse) - want) <= 8 * 2.0 ** -24 * (1 + want)
     out, lse = ops.paged_attention(q, k, v, torch.full_like(table, -1), lengths, 0.5)  # holes only
     assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,heads,kv_heads,d,n", [(1, 2, 1, 64, 1), (600, 2, 1, 64, 100), (1, 4, 2, 96, 3000),
+                                                  (2, 32, 1, 128, 300), (1, 5, 1, 256, 700)])
+def test_infinite_and_nan_values(ops, device, B, heads, kv_heads, d, n, dtype):
+    """A value that a row sees is infinite or NaN: so is the output's column, and no other one."""
+    g = torch.Generator().manual_seed(n + d)
+    page = 16
+    pages = -(-n // page) + 1
+    q = torch.randn(1, heads, d, generator=g)
+    k, v = torch.randn(pages, page, kv_heads, d, generator=g), torch.randn(pages, page, kv_heads, d, generator=g)
+    finite = v.clone()
+
+    def put(t, column, value):
+        v[t // page, t % page, :, column], finite[t // page, t % page, :, column] = value, 0
+
+    put(n // 3, 3, math.inf)
+    put(n // 2, 17, -math.inf)
+    put(n - 1, d - 1, math.nan)
+    put(0, 9, math.inf)
+    put(n - 1, 9, math.inf)
+    put(0, 12, -math.inf if n == 1 else math.inf)
+    if n > 1:
+        put(n - 1, 12, -math.inf)
+    v[pages - 1], finite[pages - 1] = math.nan, 0  # nobody's
+    q, k, v, finite = (x.to(dtype).to(device) for x in (q, k, v, finite))
+    table = torch.arange(pages - 1, dtype=torch.int32, device=device).view(1, -1)
+    lengths = torch.tensor([n], dtype=torch.int32, device=device)
+    out, lse = ops.paged_attention(q.expand(B, -1, -1).contiguous(), k, v, table.expand(B, -1).contiguous(),
+                                   lengths.expand(B).contiguous())
+    last = out[-1].cpu().double()
+    assert (last[:, 3] == math.inf).all() and (last[:, 17] == -math.inf).all() and torch.isnan(last[:, d - 1]).all()
+    assert (last[:, 9] == math.inf).all()
+    assert (last[:, 12] == -math.inf).all() if n == 1 else torch.isnan(last[:, 12]).all()
+    want = ref.attention(q, k, finite, table, lengths, d ** -0.5)
+    rest = [c for c in range(d) if c not in (3, 9, 12, 17, d - 1)]
+    _near(out[-1:, :, rest], lse[-1:], (want[0][..., rest], want[1], want[2][..., rest], want[3]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_infinite_value_of_a_small_weight(ops, device, dtype):
+    """A weight of e^-40 beside the largest is not 0 in 32 bits: its infinite value reaches the output."""
+    q = torch.zeros(1, 2, 64)
+    q[..., 0] = 1
+    k, v = torch.zeros(4, 16, 1, 64), torch.ones(4, 16, 1, 64)
+    k[1, 2, 0, 0], v[3, 5, 0, 7], v[3, 5, 0, 8] = 40, math.inf, -math.inf
+    q, k, v = (x.to(dtype).to(device) for x in (q, k, v))
+    table = torch.arange(4, dtype=torch.int32, device=device).view(1, -1)
+    out, _ = ops.paged_attention(q, k, v, table, torch.tensor([64], dtype=torch.int32, device=device), 1.0)
+    assert (out[0, :, 7] == math.inf).all() and (out[0, :, 8] == -math.inf).all() and (out[0, :, :7] == 1).all()
