@@ -19,13 +19,15 @@
 // probabilities are, as they lie in its registers, the operand of O^T = V^T
 // P^T: the order of the keys within a product is free.  V goes through LDS,
 // rows as they come, and is read transposed (ds_read_b64_tr_b16); the region is
-// the wave's own, so the loop has no barrier.  The probabilities are split into
-// hi + lo of the 16-bit type, 16 bits in bf16 and 22 in fp16: a weight in 8 bits
-// alone would add an error as large as the output's own rounding, and the matrix
-// cores have time.  fp16 ends at 2^-24, so there they are lifted by 2^15 (at most
-// 32768): a weight keeps 16 bits down to 2^-24 of the largest and is 2^-39 where it
-// is less, of which 131072 keys' are 2^-22 of it.  hi is cut, not rounded, and lo is
-// above 0 wherever the weight is: with lo at 0 or below, an infinite value would
+// the wave's own, so the loop has no barrier.  A probability is the sum of as many
+// 16-bit terms as hold it, three in bf16 (24 bits) and two in fp16 (21): one alone
+// would add an error as large as the output's own rounding, two of bf16 an error of
+// 2^-16 that shows where values cancel; the matrix cores have time (32 bf16 heads of
+// 128 at a time 51.7 us with two, 54.5 with three; all else the same).  fp16 ends at
+// 2^-24, so there they are lifted by 2^15 (at most 32768): a weight keeps 16 bits down
+// to 2^-24 of the largest and is 2^-39 where it is less, of which 131072 keys' are
+// 2^-22 of it.  All terms but the last are cut, not rounded, and all but the first are
+// above 0 wherever the weight is: with one at 0 or below, an infinite value would
 // come out as NaN.  (Looking for such values in every tile instead took 10% of the
 // time with 32 heads at a time, 3% of one short row's.)
 //
@@ -58,6 +60,10 @@ constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 // multiplied by until they are put out.
 template <bool kBf16>
 constexpr float kLift = kBf16 ? 1.f : 32768.f;
+
+// The 16-bit terms of a probability.
+template <bool kBf16>
+constexpr int kTerms = kBf16 ? 3 : 2;
 
 // Workgroups that a CU's registers hold.  A product with 32 query heads reads the cache once
 // where two with 16 read it twice: 64 rows of 8192 keys, 32 heads to one, us, 32 at a
@@ -568,7 +574,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
             found = find_page();
         }
         if (seen != 0u) {
-            u32x4_t hi[RT], lo[RT];
+            u32x4_t p[RT][kTerms<kBf16>];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 float x[8], most = -INFINITY;
@@ -609,11 +615,15 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float p0 = x[2 * e] * kLift<kBf16>, p1 = x[2 * e + 1] * kLift<kBf16>;
-                    const uint32_t h = cut2<kBf16>(p0, p1);
-                    hi[rt][e] = h;
-                    lo[rt][e] = at_least(dev::pack2_x<kBf16>(p0 - dev::x_to_f32<kBf16>(h & 0xFFFFu),
-                                                             p1 - dev::x_to_f32<kBf16>(h >> 16)),
-                                         p0, p1);
+                    float rest0 = p0, rest1 = p1;
+#pragma unroll
+                    for (int n = 0; n < kTerms<kBf16>; ++n) {
+                        const uint32_t h =
+                            n + 1 < kTerms<kBf16> ? cut2<kBf16>(rest0, rest1) : dev::pack2_x<kBf16>(rest0, rest1);
+                        p[rt][n][e] = n == 0 ? h : at_least(h, p0, p1);
+                        rest0 -= dev::x_to_f32<kBf16>(h & 0xFFFFu);
+                        rest1 -= dev::x_to_f32<kBf16>(h >> 16);
+                    }
                 }
             }
 #pragma unroll
@@ -623,8 +633,10 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                 const u32x4_t vt = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    o[rt][j] = mfma32<kBf16>(vt, hi[rt], o[rt][j]);
-                    o[rt][j] = mfma32<kBf16>(vt, lo[rt], o[rt][j]);
+#pragma unroll
+                    for (int n = 0; n < kTerms<kBf16>; ++n) {
+                        o[rt][j] = mfma32<kBf16>(vt, p[rt][n], o[rt][j]);
+                    }
                 }
             }
         }

@@ -167,3 +167,29 @@ def test_infinite_value_of_a_small_weight(ops, device, dtype):
     table = torch.arange(4, dtype=torch.int32, device=device).view(1, -1)
     out, _ = ops.paged_attention(q, k, v, table, torch.tensor([64], dtype=torch.int32, device=device), 1.0)
     assert (out[0, :, 7] == math.inf).all() and (out[0, :, 8] == -math.inf).all() and (out[0, :, :7] == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("copies,heads", [(40, 1), (1, 3), (1, 20)])
+def test_values_that_cancel(ops, device, copies, heads, dtype):
+    """Three keys of values 1, -1 and -1 whose weights nearly cancel (1 = a + b but for 2^-11): what is left shows the
+    bits that the weights are held in.  The bound: 16 roundings of 32 bits (score, exp, sums, product, quotient) of the
+    values' size, 1, and the type's."""
+    scores = torch.cat([2.0 ** i * (1 + torch.arange(128, dtype=torch.float64) / 128) for i in (-2, -1, 0)])
+    left = 1 - torch.exp(-scores)[:, None] - torch.exp(-scores)
+    a, b = torch.nonzero(left.abs() < 2.0 ** -11, as_tuple=True)
+    assert len(a) > 50
+    a, b = a.repeat(copies), b.repeat(copies)
+    B = len(a)
+    k, v = torch.zeros(B, 16, 1, 64), torch.zeros(B, 16, 1, 64)
+    k[:, 1, 0, 0], k[:, 2, 0, 0] = -scores[a].float(), -scores[b].float()
+    v[:, 0], v[:, 1:3] = 1, -1
+    q = torch.zeros(B, heads, 64)
+    q[..., 0] = 1
+    table, lengths = torch.arange(B).int().view(B, 1), torch.full((B,), 3, dtype=torch.int32)
+    q, k, v = (x.to(dtype).to(device) for x in (q, k, v))
+    out, _ = ops.paged_attention(q, k, v, table.to(device), lengths.to(device), 1.0)
+    want = (left[a, b] / (2 - left[a, b]))[:, None, None].expand(B, heads, 64)
+    bound = 16 * 2.0 ** -24 + ref.ROUND[dtype] * want.abs() + ref.TINY[dtype]
+    off = (out.cpu().double() - want).abs()
+    assert (off <= bound).all(), f"{(off / bound).max():.3g} of its bound"
