@@ -114,17 +114,21 @@ def rotary_frequencies(rot: int, base: float = 10000.0, kind: str = "plain", fac
 
 
 class _ServeOp:
-    """An executor, its workspace and the tensors that it is bound to."""
+    """An executor, its workspace and the tensors that it is bound to, which are
+    all on one GPU (ValueError otherwise: the kernels get their addresses)."""
 
     _name = ""
 
     def _create(self, args, tensors, workspace=None):
         import torch
 
-        self.lib = load_serve_library()
+        self.executor = ctypes.c_void_p(None)
         self._keep = [t for t in tensors if t is not None]
         device = self._keep[0].device
-        self.executor = ctypes.c_void_p(None)
+        for t in self._keep + ([workspace] if workspace is not None else []):
+            if not t.is_cuda or t.device != device:
+                raise ValueError(f"{self._name}: tensors must be on one GPU, not on {device} and {t.device}")
+        self.lib = load_serve_library()
         ws = ctypes.c_uint64(0)
         by_ref = [ctypes.byref(a) if isinstance(a, ctypes.Structure) else a for a in args]
         phase1 = getattr(self.lib, self._name + "GetWorkspaceSize")
@@ -183,7 +187,7 @@ class QkNormRopeOp(_ServeOp):
         self._create([_strided(q), _strided(k), _strided(v), _dense(positions), _dense(inv_freq), _dense(q_weight),
                       _dense(k_weight), eps, int(interleaved), amplitude, _dense(slots), _strided(self.q_out),
                       _strided(k_out), _strided(k_cache), _strided(v_cache)],
-                     [q, k, v, positions, inv_freq, q_weight, k_weight, slots, k_cache, v_cache])
+                     [q, k, v, positions, inv_freq, q_weight, k_weight, slots, k_cache, v_cache, self.q_out, k_out])
 
 
 class PagedAttentionOp(_ServeOp):
@@ -202,8 +206,8 @@ class PagedAttentionOp(_ServeOp):
         self.lse = lse if lse is not False else None
         scale = q.shape[-1] ** -0.5 if scale is None else scale
         self._create([_strided(q), _strided(k_cache), _strided(v_cache), _dense(page_table), _dense(lengths), scale,
-                      window, _strided(self.out), _dense(self.lse)], [q, k_cache, v_cache, page_table, lengths],
-                     workspace)
+                      window, _strided(self.out), _dense(self.lse)],
+                     [q, k_cache, v_cache, page_table, lengths, self.out, self.lse], workspace)
 
 
 class CacheUpdateOp(_ServeOp):
@@ -225,7 +229,9 @@ class CacheUpdateOp(_ServeOp):
         self.granted, self.src, self.dst = (torch.empty(rows, **i32) for _ in range(3))
         self._create([_dense(page_table), _dense(lengths), _dense(parents), _dense(counts), pages, page_size,
                       _dense(self.new_table), _dense(self.new_lengths), _dense(self.slots), _dense(self.granted),
-                      _dense(self.src), _dense(self.dst)], [page_table, lengths, parents, counts], workspace)
+                      _dense(self.src), _dense(self.dst)],
+                     [page_table, lengths, parents, counts, self.new_table, self.new_lengths, self.slots, self.granted,
+                      self.src, self.dst], workspace)
 
 
 class CacheCompactOp(_ServeOp):
@@ -241,7 +247,8 @@ class CacheCompactOp(_ServeOp):
         self.src, self.dst = torch.empty(pages // 2, **i32), torch.empty(pages // 2, **i32)
         self.used = torch.empty(1, **i32)
         self._create([_dense(page_table), _dense(lengths), pages, page_size, _dense(self.new_table), _dense(self.src),
-                      _dense(self.dst), _dense(self.used)], [page_table, lengths], workspace)
+                      _dense(self.dst), _dense(self.used)],
+                     [page_table, lengths, self.new_table, self.src, self.dst, self.used], workspace)
 
 
 class CopyPagesOp(_ServeOp):
