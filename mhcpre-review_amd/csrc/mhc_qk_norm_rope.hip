@@ -163,6 +163,14 @@ __device__ __forceinline__ float group_sum(float v)
     return v;
 }
 
+// 1 / sqrt(v): the instruction takes values below the normal ones for 0, which a tiny row's mean
+// square is where eps is as small.
+__device__ __forceinline__ float rsqrt_any(float v)
+{
+    const bool tiny = v < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(tiny ? v * 0x1p100f : v) * (tiny ? 0x1p50f : 1.f);
+}
+
 constexpr int kSteps = 4;
 
 struct Split {
@@ -228,7 +236,7 @@ __global__ __launch_bounds__(256) void norm_rope_pieces(NormRopeArgs a, Split sp
                     sum = __builtin_fmaf(u[j], u[j], sum);
                     sum = __builtin_fmaf(v[j], v[j], sum);
                 }
-                const float inv = __builtin_amdgcn_rsqf(group_sum<L>(sum) * perValue + a.eps);
+                const float inv = rsqrt_any(group_sum<L>(sum) * perValue + a.eps);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     u[j] *= inv * w[j];
