@@ -43,6 +43,9 @@ __device__ __forceinline__ int pages_for(uint32_t tokens, int pageSize)
     return tokens == 0 ? 0 : (int)((tokens - 1) / (uint32_t)pageSize) + 1;
 }
 
+// A column of a table, or one some steps beyond the last: a table may have 2^31 - 1.
+typedef uint32_t Column;
+
 // Row r of mhcCacheUpdate: what it goes on from and what it asks for.
 struct Row {
     int parent;       // row of the old table, or -1
@@ -62,8 +65,9 @@ struct Row {
         rest = length - full * a.pageSize;
         held = full + (rest > 0 ? 1 : 0);
         add = clamped(a.counts[r], a.tokens);
-        grown = full + pages_for((uint32_t)rest + (uint32_t)add, a.pageSize);
-        if (grown > a.width) {
+        const int64_t wanted = (int64_t)full + pages_for((uint32_t)rest + (uint32_t)add, a.pageSize);
+        grown = (int)wanted;
+        if (wanted > a.width) {
             add = 0;
             grown = held;
         }
@@ -78,7 +82,7 @@ struct Row {
     }
     // The same where `on`, else -1: a load in any case (of the table's first entry), so that
     // a batch of them has no branches and all are on their way before the first is used.
-    __device__ int entry_if(const CacheUpdateArgs &a, int j, bool on) const
+    __device__ int entry_if(const CacheUpdateArgs &a, Column j, bool on) const
     {
         const int page = a.table[on ? (int64_t)parent * a.width + j : 0];
         return on && page >= 0 && page < a.pages ? page : -1;
@@ -137,21 +141,22 @@ __global__ __launch_bounds__(256) void update_rows(CacheUpdateArgs a, uint32_t *
         found[r] = Found{row, row.add > 0 && row.rest > 0 ? row.entry(a, row.held - 1) : -1};
     }
     int32_t *out = a.newTable + r * a.width;
-    for (int j0 = (int)threadIdx.x; j0 < a.width; j0 += 256 * kBatch) {
+    const Column width = (Column)a.width, held = (Column)row.held, open = (Column)row.open, end = (Column)row.end;
+    for (Column j0 = threadIdx.x; j0 < width; j0 += 256 * kBatch) {
         int page[kBatch];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
-            const int j = j0 + 256 * n;
-            page[n] = row.entry_if(a, j, j < row.held);
+            const Column j = j0 + 256 * n;
+            page[n] = row.entry_if(a, j, j < held);
         }
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
-            const int j = j0 + 256 * n;
-            if (j < a.width && (j < row.open || j >= row.end)) {
+            const Column j = j0 + 256 * n;
+            if (j < width && (j < open || j >= end)) {
                 out[j] = page[n];
             }
         }
-        if (j0 - (int)threadIdx.x < row.held) {
+        if (j0 - threadIdx.x < held) {
             mark_all(page, used, many);
         }
     }
@@ -407,8 +412,8 @@ __global__ __launch_bounds__(256) void update_finish(CacheUpdateArgs a, const Fo
         }
         return copy ? mine[0] : last;
     };
-    for (int j = row.open + lane; j < row.end; j += kWave) {
-        a.newTable[r * a.width + j] = column(j);
+    for (Column j = (Column)row.open + lane; j < (Column)row.end; j += kWave) {
+        a.newTable[r * a.width + j] = column((int)j);
     }
     const int granted = served ? row.add : 0;
     for (int i = lane; i < a.tokens; i += kWave) {
@@ -525,7 +530,7 @@ __device__ __forceinline__ int held_pages(const CacheCompactArgs &a, int64_t r)
 }
 
 // (A load in any case, as Row::entry_if's.)
-__device__ __forceinline__ int held_entry(const CacheCompactArgs &a, int64_t r, int j, bool on)
+__device__ __forceinline__ int held_entry(const CacheCompactArgs &a, int64_t r, Column j, bool on)
 {
     const int page = a.table[on ? r * a.width + j : 0];
     return on && page >= 0 && page < a.pages ? page : -1;
@@ -534,8 +539,8 @@ __device__ __forceinline__ int held_entry(const CacheCompactArgs &a, int64_t r, 
 __global__ __launch_bounds__(256) void compact_mark(CacheCompactArgs a, uint32_t *used)
 {
     const int64_t r = blockIdx.x;
-    const int held = held_pages(a, r);
-    for (int j0 = (int)threadIdx.x; j0 < held; j0 += 256 * kBatch) {
+    const Column held = (Column)held_pages(a, r);
+    for (Column j0 = threadIdx.x; j0 < held; j0 += 256 * kBatch) {
         int page[kBatch];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
@@ -554,14 +559,16 @@ __global__ __launch_bounds__(1024) void compact_apply(CacheCompactArgs a, const 
     __shared__ __align__(16) uint32_t copy[kOne ? kGroups : 4];
     __shared__ uint16_t starts[kOne ? kGroups : 1];
     constexpr int kPieces = 8, kColumns = kWave * kPieces;
-    const int pieces = (a.width + kColumns - 1) / kColumns;
+    const Column width = (Column)a.width;
+    const int pieces = (int)((width + kColumns - 1) / kColumns);
     const int64_t waves = 16 * (int64_t)gridDim.x;
     int64_t n = (int64_t)blockIdx.x * 16 + threadIdx.x / kWave, r = 0;
-    int j0 = 0, page[kPieces];
+    Column j0 = 0;
+    int page[kPieces];
     const auto load = [&]() {
         r = n / pieces;
-        j0 = (int)(n - r * pieces) * kColumns + (int)threadIdx.x % kWave;
-        const int held = r < a.rows ? held_pages(a, r) : 0;
+        j0 = (Column)(n - r * pieces) * kColumns + threadIdx.x % kWave;
+        const Column held = r < a.rows ? (Column)held_pages(a, r) : 0;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             page[i] = held > 0 ? held_entry(a, r, j0 + i * kWave, j0 + i * kWave < held) : -1;
@@ -591,7 +598,7 @@ __global__ __launch_bounds__(1024) void compact_apply(CacheCompactArgs a, const 
             if (page[i] >= U) {
                 page[i] = to(counts.rank(page[i]) - stay);
             }
-            if (r < a.rows && j0 + i * kWave < a.width) {
+            if (r < a.rows && j0 + i * kWave < width) {
                 a.newTable[r * a.width + j0 + i * kWave] = page[i];
             }
         }
