@@ -137,7 +137,10 @@ MHC_API int mhcRotaryFrequencies(int32_t rot, double base, int32_t kind, double 
  *   out = sum_t exp(s_t - lse) v_t,  lse = log sum_t exp(s_t)
  *
  * with query head h reading kv head h / (heads / kvHeads), in fp32, out rounded
- * once.  A row that sees no key (L = 0, holes only) has out 0 and lse -inf.
+ * once.  (In fp16 the weights are held in 21 bits, small ones to 2^-39 of the
+ * largest.)  A row that sees no key (L = 0, holes only) has out 0 and lse -inf.
+ * What a row does not see may be infinite or NaN; an infinite value that it sees
+ * is infinite in out.
  *
  *   q          fp16 | bf16   [B, heads, d]
  *   kCache, vCache  same     [pages, pageSize, kvHeads, d]
@@ -172,7 +175,8 @@ MHC_API int mhcPagedAttention(void *workspace, uint64_t workspaceSize, mhcServeE
  *   - A row that appends into a partly filled page that another row holds too
  *     gets a free page in its place: src[r] is the shared page, dst[r] the
  *     private one, whose contents the caller copies (mhcCacheCopyPages); else
- *     both are -1.
+ *     both are -1.  Where all rows that hold the page append, all of them get one
+ *     and the page itself falls free: a page and a copy more than they need.
  *   - Free pages are given out in ascending order, to rows in ascending order;
  *     within a row first the private copy, then the pages it grows by.
  *   - A row gets what it asked for (granted[r] = counts[r]) or, if the rows up

@@ -22,11 +22,11 @@
 // the wave's own, so the loop has no barrier.  A probability is the sum of as many
 // 16-bit terms as hold it, three in bf16 (24 bits) and two in fp16 (21): one alone
 // would add an error as large as the output's own rounding, two of bf16 an error of
-// 2^-16 that shows where values cancel; the matrix cores have time (32 bf16 heads of
-// 128 at a time 51.7 us with two, 54.5 with three; all else the same).  fp16 ends at
-// 2^-24, so there they are lifted by 2^15 (at most 32768): a weight keeps 16 bits down
-// to 2^-24 of the largest and is 2^-39 where it is less, of which 131072 keys' are
-// 2^-22 of it.  All terms but the last are cut, not rounded, and all but the first are
+// 2^-16 that shows where values cancel; the matrix cores have time (32 bf16 heads
+// at a time, with two / three, us: of 64 31 / 33, of 128 51.7 / 54.5; all else the
+// same). fp16 ends at 2^-24, so there they are lifted by 2^15 (at most 32768):
+// small weights are held to 2^-39 of the largest, of which 131072 keys' are 2^-22
+// of it.  All terms but the last are cut, not rounded, and all but the first are
 // above 0 wherever the weight is: with one at 0 or below, an infinite value would
 // come out as NaN.  (Looking for such values in every tile instead took 10% of the
 // time with 32 heads at a time, 3% of one short row's.)
@@ -34,11 +34,11 @@
 // Bound: the cache is read once, 4 bytes a value pair for at most 4 * 16
 // flops, so the memory's rate decides (6.05 TB/s for a cold read of two
 // tensors of 0.5 GB in the same pieces).  Measured: 64 rows of 1 to 8192 keys,
-// 32 heads to 8 of 128, 734 MB, 137 us (5.35 TB/s); 4 rows up to 131072 keys, 1007 MB,
-// 184 us (5.5 TB/s; 174.5 in a copy that leaves the join out).  The rest is the
-// start (the first pages' addresses and translations, about 8 us) and the join's
-// chain of store, count and load, about 3 us at the end; a row of few keys is
-// nothing but these (one row of 1000 keys, 9 us).
+// 32 heads to 8 of 128, 734 MB, 139 us (5.3 TB/s); 4 rows up to 131072 keys, 1007 MB,
+// 184 us (5.5 TB/s).  The rest is the start and the join.  The same launches with one
+// key a row take 7.2 us (a launch, lengths, pages, keys, output).  The join's chain of
+// store, count and load, left out in a copy, is 2.1 us of one row of 1000 keys
+// (9.2 in all), 2.8 of the 64 rows, 7 of the 4, whose 64 heads' parts are the largest.
 #pragma once
 
 #include "mhc_pre_device.h"
@@ -67,8 +67,8 @@ constexpr int kTerms = kBf16 ? 3 : 2;
 
 // Workgroups that a CU's registers hold.  A product with 32 query heads reads the cache once
 // where two with 16 read it twice: 64 rows of 8192 keys, 32 heads to one, us, 32 at a
-// time / 16: d = 64 31.4 / 45.2, 128 51.9 / 84.5, 192 88.6 / 121.0.  At d = 256 its
-// registers spill (285 / 166).
+// time / 16, bf16: d = 64 33 / 46, 128 54.5 / 85.4, 192 87 / 123; fp16: 31.2 / 45.4,
+// 51.5 / 84.7, 85.8 / 121.  At d = 256 its registers spill (285 / 166).
 constexpr int workgroups_per_cu(int d, bool wide) { return d <= (wide ? 64 : 128) ? 2 : 1; }
 constexpr int kWideMost = 192;  // the largest d with 32 query heads at a time
 
@@ -78,7 +78,7 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8v_t __attribute__((ext_vector_type(8)));
 
-// How the units are shared out: the same arithmetic in both launches.
+// How the units are shared out.
 struct Shares {
     int units, grid;  // all units; workgroups that have some (each has at least one)
 

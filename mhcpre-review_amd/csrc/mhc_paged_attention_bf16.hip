@@ -30,7 +30,9 @@ Args plan(const PagedAttentionArgs &a, int cus, bool &wide)
 // (8 kv heads of 128): 256 rows of 16 keys 20.9 / 8.7, 64 22.1 / 14.7, 256 57.2 / 51.6,
 // 512 101.5 / 97.2, of 1 to 256 36.2 / 34.9, with a window of 128 32.1 / 27.9; 1024 rows
 // of 32 72.3 / 34.5; but 64 rows (512 of them, a quarter of the waves) of 128 10.6 / 11.7,
-// of 512 27.8 / 41.8.
+// of 512 27.8 / 41.8.  The lengths are on the device, so the rule goes by the table: short
+// rows in a table of a long context's width are shared out in units like long ones (256 rows
+// of 16 keys, width 1 / 512 pages of 16: 7.8 / 20.4).
 constexpr int64_t kShortKeys = 512;
 bool short_rows(const PagedAttentionArgs &a, const Args &p, bool wide)
 {
