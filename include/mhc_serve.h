@@ -9,6 +9,13 @@
  *                        the pages of a cache or to tensors;
  *   mhcPagedAttention    attention of one new token per sequence over a paged
  *                        key-value cache;
+ *   mhcDraftAttention    attention of several new tokens per sequence: a tree of
+ *                        drafted tokens, or a chain (a prompt's chunk);
+ *   mhcDraftAccept       the path of a drafted tree that the model's choices confirm;
+ *   mhcCacheKeep         the confirmed tokens' keys and values to their places;
+ *   mhcSparseAttention   attention of one new token per sequence over the pages that
+ *                        a score ranks highest;
+ *   mhcCacheBounds       the bounds of every page's keys, which that score reads;
  *   mhcCacheUpdate       a step's page table: keep, fork, reorder, end and
  *                        extend sequences, private copies of shared pages;
  *   mhcCacheCompact      the moves that bring the pages in use to the front;
@@ -163,6 +170,165 @@ MHC_API int mhcPagedAttentionGetWorkspaceSize(
 
 MHC_API int mhcPagedAttention(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor,
                               hipStream_t stream);
+
+/*
+ * Attention of several new tokens per sequence over a paged cache.  Row b's last
+ * n = min(max(drafted[b], 0), S, L) of L = lengths[b] cached tokens are new: node
+ * i < n is token c + i, c = L - n.  It sees the context, tokens t < c, and of the
+ * new tokens itself and its ancestors:
+ *
+ *   parents given: node i's parent is parents[b, i] where 0 <= parents[b, i] < i;
+ *     any other value: it has none and hangs under the context.  Positions are
+ *     c + (number of ancestors);
+ *   parents NULL: a chain, node i hangs under node i - 1 (a prompt's chunk).
+ *
+ * With a window w a node at position p sees tokens at positions above p - w only
+ * (context token t is at position t).  Then, for the tokens t that node i sees,
+ *
+ *   s_t = scale * q_i . k_t,  out_i = sum_t exp(s_t - lse_i) v_t,
+ *   lse_i = log sum_t exp(s_t)
+ *
+ * with query head h reading kv head h / (heads / kvHeads), in fp32, out rounded
+ * once.  (The weights are held in 16 bits in bf16 and in 22 in fp16, there small
+ * ones to 2^-39 of the largest.)  Nodes i >= n, and nodes that see no key, have out
+ * 0 and lse -inf.  What a node does not see may be infinite or NaN; an infinite
+ * value that it sees is infinite in its output.
+ *
+ *   q          fp16 | bf16   [B, S, heads, d]
+ *   kCache, vCache  same     [pages, pageSize, kvHeads, d]
+ *   pageTable  int32         [B, width]
+ *   lengths    int32         [B], the new tokens included
+ *   drafted    int32         [B]
+ *   parents    int32         [B, S], S <= 256; or NULL
+ *   out        type of q     [B, S, heads, d]   lse      fp32  [B, S, heads], or NULL
+ *
+ * Sizes, alignments and strides as for mhcPagedAttention; the blocks of work,
+ * B * kvHeads * ceil(S * heads / kvHeads / 32), are below 2^23 and, times (width *
+ * pageSize / 32 + 2), below 2^31.  The same call gives the same bits again; in another batch sums may be
+ * cut elsewhere and differ by roundings in fp32.
+ */
+MHC_API int mhcDraftAttentionGetWorkspaceSize(
+    const mhcStridedTensor *q, const mhcStridedTensor *kCache, const mhcStridedTensor *vCache,
+    const mhcTensor *pageTable, const mhcTensor *lengths, const mhcTensor *drafted,
+    const mhcTensor *parents, float scale, int64_t window, const mhcStridedTensor *out,
+    const mhcTensor *lse, uint64_t *workspaceSize, mhcServeExecutor **executor);
+
+MHC_API int mhcDraftAttention(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor,
+                              hipStream_t stream);
+
+/*
+ * What the model confirms of a drafted tree (nodes, parents and n as for
+ * mhcDraftAttention, with L = max(lengths[b], 0)).  chosen[b, i] is the token that
+ * the model puts behind node i: its likeliest, or one drawn from its distribution
+ * (what is accepted then follows that distribution).  The path begins at node 0, the
+ * row's last known token, which always stays, and goes on from node i to its first
+ * child j < n with tokens[b, j] = chosen[b, i], as long as there is one.
+ *
+ *   path       int32 [B, S]: the path's nodes, ascending, then -1
+ *   accepted   int32 [B]: how many (0 where n = 0)
+ *   next       type of tokens [B]: chosen at the path's last node, the row's next
+ *              token; -1 where n = 0
+ *   newLengths int32 [B]: L - n + accepted, the row's length once mhcCacheKeep has
+ *              put the path's tokens behind the context
+ *
+ *   tokens, chosen  int32 | int64 [B, S], S <= 256; parents int32 [B, S] or NULL (a
+ *   chain); drafted, lengths int32 [B]
+ */
+MHC_API int mhcDraftAcceptGetWorkspaceSize(
+    const mhcTensor *tokens, const mhcTensor *parents, const mhcTensor *drafted,
+    const mhcTensor *chosen, const mhcTensor *lengths, const mhcTensor *path,
+    const mhcTensor *accepted, const mhcTensor *next, const mhcTensor *newLengths,
+    uint64_t *workspaceSize, mhcServeExecutor **executor);
+
+MHC_API int mhcDraftAccept(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor,
+                           hipStream_t stream);
+
+/*
+ * Keys and values of a path's nodes to the places behind the context, in place: with
+ * c and n as for mhcDraftAttention and L clamped to the table, token c + path[b, k]
+ * goes to place c + k, for k = 0, 1, ... as long as path[b, k] is a node (0 <=
+ * path[b, k] < n) above path[b, k - 1].  Where either place is in a hole nothing is
+ * moved.  lengths is the one that mhcDraftAttention and mhcDraftAccept were given.
+ * Pages that the moves touch must be held by one row only (mhcCacheUpdate sees to
+ * that for rows that append).
+ *
+ *   kCache, vCache  fp16 | bf16 | fp32 [pages, pageSize, kvHeads, d]
+ *   pageTable int32 [B, width]   lengths, drafted int32 [B]   path int32 [B, S]
+ */
+MHC_API int mhcCacheKeepGetWorkspaceSize(
+    const mhcStridedTensor *kCache, const mhcStridedTensor *vCache, const mhcTensor *pageTable,
+    const mhcTensor *lengths, const mhcTensor *drafted, const mhcTensor *path,
+    uint64_t *workspaceSize, mhcServeExecutor **executor);
+
+MHC_API int mhcCacheKeep(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor,
+                         hipStream_t stream);
+
+/*
+ * The smallest and the largest value, per kv head and dimension, of each page's keys:
+ * lo, hi [pages, kvHeads, d].  For the pages that hold row b's last
+ * min(max(counts[b], 0), tokens, L) tokens (L: lengths[b] clamped to the table), in
+ * place:
+ *
+ *   lo = min over these tokens in the page, and of the old lo if the page also holds
+ *   tokens of the row in front of them; hi likewise.
+ *
+ * So counts = what a step appended keeps the bounds of a growing cache, and counts =
+ * L makes them anew.  After tokens were taken away (mhcCacheKeep) the last page's
+ * bounds may be wider than need be; counts that reach back to the page's start mend
+ * that.  A NaN among the keys, or in the old bounds that count, makes both bounds NaN.
+ * -0 is below 0.  No two rows' new tokens lie in one page.
+ *
+ *   kCache  fp16 | bf16 [pages, pageSize, kvHeads, d]   lo, hi  same [pages, kvHeads, d]
+ *   pageTable int32 [B, width]   lengths, counts int32 [B]   tokens >= 0
+ *
+ * d, alignments and strides as for mhcPagedAttention.  cache_copy_pages copies bounds
+ * too: they are caches with pages of one slot.
+ */
+MHC_API int mhcCacheBoundsGetWorkspaceSize(
+    const mhcStridedTensor *kCache, const mhcTensor *pageTable, const mhcTensor *lengths,
+    const mhcTensor *counts, int64_t tokens, const mhcStridedTensor *lo,
+    const mhcStridedTensor *hi, uint64_t *workspaceSize, mhcServeExecutor **executor);
+
+MHC_API int mhcCacheBounds(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor,
+                           hipStream_t stream);
+
+/*
+ * Attention of one new token per sequence over `top` pages for each of its kv heads.
+ * Row b holds its table's first ceil(L / pageSize) columns (L: lengths[b] clamped to
+ * the table); holes are left out.  kv head g takes the first `first` and the last
+ * `last` of these columns that are no holes of their own, and of the others those with
+ * the highest scores, until it has `top` (or all); of equal scores the lower column.
+ * With the query heads h that share g
+ *
+ *   score = sum_h sum_i max(q_hi lo_i, q_hi hi_i)
+ *         = sum_i (sum_h max(q_hi, 0)) hi_i + (sum_h min(q_hi, 0)) lo_i,
+ *
+ * the largest value that the sum of the heads' products with a key between the bounds
+ * lo and hi can have, in 64 bits; a score that is NaN is above all others.  Over the
+ * tokens of these pages
+ *
+ *   s_t = scale * q . k_t,  out = sum_t exp(s_t - lse) v_t,  lse = log sum_t exp(s_t)
+ *
+ * as mhcPagedAttention computes it, with its limits, holes and exceptional values.
+ *
+ *   q          fp16 | bf16   [B, heads, d]
+ *   kCache, vCache  same     [pages, pageSize, kvHeads, d]
+ *   lo, hi     same          [pages, kvHeads, d], 16-byte aligned rows
+ *   pageTable  int32         [B, width]      lengths  int32 [B], the new token included
+ *   out        type of q     [B, heads, d]   lse      fp32  [B, heads], or NULL
+ *   columns    int32         [B, kvHeads, top]: the columns taken, ascending, then -1
+ *
+ * 0 <= first, last; first + last <= top; top >= 1; top * pageSize below 2^31.
+ */
+MHC_API int mhcSparseAttentionGetWorkspaceSize(
+    const mhcStridedTensor *q, const mhcStridedTensor *kCache, const mhcStridedTensor *vCache,
+    const mhcStridedTensor *lo, const mhcStridedTensor *hi, const mhcTensor *pageTable,
+    const mhcTensor *lengths, int64_t top, int64_t first, int64_t last, float scale,
+    const mhcStridedTensor *out, const mhcTensor *lse, const mhcTensor *columns,
+    uint64_t *workspaceSize, mhcServeExecutor **executor);
+
+MHC_API int mhcSparseAttention(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor,
+                               hipStream_t stream);
 
 /*
  * A step's page table.  Row r of the new state goes on from row parents[r] of

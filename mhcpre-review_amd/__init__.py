@@ -28,12 +28,17 @@ from .binding import (  # noqa: F401
     stream_probe,
 )
 from .serve import (  # noqa: F401
+    CacheBoundsOp,
     CacheCompactOp,
+    CacheKeepOp,
     CacheUpdateOp,
     CopyPagesOp,
+    DraftAcceptOp,
+    DraftAttentionOp,
     MhcStridedTensor,
     PagedAttentionOp,
     QkNormRopeOp,
+    SparseAttentionOp,
     load_serve_library,
     make_strided,
     rotary_frequencies,

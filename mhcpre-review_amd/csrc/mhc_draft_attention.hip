@@ -1,0 +1,80 @@
+// mhcDraftAttention's host side.
+
+#include "mhc_draft_attention.h"
+
+namespace mhc {
+namespace draft {
+namespace {
+
+// The layout for rows of a (sequence, kv head).
+Kind kind_of(const DraftAttentionArgs &a)
+{
+    const int64_t rows = (int64_t)a.S * (a.heads / a.kvHeads);
+    return rows <= 32 ? Kind::kOne : rows <= 64 ? Kind::kTwo : Kind::kFour;
+}
+
+template <Kind kKind>
+void plan_kind(Args &p, int cus)
+{
+    with_size<kKind>(p.a.d, [&](auto l) {
+        using L = decltype(l);
+        p.rows = L::kBlock;
+        p.unit = L::kUnit;
+        p.most = cus * L::kPerCu;
+        return 0;
+    });
+}
+
+Args plan(const DraftAttentionArgs &a, int cus)
+{
+    Args p{};
+    p.a = a;
+    p.group = a.heads / a.kvHeads;
+    switch (kind_of(a)) {
+    case Kind::kOne: plan_kind<Kind::kOne>(p, cus); break;
+    case Kind::kTwo: plan_kind<Kind::kTwo>(p, cus); break;
+    case Kind::kFour: plan_kind<Kind::kFour>(p, cus); break;
+    }
+    p.blocks = (int)(((int64_t)a.S * p.group + p.rows - 1) / p.rows);
+    return p;
+}
+
+int padded(int d) { return with_size<Kind::kOne>(d, [](auto l) { return decltype(l)::D; }); }
+
+}  // namespace
+}  // namespace draft
+
+bool draft_attention_units_fit(const DraftAttentionArgs &a)
+{
+    const int64_t blocks = ((int64_t)a.S * (a.heads / a.kvHeads) + draft::kRows - 1) / draft::kRows;
+    const int64_t units = (int64_t)a.width * a.pageSize / 32 + 2;
+    int64_t all;
+    return !__builtin_mul_overflow(units, blocks, &all) && !__builtin_mul_overflow(all, (int64_t)a.B * a.kvHeads, &all) &&
+           all < INT32_MAX && (int64_t)a.B * a.kvHeads * blocks < (1 << 23);  // (workgroups of the joining launch)
+}
+
+size_t draft_attention_workspace(const DraftAttentionArgs &a, int cus)
+{
+    const draft::Args p = draft::plan(a, cus);
+    return (size_t)2 * p.most * p.rows * (draft::padded(a.d) + 2) * 4;
+}
+
+hipError_t launch_draft_attention(const DraftAttentionArgs &a, void *workspace, int cus, hipStream_t stream)
+{
+    draft::Args p = draft::plan(a, cus);
+    p.outs = static_cast<float *>(workspace);
+    p.ends = p.outs + (size_t)2 * p.most * p.rows * draft::padded(a.d);
+    switch (draft::kind_of(a)) {
+    case draft::Kind::kOne:
+        return a.isBf16 ? draft::launch_kind<true, draft::Kind::kOne>(p, stream)
+                        : draft::launch_kind<false, draft::Kind::kOne>(p, stream);
+    case draft::Kind::kTwo:
+        return a.isBf16 ? draft::launch_kind<true, draft::Kind::kTwo>(p, stream)
+                        : draft::launch_kind<false, draft::Kind::kTwo>(p, stream);
+    default:
+        return a.isBf16 ? draft::launch_kind<true, draft::Kind::kFour>(p, stream)
+                        : draft::launch_kind<false, draft::Kind::kFour>(p, stream);
+    }
+}
+
+}  // namespace mhc

@@ -102,6 +102,7 @@ struct Args {
     int most;     // workgroups of the launch
     char *parts;  // see Parts; null: the kernel of short rows
     LaunchTag tag;
+    int each = 1;  // kEach: kv heads of a sequence
 };
 
 // A stretch leaves at most two parts in the workspace, of the (row, kv head,
@@ -288,14 +289,23 @@ __device__ __forceinline__ uint32_t at_least(uint32_t two, float p0, float p1)
                                                                   __builtin_elementwise_min(some, u16x2_t{1, 1})));
 }
 
+// Where the query heads of row b and kv head `kv` begin in q or out.  kEach: a row is one
+// kv head of a sequence of `each` (its own page table and length; a.kvHeads is 1).
+template <bool kEach>
+__device__ __forceinline__ int64_t first_head(const HeadRows &t, int b, int kv, int group, int each)
+{
+    return kEach ? b / each * t.row + (int64_t)(b % each * group) * t.head : b * t.row + (int64_t)(kv * group) * t.head;
+}
+
 // 4 values of the output from their sum, its weights' sum and their maximum; the
 // first ones' thread also writes the head's lse.
-template <bool kBf16>
+template <bool kBf16, bool kEach = false>
 __device__ __forceinline__ void finish(const PagedAttentionArgs &a, int b, int head, int e, f32x4_t all, float top,
-                                       float total)
+                                       float total, int each = 1)
 {
     const float inv = total == 0.f ? 0.f : 1.f / kLift<kBf16> / total;
-    uint16_t *out = static_cast<uint16_t *>(a.out.data) + b * a.out.row + head * a.out.head + e;
+    uint16_t *out = static_cast<uint16_t *>(a.out.data) +
+                    (kEach ? first_head<true>(a.out, b, 0, a.heads, each) : b * a.out.row) + head * a.out.head + e;
     *reinterpret_cast<u32x2_t *>(out) =
         u32x2_t{dev::pack2_x<kBf16>(all[0] * inv, all[1] * inv), dev::pack2_x<kBf16>(all[2] * inv, all[3] * inv)};
     if (e == 0 && a.lse != nullptr) {
@@ -334,7 +344,8 @@ __device__ __forceinline__ int span_bits(int parts, int round)
 // wave is on its own: a share of the (row, kv head, block)s, each of which it does
 // alone, 32 keys at a time, with no join and no workspace.  (Otherwise a row of up
 // to 32 keys leaves three waves of its workgroup without any.)
-template <bool kBf16, int D, int RT, bool kShort>
+// kEach: rows are the kv heads of sequences, each with a table and a length of its own.
+template <bool kBf16, int D, int RT, bool kShort, bool kEach = false>
 __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void attention_units(Args args)
 {
     using S = Shape<D>;
@@ -450,7 +461,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
         Found f{-1, 0, 0};
         if (inside(ahead, unit)) {
             const int t = (ahead.keys.first + ahead.tile) * kPer + (kShort ? 0 : wave * kTile) + lane % kTile;
-            f.kvHead = ahead.hg / args.blocks;
+            f.kvHead = kEach ? ahead.b % args.each : ahead.hg / args.blocks;
             if (t >= ahead.keys.low && t < ahead.keys.high) {
                 const uint32_t at = (uint32_t)t / (uint32_t)a.pageSize;
                 f.page = a.table[(int64_t)ahead.b * a.width + at];
@@ -500,8 +511,8 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
             const int h = x.hg % args.blocks * 16 * RT + rt * 16 + col;
             q[rt].clear();
             if (h < args.group) {
-                q[rt].load(static_cast<const uint16_t *>(a.q.data) + x.b * a.q.row +
-                               (int64_t)(x.hg / args.blocks * args.group + h) * a.q.head,
+                q[rt].load(static_cast<const uint16_t *>(a.q.data) +
+                               first_head<kEach>(a.q, x.b, x.hg / args.blocks, args.group, args.each) + h * a.q.head,
                            lane);
             }
         }
@@ -653,8 +664,8 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                 if (h < args.group) {
 #pragma unroll
                     for (int j = 0; j < S::kDims; ++j) {
-                        finish<kBf16>(a, here.b, here.hg / args.blocks * args.group + h, 16 * j + 4 * c, o[rt][j],
-                                      top[rt] == -INFINITY ? 0.f : top[rt], sum[rt]);
+                        finish<kBf16, kEach>(a, here.b, here.hg / args.blocks * args.group + h, 16 * j + 4 * c,
+                                             o[rt][j], top[rt] == -INFINITY ? 0.f : top[rt], sum[rt], args.each);
                     }
                 }
             }
@@ -711,7 +722,7 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
                         parts.put_ends(slot, rt * 16 + row, most, total);
                     }
                 } else {
-                    finish<kBf16>(a, here.b, kvHead * args.group + h, e, all, zero, total);
+                    finish<kBf16, kEach>(a, here.b, kvHead * args.group + h, e, all, zero, total, args.each);
                 }
             }
             __syncthreads();
@@ -821,8 +832,8 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
             for (int t = 0; t < kTasks; ++t) {
                 if (at0 + t * 64 * kWaves >= rows * (D / 4)) {
                 } else if (whole) {
-                    finish<kBf16>(a, part.b, part.hg / args.blocks * args.group + head0 + row[t], e[t], all[t], zero[t],
-                                  total[t]);
+                    finish<kBf16, kEach>(a, part.b, part.hg / args.blocks * args.group + head0 + row[t], e[t], all[t],
+                                         zero[t], total[t], args.each);
                 } else {
                     parts.put(part.slot(first), row[t], e[t], all[t]);
                     if (e[t] == 0) {
@@ -869,14 +880,14 @@ __global__ __launch_bounds__(64 * kWaves, workgroups_per_cu(D, RT > 1)) void att
     }
 }
 
-template <bool kBf16, int D, int RT>
+template <bool kBf16, int D, int RT, bool kEach>
 hipError_t launch_size(const Args &args, hipStream_t stream)
 {
     int grid = args.most;
-    auto kernel = attention_units<kBf16, D, RT, false>;
+    auto kernel = attention_units<kBf16, D, RT, false, kEach>;
     if constexpr (RT == 1) {
         if (args.parts == nullptr) {
-            kernel = attention_units<kBf16, D, RT, true>;
+            kernel = attention_units<kBf16, D, RT, true, kEach>;
             const int items = args.a.B * args.a.kvHeads * args.blocks;
             grid = (items + kWaves - 1) / kWaves < grid ? (items + kWaves - 1) / kWaves : grid;
         }
@@ -885,21 +896,21 @@ hipError_t launch_size(const Args &args, hipStream_t stream)
     return hipGetLastError();
 }
 
-template <bool kBf16, int RT>
+template <bool kBf16, int RT, bool kEach = false>
 hipError_t launch_heads(const Args &args, hipStream_t stream)
 {
     switch (args.a.d) {
-    case 32: return launch_size<kBf16, 32, RT>(args, stream);
-    case 64: return launch_size<kBf16, 64, RT>(args, stream);
-    case 80: return launch_size<kBf16, 80, RT>(args, stream);
-    case 96: return launch_size<kBf16, 96, RT>(args, stream);
-    case 112: return launch_size<kBf16, 112, RT>(args, stream);
-    case 128: return launch_size<kBf16, 128, RT>(args, stream);
-    case 160: return launch_size<kBf16, 160, RT>(args, stream);
-    case 192: return launch_size<kBf16, 192, RT>(args, stream);
+    case 32: return launch_size<kBf16, 32, RT, kEach>(args, stream);
+    case 64: return launch_size<kBf16, 64, RT, kEach>(args, stream);
+    case 80: return launch_size<kBf16, 80, RT, kEach>(args, stream);
+    case 96: return launch_size<kBf16, 96, RT, kEach>(args, stream);
+    case 112: return launch_size<kBf16, 112, RT, kEach>(args, stream);
+    case 128: return launch_size<kBf16, 128, RT, kEach>(args, stream);
+    case 160: return launch_size<kBf16, 160, RT, kEach>(args, stream);
+    case 192: return launch_size<kBf16, 192, RT, kEach>(args, stream);
     case 256:
         if constexpr (RT == 1) {
-            return launch_size<kBf16, 256, RT>(args, stream);
+            return launch_size<kBf16, 256, RT, kEach>(args, stream);
         }
         return hipErrorInvalidValue;
     default: return hipErrorInvalidValue;
@@ -909,6 +920,14 @@ hipError_t launch_heads(const Args &args, hipStream_t stream)
 // One file per instance: mhc_paged_attention_{bf16,f16}.hip, RT 1 and 2.
 hipError_t launch_bf16(const Args &args, bool wide, hipStream_t stream);
 hipError_t launch_f16(const Args &args, bool wide, hipStream_t stream);
+// kEach's: mhc_sparse_attention_{bf16,f16}.hip.
+hipError_t launch_each_bf16(const Args &args, bool wide, hipStream_t stream);
+hipError_t launch_each_f16(const Args &args, bool wide, hipStream_t stream);
+
+// How a call is laid out (mhc_paged_attention_bf16.hip): 32 query heads at a time or 16, and
+// whether rows are short enough for a wave each.
+Args plan(const PagedAttentionArgs &a, int cus, bool &wide);
+bool short_rows(const PagedAttentionArgs &a, const Args &p, bool wide);
 
 }  // namespace attention
 }  // namespace mhc

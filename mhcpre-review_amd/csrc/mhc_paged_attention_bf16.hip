@@ -10,8 +10,6 @@ hipError_t launch_bf16(const Args &args, bool wide, hipStream_t stream)
     return wide ? launch_heads<true, 2>(args, stream) : launch_heads<true, 1>(args, stream);
 }
 
-namespace {
-
 Args plan(const PagedAttentionArgs &a, int cus, bool &wide)
 {
     Args p{};
@@ -41,7 +39,6 @@ bool short_rows(const PagedAttentionArgs &a, const Args &p, bool wide)
     return !wide && keys <= kShortKeys && (int64_t)a.B * a.kvHeads * p.blocks >= 2 * (int64_t)p.most;
 }
 
-}  // namespace
 }  // namespace attention
 
 bool paged_attention_head_size(int64_t d)

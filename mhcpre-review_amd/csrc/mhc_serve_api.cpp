@@ -15,7 +15,7 @@
 
 namespace {
 
-enum class Op { kNormRope, kAttention, kUpdate, kCompact, kCopy };
+enum class Op { kNormRope, kAttention, kUpdate, kCompact, kCopy, kDraft, kAccept, kKeep, kBounds, kSparse };
 
 // The most rows, pages and elements a tensor may have: every index below fits
 // its kernel's type, every byte offset 62 bits.
@@ -38,6 +38,11 @@ struct mhcServeExecutor {
         mhc::CacheUpdateArgs update;
         mhc::CacheCompactArgs compact;
         mhc::CopyPagesArgs copy;
+        mhc::DraftAttentionArgs draft;
+        mhc::DraftAcceptArgs accept;
+        mhc::CacheKeepArgs keep;
+        mhc::CacheBoundsArgs bounds;
+        mhc::SparseAttentionArgs sparse;
     };
     mhcServeExecutor() : rope{} {}
 };
@@ -179,6 +184,11 @@ mhc::HeadRows head_rows(const mhcStridedTensor *t)
     return {t->data, stride_of(t, 0), stride_of(t, 1)};
 }
 
+mhc::TokenRows token_rows(const mhcStridedTensor *t)
+{
+    return {t->data, stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)};
+}
+
 mhc::CacheRows cache_rows(const mhcStridedTensor *t)
 {
     return {t->data, stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)};
@@ -213,8 +223,18 @@ int finish(mhcServeExecutor *ex, const void *someTensor, uint64_t *workspaceSize
     case Op::kCompact:
         ex->workspace = mhc::cache_compact_workspace(ex->compact);
         break;
+    case Op::kDraft:
+        ex->workspace = ex->empty ? 0 : mhc::draft_attention_workspace(ex->draft, ex->cus);
+        break;
+    case Op::kSparse:
+        ex->workspace = ex->empty ? 0 : mhc::sparse_attention_workspace(ex->sparse, ex->cus);
+        prime_replay_words(*ex);
+        break;
     case Op::kNormRope:
     case Op::kCopy:
+    case Op::kAccept:
+    case Op::kKeep:
+    case Op::kBounds:
         break;
     }
     *workspaceSize = ex->workspace;
@@ -262,6 +282,21 @@ int launch(Op op, void *workspace, uint64_t workspaceSize, mhcServeExecutor *ex,
     case Op::kCopy:
         err = mhc::launch_copy_pages(ex->copy, ex->cus, stream);
         break;
+    case Op::kDraft:
+        err = mhc::launch_draft_attention(ex->draft, workspace, ex->cus, stream);
+        break;
+    case Op::kAccept:
+        err = mhc::launch_draft_accept(ex->accept, stream);
+        break;
+    case Op::kKeep:
+        err = mhc::launch_cache_keep(ex->keep, stream);
+        break;
+    case Op::kBounds:
+        err = mhc::launch_cache_bounds(ex->bounds, stream);
+        break;
+    case Op::kSparse:
+        err = mhc::launch_sparse_attention(ex->sparse, workspace, current, ex->cus, stream);
+        break;
     }
     return err == hipSuccess ? MHC_STATUS_SUCCESS : MHC_STATUS_HIP_ERROR;
 }
@@ -301,6 +336,66 @@ int table_limits(const mhcTensor *table, const mhcTensor *lengths, int64_t pages
     }
     return first_of({check_dense(table, {MHC_DTYPE_INT32}, {table->dims[0], table->dims[1]}),
                      check_dense(lengths, {MHC_DTYPE_INT32}, {table->dims[0]})});
+}
+
+// The arguments that attention of single tokens takes, checked.
+int attention_args(const mhcStridedTensor *q, const mhcStridedTensor *kCache, const mhcStridedTensor *vCache,
+                   const mhcTensor *pageTable, const mhcTensor *lengths, float scale, int64_t window,
+                   const mhcStridedTensor *out, const mhcTensor *lse, uint64_t *workspaceSize,
+                   mhcServeExecutor **executor, mhc::PagedAttentionArgs &a)
+{
+    if (q == nullptr || out == nullptr || vCache == nullptr || workspaceSize == nullptr || executor == nullptr) {
+        return MHC_STATUS_NULL_ARGUMENT;
+    }
+    int st = cache_limits(kCache);
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    const int64_t pages = kCache->dims[0], pageSize = kCache->dims[1], kvHeads = kCache->dims[2], d = kCache->dims[3];
+    if (q->ndim != 3 || window < 0) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    if (q->dtype != MHC_DTYPE_FLOAT16 && q->dtype != MHC_DTYPE_BF16) {
+        return MHC_STATUS_INVALID_DTYPE;
+    }
+    const int64_t B = q->dims[0], heads = q->dims[1];
+    if (B < 0 || heads < 1 || heads % kvHeads != 0) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    if ((st = table_limits(pageTable, lengths, pages, pageSize)) != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    if (pageTable->dims[0] != B) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    if (!mhc::paged_attention_head_size(d) || heads > 65536 || B > (1 << 20)) {
+        return MHC_STATUS_UNSUPPORTED_SHAPE;
+    }
+    st = first_of({check_strided(q, q->dtype, {B, heads, d}, 16), check_strided(out, q->dtype, {B, heads, d}, 16),
+                   check_strided(kCache, q->dtype, {pages, pageSize, kvHeads, d}, 16),
+                   check_strided(vCache, q->dtype, {pages, pageSize, kvHeads, d}, 16),
+                   lse != nullptr ? check_dense(lse, {MHC_DTYPE_FLOAT}, {B, heads}) : MHC_STATUS_SUCCESS});
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    a.isBf16 = q->dtype == MHC_DTYPE_BF16;
+    a.B = static_cast<int>(B);
+    a.heads = static_cast<int>(heads);
+    a.kvHeads = static_cast<int>(kvHeads);
+    a.d = static_cast<int>(d);
+    a.q = head_rows(q);
+    a.out = head_rows(out);
+    a.kCache = cache_rows(kCache);
+    a.vCache = cache_rows(vCache);
+    a.pages = pages;
+    a.pageSize = static_cast<int>(pageSize);
+    a.width = static_cast<int>(pageTable->dims[1]);
+    a.table = static_cast<const int32_t *>(pageTable->data);
+    a.lengths = static_cast<const int32_t *>(lengths->data);
+    a.scale = scale;
+    a.window = window;
+    a.lse = lse != nullptr ? static_cast<float *>(lse->data) : nullptr;
+    return MHC_STATUS_SUCCESS;
 }
 
 }  // namespace
@@ -470,69 +565,21 @@ int mhcPagedAttentionGetWorkspaceSize(const mhcStridedTensor *q, const mhcStride
                                       const mhcStridedTensor *out, const mhcTensor *lse, uint64_t *workspaceSize,
                                       mhcServeExecutor **executor)
 {
-    if (q == nullptr || out == nullptr || vCache == nullptr || workspaceSize == nullptr || executor == nullptr) {
-        return MHC_STATUS_NULL_ARGUMENT;
-    }
-    int st = cache_limits(kCache);
+    mhc::PagedAttentionArgs a{};
+    const int st = attention_args(q, kCache, vCache, pageTable, lengths, scale, window, out, lse, workspaceSize, executor, a);
     if (st != MHC_STATUS_SUCCESS) {
         return st;
     }
-    const int64_t pages = kCache->dims[0], pageSize = kCache->dims[1], kvHeads = kCache->dims[2], d = kCache->dims[3];
-    if (q->ndim != 3 || window < 0) {
-        return MHC_STATUS_INVALID_SHAPE;
-    }
-    if (q->dtype != MHC_DTYPE_FLOAT16 && q->dtype != MHC_DTYPE_BF16) {
-        return MHC_STATUS_INVALID_DTYPE;
-    }
-    const int64_t B = q->dims[0], heads = q->dims[1];
-    if (B < 0 || heads < 1 || heads % kvHeads != 0) {
-        return MHC_STATUS_INVALID_SHAPE;
-    }
-    if ((st = table_limits(pageTable, lengths, pages, pageSize)) != MHC_STATUS_SUCCESS) {
-        return st;
-    }
-    if (pageTable->dims[0] != B) {
-        return MHC_STATUS_INVALID_SHAPE;
-    }
-    if (!mhc::paged_attention_head_size(d) || heads > 65536 || B > (1 << 20)) {
+    if (!mhc::paged_attention_units_fit(a)) {
         return MHC_STATUS_UNSUPPORTED_SHAPE;
-    }
-    st = first_of({check_strided(q, q->dtype, {B, heads, d}, 16), check_strided(out, q->dtype, {B, heads, d}, 16),
-                   check_strided(kCache, q->dtype, {pages, pageSize, kvHeads, d}, 16),
-                   check_strided(vCache, q->dtype, {pages, pageSize, kvHeads, d}, 16),
-                   lse != nullptr ? check_dense(lse, {MHC_DTYPE_FLOAT}, {B, heads}) : MHC_STATUS_SUCCESS});
-    if (st != MHC_STATUS_SUCCESS) {
-        return st;
     }
     mhcServeExecutor *ex = new (std::nothrow) mhcServeExecutor;
     if (ex == nullptr) {
         return MHC_STATUS_HIP_ERROR;
     }
     ex->op = Op::kAttention;
-    ex->empty = B == 0;
-    ex->attention = mhc::PagedAttentionArgs{};
-    mhc::PagedAttentionArgs &a = ex->attention;
-    a.isBf16 = q->dtype == MHC_DTYPE_BF16;
-    a.B = static_cast<int>(B);
-    a.heads = static_cast<int>(heads);
-    a.kvHeads = static_cast<int>(kvHeads);
-    a.d = static_cast<int>(d);
-    a.q = head_rows(q);
-    a.out = head_rows(out);
-    a.kCache = cache_rows(kCache);
-    a.vCache = cache_rows(vCache);
-    a.pages = pages;
-    a.pageSize = static_cast<int>(pageSize);
-    a.width = static_cast<int>(pageTable->dims[1]);
-    a.table = static_cast<const int32_t *>(pageTable->data);
-    a.lengths = static_cast<const int32_t *>(lengths->data);
-    a.scale = scale;
-    a.window = window;
-    a.lse = lse != nullptr ? static_cast<float *>(lse->data) : nullptr;
-    if (!mhc::paged_attention_units_fit(a)) {
-        delete ex;
-        return MHC_STATUS_UNSUPPORTED_SHAPE;
-    }
+    ex->empty = a.B == 0;
+    ex->attention = a;
     return finish(ex, q->data, workspaceSize, executor);
 }
 
@@ -687,6 +734,309 @@ int mhcCacheCopyPagesGetWorkspaceSize(const mhcStridedTensor *kCache, const mhcS
 int mhcCacheCopyPages(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor, hipStream_t stream)
 {
     return launch(Op::kCopy, workspace, workspaceSize, executor, stream);
+}
+
+int mhcDraftAttentionGetWorkspaceSize(const mhcStridedTensor *q, const mhcStridedTensor *kCache,
+                                      const mhcStridedTensor *vCache, const mhcTensor *pageTable,
+                                      const mhcTensor *lengths, const mhcTensor *drafted, const mhcTensor *parents,
+                                      float scale, int64_t window, const mhcStridedTensor *out, const mhcTensor *lse,
+                                      uint64_t *workspaceSize, mhcServeExecutor **executor)
+{
+    if (q == nullptr || out == nullptr || vCache == nullptr || workspaceSize == nullptr || executor == nullptr) {
+        return MHC_STATUS_NULL_ARGUMENT;
+    }
+    int st = cache_limits(kCache);
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    const int64_t pages = kCache->dims[0], pageSize = kCache->dims[1], kvHeads = kCache->dims[2], d = kCache->dims[3];
+    if (q->ndim != 4 || window < 0) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    if (q->dtype != MHC_DTYPE_FLOAT16 && q->dtype != MHC_DTYPE_BF16) {
+        return MHC_STATUS_INVALID_DTYPE;
+    }
+    const int64_t B = q->dims[0], S = q->dims[1], heads = q->dims[2];
+    if (B < 0 || S < 0 || heads < 1 || heads % kvHeads != 0) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    if ((st = table_limits(pageTable, lengths, pages, pageSize)) != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    if (pageTable->dims[0] != B) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    if (!mhc::paged_attention_head_size(d) || heads > 65536 || B > (1 << 20) || S > (1 << 20) ||
+        (parents != nullptr && S > mhc::kDraftNodes)) {
+        return MHC_STATUS_UNSUPPORTED_SHAPE;
+    }
+    st = first_of(
+        {check_strided(q, q->dtype, {B, S, heads, d}, 16), check_strided(out, q->dtype, {B, S, heads, d}, 16),
+         check_strided(kCache, q->dtype, {pages, pageSize, kvHeads, d}, 16),
+         check_strided(vCache, q->dtype, {pages, pageSize, kvHeads, d}, 16),
+         check_dense(drafted, {MHC_DTYPE_INT32}, {B}),
+         parents != nullptr ? check_dense(parents, {MHC_DTYPE_INT32}, {B, S}) : MHC_STATUS_SUCCESS,
+         lse != nullptr ? check_dense(lse, {MHC_DTYPE_FLOAT}, {B, S, heads}) : MHC_STATUS_SUCCESS});
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    mhcServeExecutor *ex = new (std::nothrow) mhcServeExecutor;
+    if (ex == nullptr) {
+        return MHC_STATUS_HIP_ERROR;
+    }
+    ex->op = Op::kDraft;
+    ex->empty = B == 0 || S == 0;
+    ex->draft = mhc::DraftAttentionArgs{};
+    mhc::DraftAttentionArgs &a = ex->draft;
+    a.isBf16 = q->dtype == MHC_DTYPE_BF16;
+    a.B = static_cast<int>(B);
+    a.S = static_cast<int>(S);
+    a.heads = static_cast<int>(heads);
+    a.kvHeads = static_cast<int>(kvHeads);
+    a.d = static_cast<int>(d);
+    a.q = token_rows(q);
+    a.out = token_rows(out);
+    a.kCache = cache_rows(kCache);
+    a.vCache = cache_rows(vCache);
+    a.pages = pages;
+    a.pageSize = static_cast<int>(pageSize);
+    a.width = static_cast<int>(pageTable->dims[1]);
+    a.table = static_cast<const int32_t *>(pageTable->data);
+    a.lengths = static_cast<const int32_t *>(lengths->data);
+    a.drafted = static_cast<const int32_t *>(drafted->data);
+    a.parents = parents != nullptr ? static_cast<const int32_t *>(parents->data) : nullptr;
+    a.scale = scale;
+    a.window = window;
+    a.lse = lse != nullptr ? static_cast<float *>(lse->data) : nullptr;
+    if (!ex->empty && !mhc::draft_attention_units_fit(a)) {
+        delete ex;
+        return MHC_STATUS_UNSUPPORTED_SHAPE;
+    }
+    return finish(ex, q->data, workspaceSize, executor);
+}
+
+int mhcDraftAttention(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor, hipStream_t stream)
+{
+    return launch(Op::kDraft, workspace, workspaceSize, executor, stream);
+}
+
+int mhcDraftAcceptGetWorkspaceSize(const mhcTensor *tokens, const mhcTensor *parents, const mhcTensor *drafted,
+                                   const mhcTensor *chosen, const mhcTensor *lengths, const mhcTensor *path,
+                                   const mhcTensor *accepted, const mhcTensor *next, const mhcTensor *newLengths,
+                                   uint64_t *workspaceSize, mhcServeExecutor **executor)
+{
+    if (tokens == nullptr || workspaceSize == nullptr || executor == nullptr) {
+        return MHC_STATUS_NULL_ARGUMENT;
+    }
+    if (tokens->ndim != 2 || tokens->dims[0] < 0 || tokens->dims[1] < 0) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    const int64_t B = tokens->dims[0], S = tokens->dims[1];
+    if (B > kMaxTableRows || S > mhc::kDraftNodes) {
+        return MHC_STATUS_UNSUPPORTED_SHAPE;
+    }
+    const int32_t type = tokens->dtype;
+    const int st = first_of(
+        {check_dense(tokens, {MHC_DTYPE_INT32, MHC_DTYPE_INT64}, {B, S}), check_dense(chosen, {type}, {B, S}),
+         parents != nullptr ? check_dense(parents, {MHC_DTYPE_INT32}, {B, S}) : MHC_STATUS_SUCCESS,
+         check_dense(drafted, {MHC_DTYPE_INT32}, {B}), check_dense(lengths, {MHC_DTYPE_INT32}, {B}),
+         check_dense(path, {MHC_DTYPE_INT32}, {B, S}), check_dense(accepted, {MHC_DTYPE_INT32}, {B}),
+         check_dense(next, {type}, {B}), check_dense(newLengths, {MHC_DTYPE_INT32}, {B})});
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    mhcServeExecutor *ex = new (std::nothrow) mhcServeExecutor;
+    if (ex == nullptr) {
+        return MHC_STATUS_HIP_ERROR;
+    }
+    ex->op = Op::kAccept;
+    ex->empty = B == 0;
+    ex->accept = {static_cast<int>(B),
+                  static_cast<int>(S),
+                  type == MHC_DTYPE_INT64,
+                  tokens->data,
+                  chosen->data,
+                  parents != nullptr ? static_cast<const int32_t *>(parents->data) : nullptr,
+                  static_cast<const int32_t *>(drafted->data),
+                  static_cast<const int32_t *>(lengths->data),
+                  static_cast<int32_t *>(path->data),
+                  static_cast<int32_t *>(accepted->data),
+                  static_cast<int32_t *>(newLengths->data),
+                  next->data};
+    return finish(ex, accepted->data, workspaceSize, executor);
+}
+
+int mhcDraftAccept(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor, hipStream_t stream)
+{
+    return launch(Op::kAccept, workspace, workspaceSize, executor, stream);
+}
+
+int mhcCacheKeepGetWorkspaceSize(const mhcStridedTensor *kCache, const mhcStridedTensor *vCache,
+                                 const mhcTensor *pageTable, const mhcTensor *lengths, const mhcTensor *drafted,
+                                 const mhcTensor *path, uint64_t *workspaceSize, mhcServeExecutor **executor)
+{
+    if (vCache == nullptr || path == nullptr || workspaceSize == nullptr || executor == nullptr) {
+        return MHC_STATUS_NULL_ARGUMENT;
+    }
+    int st = cache_limits(kCache);
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    const int64_t pages = kCache->dims[0], pageSize = kCache->dims[1], kvHeads = kCache->dims[2], d = kCache->dims[3];
+    if (path->ndim != 2 || path->dims[1] < 0) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    if ((st = table_limits(pageTable, lengths, pages, pageSize)) != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    const int64_t B = pageTable->dims[0], S = path->dims[1];
+    const int size = elem_bytes(kCache->dtype);
+    if (S > kMaxCount || d > (1 << 16) || kvHeads > 65536 || kvHeads * d > kMaxCount) {
+        return MHC_STATUS_UNSUPPORTED_SHAPE;
+    }
+    st = first_of({check_strided(kCache, kCache->dtype, {pages, pageSize, kvHeads, d}, size > 0 ? size : 2),
+                   check_strided(vCache, kCache->dtype, {pages, pageSize, kvHeads, d}, size > 0 ? size : 2),
+                   check_dense(drafted, {MHC_DTYPE_INT32}, {B}), check_dense(path, {MHC_DTYPE_INT32}, {B, S})});
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    mhcServeExecutor *ex = new (std::nothrow) mhcServeExecutor;
+    if (ex == nullptr) {
+        return MHC_STATUS_HIP_ERROR;
+    }
+    ex->op = Op::kKeep;
+    ex->empty = B == 0 || S == 0;
+    ex->keep = {cache_rows(kCache),
+                cache_rows(vCache),
+                pages,
+                static_cast<int>(pageSize),
+                static_cast<int>(pageTable->dims[1]),
+                static_cast<int>(kvHeads),
+                static_cast<int>(d) * size,
+                size,
+                static_cast<int>(B),
+                static_cast<int>(S),
+                static_cast<const int32_t *>(pageTable->data),
+                static_cast<const int32_t *>(lengths->data),
+                static_cast<const int32_t *>(drafted->data),
+                static_cast<const int32_t *>(path->data)};
+    return finish(ex, kCache->data, workspaceSize, executor);
+}
+
+int mhcCacheKeep(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor, hipStream_t stream)
+{
+    return launch(Op::kKeep, workspace, workspaceSize, executor, stream);
+}
+
+int mhcCacheBoundsGetWorkspaceSize(const mhcStridedTensor *kCache, const mhcTensor *pageTable, const mhcTensor *lengths,
+                                   const mhcTensor *counts, int64_t tokens, const mhcStridedTensor *lo,
+                                   const mhcStridedTensor *hi, uint64_t *workspaceSize, mhcServeExecutor **executor)
+{
+    if (lo == nullptr || hi == nullptr || workspaceSize == nullptr || executor == nullptr) {
+        return MHC_STATUS_NULL_ARGUMENT;
+    }
+    int st = cache_limits(kCache);
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    const int64_t pages = kCache->dims[0], pageSize = kCache->dims[1], kvHeads = kCache->dims[2], d = kCache->dims[3];
+    if (kCache->dtype != MHC_DTYPE_FLOAT16 && kCache->dtype != MHC_DTYPE_BF16) {
+        return MHC_STATUS_INVALID_DTYPE;
+    }
+    if ((st = table_limits(pageTable, lengths, pages, pageSize)) != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    const int64_t B = pageTable->dims[0];
+    if (tokens < 0) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    if (!mhc::paged_attention_head_size(d) || kvHeads > 65536) {
+        return MHC_STATUS_UNSUPPORTED_SHAPE;
+    }
+    st = first_of({check_strided(kCache, kCache->dtype, {pages, pageSize, kvHeads, d}, 16),
+                   check_strided(lo, kCache->dtype, {pages, kvHeads, d}, 16),
+                   check_strided(hi, kCache->dtype, {pages, kvHeads, d}, 16),
+                   check_dense(counts, {MHC_DTYPE_INT32}, {B})});
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    mhcServeExecutor *ex = new (std::nothrow) mhcServeExecutor;
+    if (ex == nullptr) {
+        return MHC_STATUS_HIP_ERROR;
+    }
+    ex->op = Op::kBounds;
+    ex->empty = B == 0 || tokens == 0;
+    ex->bounds = mhc::CacheBoundsArgs{};
+    mhc::CacheBoundsArgs &a = ex->bounds;
+    a.isBf16 = kCache->dtype == MHC_DTYPE_BF16;
+    a.B = static_cast<int>(B);
+    a.kvHeads = static_cast<int>(kvHeads);
+    a.d = static_cast<int>(d);
+    a.k = cache_rows(kCache);
+    a.lo = head_rows(lo);
+    a.hi = head_rows(hi);
+    a.pages = pages;
+    a.pageSize = static_cast<int>(pageSize);
+    a.width = static_cast<int>(pageTable->dims[1]);
+    a.tokens = static_cast<int>(tokens < kMaxCount ? tokens : kMaxCount);
+    a.table = static_cast<const int32_t *>(pageTable->data);
+    a.lengths = static_cast<const int32_t *>(lengths->data);
+    a.counts = static_cast<const int32_t *>(counts->data);
+    return finish(ex, kCache->data, workspaceSize, executor);
+}
+
+int mhcCacheBounds(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor, hipStream_t stream)
+{
+    return launch(Op::kBounds, workspace, workspaceSize, executor, stream);
+}
+
+int mhcSparseAttentionGetWorkspaceSize(const mhcStridedTensor *q, const mhcStridedTensor *kCache,
+                                       const mhcStridedTensor *vCache, const mhcStridedTensor *lo,
+                                       const mhcStridedTensor *hi, const mhcTensor *pageTable,
+                                       const mhcTensor *lengths, int64_t top, int64_t first, int64_t last, float scale,
+                                       const mhcStridedTensor *out, const mhcTensor *lse, const mhcTensor *columns,
+                                       uint64_t *workspaceSize, mhcServeExecutor **executor)
+{
+    mhc::SparseAttentionArgs s{};
+    int st = attention_args(q, kCache, vCache, pageTable, lengths, scale, 0, out, lse, workspaceSize, executor,
+                            s.attention);
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    const int64_t pages = kCache->dims[0], kvHeads = kCache->dims[2], d = kCache->dims[3], B = q->dims[0];
+    if (first < 0 || last < 0 || top < 1 || first > top || last > top - first) {
+        return MHC_STATUS_INVALID_SHAPE;
+    }
+    if (top > kMaxCount / kCache->dims[1]) {
+        return MHC_STATUS_UNSUPPORTED_SHAPE;
+    }
+    st = first_of({check_strided(lo, q->dtype, {pages, kvHeads, d}, 16), check_strided(hi, q->dtype, {pages, kvHeads, d}, 16),
+                   check_dense(columns, {MHC_DTYPE_INT32}, {B, kvHeads, top})});
+    if (st != MHC_STATUS_SUCCESS) {
+        return st;
+    }
+    s.lo = head_rows(lo);
+    s.hi = head_rows(hi);
+    s.top = static_cast<int>(top);
+    s.first = static_cast<int>(first);
+    s.last = static_cast<int>(last);
+    s.columns = static_cast<int32_t *>(columns->data);
+    if (!mhc::sparse_attention_fits(s)) {
+        return MHC_STATUS_UNSUPPORTED_SHAPE;
+    }
+    mhcServeExecutor *ex = new (std::nothrow) mhcServeExecutor;
+    if (ex == nullptr) {
+        return MHC_STATUS_HIP_ERROR;
+    }
+    ex->op = Op::kSparse;
+    ex->empty = B == 0;
+    ex->sparse = s;
+    return finish(ex, q->data, workspaceSize, executor);
+}
+
+int mhcSparseAttention(void *workspace, uint64_t workspaceSize, mhcServeExecutor *executor, hipStream_t stream)
+{
+    return launch(Op::kSparse, workspace, workspaceSize, executor, stream);
 }
 
 }  // extern "C"

@@ -1,6 +1,7 @@
 // PyTorch operators over the serving operators' C ABI (include/mhc_serve.h):
 //   torch.ops.mhcpre.qk_norm_rope, qk_norm_rope_append, paged_attention,
-//   cache_update, cache_compact, cache_copy_pages
+//   cache_update, cache_compact, cache_copy_pages, draft_attention,
+//   draft_accept, cache_keep, cache_bounds, sparse_attention
 //
 // Each call runs phase 1 on the given tensors, takes outputs and workspace
 // from PyTorch's caching allocator and launches on the current stream.  The
@@ -13,6 +14,7 @@
 #include <torch/library.h>
 
 #include <cmath>
+#include <vector>
 
 #include "mhc_serve.h"
 
@@ -285,6 +287,145 @@ void cache_copy_pages(const at::Tensor &kCache, const at::Tensor &vCache, const 
     enqueue("mhcCacheCopyPagesGetWorkspaceSize", st, "mhcCacheCopyPages", mhcCacheCopyPages, owner, bytes, kCache);
 }
 
+// x [B, S, heads, d] with rows and heads that start at multiples of 8 elements, copied where
+// they do not.
+at::Tensor token_rows(const at::Tensor &x, const char *name)
+{
+    TORCH_CHECK(x.dim() == 4, "mhcpre: ", name, " must be [B, S, heads, d]");
+    bool whole = (x.size(3) <= 1 || x.stride(3) == 1) &&
+                 reinterpret_cast<uintptr_t>(x.data_ptr()) % (8 * x.element_size()) == 0;
+    for (int64_t i = 0; i < 3; ++i) {
+        whole = whole && (x.size(i) <= 1 || (x.stride(i) >= 0 && x.stride(i) % 8 == 0));
+    }
+    return whole ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+bool given(const std::optional<at::Tensor> &t) { return t.has_value() && t->defined(); }
+
+std::tuple<at::Tensor, at::Tensor> draft_attention(const at::Tensor &q_, const at::Tensor &kCache,
+                                                   const at::Tensor &vCache, const at::Tensor &pageTable_,
+                                                   const at::Tensor &lengths_, const at::Tensor &drafted_,
+                                                   const std::optional<at::Tensor> &parents_,
+                                                   std::optional<double> scale, int64_t window)
+{
+    same_device(q_, {&kCache, &vCache, &pageTable_, &lengths_, &drafted_});
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(q_.device());
+    const at::Tensor q = token_rows(q_, "q"), pageTable = pageTable_.contiguous(), lengths = flat(lengths_),
+                     drafted = flat(drafted_);
+    at::Tensor parents;
+    mhcTensor dp{};
+    if (given(parents_)) {
+        same_device(q, {&*parents_});
+        parents = parents_->contiguous();
+        dp = dense(parents);
+    }
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    at::Tensor lse = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
+    const mhcStridedTensor dq = strided(q), dkc = strided(kCache), dvc = strided(vCache), dout = strided(out);
+    const mhcTensor dt = dense(pageTable), dl = dense(lengths), dd = dense(drafted), dlse = dense(lse);
+    const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(3)));
+    uint64_t bytes = 0;
+    ExecutorOwner owner;
+    const int st = mhcDraftAttentionGetWorkspaceSize(&dq, &dkc, &dvc, &dt, &dl, &dd,
+                                                     parents.defined() ? &dp : nullptr, static_cast<float>(s), window,
+                                                     &dout, &dlse, &bytes, &owner.exe);
+    enqueue("mhcDraftAttentionGetWorkspaceSize", st, "mhcDraftAttention", mhcDraftAttention, owner, bytes, q);
+    return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> draft_accept(const at::Tensor &tokens_,
+                                                                        const std::optional<at::Tensor> &parents_,
+                                                                        const at::Tensor &drafted_,
+                                                                        const at::Tensor &chosen_,
+                                                                        const at::Tensor &lengths_)
+{
+    same_device(tokens_, {&drafted_, &chosen_, &lengths_});
+    TORCH_CHECK(tokens_.dim() == 2, "mhcpre: tokens must be [B, S]");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(tokens_.device());
+    const at::Tensor tokens = tokens_.contiguous(), chosen = chosen_.contiguous(), drafted = flat(drafted_),
+                     lengths = flat(lengths_);
+    at::Tensor parents;
+    mhcTensor dp{};
+    if (given(parents_)) {
+        same_device(tokens, {&*parents_});
+        parents = parents_->contiguous();
+        dp = dense(parents);
+    }
+    const auto i32 = tokens.options().dtype(at::kInt);
+    const int64_t B = tokens.size(0);
+    at::Tensor path = at::empty(tokens.sizes(), i32), accepted = at::empty({B}, i32),
+               next = at::empty({B}, tokens.options()), newLengths = at::empty({B}, i32);
+    const mhcTensor dt = dense(tokens), dc = dense(chosen), dd = dense(drafted), dl = dense(lengths),
+                    dpath = dense(path), da = dense(accepted), dn = dense(next), dnl = dense(newLengths);
+    uint64_t bytes = 0;
+    ExecutorOwner owner;
+    const int st = mhcDraftAcceptGetWorkspaceSize(&dt, parents.defined() ? &dp : nullptr, &dd, &dc, &dl, &dpath, &da,
+                                                  &dn, &dnl, &bytes, &owner.exe);
+    enqueue("mhcDraftAcceptGetWorkspaceSize", st, "mhcDraftAccept", mhcDraftAccept, owner, bytes, tokens);
+    return {path, accepted, next, newLengths};
+}
+
+void cache_keep(const at::Tensor &kCache, const at::Tensor &vCache, const at::Tensor &pageTable_,
+                const at::Tensor &lengths_, const at::Tensor &drafted_, const at::Tensor &path_)
+{
+    same_device(kCache, {&vCache, &pageTable_, &lengths_, &drafted_, &path_});
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(kCache.device());
+    const at::Tensor pageTable = pageTable_.contiguous(), lengths = flat(lengths_), drafted = flat(drafted_),
+                     path = path_.contiguous();
+    const mhcStridedTensor dk = strided(kCache), dv = strided(vCache);
+    const mhcTensor dt = dense(pageTable), dl = dense(lengths), dd = dense(drafted), dp = dense(path);
+    uint64_t bytes = 0;
+    ExecutorOwner owner;
+    const int st = mhcCacheKeepGetWorkspaceSize(&dk, &dv, &dt, &dl, &dd, &dp, &bytes, &owner.exe);
+    enqueue("mhcCacheKeepGetWorkspaceSize", st, "mhcCacheKeep", mhcCacheKeep, owner, bytes, kCache);
+}
+
+void cache_bounds(const at::Tensor &kCache, const at::Tensor &pageTable_, const at::Tensor &lengths_,
+                  const at::Tensor &counts_, const at::Tensor &lo, const at::Tensor &hi, int64_t tokens)
+{
+    same_device(kCache, {&pageTable_, &lengths_, &counts_, &lo, &hi});
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(kCache.device());
+    const at::Tensor pageTable = pageTable_.contiguous(), lengths = flat(lengths_), counts = flat(counts_);
+    const mhcStridedTensor dk = strided(kCache), dlo = strided(lo), dhi = strided(hi);
+    const mhcTensor dt = dense(pageTable), dl = dense(lengths), dc = dense(counts);
+    uint64_t bytes = 0;
+    ExecutorOwner owner;
+    const int st = mhcCacheBoundsGetWorkspaceSize(&dk, &dt, &dl, &dc, tokens, &dlo, &dhi, &bytes, &owner.exe);
+    enqueue("mhcCacheBoundsGetWorkspaceSize", st, "mhcCacheBounds", mhcCacheBounds, owner, bytes, kCache);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> sparse_attention(const at::Tensor &q_, const at::Tensor &kCache,
+                                                                const at::Tensor &vCache, const at::Tensor &lo,
+                                                                const at::Tensor &hi, const at::Tensor &pageTable_,
+                                                                const at::Tensor &lengths_, int64_t top, int64_t first,
+                                                                int64_t last, std::optional<double> scale)
+{
+    same_device(q_, {&kCache, &vCache, &lo, &hi, &pageTable_, &lengths_});
+    TORCH_CHECK(kCache.dim() == 4, "mhcpre: k_cache must be [pages, page_size, kv_heads, d]");
+    TORCH_CHECK(top >= 1, "mhcpre: top ", top);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(q_.device());
+    const at::Tensor q = head_rows(q_, "q", 8), pageTable = pageTable_.contiguous(), lengths = flat(lengths_);
+    at::Tensor out = at::empty(q.sizes(), q.options());
+    at::Tensor lse = at::empty(q.sizes().slice(0, 2), q.options().dtype(at::kFloat));
+    at::Tensor columns = at::empty({q.size(0), kCache.size(2), top}, q.options().dtype(at::kInt));
+    const mhcStridedTensor dq = strided(q), dkc = strided(kCache), dvc = strided(vCache), dlo = strided(lo),
+                           dhi = strided(hi), dout = strided(out);
+    const mhcTensor dt = dense(pageTable), dl = dense(lengths), dlse = dense(lse), dc = dense(columns);
+    const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(2)));
+    uint64_t bytes = 0;
+    ExecutorOwner owner;
+    const int st = mhcSparseAttentionGetWorkspaceSize(&dq, &dkc, &dvc, &dlo, &dhi, &dt, &dl, top, first, last,
+                                                      static_cast<float>(s), &dout, &dlse, &dc, &bytes, &owner.exe);
+    enqueue("mhcSparseAttentionGetWorkspaceSize", st, "mhcSparseAttention", mhcSparseAttention, owner, bytes, q);
+    if (q_.dim() == 3) {
+        return {out, lse, columns};
+    }
+    std::vector<int64_t> shape(q_.sizes().begin(), q_.sizes().end() - 2);
+    shape.push_back(kCache.size(2));
+    shape.push_back(top);
+    return {out.view(q_.sizes()), lse.view(q_.sizes().slice(0, q_.dim() - 1)), columns.view(shape)};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(mhcpre, m)
@@ -302,6 +443,16 @@ TORCH_LIBRARY_FRAGMENT(mhcpre, m)
     m.def("cache_compact(Tensor page_table, Tensor lengths, int pages, int page_size) "
           "-> (Tensor, Tensor, Tensor, Tensor)");
     m.def("cache_copy_pages(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor src, Tensor dst) -> ()");
+    m.def("draft_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor lengths, "
+          "Tensor drafted, Tensor? parents=None, float? scale=None, int window=0) -> (Tensor, Tensor)");
+    m.def("draft_accept(Tensor tokens, Tensor? parents, Tensor drafted, Tensor chosen, Tensor lengths) "
+          "-> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("cache_keep(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor page_table, Tensor lengths, Tensor drafted, "
+          "Tensor path) -> ()");
+    m.def("cache_bounds(Tensor k_cache, Tensor page_table, Tensor lengths, Tensor counts, Tensor(a!) lo, "
+          "Tensor(b!) hi, int tokens=1) -> ()");
+    m.def("sparse_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor lo, Tensor hi, Tensor page_table, "
+          "Tensor lengths, int top, int first=1, int last=1, float? scale=None) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mhcpre, CUDA, m)
@@ -312,4 +463,9 @@ TORCH_LIBRARY_IMPL(mhcpre, CUDA, m)
     m.impl("cache_update", &cache_update);
     m.impl("cache_compact", &cache_compact);
     m.impl("cache_copy_pages", &cache_copy_pages);
+    m.impl("draft_attention", &draft_attention);
+    m.impl("draft_accept", &draft_accept);
+    m.impl("cache_keep", &cache_keep);
+    m.impl("cache_bounds", &cache_bounds);
+    m.impl("sparse_attention", &sparse_attention);
 }

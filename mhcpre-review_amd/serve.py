@@ -50,6 +50,11 @@ def load_serve_library() -> ctypes.CDLL:
         "mhcCacheUpdate": [T, T, T, T, i64, i64, T, T, T, T, T, T],
         "mhcCacheCompact": [T, T, i64, i64, T, T, T, T],
         "mhcCacheCopyPages": [S, S, T, T],
+        "mhcDraftAttention": [S, S, S, T, T, T, T, f32, i64, S, T],
+        "mhcDraftAccept": [T, T, T, T, T, T, T, T, T],
+        "mhcCacheKeep": [S, S, T, T, T, T],
+        "mhcCacheBounds": [S, T, T, T, i64, S, S],
+        "mhcSparseAttention": [S, S, S, S, S, T, T, i64, i64, i64, f32, S, T, T],
     }
     for name, args in phase1.items():
         first, second = getattr(lib, name + "GetWorkspaceSize"), getattr(lib, name)
@@ -258,3 +263,88 @@ class CopyPagesOp(_ServeOp):
 
     def __init__(self, k_cache, v_cache, src, dst):
         self._create([_strided(k_cache), _strided(v_cache), _dense(src), _dense(dst)], [k_cache, v_cache, src, dst])
+
+
+class DraftAttentionOp(_ServeOp):
+    """mhcDraftAttention on q ``[B, S, heads, d]``: a tree of drafted tokens
+    (``parents`` int32 ``[B, S]``) or a chain (None).  ``out`` and ``lse`` (fp32
+    ``[B, S, heads]``; ``lse=False``: not written) are attributes."""
+
+    _name = "mhcDraftAttention"
+
+    def __init__(self, q, k_cache, v_cache, page_table, lengths, drafted, parents=None, scale: Optional[float] = None,
+                 window: int = 0, out=None, lse=None, workspace=None):
+        import torch
+
+        self.out = out if out is not None else torch.empty_like(q, memory_format=torch.contiguous_format)
+        if lse is None:
+            lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
+        self.lse = lse if lse is not False else None
+        scale = q.shape[-1] ** -0.5 if scale is None else scale
+        self._create([_strided(q), _strided(k_cache), _strided(v_cache), _dense(page_table), _dense(lengths),
+                      _dense(drafted), _dense(parents), scale, window, _strided(self.out), _dense(self.lse)],
+                     [q, k_cache, v_cache, page_table, lengths, drafted, parents, self.out, self.lse], workspace)
+
+
+class DraftAcceptOp(_ServeOp):
+    """mhcDraftAccept on tokens ``[B, S]``; attributes ``path``, ``accepted``,
+    ``next`` and ``new_lengths``."""
+
+    _name = "mhcDraftAccept"
+
+    def __init__(self, tokens, parents, drafted, chosen, lengths):
+        import torch
+
+        i32 = dict(dtype=torch.int32, device=tokens.device)
+        rows = tokens.shape[0]
+        self.path = torch.empty(tokens.shape, **i32)
+        self.accepted, self.new_lengths = torch.empty(rows, **i32), torch.empty(rows, **i32)
+        self.next = torch.empty(rows, dtype=tokens.dtype, device=tokens.device)
+        self._create([_dense(tokens), _dense(parents), _dense(drafted), _dense(chosen), _dense(lengths),
+                      _dense(self.path), _dense(self.accepted), _dense(self.next), _dense(self.new_lengths)],
+                     [tokens, parents, drafted, chosen, lengths, self.path, self.accepted, self.next,
+                      self.new_lengths])
+
+
+class CacheKeepOp(_ServeOp):
+    """mhcCacheKeep: the tokens of ``path`` to the places behind the context."""
+
+    _name = "mhcCacheKeep"
+
+    def __init__(self, k_cache, v_cache, page_table, lengths, drafted, path):
+        self._create([_strided(k_cache), _strided(v_cache), _dense(page_table), _dense(lengths), _dense(drafted),
+                      _dense(path)], [k_cache, v_cache, page_table, lengths, drafted, path])
+
+
+class CacheBoundsOp(_ServeOp):
+    """mhcCacheBounds: ``lo`` and ``hi`` ``[pages, kv_heads, d]`` of the pages with
+    the rows' last ``counts`` tokens, ``tokens`` at most."""
+
+    _name = "mhcCacheBounds"
+
+    def __init__(self, k_cache, page_table, lengths, counts, lo, hi, tokens: int = 1):
+        self._create([_strided(k_cache), _dense(page_table), _dense(lengths), _dense(counts), tokens, _strided(lo),
+                      _strided(hi)], [k_cache, page_table, lengths, counts, lo, hi])
+
+
+class SparseAttentionOp(_ServeOp):
+    """mhcSparseAttention on q ``[B, heads, d]``; ``out``, ``lse`` (as for
+    :class:`PagedAttentionOp`) and ``columns`` int32 ``[B, kv_heads, top]`` are
+    attributes."""
+
+    _name = "mhcSparseAttention"
+
+    def __init__(self, q, k_cache, v_cache, lo, hi, page_table, lengths, top: int, first: int = 1, last: int = 1,
+                 scale: Optional[float] = None, out=None, lse=None, workspace=None):
+        import torch
+
+        self.out = out if out is not None else torch.empty_like(q, memory_format=torch.contiguous_format)
+        if lse is None:
+            lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
+        self.lse = lse if lse is not False else None
+        self.columns = torch.empty((q.shape[0], k_cache.shape[2], top), dtype=torch.int32, device=q.device)
+        scale = q.shape[-1] ** -0.5 if scale is None else scale
+        self._create([_strided(q), _strided(k_cache), _strided(v_cache), _strided(lo), _strided(hi),
+                      _dense(page_table), _dense(lengths), top, first, last, scale, _strided(self.out),
+                      _dense(self.lse), _dense(self.columns)],
+                     [q, k_cache, v_cache, lo, hi, page_table, lengths, self.out, self.lse, self.columns], workspace)

@@ -1,9 +1,10 @@
 """PyTorch operators ``torch.ops.mhcpre.mhc_pre`` and
 ``torch.ops.mhcpre.mhc_pre_with_h_pre``, and the serving operators
 ``qk_norm_rope``, ``qk_norm_rope_append``, ``paged_attention``,
-``cache_update``, ``cache_compact`` and ``cache_copy_pages`` (native too, from
-``csrc/mhc_serve_torch.cpp`` over ``include/mhc_serve.h``, which says what each
-computes).
+``cache_update``, ``cache_compact``, ``cache_copy_pages``, ``draft_attention``,
+``draft_accept``, ``cache_keep``, ``cache_bounds`` and ``sparse_attention``
+(native too, from ``csrc/mhc_serve_torch.cpp`` over ``include/mhc_serve.h``, which
+says what each computes).
 
 The serving operators take x-like tensors as ``[..., heads, d]`` with any
 leading dimensions; inputs that are not laid out as the C ABI wants them are
@@ -148,3 +149,31 @@ def _(page_table, lengths, pages, page_size):
 @torch.library.register_fake(f"{_LIB_NAME}::cache_copy_pages")
 def _(k_cache, v_cache, src, dst):
     return None
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::draft_attention")
+def _(q, k_cache, v_cache, page_table, lengths, drafted, parents=None, scale=None, window=0):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::draft_accept")
+def _(tokens, parents, drafted, chosen, lengths):
+    rows = tokens.shape[:1]
+    return (tokens.new_empty(tokens.shape, dtype=torch.int32), tokens.new_empty(rows, dtype=torch.int32),
+            tokens.new_empty(rows), tokens.new_empty(rows, dtype=torch.int32))
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::cache_keep")
+def _(k_cache, v_cache, page_table, lengths, drafted, path):
+    return None
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::cache_bounds")
+def _(k_cache, page_table, lengths, counts, lo, hi, tokens=1):
+    return None
+
+
+@torch.library.register_fake(f"{_LIB_NAME}::sparse_attention")
+def _(q, k_cache, v_cache, lo, hi, page_table, lengths, top, first=1, last=1, scale=None):
+    return (q.new_empty(q.shape), q.new_empty(q.shape[:-1], dtype=torch.float32),
+            q.new_empty(q.shape[:-2] + (k_cache.shape[2], top), dtype=torch.int32))
