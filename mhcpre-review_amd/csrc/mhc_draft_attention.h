@@ -35,7 +35,6 @@ using attention::bf16x8v_t;
 using attention::f16x8_t;
 using attention::kLn2;
 using attention::kLog2e;
-using attention::read_transposed;
 using attention::shfl64;
 using attention::u32x2_t;
 using dev::f32x4_t;
@@ -46,28 +45,60 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kRows = 32;  // of a wave
 
+// What is loaded in the place of keys that nobody sees (a row of the largest size).
+__device__ const uint32_t kZeros[128] = {};
+
+// 16 bytes a lane from memory to LDS, lane by lane from `to` on.  In assembly, for the
+// compiler would let every read of LDS wait for all such loads: the caller waits
+// (dev::wait_vm) before a tile is read.  (m0 is no register that the compiler hands out.)
+__device__ __forceinline__ void load_to_lds(const void *from, __attribute__((address_space(3))) char *to)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"((uint32_t)(uintptr_t)to), "v"(from)
+                 : "memory");
+}
+
 // How a workgroup's waves are laid out: kRowWaves share a tile, each with rows of its
-// own, and kKeyWaves such groups have tiles of their own.
+// own, and kKeyWaves such groups have tiles of their own.  Tiles come from memory
+// straight into LDS, the next one while this one is worked on.
 template <int D_, int kRowWaves_, int kKeyWaves_, int kTile_>
 struct Layout {
     static constexpr int D = D_, kRowWaves = kRowWaves_, kKeyWaves = kKeyWaves_, kTile = kTile_;
-    static constexpr int kThreads = kWave * kRowWaves * kKeyWaves;
+    static constexpr int kWaves = kRowWaves * kKeyWaves, kThreads = kWave * kWaves;
     static constexpr int kUnit = kTile * kKeyWaves;  // keys of a unit
     static constexpr int kBlock = kRows * kRowWaves;
-    static constexpr int kBuffers = kRowWaves > 1 ? 2 : 1;  // (a wave alone needs no barrier)
-    static constexpr int kChunks = D / 8;                   // 16-byte chunks of a row
-    static constexpr int kLoads = (kTile * kChunks + kWave * kRowWaves - 1) / (kWave * kRowWaves);
-    // LDS bytes between two rows: of K so that 16 rows' chunks, of V so that 4 rows' 64 bytes
-    // lie in different banks.
-    static constexpr int kPitchK = 2 * D + 16, kPitchV = 2 * D + (D % 64 == 0 ? 64 : 0);
-    static constexpr int kBytes = kTile * (kPitchK + kPitchV);  // of a tile
-    static constexpr int kGroup = kBuffers * kBytes;            // of a group of waves
-    static constexpr int kJoin = kKeyWaves > 1 ? kRows * (D + 4) * 4 * kRowWaves * kKeyWaves : 0;
-    static constexpr int kSetup = 256 * 32 + 256 * 4;
-    static constexpr int kTiles = kGroup * kKeyWaves;
+    static constexpr int kChunks = D / 8;                       // 16-byte chunks of a row
+    static constexpr int kSide = kTile * kChunks * 16;          // bytes of a tile of K or V
+    static constexpr int kBuffer = 2 * kSide;                   // K, then V
+    static constexpr int kLoads = kSide / 1024 / kRowWaves;     // of a wave, for either
+    static constexpr int kTiles = 2 * kBuffer * kKeyWaves;
+    static constexpr int kJoin = kKeyWaves > 1 ? kRows * (D + 4) * 4 * kWaves : 0;
+    static constexpr int kSetup = kDraftNodes * (32 + 4);
     static constexpr int kLds = kTiles > kJoin ? (kTiles > kSetup ? kTiles : kSetup) : (kJoin > kSetup ? kJoin : kSetup);
     // Workgroups of a CU: what its registers (two waves a SIMD up to D = 128) and LDS hold.
-    static constexpr int kPerCu = kThreads == 256 && D <= 128 && 2 * (kLds + 4096) <= 160 * 1024 ? 2 : 1;
+    static constexpr int kPerCu = kThreads == 256 && D <= 128 && 2 * (kLds + kBlock * 48) <= 160 * 1024 ? 2 : 1;
+    static_assert(kLoads * kRowWaves * 1024 == kSide && kLds + kBlock * 48 <= 160 * 1024);
+
+    // Where chunk c of row r lies among its row's chunks: turned so that what 16 lanes read at
+    // a time lies in different banks, of K the same chunk of 16 rows, of V 64 bytes of 4 rows.
+    __device__ static constexpr int turn(int r)
+    {
+        return kChunks % 16 == 0  ? (r & 3) << 2 | (r >> 2 & 3)
+               : kChunks % 8 == 0 ? (r >> 1 & 1) << 2 | (r >> 2 & 3)
+                                  : r >> 2 & 3;
+    }
+    __device__ static constexpr uint32_t at(int r, int c) { return (r * kChunks + (c ^ turn(r))) * 16; }
+    // A constant step of `by` chunks (a multiple of the lanes' own range) from place p of a row
+    // whose turn is in p: what the turn reaches changes by an exclusive or, the rest by a sum.
+    static constexpr int kTurned = kChunks % 16 == 0 ? 16 : kChunks % 8 == 0 ? 8 : 4;
+    __device__ static uint32_t step(uint32_t p, int by) { return (p ^ by % kTurned * 16) + by / kTurned * kTurned * 16; }
+};
+
+// What a stretch begins and does not finish: a (sequence, kv head, block), the line's unit
+// at which it begins and its units, and the units of the line.  units 0: nothing.
+struct Open {
+    int b, kv, block, start, units, all;
 };
 
 struct Args {
@@ -78,6 +109,7 @@ struct Args {
     int unit;    // keys of a unit
     int most;    // workgroups of the launch
     float *outs, *ends;  // the parts: [2 * most][rows][D], [2 * most][rows][2]
+    Open *open;          // [most]
 };
 
 // The keys of a block of a sequence with c + n tokens, n of them new: [low, high).
@@ -228,27 +260,127 @@ __device__ __forceinline__ void finish(const Args &args, const Place &p, int nod
     }
 }
 
+// The ancestors of every node of row b, 256 bits each (itself among them), at the start of
+// `lds`.  A node's farthest known ancestor's are its own too: each round doubles how far.
+template <int kThreads>
+__device__ __forceinline__ void find_ancestors(const DraftAttentionArgs &a, int b, int n, char *lds)
+{
+    constexpr int kNodes = kDraftNodes / kThreads > 0 ? kDraftNodes / kThreads : 1;  // of a thread
+    uint64_t *known = reinterpret_cast<uint64_t *>(lds);
+    int *farthest = reinterpret_cast<int *>(lds + kDraftNodes * 32);
+    uint64_t own[kNodes][4];
+    int far[kNodes];
+#pragma unroll
+    for (int k = 0; k < kNodes; ++k) {
+        const int i = k * kThreads + (int)threadIdx.x;
+        far[k] = -1;
+        if (i < n) {
+            const int p = a.parents[(int64_t)b * a.S + i];
+            far[k] = p >= 0 && p < i ? p : -1;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            own[k][x] = i / 64 == x ? 1ull << (i % 64) : 0ull;
+        }
+    }
+    for (int reach = 1;; reach *= 2) {
+#pragma unroll
+        for (int k = 0; k < kNodes; ++k) {
+            const int i = k * kThreads + (int)threadIdx.x;
+            if (i < n) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    known[4 * i + x] = own[k][x];
+                }
+                farthest[i] = far[k];
+            }
+        }
+        __syncthreads();
+        if (reach >= n) {
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < kNodes; ++k) {
+            if (far[k] >= 0) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    own[k][x] |= known[4 * far[k] + x];
+                }
+                far[k] = farthest[far[k]];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Which of the 64 keys from t0 on a node sees: the context from `from` on, and of the new
+// tokens its ancestors, or in a chain those up to itself.
+__device__ __forceinline__ uint64_t seen_keys(bool tree, int c, int node, uint32_t from, int64_t t0,
+                                              const uint64_t (&ancestors)[4])
+{
+    // (positions below 2^31 and their differences fit 33 bits)
+    const int64_t to = (tree ? c : (int64_t)c + node + 1) - t0, first = (int64_t)from - t0;
+    uint64_t seen = low_bits(to > 64 ? 64 : to < 0 ? 0 : (int)to) & ~low_bits(first > 64 ? 64 : first < 0 ? 0 : (int)first);
+    if (tree) {
+        // Bit x of the tile is node x + t0 - c.
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int64_t by = t0 - c - 64 * x;
+            if (by > -64 && by < 64) {
+                seen |= by >= 0 ? ancestors[x] >> by : ancestors[x] << -by;
+            }
+        }
+    }
+    return seen;
+}
+
+// What one of two packed 16-bit values leaves of x.
+template <bool kBf16>
+__device__ __forceinline__ float rest(float x, uint32_t two, int which)
+{
+    if constexpr (kBf16) {  // (cut: the upper half of x itself)
+        return x - __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+    } else {
+        const _Float16 h = __builtin_bit_cast(_Float16, (uint16_t)(which == 0 ? two : two >> 16));
+        return __builtin_fmaf(-(float)h, 1.f, x);
+    }
+}
+
+// 4 values at the same column of 4 rows of LDS (the lane's column of 16).
+__device__ __forceinline__ u32x2_t transposed(uint32_t at)
+{
+    return __builtin_bit_cast(
+        u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attention::s16x4_t *)(uintptr_t)at));
+}
+
+// Keeps the instructions on both sides in the order that they are written in.  (Left to
+// itself the compiler waits for every operand where registers are short.)
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 template <bool kBf16, typename L>
-__global__ __launch_bounds__(L::kThreads, L::kThreads / 256 * L::kPerCu) void draft_units(Args args)
+__global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256) void draft_units(Args args)
 {
     constexpr int D = L::D, kTile = L::kTile, kKt = kTile / 32, kSteps = D / 16, kDims = D / 32;
-    __shared__ __align__(16) char lds[L::kLds];
-    __shared__ uint64_t badKeys[L::kKeyWaves][L::kBuffers];
+    __shared__ __align__(256) char lds[L::kLds];
+    __shared__ uint64_t rowMasks[L::kBlock][4];  // the rows' ancestors
+    __shared__ uint64_t badKeys[L::kKeyWaves][2];
     __shared__ float tops[L::kKeyWaves][L::kBlock], sums[L::kKeyWaves][L::kBlock];
-    __shared__ int again;
+    __shared__ bool odd[L::kWaves];
     const DraftAttentionArgs &a = args.a;
     const int w = (int)blockIdx.x;
     const int lane = (int)threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int rowWave = wave % L::kRowWaves, keyWave = wave / L::kRowWaves;
     const int half = lane / 32, col = lane % 32;
-    char *mine = lds + keyWave * L::kGroup;
-    const auto barrier = [] {
-        if constexpr (L::kRowWaves > 1) {
-            __syncthreads();
-        }
-    };
+    auto *const mine = (__attribute__((address_space(3))) char *)lds + keyWave * 2 * L::kBuffer;
+    // Where a lane reads in a tile: of K row `col` and every second chunk from `half` on; of V
+    // (turned) rows 4 half + .. and + 8, 4 columns of 32.
+    const uint32_t kPlace = L::at(col, half);
+    const uint32_t vPlace = L::at(4 * half + lane % 16 / 4, lane / 16 % 2 * 2 + lane % 4 / 2) + lane % 2 * 8;
 
     const attention::Shares shares(all_units(args), args.most);
+    if (threadIdx.x == 0) {
+        args.open[w].units = 0;
+    }
     if (w >= shares.grid) {
         return;
     }
@@ -263,68 +395,31 @@ __global__ __launch_bounds__(L::kThreads, L::kThreads / 256 * L::kPerCu) void dr
         const bool there = node < seq.n;
 
         // The node's ancestors (itself one of them) among the new tokens, and its depth.
-        uint64_t ancestors[4] = {0, 0, 0, 0};
         int depth = node;
         const bool tree = a.parents != nullptr;
         const int draftFrom = (place.keys.first + place.tile) * L::kUnit;
-        const bool masks = tree && seq.n > 0 &&
-                           (a.window > 0 || (int64_t)draftFrom + (int64_t)tiles * L::kUnit > seq.c);
-        if (masks) {
-            uint64_t *known = reinterpret_cast<uint64_t *>(lds);
-            int *farthest = reinterpret_cast<int *>(lds + 256 * 32);
-            __syncthreads();
-            const int i = (int)threadIdx.x;  // (256 threads at least)
-            uint64_t own[4] = {0, 0, 0, 0};
-            int far = -1;
-            if (i < seq.n) {
-                const int p = a.parents[(int64_t)place.b * a.S + i];
-                far = p >= 0 && p < i ? p : -1;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    own[x] = i / 64 == x ? 1ull << (i % 64) : 0ull;
-                }
-            }
-            for (int reach = 1; reach < seq.n; reach *= 2) {
-                if (i < seq.n) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        known[4 * i + x] = own[x];
-                    }
-                    farthest[i] = far;
-                }
-                __syncthreads();
-                if (far >= 0) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        own[x] |= known[4 * far + x];
-                    }
-                    far = farthest[far];
-                }
-                __syncthreads();
-            }
-            if (i < seq.n) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    known[4 * i + x] = own[x];
-                }
-            }
-            __syncthreads();
+        __syncthreads();  // (the LDS is free)
+        if (tree && seq.n > 0 && (a.window > 0 || (int64_t)draftFrom + (int64_t)tiles * L::kUnit > seq.c)) {
+            find_ancestors<L::kThreads>(a, place.b, seq.n, lds);
+            const uint64_t *known = reinterpret_cast<const uint64_t *>(lds);
             depth = 0;
             if (there) {
+                uint64_t own[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    ancestors[x] = known[4 * node + x];
-                    depth += __popcll(ancestors[x]);
+                    own[x] = known[4 * node + x];
+                    depth += __popcll(own[x]);
                 }
                 depth -= 1;
                 // Of the path only the window's length, from the node up: the lower numbers go.
                 int over = a.window > 0 && a.window < depth + 1 ? depth + 1 - (int)a.window : 0;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    while (over > 0 && ancestors[x] != 0) {
-                        ancestors[x] &= ancestors[x] - 1;
+                    while (over > 0 && own[x] != 0) {
+                        own[x] &= own[x] - 1;
                         --over;
                     }
+                    rowMasks[rowWave * kRows + col][x] = own[x];  // (by all key waves, the same)
                 }
             }
             __syncthreads();
@@ -338,25 +433,25 @@ __global__ __launch_bounds__(L::kThreads, L::kThreads / 256 * L::kPerCu) void dr
         const int64_t wholeFrom = a.window > 0 ? (int64_t)seq.c + seq.n - a.window : 0;
 
         u32x4_t q[kSteps];
-        float c = a.scale * kLog2e;
+        // (Its sign goes to q, for the maximum wants a factor above 0; with a scale of 0 q is 0.)
+        const float c = a.scale == 0.f ? 1.f : fabsf(a.scale * kLog2e);
         {
             const uint16_t *at = static_cast<const uint16_t *>(a.q.data) + place.b * a.q.row + node * a.q.token +
                                  (int64_t)(place.kv * args.group + head) * a.q.head;
-            // (a factor of at least 0 for the maximum's sake: its sign goes to q)
             const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-            c = fabsf(c);
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 q[s] = u32x4_t{0, 0, 0, 0};
-                if (there && 16 * s < a.d) {
+                if (there && a.scale != 0.f && 16 * s < a.d) {
                     q[s] = *reinterpret_cast<const u32x4_t *>(at + 16 * s + 8 * half);
                     q[s] ^= u32x4_t{flip, flip, flip, flip};
                 }
             }
         }
 
-        const uint16_t *kBase = static_cast<const uint16_t *>(a.kCache.data) + place.kv * a.kCache.head;
-        const uint16_t *vBase = static_cast<const uint16_t *>(a.vCache.data) + place.kv * a.vCache.head;
+        const char *kBase = static_cast<const char *>(a.kCache.data) + 2 * place.kv * a.kCache.head;
+        const char *vBase = static_cast<const char *>(a.vCache.data) + 2 * place.kv * a.vCache.head;
+        const int32_t *table = a.table + (int64_t)place.b * a.width;
         f32x16_t o[kDims];
         float top, sum;
         // kChecked: with infinite and NaN values of V set apart.
@@ -373,158 +468,143 @@ __global__ __launch_bounds__(L::kThreads, L::kThreads / 256 * L::kPerCu) void dr
             sum = 0.f;
 
             // The lane's key (lane % kTile) of a tile: its page and slot, then its rows.
-            struct Found {
-                int page, slot;
+            uint32_t t = (uint32_t)(place.keys.first + place.tile) * L::kUnit + keyWave * kTile + lane % kTile;
+            // (Always a load, of the row's first entry where there is no key: under a branch it
+            // would be waited for at once.)
+            int page = -1, slot = 0;
+            bool key = false;
+            const auto find_page = [&](bool more) {
+                key = more && t >= (uint32_t)place.keys.low && t < (uint32_t)place.keys.high;
+                const uint32_t at = (key ? t : 0u) / (uint32_t)a.pageSize;
+                page = table[at];
+                slot = (int)(t - at * (uint32_t)a.pageSize);
+                t += L::kUnit;
             };
-            int ahead = 0;
-            const auto find_page = [&]() {
-                Found f{-1, 0};
-                if (ahead < tiles) {
-                    const uint32_t t = (uint32_t)(place.keys.first + place.tile + ahead) * L::kUnit + keyWave * kTile +
-                                       lane % kTile;
-                    if (t >= (uint32_t)place.keys.low && t < (uint32_t)place.keys.high) {
-                        const uint32_t at = t / (uint32_t)a.pageSize;
-                        f.page = a.table[(int64_t)place.b * a.width + at];
-                        f.slot = (int)(t - at * (uint32_t)a.pageSize);
-                    }
-                    ++ahead;
-                }
-                return f;
-            };
-            u32x4_t kReg[L::kLoads], vReg[L::kLoads];
-            uint64_t loaded = 0;  // keys of the tile in kReg and vReg
-            int64_t vAt = 0;
-            const auto load = [&](const Found &f) {
-                const bool seen = f.page >= 0 && f.page < a.pages;
+            uint64_t loaded = 0;  // keys of the tile on its way
+            const auto load = [&](int buffer) {
+                const bool seen = key && page >= 0 && page < a.pages;
                 loaded = __ballot(seen);
                 if constexpr (kTile == 32) {
                     loaded &= 0xFFFFFFFFull;
                 }
-                // Where there is no key the cache's first row is read instead, and not used.
-                const int64_t kAt = seen ? f.page * a.kCache.page + f.slot * a.kCache.slot : 0;
-                vAt = seen ? f.page * a.vCache.page + f.slot * a.vCache.slot : 0;
+                const char *kRow = seen ? kBase + 2 * (page * a.kCache.page + slot * a.kCache.slot)
+                                        : reinterpret_cast<const char *>(kZeros);
+                const char *vRow = seen ? vBase + 2 * (page * a.vCache.page + slot * a.vCache.slot)
+                                        : reinterpret_cast<const char *>(kZeros);
+                auto *const to = mine + buffer * L::kBuffer;
 #pragma unroll
                 for (int n = 0; n < L::kLoads; ++n) {
-                    const int at = (n * L::kRowWaves + rowWave) * kWave + lane;
-                    const int r = at / L::kChunks, ch = at % L::kChunks;
-                    const int64_t kRow = shfl64(kAt, r % kTile), vRow = shfl64(vAt, r % kTile);
-                    kReg[n] = vReg[n] = u32x4_t{0, 0, 0, 0};
-                    if (ch * 8 < a.d && r < kTile) {
-                        kReg[n] = *reinterpret_cast<const u32x4_t *>(kBase + kRow + ch * 8);
-                        vReg[n] = *reinterpret_cast<const u32x4_t *>(vBase + vRow + ch * 8);
+                    const int first = (n * L::kRowWaves + rowWave) * kWave, at = first + lane;
+                    const int r = at / L::kChunks, ch = at % L::kChunks ^ L::turn(r);
+                    const char *k = reinterpret_cast<const char *>(shfl64(reinterpret_cast<int64_t>(kRow), r)) + ch * 16;
+                    const char *v = reinterpret_cast<const char *>(shfl64(reinterpret_cast<int64_t>(vRow), r)) + ch * 16;
+                    if (ch * 8 >= a.d) {
+                        k = v = reinterpret_cast<const char *>(kZeros);
                     }
+                    load_to_lds(k, to + first * 16);
+                    load_to_lds(v, to + L::kSide + first * 16);
                 }
             };
-            Found next = find_page();
-            load(next);
-            next = find_page();
+            find_page(true);
+            load(0);
+            find_page(tiles > 1);
             for (int tile = 0; tile < tiles; ++tile) {
-                char *kLds = mine + tile % L::kBuffers * L::kBytes, *vLds = kLds + kTile * L::kPitchK;
+                const uint32_t buffer = (uint32_t)(uintptr_t)mine + tile % 2 * L::kBuffer;
+                const uint32_t kFrom = buffer + kPlace, vFrom = buffer + L::kSide + vPlace;
                 const uint64_t valid = loaded;
-                const int64_t vRows = vAt;
-                if constexpr (checked) {
-                    __syncthreads();
-                    if (rowWave == 0 && lane == 0) {
-                        badKeys[keyWave][tile % L::kBuffers] = 0;
-                    }
+                const int64_t t0 = (int64_t)(place.keys.first + place.tile + tile) * L::kUnit + keyWave * kTile;
+                dev::wait_vm<0>();  // (the tile is there, and the next one's pages are known)
+                if constexpr (L::kRowWaves > 1 || checked) {
                     __syncthreads();
                 }
+                if constexpr (checked) {
+                    if (rowWave == 0 && lane == 0) {
+                        badKeys[keyWave][tile % 2] = 0;
+                    }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int n = 0; n < L::kLoads; ++n) {
+                        const int at = (n * L::kRowWaves + rowWave) * kWave + lane;
+                        auto *const place16 = (__attribute__((address_space(3))) u32x4_t *)(uintptr_t)(buffer + L::kSide + at * 16);
+                        u32x4_t v = *place16;
+                        bool bad = false;
 #pragma unroll
-                for (int n = 0; n < L::kLoads; ++n) {
-                    const int at = (n * L::kRowWaves + rowWave) * kWave + lane;
-                    const int r = at / L::kChunks, ch = at % L::kChunks;
-                    if (r < kTile) {
-                        // What the block does not see is zero, whatever the cache holds.
-                        u32x4_t v = (valid >> r & 1u) != 0u ? vReg[n] : u32x4_t{0, 0, 0, 0};
-                        if constexpr (checked) {
-                            bool bad = false;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                if (infinite<kBf16>(v[e])) {
-                                    v[e] &= 0xFFFF0000u;
-                                    bad = true;
-                                }
-                                if (infinite<kBf16>(v[e] >> 16)) {
-                                    v[e] &= 0xFFFFu;
-                                    bad = true;
-                                }
+                        for (int e = 0; e < 4; ++e) {
+                            if (infinite<kBf16>(v[e])) {
+                                v[e] &= 0xFFFF0000u;
+                                bad = true;
                             }
-                            if (bad) {
-                                atomicOr(reinterpret_cast<unsigned long long *>(&badKeys[keyWave][tile % L::kBuffers]),
-                                         1ull << r);
+                            if (infinite<kBf16>(v[e] >> 16)) {
+                                v[e] &= 0xFFFFu;
+                                bad = true;
                             }
                         }
-                        *reinterpret_cast<u32x4_t *>(kLds + r * L::kPitchK + ch * 16) = kReg[n];
-                        *reinterpret_cast<u32x4_t *>(vLds + r * L::kPitchV + ch * 16) = v;
+                        if (bad) {
+                            *place16 = v;
+                            atomicOr(reinterpret_cast<unsigned long long *>(&badKeys[keyWave][tile % 2]),
+                                     1ull << (at / L::kChunks));
+                        }
                     }
-                }
-                if constexpr (checked) {
                     __syncthreads();
-                } else {
-                    barrier();
                 }
-                if (tile + 1 < tiles) {
-                    load(next);
-                    next = find_page();
-                }
+                // (After the last tile: rows of zeros.  Under a branch the page would be waited for.)
+                load((tile + 1) % 2);
+                find_page(tile + 2 < tiles);
 
                 // What the row sees of the tile (its keys from t0 on).
-                const int64_t t0 = (int64_t)(place.keys.first + place.tile + tile) * L::kUnit + keyWave * kTile;
                 constexpr uint64_t kAll = kTile == 64 ? ~0ull : 0xFFFFFFFFull;
                 const bool whole = valid == kAll && t0 >= wholeFrom && t0 + kTile <= wholeTo;
                 uint64_t seen = kAll;
                 if (!whole) {
-                    // (positions below 2^31 and their differences fit 33 bits)
-                    const int64_t ctx = tree ? seq.c : (int64_t)seq.c + node + 1;
-                    const int64_t toCtx = ctx - t0, fromCtx = (int64_t)from - t0;
-                    seen = low_bits(toCtx > 64 ? 64 : toCtx < 0 ? 0 : (int)toCtx) &
-                           ~low_bits(fromCtx > 64 ? 64 : fromCtx < 0 ? 0 : (int)fromCtx);
-                    if (tree) {
-                        // Bit x of the tile is node x + t0 - c.
-                        const int64_t shift = t0 - seq.c;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int64_t by = shift - 64 * x;
-                            if (by > -64 && by < 64) {
-                                seen |= by >= 0 ? ancestors[x] >> by : ancestors[x] << -by;
-                            }
-                        }
-                    }
+                    seen = seen_keys(tree, seq.c, node, from, t0, rowMasks[rowWave * kRows + col]);
                     seen = there ? seen & valid : 0ull;
-                }
-                if (!__any((int)(seen != 0ull))) {
-                    continue;
+                    if (!__any((int)(seen != 0ull))) {
+                        continue;
+                    }
                 }
 
-                f32x16_t s[kKt];
+                f32x16_t s[kKt] = {};
+                {
+                    constexpr int kAll = kSteps * kKt, kAhead = kAll < 6 ? kAll : 6;
+                    u32x4_t k[kAhead];
+                    const auto read = [&](int x) {
+                        return *(__attribute__((address_space(3))) const u32x4_t *)(uintptr_t)(
+                            L::step(kFrom, 2 * (x / kKt)) + x % kKt * 32 * L::kChunks * 16);
+                    };
 #pragma unroll
-                for (int kt = 0; kt < kKt; ++kt) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        s[kt][i] = 0.f;
+                    for (int x = 0; x < kAhead; ++x) {
+                        k[x] = read(x);
                     }
+                    in_order();
 #pragma unroll
-                    for (int x = 0; x < kSteps; ++x) {
-                        const u32x4_t k =
-                            *reinterpret_cast<const u32x4_t *>(kLds + (32 * kt + col) * L::kPitchK + (2 * x + half) * 16);
-                        s[kt] = mfma<kBf16>(k, q[x], s[kt]);
+                    for (int x = 0; x < kAll; ++x) {
+                        s[x % kKt] = mfma<kBf16>(k[x % kAhead], q[x / kKt], s[x % kKt]);
+                        if (x + kAhead < kAll) {
+                            k[x % kAhead] = read(x + kAhead);
+                        }
+                        in_order();
                     }
                 }
-                float most = -INFINITY;
+                if (!whole) {
 #pragma unroll
-                for (int kt = 0; kt < kKt; ++kt) {
-                    const uint32_t bits = (uint32_t)(seen >> (32 * kt)) >> (4 * half);
+                    for (int kt = 0; kt < kKt; ++kt) {
+                        const uint32_t bits = (uint32_t)(seen >> (32 * kt)) >> (4 * half);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (!whole) {
+                        for (int i = 0; i < 16; ++i) {
                             s[kt][i] = (bits >> (8 * (i / 4) + i % 4) & 1u) != 0u ? s[kt][i] : -INFINITY;
                         }
+                    }
+                }
+                float most = s[0][0];
+#pragma unroll
+                for (int kt = 0; kt < kKt; ++kt) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
                         most = fmaxf(most, s[kt][i]);
                     }
                 }
                 most = fmaxf(most, __shfl_xor(most, 32));
-                // (nothing seen: -inf whatever the factor, also 0)
-                const float next_top = fmaxf(top, most == -INFINITY ? -INFINITY : most * c);
+                const float next_top = fmaxf(top, most * c);
                 const float zero = next_top == -INFINITY ? 0.f : next_top;
                 if (__any((int)(next_top > top))) {  // (else the sums are on the right scale)
                     const float keep = __builtin_amdgcn_exp2f(top - zero);
@@ -539,43 +619,53 @@ __global__ __launch_bounds__(L::kThreads, L::kThreads / 256 * L::kPerCu) void dr
                     }
                 }
                 const float shift = kLiftBits<kBf16> - zero;
-                u32x4_t p[kTile / 16][2];
+                // The weights of 16 keys, two at a time, between the products of the 16 before, whose
+                // values of V are read ahead.
+                constexpr int kGroups = kTile / 16, kProducts = kGroups * kDims, kAhead = kProducts < 4 ? kProducts : 4;
+                u32x4_t p[kGroups][2], v[kAhead];
+                const auto weigh = [&](int t, int x) {  // (keys 2 x and 2 x + 1 of the lane's 8)
+                    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x], c, shift));
+                    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x + 1], c, shift));
+                    sum += x0;
+                    sum += x1;
+                    const uint32_t first = attention::cut2<kBf16>(x0, x1);
+                    p[t][0][x] = first;
+                    p[t][1][x] = dev::pack2_x<kBf16>(rest<kBf16>(x0, first, 0), rest<kBf16>(x1, first, 1));
+                };
+                const auto read = [&](int x) {  // (rows r and r + 8 of the tile, the lane's 4 columns of 32)
+                    const uint32_t rows = x / kDims * 16 * L::kChunks * 16;
+                    const u32x2_t v0 = transposed(L::step(vFrom, 4 * (x % kDims)) + rows);
+                    const u32x2_t v1 = transposed(L::step(vFrom ^ 32, 4 * (x % kDims)) + rows + 8 * L::kChunks * 16);
+                    return u32x4_t{v0[0], v0[1], v1[0], v1[1]};
+                };
 #pragma unroll
-                for (int kt = 0; kt < kKt; ++kt) {
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        float x[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            x[e] = __builtin_fmaf(s[kt][i + e], c, shift);
-                            if (!whole) {
-                                x[e] = s[kt][i + e] == -INFINITY ? -INFINITY : x[e];
-                            }
-                            x[e] = __builtin_amdgcn_exp2f(x[e]);
-                            sum += x[e];
-                        }
-                        const uint32_t first = attention::cut2<kBf16>(x[0], x[1]);
-                        p[2 * kt + i / 8][0][i % 8 / 2] = first;
-                        p[2 * kt + i / 8][1][i % 8 / 2] =
-                            dev::pack2_x<kBf16>(x[0] - dev::x_to_f32<kBf16>(first & 0xFFFFu),
-                                                x[1] - dev::x_to_f32<kBf16>(first >> 16));
-                    }
+                for (int x = 0; x < kAhead; ++x) {
+                    v[x] = read(x);
                 }
 #pragma unroll
-                for (int t = 0; t < kTile / 16; ++t) {
+                for (int x = 0; x < 4; ++x) {
+                    weigh(0, x);
+                }
+                in_order();
 #pragma unroll
-                    for (int j = 0; j < kDims; ++j) {
-                        const char *at = vLds + (16 * t + 4 * half + lane % 16 / 4) * L::kPitchV +
-                                         (32 * j + lane / 16 % 2 * 16 + lane % 4 * 4) * 2;
-                        const u32x2_t v0 = read_transposed(at), v1 = read_transposed(at + 8 * L::kPitchV);
-                        const u32x4_t vt = {v0[0], v0[1], v1[0], v1[1]};
-                        o[j] = mfma<kBf16>(vt, p[t][0], o[j]);
-                        o[j] = mfma<kBf16>(vt, p[t][1], o[j]);
+                for (int x = 0; x < kProducts; ++x) {
+                    const int t = x / kDims, j = x % kDims;
+                    o[j] = mfma<kBf16>(v[x % kAhead], p[t][0], o[j]);
+                    o[j] = mfma<kBf16>(v[x % kAhead], p[t][1], o[j]);
+                    if (x + kAhead < kProducts) {
+                        v[x % kAhead] = read(x + kAhead);
                     }
+                    if (t + 1 < kGroups) {
+#pragma unroll
+                        for (int y = j * 4 / kDims; y < (j + 1) * 4 / kDims; ++y) {
+                            weigh(t + 1, y);
+                        }
+                    }
+                    in_order();
                 }
                 if constexpr (checked) {
                     // The infinite and NaN values of the rows that see them.
-                    uint64_t bad = badKeys[keyWave][tile % L::kBuffers];
+                    uint64_t bad = badKeys[keyWave][tile % 2];
                     while (bad != 0) {
                         const int key = __ffsll((unsigned long long)bad) - 1;
                         bad &= bad - 1;
@@ -595,43 +685,51 @@ __global__ __launch_bounds__(L::kThreads, L::kThreads / 256 * L::kPerCu) void dr
                         const bool on = (seen >> key & 1u) != 0u;
                         // (a weight that is 0 in 32 bits is above 0 all the same)
                         weight = weight == 0.f ? 1e-30f : weight;
-                        const uint16_t *from_ = vBase + shfl64(vRows, key);
+                        const uint32_t at = (uint32_t)t0 + key, column = at / (uint32_t)a.pageSize;
+                        const uint16_t *v = reinterpret_cast<const uint16_t *>(
+                            vBase + 2 * (table[column] * a.vCache.page + (at - column * (uint32_t)a.pageSize) * a.vCache.slot));
 #pragma unroll
                         for (int j = 0; j < kDims; ++j) {
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
                                 const int e = 32 * j + 8 * (i / 4) + 4 * half + i % 4;
-                                const uint32_t bits = e < a.d ? from_[e] : 0u;
-                                if (on && infinite<kBf16>(bits)) {
-                                    o[j][i] += weight * dev::x_to_f32<kBf16>(bits);
+                                if (32 * j + i / 8 * 16 < a.d) {  // (e < d, for d % 16 is 0)
+                                    const uint32_t bits = v[e];
+                                    if (on && infinite<kBf16>(bits)) {
+                                        o[j][i] += weight * dev::x_to_f32<kBf16>(bits);
+                                    }
                                 }
                             }
                         }
                     }
                 }
             }
+            dev::wait_vm<0>();  // (the rows of zeros, before the LDS serves for something else)
         };
         pass(std::false_type{});
-        bool odd = false;
+        bool all = true;
 #pragma unroll
         for (int j = 0; j < kDims; ++j) {
-            float all = 0.f;
+            float none = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                all += o[j][i] * 0.f;
+                none += o[j][i] * 0.f;
             }
-            odd = odd || all != 0.f;
+            all = all && none == 0.f;
+        }
+        if (lane == 0) {
+            odd[wave] = false;
+        }
+        if (!all) {
+            odd[wave] = true;
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            again = 0;
+        bool again = false;
+#pragma unroll
+        for (int x = 0; x < L::kWaves; ++x) {
+            again = again || odd[x];
         }
-        __syncthreads();
-        if (odd) {
-            again = 1;
-        }
-        __syncthreads();
-        if (again != 0) {
+        if (again) {
             pass(std::true_type{});
         }
 
@@ -648,6 +746,9 @@ __global__ __launch_bounds__(L::kThreads, L::kThreads / 256 * L::kPerCu) void dr
             }
         }
         const bool whole = place.tile == 0 && tiles == place.keys.units;
+        if (threadIdx.x == 0 && place.tile == 0 && !whole) {
+            args.open[w] = Open{place.b, place.kv, place.block, place.start, place.keys.units, shares.units};
+        }
         const int slot = 2 * w + (unit == begin ? 0 : 1);
         // 4 values of row r of the block.
         const auto put = [&](int r, int e, f32x4_t all, float t, float s) {
@@ -732,8 +833,8 @@ __global__ __launch_bounds__(L::kThreads, L::kThreads / 256 * L::kPerCu) void dr
     }
 }
 
-// Joins the parts of the (sequence, kv head, block)s that no stretch finished: one
-// workgroup for some rows of one.
+// Joins the parts of the (sequence, kv head, block)s that no stretch finished: a workgroup
+// for some rows of the one that stretch blockIdx.x began.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBatch = 8;
 
@@ -741,33 +842,21 @@ template <bool kBf16, int D>
 __global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
 {
     const DraftAttentionArgs &a = args.a;
-    const int perRow = a.kvHeads * args.blocks;
-    const int item = (int)blockIdx.x;
+    const Open open = args.open[blockIdx.x];
+    if (open.units == 0) {
+        return;
+    }
     const int r = (int)blockIdx.y * (kJoinThreads / (D / 4)) + (int)threadIdx.x / (D / 4);
     const int e = (int)threadIdx.x % (D / 4) * 4;
-    const attention::Shares shares(all_units(args), args.most);
-    // Where the item begins.
+    const attention::Shares shares(open.all, args.most);
     Place p{};
-    p.b = item / perRow;
-    p.kv = item % perRow / args.blocks;
-    p.block = item % args.blocks;
-    const int lane = (int)threadIdx.x % kWave;
-    int base = 0;
-    for (int b0 = 0; b0 < p.b; b0 += kWave) {
-        const int x = b0 + lane;
-        base += __builtin_amdgcn_readlane(
-            dev::wave_scan(x < p.b ? Sequence(a, x).units(args) * a.kvHeads : 0), kWave - 1);
-    }
-    const Sequence seq(a, p.b);
-    base += p.kv * seq.units(args);
-    for (int x = 0; x < p.block; ++x) {
-        base += seq.keys(args, x).units;
-    }
-    p.keys = seq.keys(args, p.block);
-    const int first = shares.owner(base), last = shares.owner(base + p.keys.units - 1);
+    p.b = open.b;
+    p.kv = open.kv;
+    p.block = open.block;
+    const int base = open.start, first = (int)blockIdx.x, last = shares.owner(open.start + open.units - 1);
     const int64_t row = (int64_t)p.block * args.rows + r;
     const int node = (int)(row / args.group), head = (int)(row % args.group);
-    if (first == last || r >= args.rows || node >= a.S || (int)threadIdx.x >= kJoinThreads / (D / 4) * (D / 4)) {
+    if (r >= args.rows || node >= a.S || (int)threadIdx.x >= kJoinThreads / (D / 4) * (D / 4)) {
         return;
     }
     const int firstSlot = 2 * first + (shares.start(first) == base ? 0 : 1);
@@ -822,8 +911,7 @@ hipError_t launch_layout(const Args &args, hipStream_t stream)
     constexpr int kPer = kJoinThreads / (L::D / 4);
     const int64_t rows = (int64_t)args.a.S * args.group < args.rows ? (int64_t)args.a.S * args.group : args.rows;
     hipLaunchKernelGGL((draft_join<kBf16, L::D>),
-                       dim3((unsigned)(args.a.B * args.a.kvHeads * args.blocks), (unsigned)((rows + kPer - 1) / kPer)),
-                       dim3(kJoinThreads), 0, stream, args);
+                       dim3((unsigned)args.most, (unsigned)((rows + kPer - 1) / kPer)), dim3(kJoinThreads), 0, stream, args);
     return hipGetLastError();
 }
 
@@ -833,11 +921,11 @@ enum class Kind { kOne, kTwo, kFour };
 template <int D, Kind kKind>
 struct LayoutOf;
 template <int D>
-struct LayoutOf<D, Kind::kOne> : Layout<D, 1, 4, 32> {};
+struct LayoutOf<D, Kind::kOne> : Layout<D, 1, (D > 128 ? 2 : 4), 32> {};
 template <int D>
 struct LayoutOf<D, Kind::kTwo> : Layout<D, 2, 2, 32> {};
 template <int D>
-struct LayoutOf<D, Kind::kFour> : Layout<D, 4, 1, (D > 192 ? 32 : 64)> {};
+struct LayoutOf<D, Kind::kFour> : Layout<D, 4, 1, 64> {};
 
 // Calls f(layout) for a kind and (padded) head size.
 template <Kind kKind, typename F>

@@ -50,13 +50,13 @@ bool draft_attention_units_fit(const DraftAttentionArgs &a)
     const int64_t units = (int64_t)a.width * a.pageSize / 32 + 2;
     int64_t all;
     return !__builtin_mul_overflow(units, blocks, &all) && !__builtin_mul_overflow(all, (int64_t)a.B * a.kvHeads, &all) &&
-           all < INT32_MAX && (int64_t)a.B * a.kvHeads * blocks < (1 << 23);  // (workgroups of the joining launch)
+           all < INT32_MAX;
 }
 
 size_t draft_attention_workspace(const DraftAttentionArgs &a, int cus)
 {
     const draft::Args p = draft::plan(a, cus);
-    return (size_t)2 * p.most * p.rows * (draft::padded(a.d) + 2) * 4;
+    return (size_t)2 * p.most * p.rows * (draft::padded(a.d) + 2) * 4 + p.most * sizeof(draft::Open);
 }
 
 hipError_t launch_draft_attention(const DraftAttentionArgs &a, void *workspace, int cus, hipStream_t stream)
@@ -64,6 +64,7 @@ hipError_t launch_draft_attention(const DraftAttentionArgs &a, void *workspace, 
     draft::Args p = draft::plan(a, cus);
     p.outs = static_cast<float *>(workspace);
     p.ends = p.outs + (size_t)2 * p.most * p.rows * draft::padded(a.d);
+    p.open = reinterpret_cast<draft::Open *>(p.ends + (size_t)2 * p.most * p.rows * 2);
     switch (draft::kind_of(a)) {
     case draft::Kind::kOne:
         return a.isBf16 ? draft::launch_kind<true, draft::Kind::kOne>(p, stream)
