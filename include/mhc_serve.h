@@ -203,7 +203,7 @@ MHC_API int mhcPagedAttention(void *workspace, uint64_t workspaceSize, mhcServeE
  *   out        type of q     [B, S, heads, d]   lse      fp32  [B, S, heads], or NULL
  *
  * Sizes, alignments and strides as for mhcPagedAttention; the units of work,
- * B * kvHeads * ceil(S * heads / kvHeads / 32) * (width * pageSize / 32 + 2), are
+ * B * kvHeads * ceil(S * heads / kvHeads / 32) * (width * pageSize / 32 + 5), are
  * below 2^31.  The same call gives the same bits again; in another batch sums may be
  * cut elsewhere and differ by roundings in fp32.
  */

@@ -72,13 +72,13 @@ struct Layout {
     static constexpr int kSide = kTile * kChunks * 16;          // bytes of a tile of K or V
     static constexpr int kBuffer = 2 * kSide;                   // K, then V
     static constexpr int kLoads = kSide / 1024 / kRowWaves;     // of a wave, for either
-    static constexpr int kTiles = 2 * kBuffer * kKeyWaves;
-    static constexpr int kJoin = kKeyWaves > 1 ? kRows * (D + 4) * 4 * kWaves : 0;
-    static constexpr int kSetup = kDraftNodes * (32 + 4);
-    static constexpr int kLds = kTiles > kJoin ? (kTiles > kSetup ? kTiles : kSetup) : (kJoin > kSetup ? kJoin : kSetup);
+    static constexpr int kLds = 2 * kBuffer * kKeyWaves;
+    static constexpr int kMore = kDraftNodes * 36 + kKeyWaves * kBlock * 8 + 256;  // the other LDS
     // Workgroups of a CU: what its registers (two waves a SIMD up to D = 128) and LDS hold.
-    static constexpr int kPerCu = kThreads == 256 && D <= 128 && 2 * (kLds + kBlock * 48) <= 160 * 1024 ? 2 : 1;
-    static_assert(kLoads * kRowWaves * 1024 == kSide && kLds + kBlock * 48 <= 160 * 1024);
+    static constexpr int kPerCu = kThreads == 256 && D <= 128 && 2 * (kLds + kMore) <= 160 * 1024 ? 2 : 1;
+    static_assert(kLoads * kRowWaves * 1024 == kSide && kLds + kMore <= 160 * 1024);
+    // A wave's output fits a buffer (the groups of key waves leave theirs there to be joined).
+    static_assert(kKeyWaves == 1 || (kRows * D * 4 <= kBuffer && (kRowWaves == 1 || kRowWaves <= kKeyWaves)));
 
     // Where chunk c of row r lies among its row's chunks: turned so that what 16 lanes read at
     // a time lies in different banks, of K the same chunk of 16 rows, of V 64 bytes of 4 rows.
@@ -95,10 +95,15 @@ struct Layout {
     __device__ static uint32_t step(uint32_t p, int by) { return (p ^ by % kTurned * 16) + by / kTurned * kTurned * 16; }
 };
 
-// What a stretch begins and does not finish: a (sequence, kv head, block), the line's unit
-// at which it begins and its units, and the units of the line.  units 0: nothing.
+// What a (sequence, kv head, block) costs beside its tiles (its start and end), in tiles: it
+// stands for that in the line, in front of its tiles.
+constexpr int kItemUnits = 3;
+
+// What a stretch begins and does not finish: a (sequence, kv head, block), the line's units
+// of its first and its last tile, the units of the line, and the slot of its part.  last
+// < 0: nothing.
 struct Open {
-    int b, kv, block, start, units, all;
+    int b, kv, block, first, last, all, slot, none;
 };
 
 struct Args {
@@ -112,22 +117,30 @@ struct Args {
     Open *open;          // [most]
 };
 
-// The keys of a block of a sequence with c + n tokens, n of them new: [low, high).
+// The keys of a block of a sequence with c + n tokens, n of them new: [low, high), in
+// `tiles` (units of the launch, one at least) from `first` on.
 struct Keys {
-    int low, high, first, units;
+    int low, high, first, tiles;
 };
 
 struct Sequence {
     int c, n;  // tokens in front of the new ones, new ones
 
-    __device__ Sequence(const DraftAttentionArgs &a, int b)
+    __device__ Sequence(const DraftAttentionArgs &a, int L, int m)
     {
         const int most = a.width * a.pageSize;
-        int L = a.lengths[b], m = a.drafted[b];
         L = L < 0 ? 0 : L > most ? most : L;
         m = m < 0 ? 0 : m > a.S ? a.S : m;
         n = m < L ? m : L;
         c = L - n;
+    }
+    // A lane's own row, and the same row for all lanes (by scalar loads, which do not wait for
+    // vector ones).
+    __device__ static Sequence of(const DraftAttentionArgs &a, int b) { return {a, a.lengths[b], a.drafted[b]}; }
+    __device__ static Sequence same(const DraftAttentionArgs &a, int b)
+    {
+        typedef const __attribute__((address_space(4))) int32_t *Scalar;
+        return {a, ((Scalar)(uintptr_t)a.lengths)[b], ((Scalar)(uintptr_t)a.drafted)[b]};
     }
     __device__ Keys keys(const Args &args, int block) const
     {
@@ -141,15 +154,16 @@ struct Sequence {
             k.low = args.a.window > 0 && from > 0 ? (int)from : 0;
             k.high = c + i1;
             k.first = k.low / args.unit;
-            k.units = (k.high - 1) / args.unit + 1 - k.first;
+            k.tiles = (k.high - 1) / args.unit + 1 - k.first;
         }
         return k;
     }
+    // Of a kv head, in the line.
     __device__ int units(const Args &args) const
     {
-        int all = 0;
+        int all = args.blocks * kItemUnits;
         for (int x = 0; x < args.blocks; ++x) {
-            all += keys(args, x).units;
+            all += keys(args, x).tiles;
         }
         return all;
     }
@@ -186,60 +200,90 @@ __device__ __forceinline__ float scaled(float x, float f)
     return __builtin_isfinite(x) ? x * f : x * fmaxf(f, 1e-30f);
 }
 
-// Place of a stretch's first unit: sequence, kv head, block, and the unit in its keys.
+// A tile of the line: sequence (its context and new tokens), kv head, block, and the tile of
+// its keys.
 struct Place {
     int b, kv, block, tile;
-    int start;  // the line's unit at which the (sequence, kv head, block) begins
+    int start;  // the line's unit of tile 0
+    int c, n;
     Keys keys;
+
+    __device__ void enter(const Args &args)
+    {
+        const Sequence s = Sequence::same(args.a, b);
+        c = s.c;
+        n = s.n;
+        keys = s.keys(args, block);
+    }
+    __device__ bool inside(const Args &args, int end) const { return b < args.a.B && start + tile < end; }
+    __device__ void advance(const Args &args)
+    {
+        if (++tile < keys.tiles) {
+            return;
+        }
+        tile = 0;
+        start += keys.tiles + kItemUnits;
+        if (++block == args.blocks) {
+            block = 0;
+            if (++kv == args.a.kvHeads) {
+                kv = 0;
+                ++b;
+            }
+        }
+        if (b < args.a.B) {
+            enter(args);
+        }
+    }
 };
 
-// The place of unit `at` of the line, from the units of sequences (lane's: of `first`).
-__device__ __forceinline__ Place find_place(const Args &args, int at)
-{
-    const DraftAttentionArgs &a = args.a;
-    const int lane = (int)threadIdx.x % kWave;
-    int base = 0;
-    for (int b0 = 0;; b0 += kWave) {
-        const int x = b0 + lane;
-        const int units = x < a.B ? Sequence(a, x).units(args) * a.kvHeads : 0;
-        const int upto = dev::wave_scan(units);
-        const uint64_t past = __ballot(base + upto > at);
-        if (past == 0 && b0 + kWave < a.B) {
-            base += __builtin_amdgcn_readlane(upto, kWave - 1);
-            continue;
-        }
-        const int hit = __ffsll((unsigned long long)past) - 1;
-        Place p;
-        p.b = b0 + hit;
-        const int all = __builtin_amdgcn_readlane(units, hit) / a.kvHeads;
-        base += __builtin_amdgcn_readlane(upto, hit) - all * a.kvHeads;
-        p.kv = (at - base) / all;
-        base += p.kv * all;
-        const Sequence s(a, p.b);
-        for (p.block = 0;; ++p.block) {
-            p.keys = s.keys(args, p.block);
-            if (at < base + p.keys.units) {
-                break;
-            }
-            base += p.keys.units;
-        }
-        p.start = base;
-        p.tile = at - base;
-        return p;
-    }
-}
+// The line of all tiles.
+struct Line {
+    int all;  // all units
 
-__device__ __forceinline__ int all_units(const Args &args)
-{
-    const int lane = (int)threadIdx.x % kWave;
-    int all = 0;
-    for (int b0 = 0; b0 < args.a.B; b0 += kWave) {
-        const int x = b0 + lane;
-        all += __builtin_amdgcn_readlane(
-            dev::wave_scan(x < args.a.B ? Sequence(args.a, x).units(args) * args.a.kvHeads : 0), kWave - 1);
+    // Finds the first tile at unit `at` of the line or behind it.
+    __device__ static Place find(const Args &args, int at)
+    {
+        const DraftAttentionArgs &a = args.a;
+        const int lane = (int)threadIdx.x % kWave;
+        int base = 0;
+        for (int b0 = 0;; b0 += kWave) {
+            const int x = b0 + lane;
+            const int units = x < a.B ? Sequence::of(a, x).units(args) * a.kvHeads : 0;
+            const int upto = dev::wave_scan(units);
+            const uint64_t past = __ballot(base + upto > at);
+            if (past == 0 && b0 + kWave < a.B) {
+                base += __builtin_amdgcn_readlane(upto, kWave - 1);
+                continue;
+            }
+            const int hit = __ffsll((unsigned long long)past) - 1;
+            Place p;
+            p.b = b0 + hit;
+            const int all = __builtin_amdgcn_readlane(units, hit) / a.kvHeads;
+            base += __builtin_amdgcn_readlane(upto, hit) - all * a.kvHeads;
+            p.kv = (at - base) / all;
+            base += p.kv * all;
+            for (p.block = 0;; ++p.block) {
+                p.enter(args);
+                if (at < base + kItemUnits + p.keys.tiles) {
+                    break;
+                }
+                base += kItemUnits + p.keys.tiles;
+            }
+            p.start = base + kItemUnits;
+            p.tile = at > p.start ? at - p.start : 0;
+            return p;
+        }
     }
-    return all;
-}
+    __device__ explicit Line(const Args &args) : all(0)
+    {
+        const int lane = (int)threadIdx.x % kWave;
+        for (int b0 = 0; b0 < args.a.B; b0 += kWave) {
+            const int x = b0 + lane;
+            all += __builtin_amdgcn_readlane(
+                dev::wave_scan(x < args.a.B ? Sequence::of(args.a, x).units(args) * args.a.kvHeads : 0), kWave - 1);
+        }
+    }
+};
 
 // 4 values of row `row` of a block, from their sum and its weights' sum and maximum.
 template <bool kBf16>
@@ -260,14 +304,13 @@ __device__ __forceinline__ void finish(const Args &args, const Place &p, int nod
     }
 }
 
-// The ancestors of every node of row b, 256 bits each (itself among them), at the start of
-// `lds`.  A node's farthest known ancestor's are its own too: each round doubles how far.
+// The ancestors of every node of row b, 256 bits each (itself among them).  A node's
+// farthest known ancestor's are its own too: each round doubles how far.
 template <int kThreads>
-__device__ __forceinline__ void find_ancestors(const DraftAttentionArgs &a, int b, int n, char *lds)
+__device__ __forceinline__ void find_ancestors(const DraftAttentionArgs &a, int b, int n,
+                                               uint64_t (&known)[kDraftNodes][4], int (&farthest)[kDraftNodes])
 {
     constexpr int kNodes = kDraftNodes / kThreads > 0 ? kDraftNodes / kThreads : 1;  // of a thread
-    uint64_t *known = reinterpret_cast<uint64_t *>(lds);
-    int *farthest = reinterpret_cast<int *>(lds + kDraftNodes * 32);
     uint64_t own[kNodes][4];
     int far[kNodes];
 #pragma unroll
@@ -290,7 +333,7 @@ __device__ __forceinline__ void find_ancestors(const DraftAttentionArgs &a, int 
             if (i < n) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    known[4 * i + x] = own[k][x];
+                    known[i][x] = own[k][x];
                 }
                 farthest[i] = far[k];
             }
@@ -304,7 +347,7 @@ __device__ __forceinline__ void find_ancestors(const DraftAttentionArgs &a, int 
             if (far[k] >= 0) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    own[k][x] |= known[4 * far[k] + x];
+                    own[k][x] |= known[far[k]][x];
                 }
                 far[k] = farthest[far[k]];
             }
@@ -314,20 +357,25 @@ __device__ __forceinline__ void find_ancestors(const DraftAttentionArgs &a, int 
 }
 
 // Which of the 64 keys from t0 on a node sees: the context from `from` on, and of the new
-// tokens its ancestors, or in a chain those up to itself.
-__device__ __forceinline__ uint64_t seen_keys(bool tree, int c, int node, uint32_t from, int64_t t0,
-                                              const uint64_t (&ancestors)[4])
+// tokens its ancestors but the first `over`, or in a chain those from `from` up to itself.
+__device__ __forceinline__ uint64_t seen_keys(bool tree, int c, int node, uint32_t from, int over, int64_t t0,
+                                              const uint64_t (&known)[kDraftNodes][4])
 {
     // (positions below 2^31 and their differences fit 33 bits)
     const int64_t to = (tree ? c : (int64_t)c + node + 1) - t0, first = (int64_t)from - t0;
     uint64_t seen = low_bits(to > 64 ? 64 : to < 0 ? 0 : (int)to) & ~low_bits(first > 64 ? 64 : first < 0 ? 0 : (int)first);
-    if (tree) {
+    if (tree && t0 + 64 > c) {
         // Bit x of the tile is node x + t0 - c.
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int64_t by = t0 - c - 64 * x;
+            uint64_t own = known[node][x];
+            while (over > 0 && own != 0) {
+                own &= own - 1;
+                --over;
+            }
             if (by > -64 && by < 64) {
-                seen |= by >= 0 ? ancestors[x] >> by : ancestors[x] << -by;
+                seen |= by >= 0 ? own >> by : own << -by;
             }
         }
     }
@@ -362,9 +410,10 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
 {
     constexpr int D = L::D, kTile = L::kTile, kKt = kTile / 32, kSteps = D / 16, kDims = D / 32;
     __shared__ __align__(256) char lds[L::kLds];
-    __shared__ uint64_t rowMasks[L::kBlock][4];  // the rows' ancestors
+    __shared__ uint64_t known[kDraftNodes][4];  // the new tokens' ancestors
+    __shared__ int farthest[kDraftNodes];
     __shared__ uint64_t badKeys[L::kKeyWaves][2];
-    __shared__ float tops[L::kKeyWaves][L::kBlock], sums[L::kKeyWaves][L::kBlock];
+    __shared__ float2 ends[L::kKeyWaves][L::kBlock];
     __shared__ bool odd[L::kWaves];
     const DraftAttentionArgs &a = args.a;
     const int w = (int)blockIdx.x;
@@ -376,338 +425,384 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     // (turned) rows 4 half + .. and + 8, 4 columns of 32.
     const uint32_t kPlace = L::at(col, half);
     const uint32_t vPlace = L::at(4 * half + lane % 16 / 4, lane / 16 % 2 * 2 + lane % 4 / 2) + lane % 2 * 8;
+    const bool tree = a.parents != nullptr;
+    // (The scale's sign goes to q, for the maximum wants a factor above 0; with a scale of 0 q is 0.)
+    const float factor = a.scale == 0.f ? 1.f : fabsf(a.scale * kLog2e);
 
-    const attention::Shares shares(all_units(args), args.most);
+    const Line line(args);
+    const attention::Shares shares(line.all, args.most);
     if (threadIdx.x == 0) {
-        args.open[w].units = 0;
+        args.open[w].last = -1;
     }
     if (w >= shares.grid) {
         return;
     }
     const int begin = shares.start(w), end = shares.start(w + 1);
-    Place place = find_place(args, begin);
+    Place here = Line::find(args, begin);
+    if (!here.inside(args, end)) {
+        return;
+    }
 
-    for (int unit = begin; unit < end;) {
-        const Sequence seq(a, place.b);
-        const int tiles = end - unit < place.keys.units - place.tile ? end - unit : place.keys.units - place.tile;
-        const int row = place.block * L::kBlock + rowWave * kRows + col;
+    // The lane's key (lane % kTile) of the tile at `ahead`: its page and slot.
+    Place ahead = here;
+    const int32_t *table = a.table + (int64_t)here.b * a.width;
+    int page = -1, slot = 0, foundKv = here.kv;
+    bool key = false;
+    const auto find_page = [&]() {
+        uint32_t t = 0;
+        key = false;
+        if (ahead.inside(args, end)) {
+            t = (uint32_t)(ahead.keys.first + ahead.tile) * L::kUnit + keyWave * kTile + lane % kTile;
+            key = t >= (uint32_t)ahead.keys.low && t < (uint32_t)ahead.keys.high;
+            table = a.table + (int64_t)ahead.b * a.width;
+            foundKv = ahead.kv;
+            ahead.advance(args);
+        }
+        // (Always a load, of the row's first entry where there is no key: under a branch it would
+        // be waited for at once.)
+        const uint32_t at = (key ? t : 0u) / (uint32_t)a.pageSize;
+        page = table[at];
+        slot = (int)(t - at * (uint32_t)a.pageSize);
+    };
+    uint64_t loaded = 0;  // keys of the tile on its way
+    const auto load = [&](int buffer) {
+        const bool seen = key && page >= 0 && page < a.pages;
+        loaded = __ballot(seen);
+        if constexpr (kTile == 32) {
+            loaded &= 0xFFFFFFFFull;
+        }
+        const char *zeros = reinterpret_cast<const char *>(kZeros);
+        const char *kRow = seen ? static_cast<const char *>(a.kCache.data) +
+                                      2 * (foundKv * a.kCache.head + page * a.kCache.page + slot * a.kCache.slot)
+                                : zeros;
+        const char *vRow = seen ? static_cast<const char *>(a.vCache.data) +
+                                      2 * (foundKv * a.vCache.head + page * a.vCache.page + slot * a.vCache.slot)
+                                : zeros;
+        auto *const to = mine + buffer * L::kBuffer;
+#pragma unroll
+        for (int n = 0; n < L::kLoads; ++n) {
+            const int first = (n * L::kRowWaves + rowWave) * kWave, at = first + lane;
+            const int r = at / L::kChunks, ch = at % L::kChunks ^ L::turn(r);
+            const char *k = reinterpret_cast<const char *>(shfl64(reinterpret_cast<int64_t>(kRow), r)) + ch * 16;
+            const char *v = reinterpret_cast<const char *>(shfl64(reinterpret_cast<int64_t>(vRow), r)) + ch * 16;
+            if (ch * 8 >= a.d) {
+                k = v = zeros;
+            }
+            load_to_lds(k, to + first * 16);
+            load_to_lds(v, to + L::kSide + first * 16);
+        }
+    };
+    // The operand of the rows of a place's block.  (It is turned where it is used first: what a
+    // load brings must not be touched before the wait at the loop's head.)
+    u32x4_t q[kSteps];
+    const auto load_q = [&](const Place &p) {
+        const int row = p.block * L::kBlock + rowWave * kRows + col;
         const int node = row / args.group, head = row % args.group;
-        const bool there = node < seq.n;
+        const uint16_t *from = static_cast<const uint16_t *>(a.q.data) + p.b * a.q.row + node * a.q.token +
+                               (int64_t)(p.kv * args.group + head) * a.q.head + 8 * half;
+        const bool on = node < p.n && a.scale != 0.f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            q[s] = *reinterpret_cast<const u32x4_t *>(on && 16 * s < a.d ? from + 16 * s
+                                                                         : reinterpret_cast<const uint16_t *>(kZeros));
+        }
+    };
+    const auto turn_q = [&]() {
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            q[s] ^= u32x4_t{flip, flip, flip, flip};
+        }
+    };
 
-        // The node's ancestors (itself one of them) among the new tokens, and its depth.
+    f32x16_t o[kDims];
+    float top, sum;
+    const auto clear = [&]() {
+#pragma unroll
+        for (int j = 0; j < kDims; ++j) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                o[j][i] = 0.f;
+            }
+        }
+        top = -INFINITY;
+        sum = 0.f;
+    };
+    // The lane's row of the block at `here`: its node, where its context begins, how many of its
+    // first ancestors lie in front of its window; and tiles in [wholeFrom, wholeTo) that all rows
+    // of the wave see whole.
+    int node = 0, over = 0, maskedRow = -1;
+    bool there = false;
+    uint32_t from = 0;
+    int64_t wholeFrom = 0, wholeTo = 0;
+    const auto enter = [&]() {
+        const int row0 = here.block * L::kBlock + rowWave * kRows;
+        node = (row0 + col) / args.group;
+        there = node < here.n;
         int depth = node;
-        const bool tree = a.parents != nullptr;
-        const int draftFrom = (place.keys.first + place.tile) * L::kUnit;
-        __syncthreads();  // (the LDS is free)
-        if (tree && seq.n > 0 && (a.window > 0 || (int64_t)draftFrom + (int64_t)tiles * L::kUnit > seq.c)) {
-            find_ancestors<L::kThreads>(a, place.b, seq.n, lds);
-            const uint64_t *known = reinterpret_cast<const uint64_t *>(lds);
-            depth = 0;
-            if (there) {
-                uint64_t own[4];
+        const int lastTile = end - 1 - here.start < here.keys.tiles - 1 ? end - 1 - here.start : here.keys.tiles - 1;
+        if (tree && here.n > 0 &&
+            (a.window > 0 || (int64_t)(here.keys.first + lastTile + 1) * L::kUnit > here.c)) {
+            if (maskedRow != here.b) {
+                __syncthreads();  // (the ones before are read)
+                find_ancestors<L::kThreads>(a, here.b, here.n, known, farthest);
+                maskedRow = here.b;
+            }
+            if (a.window > 0) {
+                depth = -1;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    own[x] = known[4 * node + x];
-                    depth += __popcll(own[x]);
-                }
-                depth -= 1;
-                // Of the path only the window's length, from the node up: the lower numbers go.
-                int over = a.window > 0 && a.window < depth + 1 ? depth + 1 - (int)a.window : 0;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    while (over > 0 && own[x] != 0) {
-                        own[x] &= own[x] - 1;
-                        --over;
-                    }
-                    rowMasks[rowWave * kRows + col][x] = own[x];  // (by all key waves, the same)
+                    depth += there ? __popcll(known[node][x]) : 0;
                 }
             }
-            __syncthreads();
         }
-        // The context that the row sees: [from, c).  (A chain's row: [from, c + node].)
-        const int64_t from64 = (int64_t)seq.c + depth + 1 - a.window;
-        const uint32_t from = a.window > 0 && from64 > 0 ? (uint32_t)from64 : 0u;
-        // Tiles in [wholeFrom, wholeTo) all rows of the wave see whole.
-        const int64_t wholeTo =
-            tree ? seq.c : (int64_t)seq.c + (place.block * L::kBlock + rowWave * kRows) / args.group + 1;
-        const int64_t wholeFrom = a.window > 0 ? (int64_t)seq.c + seq.n - a.window : 0;
+        over = a.window > 0 && a.window < depth + 1 ? depth + 1 - (int)a.window : 0;
+        // (The context that the row sees: [from, c); a chain's row: [from, c + node].)
+        const int64_t from64 = (int64_t)here.c + depth + 1 - a.window;
+        from = a.window > 0 && from64 > 0 ? (uint32_t)from64 : 0u;
+        wholeTo = tree ? here.c : (int64_t)here.c + row0 / args.group + 1;
+        wholeFrom = a.window > 0 ? (int64_t)here.c + here.n - a.window : 0;
+    };
 
-        u32x4_t q[kSteps];
-        // (Its sign goes to q, for the maximum wants a factor above 0; with a scale of 0 q is 0.)
-        const float c = a.scale == 0.f ? 1.f : fabsf(a.scale * kLog2e);
+    // A tile: its keys from t0 on, of which `valid` are in the cache.  kChecked: with infinite and
+    // NaN values of V set apart.
+    const auto attend = [&](auto kChecked, uint32_t buffer, int64_t t0, uint64_t valid, const uint64_t &badHere) {
+        constexpr bool checked = decltype(kChecked)::value;
+        const uint32_t kFrom = buffer + kPlace, vFrom = buffer + L::kSide + vPlace;
+        constexpr uint64_t kAll = kTile == 64 ? ~0ull : 0xFFFFFFFFull;
+        const bool whole = valid == kAll && t0 >= wholeFrom && t0 + kTile <= wholeTo;
+        uint64_t seen = kAll;
+        if (!whole) {
+            seen = there ? seen_keys(tree, here.c, node, from, over, t0, known) & valid : 0ull;
+            if (!__any((int)(seen != 0ull))) {
+                return;
+            }
+        }
+
+        f32x16_t s[kKt] = {};
         {
-            const uint16_t *at = static_cast<const uint16_t *>(a.q.data) + place.b * a.q.row + node * a.q.token +
-                                 (int64_t)(place.kv * args.group + head) * a.q.head;
-            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+            constexpr int kReads = kSteps * kKt, kAhead = kReads < 6 ? kReads : 6;
+            u32x4_t k[kAhead];
+            const auto read = [&](int x) {
+                return *(__attribute__((address_space(3))) const u32x4_t *)(uintptr_t)(
+                    L::step(kFrom, 2 * (x / kKt)) + x % kKt * 32 * L::kChunks * 16);
+            };
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                q[s] = u32x4_t{0, 0, 0, 0};
-                if (there && a.scale != 0.f && 16 * s < a.d) {
-                    q[s] = *reinterpret_cast<const u32x4_t *>(at + 16 * s + 8 * half);
-                    q[s] ^= u32x4_t{flip, flip, flip, flip};
+            for (int x = 0; x < kAhead; ++x) {
+                k[x] = read(x);
+            }
+            in_order();
+#pragma unroll
+            for (int x = 0; x < kReads; ++x) {
+                s[x % kKt] = mfma<kBf16>(k[x % kAhead], q[x / kKt], s[x % kKt]);
+                if (x + kAhead < kReads) {
+                    k[x % kAhead] = read(x + kAhead);
+                }
+                in_order();
+            }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int kt = 0; kt < kKt; ++kt) {
+                const uint32_t bits = (uint32_t)(seen >> (32 * kt)) >> (4 * half);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[kt][i] = (bits >> (8 * (i / 4) + i % 4) & 1u) != 0u ? s[kt][i] : -INFINITY;
                 }
             }
         }
-
-        const char *kBase = static_cast<const char *>(a.kCache.data) + 2 * place.kv * a.kCache.head;
-        const char *vBase = static_cast<const char *>(a.vCache.data) + 2 * place.kv * a.vCache.head;
-        const int32_t *table = a.table + (int64_t)place.b * a.width;
-        f32x16_t o[kDims];
-        float top, sum;
-        // kChecked: with infinite and NaN values of V set apart.
-        const auto pass = [&](auto kChecked) {
-            constexpr bool checked = decltype(kChecked)::value;
+        float most = s[0][0];
+#pragma unroll
+        for (int kt = 0; kt < kKt; ++kt) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                most = fmaxf(most, s[kt][i]);
+            }
+        }
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const float next = fmaxf(top, most * factor);
+        const float zero = next == -INFINITY ? 0.f : next;
+        if (__any((int)(next > top))) {  // (else the sums are on the right scale)
+            const float keep = __builtin_amdgcn_exp2f(top - zero);
+            top = next;
+            sum *= keep;
 #pragma unroll
             for (int j = 0; j < kDims; ++j) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    o[j][i] = 0.f;
+                    o[j][i] = checked ? scaled(o[j][i], keep) : o[j][i] * keep;
                 }
             }
-            top = -INFINITY;
-            sum = 0.f;
-
-            // The lane's key (lane % kTile) of a tile: its page and slot, then its rows.
-            uint32_t t = (uint32_t)(place.keys.first + place.tile) * L::kUnit + keyWave * kTile + lane % kTile;
-            // (Always a load, of the row's first entry where there is no key: under a branch it
-            // would be waited for at once.)
-            int page = -1, slot = 0;
-            bool key = false;
-            const auto find_page = [&](bool more) {
-                key = more && t >= (uint32_t)place.keys.low && t < (uint32_t)place.keys.high;
-                const uint32_t at = (key ? t : 0u) / (uint32_t)a.pageSize;
-                page = table[at];
-                slot = (int)(t - at * (uint32_t)a.pageSize);
-                t += L::kUnit;
-            };
-            uint64_t loaded = 0;  // keys of the tile on its way
-            const auto load = [&](int buffer) {
-                const bool seen = key && page >= 0 && page < a.pages;
-                loaded = __ballot(seen);
-                if constexpr (kTile == 32) {
-                    loaded &= 0xFFFFFFFFull;
-                }
-                const char *kRow = seen ? kBase + 2 * (page * a.kCache.page + slot * a.kCache.slot)
-                                        : reinterpret_cast<const char *>(kZeros);
-                const char *vRow = seen ? vBase + 2 * (page * a.vCache.page + slot * a.vCache.slot)
-                                        : reinterpret_cast<const char *>(kZeros);
-                auto *const to = mine + buffer * L::kBuffer;
+        }
+        const float shift = kLiftBits<kBf16> - zero;
+        // The weights of 16 keys, two at a time, between the products of the 16 before, whose
+        // values of V are read ahead.
+        constexpr int kGroups = kTile / 16, kProducts = kGroups * kDims, kAhead = kProducts < 4 ? kProducts : 4;
+        u32x4_t p[kGroups][2], v[kAhead];
+        const auto weigh = [&](int t, int x) {  // (keys 2 x and 2 x + 1 of the lane's 8)
+            const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x], factor, shift));
+            const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x + 1], factor, shift));
+            sum += x0;
+            sum += x1;
+            const uint32_t first = attention::cut2<kBf16>(x0, x1);
+            p[t][0][x] = first;
+            p[t][1][x] = dev::pack2_x<kBf16>(rest<kBf16>(x0, first, 0), rest<kBf16>(x1, first, 1));
+        };
+        const auto read = [&](int x) {  // (rows r and r + 8 of the tile, the lane's 4 columns of 32)
+            const uint32_t rows = x / kDims * 16 * L::kChunks * 16;
+            const u32x2_t v0 = transposed(L::step(vFrom, 4 * (x % kDims)) + rows);
+            const u32x2_t v1 = transposed(L::step(vFrom ^ 32, 4 * (x % kDims)) + rows + 8 * L::kChunks * 16);
+            return u32x4_t{v0[0], v0[1], v1[0], v1[1]};
+        };
 #pragma unroll
-                for (int n = 0; n < L::kLoads; ++n) {
-                    const int first = (n * L::kRowWaves + rowWave) * kWave, at = first + lane;
-                    const int r = at / L::kChunks, ch = at % L::kChunks ^ L::turn(r);
-                    const char *k = reinterpret_cast<const char *>(shfl64(reinterpret_cast<int64_t>(kRow), r)) + ch * 16;
-                    const char *v = reinterpret_cast<const char *>(shfl64(reinterpret_cast<int64_t>(vRow), r)) + ch * 16;
-                    if (ch * 8 >= a.d) {
-                        k = v = reinterpret_cast<const char *>(kZeros);
-                    }
-                    load_to_lds(k, to + first * 16);
-                    load_to_lds(v, to + L::kSide + first * 16);
-                }
-            };
-            find_page(true);
-            load(0);
-            find_page(tiles > 1);
-            for (int tile = 0; tile < tiles; ++tile) {
-                const uint32_t buffer = (uint32_t)(uintptr_t)mine + tile % 2 * L::kBuffer;
-                const uint32_t kFrom = buffer + kPlace, vFrom = buffer + L::kSide + vPlace;
-                const uint64_t valid = loaded;
-                const int64_t t0 = (int64_t)(place.keys.first + place.tile + tile) * L::kUnit + keyWave * kTile;
-                dev::wait_vm<0>();  // (the tile is there, and the next one's pages are known)
-                if constexpr (L::kRowWaves > 1 || checked) {
-                    __syncthreads();
-                }
-                if constexpr (checked) {
-                    if (rowWave == 0 && lane == 0) {
-                        badKeys[keyWave][tile % 2] = 0;
-                    }
-                    __syncthreads();
-#pragma unroll 1
-                    for (int n = 0; n < L::kLoads; ++n) {
-                        const int at = (n * L::kRowWaves + rowWave) * kWave + lane;
-                        auto *const place16 = (__attribute__((address_space(3))) u32x4_t *)(uintptr_t)(buffer + L::kSide + at * 16);
-                        u32x4_t v = *place16;
-                        bool bad = false;
+        for (int x = 0; x < kAhead; ++x) {
+            v[x] = read(x);
+        }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (infinite<kBf16>(v[e])) {
-                                v[e] &= 0xFFFF0000u;
-                                bad = true;
-                            }
-                            if (infinite<kBf16>(v[e] >> 16)) {
-                                v[e] &= 0xFFFFu;
-                                bad = true;
-                            }
-                        }
-                        if (bad) {
-                            *place16 = v;
-                            atomicOr(reinterpret_cast<unsigned long long *>(&badKeys[keyWave][tile % 2]),
-                                     1ull << (at / L::kChunks));
-                        }
-                    }
-                    __syncthreads();
-                }
-                // (After the last tile: rows of zeros.  Under a branch the page would be waited for.)
-                load((tile + 1) % 2);
-                find_page(tile + 2 < tiles);
-
-                // What the row sees of the tile (its keys from t0 on).
-                constexpr uint64_t kAll = kTile == 64 ? ~0ull : 0xFFFFFFFFull;
-                const bool whole = valid == kAll && t0 >= wholeFrom && t0 + kTile <= wholeTo;
-                uint64_t seen = kAll;
-                if (!whole) {
-                    seen = seen_keys(tree, seq.c, node, from, t0, rowMasks[rowWave * kRows + col]);
-                    seen = there ? seen & valid : 0ull;
-                    if (!__any((int)(seen != 0ull))) {
-                        continue;
-                    }
-                }
-
-                f32x16_t s[kKt] = {};
-                {
-                    constexpr int kAll = kSteps * kKt, kAhead = kAll < 6 ? kAll : 6;
-                    u32x4_t k[kAhead];
-                    const auto read = [&](int x) {
-                        return *(__attribute__((address_space(3))) const u32x4_t *)(uintptr_t)(
-                            L::step(kFrom, 2 * (x / kKt)) + x % kKt * 32 * L::kChunks * 16);
-                    };
+        for (int x = 0; x < 4; ++x) {
+            weigh(0, x);
+        }
+        in_order();
 #pragma unroll
-                    for (int x = 0; x < kAhead; ++x) {
-                        k[x] = read(x);
-                    }
-                    in_order();
+        for (int x = 0; x < kProducts; ++x) {
+            const int t = x / kDims, j = x % kDims;
+            o[j] = mfma<kBf16>(v[x % kAhead], p[t][0], o[j]);
+            o[j] = mfma<kBf16>(v[x % kAhead], p[t][1], o[j]);
+            if (x + kAhead < kProducts) {
+                v[x % kAhead] = read(x + kAhead);
+            }
+            if (t + 1 < kGroups) {
 #pragma unroll
-                    for (int x = 0; x < kAll; ++x) {
-                        s[x % kKt] = mfma<kBf16>(k[x % kAhead], q[x / kKt], s[x % kKt]);
-                        if (x + kAhead < kAll) {
-                            k[x % kAhead] = read(x + kAhead);
-                        }
-                        in_order();
-                    }
+                for (int y = j * 4 / kDims; y < (j + 1) * 4 / kDims; ++y) {
+                    weigh(t + 1, y);
                 }
-                if (!whole) {
-#pragma unroll
-                    for (int kt = 0; kt < kKt; ++kt) {
-                        const uint32_t bits = (uint32_t)(seen >> (32 * kt)) >> (4 * half);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            s[kt][i] = (bits >> (8 * (i / 4) + i % 4) & 1u) != 0u ? s[kt][i] : -INFINITY;
-                        }
-                    }
-                }
-                float most = s[0][0];
+            }
+            in_order();
+        }
+        if constexpr (checked) {
+            // The infinite and NaN values of the rows that see them.
+            uint64_t bad = badHere;
+            while (bad != 0) {
+                const int at = __ffsll((unsigned long long)bad) - 1;
+                bad &= bad - 1;
+                float weight = 0.f;
 #pragma unroll
                 for (int kt = 0; kt < kKt; ++kt) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        most = fmaxf(most, s[kt][i]);
-                    }
-                }
-                most = fmaxf(most, __shfl_xor(most, 32));
-                const float next_top = fmaxf(top, most * c);
-                const float zero = next_top == -INFINITY ? 0.f : next_top;
-                if (__any((int)(next_top > top))) {  // (else the sums are on the right scale)
-                    const float keep = __builtin_amdgcn_exp2f(top - zero);
-                    top = next_top;
-                    sum *= keep;
-#pragma unroll
-                    for (int j = 0; j < kDims; ++j) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            o[j][i] = checked ? scaled(o[j][i], keep) : o[j][i] * keep;
+                        if (32 * kt + 8 * (i / 4) + i % 4 == (at & ~4)) {
+                            const uint32_t hi = p[2 * kt + i / 8][0][i % 8 / 2] >> (i % 2 * 16) & 0xFFFFu;
+                            const uint32_t lo = p[2 * kt + i / 8][1][i % 8 / 2] >> (i % 2 * 16) & 0xFFFFu;
+                            weight = dev::x_to_f32<kBf16>(hi) + dev::x_to_f32<kBf16>(lo);
                         }
                     }
                 }
-                const float shift = kLiftBits<kBf16> - zero;
-                // The weights of 16 keys, two at a time, between the products of the 16 before, whose
-                // values of V are read ahead.
-                constexpr int kGroups = kTile / 16, kProducts = kGroups * kDims, kAhead = kProducts < 4 ? kProducts : 4;
-                u32x4_t p[kGroups][2], v[kAhead];
-                const auto weigh = [&](int t, int x) {  // (keys 2 x and 2 x + 1 of the lane's 8)
-                    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x], c, shift));
-                    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x + 1], c, shift));
-                    sum += x0;
-                    sum += x1;
-                    const uint32_t first = attention::cut2<kBf16>(x0, x1);
-                    p[t][0][x] = first;
-                    p[t][1][x] = dev::pack2_x<kBf16>(rest<kBf16>(x0, first, 0), rest<kBf16>(x1, first, 1));
-                };
-                const auto read = [&](int x) {  // (rows r and r + 8 of the tile, the lane's 4 columns of 32)
-                    const uint32_t rows = x / kDims * 16 * L::kChunks * 16;
-                    const u32x2_t v0 = transposed(L::step(vFrom, 4 * (x % kDims)) + rows);
-                    const u32x2_t v1 = transposed(L::step(vFrom ^ 32, 4 * (x % kDims)) + rows + 8 * L::kChunks * 16);
-                    return u32x4_t{v0[0], v0[1], v1[0], v1[1]};
-                };
+                weight = __shfl(weight, col + 32 * (at >> 2 & 1));
+                const bool on = (seen >> at & 1u) != 0u;
+                // (a weight that is 0 in 32 bits is above 0 all the same)
+                weight = weight == 0.f ? 1e-30f : weight;
+                const uint32_t t = (uint32_t)t0 + at, column = t / (uint32_t)a.pageSize;
+                const uint16_t *value = static_cast<const uint16_t *>(a.vCache.data) + here.kv * a.vCache.head +
+                                        a.table[(int64_t)here.b * a.width + column] * a.vCache.page +
+                                        (t - column * (uint32_t)a.pageSize) * a.vCache.slot;
 #pragma unroll
-                for (int x = 0; x < kAhead; ++x) {
-                    v[x] = read(x);
-                }
+                for (int j = 0; j < kDims; ++j) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    weigh(0, x);
-                }
-                in_order();
-#pragma unroll
-                for (int x = 0; x < kProducts; ++x) {
-                    const int t = x / kDims, j = x % kDims;
-                    o[j] = mfma<kBf16>(v[x % kAhead], p[t][0], o[j]);
-                    o[j] = mfma<kBf16>(v[x % kAhead], p[t][1], o[j]);
-                    if (x + kAhead < kProducts) {
-                        v[x % kAhead] = read(x + kAhead);
-                    }
-                    if (t + 1 < kGroups) {
-#pragma unroll
-                        for (int y = j * 4 / kDims; y < (j + 1) * 4 / kDims; ++y) {
-                            weigh(t + 1, y);
-                        }
-                    }
-                    in_order();
-                }
-                if constexpr (checked) {
-                    // The infinite and NaN values of the rows that see them.
-                    uint64_t bad = badKeys[keyWave][tile % 2];
-                    while (bad != 0) {
-                        const int key = __ffsll((unsigned long long)bad) - 1;
-                        bad &= bad - 1;
-                        float weight = 0.f;
-#pragma unroll
-                        for (int kt = 0; kt < kKt; ++kt) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                if (32 * kt + 8 * (i / 4) + i % 4 == (key & ~4)) {
-                                    const uint32_t hi = p[2 * kt + i / 8][0][i % 8 / 2] >> (i % 2 * 16) & 0xFFFFu;
-                                    const uint32_t lo = p[2 * kt + i / 8][1][i % 8 / 2] >> (i % 2 * 16) & 0xFFFFu;
-                                    weight = dev::x_to_f32<kBf16>(hi) + dev::x_to_f32<kBf16>(lo);
-                                }
-                            }
-                        }
-                        weight = __shfl(weight, col + 32 * (key >> 2 & 1));
-                        const bool on = (seen >> key & 1u) != 0u;
-                        // (a weight that is 0 in 32 bits is above 0 all the same)
-                        weight = weight == 0.f ? 1e-30f : weight;
-                        const uint32_t at = (uint32_t)t0 + key, column = at / (uint32_t)a.pageSize;
-                        const uint16_t *v = reinterpret_cast<const uint16_t *>(
-                            vBase + 2 * (table[column] * a.vCache.page + (at - column * (uint32_t)a.pageSize) * a.vCache.slot));
-#pragma unroll
-                        for (int j = 0; j < kDims; ++j) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const int e = 32 * j + 8 * (i / 4) + 4 * half + i % 4;
-                                if (32 * j + i / 8 * 16 < a.d) {  // (e < d, for d % 16 is 0)
-                                    const uint32_t bits = v[e];
-                                    if (on && infinite<kBf16>(bits)) {
-                                        o[j][i] += weight * dev::x_to_f32<kBf16>(bits);
-                                    }
-                                }
+                    for (int i = 0; i < 16; ++i) {
+                        const int e = 32 * j + 8 * (i / 4) + 4 * half + i % 4;
+                        if (32 * j + i / 8 * 16 < a.d) {  // (e < d, for d % 16 is 0)
+                            const uint32_t bits = value[e];
+                            if (on && infinite<kBf16>(bits)) {
+                                o[j][i] += weight * dev::x_to_f32<kBf16>(bits);
                             }
                         }
                     }
                 }
             }
-            dev::wait_vm<0>();  // (the rows of zeros, before the LDS serves for something else)
-        };
-        pass(std::false_type{});
-        bool all = true;
+        }
+    };
+
+    // The block at `here` again, tile `firstTile` to the one at `here`.
+    const auto again = [&](int firstTile) {
+        const int lastTile = here.tile;
+        clear();
+        load_q(here);
+        ahead = here;
+        ahead.tile = firstTile;
+        for (int tile = firstTile; tile <= lastTile; ++tile) {
+            find_page();
+            __syncthreads();  // (the tile before is done)
+            load(0);
+            const uint64_t valid = loaded;
+            if (rowWave == 0 && lane == 0) {
+                badKeys[keyWave][0] = 0;
+            }
+            dev::wait_vm<0>();
+            if (tile == firstTile) {
+                turn_q();
+            }
+            __syncthreads();
+            const uint32_t buffer = (uint32_t)(uintptr_t)mine;
+#pragma unroll 1
+            for (int n = 0; n < L::kLoads; ++n) {
+                const int at = (n * L::kRowWaves + rowWave) * kWave + lane;
+                auto *const place16 = (__attribute__((address_space(3))) u32x4_t *)(uintptr_t)(buffer + L::kSide + at * 16);
+                u32x4_t v = *place16;
+                bool bad = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (infinite<kBf16>(v[e])) {
+                        v[e] &= 0xFFFF0000u;
+                        bad = true;
+                    }
+                    if (infinite<kBf16>(v[e] >> 16)) {
+                        v[e] &= 0xFFFFu;
+                        bad = true;
+                    }
+                }
+                if (bad) {
+                    *place16 = v;
+                    atomicOr(reinterpret_cast<unsigned long long *>(&badKeys[keyWave][0]), 1ull << (at / L::kChunks));
+                }
+            }
+            __syncthreads();
+            attend(std::true_type{}, buffer, (int64_t)(here.keys.first + tile) * L::kUnit + keyWave * kTile, valid,
+                   badKeys[keyWave][0]);
+        }
+        __syncthreads();
+    };
+
+    find_page();
+    load(0);
+    find_page();
+    load_q(here);
+    clear();
+    int firstTile = here.tile;  // of the block, in this stretch
+    bool fresh = true, wholeStretch = true;
+    for (int buffer = 0;; buffer ^= 1) {
+        const uint64_t valid = loaded;
+        dev::wait_vm<0>();  // (the tile is there, the next one's pages are known, and so is q)
+        if constexpr (L::kRowWaves > 1) {
+            __syncthreads();
+        }
+        if (fresh) {
+            enter();
+            turn_q();
+            fresh = false;
+        }
+        // The next tile, of this block or the next one (behind the last one rows of zeros: under a
+        // branch the page would be waited for).
+        load(buffer ^ 1);
+        find_page();
+        attend(std::false_type{}, (uint32_t)(uintptr_t)mine + buffer * L::kBuffer,
+               (int64_t)(here.keys.first + here.tile) * L::kUnit + keyWave * kTile, valid, 0ull);
+        if (here.tile + 1 < here.keys.tiles && here.start + here.tile + 1 < end) {
+            ++here.tile;
+            continue;
+        }
+
+        // The block's end, or the stretch's.
+        bool finite = true;
 #pragma unroll
         for (int j = 0; j < kDims; ++j) {
             float none = 0.f;
@@ -715,22 +810,37 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
             for (int i = 0; i < 16; ++i) {
                 none += o[j][i] * 0.f;
             }
-            all = all && none == 0.f;
+            finite = finite && none == 0.f;
         }
         if (lane == 0) {
             odd[wave] = false;
         }
-        if (!all) {
+        if (!finite) {
             odd[wave] = true;
         }
+        Place next = here;
+        next.advance(args);
+        const bool more = next.inside(args, end);
+        if (more) {
+            load_q(next);
+        }
         __syncthreads();
-        bool again = false;
+        bool redo = false;
 #pragma unroll
         for (int x = 0; x < L::kWaves; ++x) {
-            again = again || odd[x];
+            redo = redo || odd[x];
         }
-        if (again) {
-            pass(std::true_type{});
+        if (redo) {
+            dev::wait_vm<0>();  // (the tile on its way)
+            again(firstTile);
+            // The next one anew.
+            ahead = next;
+            find_page();
+            load(buffer ^ 1);
+            find_page();
+            if (more) {
+                load_q(next);
+            }
         }
 
         sum += __shfl_xor(sum, 32);
@@ -745,92 +855,105 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                 }
             }
         }
-        const bool whole = place.tile == 0 && tiles == place.keys.units;
-        if (threadIdx.x == 0 && place.tile == 0 && !whole) {
-            args.open[w] = Open{place.b, place.kv, place.block, place.start, place.keys.units, shares.units};
-        }
-        const int slot = 2 * w + (unit == begin ? 0 : 1);
-        // 4 values of row r of the block.
-        const auto put = [&](int r, int e, f32x4_t all, float t, float s) {
-            const int x = place.block * L::kBlock + r;
-            const int i = x / args.group, h = x % args.group;
-            if (i >= a.S) {
-            } else if (whole) {
-                finish<kBf16>(args, place, i, h, e, all, t, s);
-            } else {
-                *reinterpret_cast<f32x4_t *>(args.outs + ((int64_t)slot * L::kBlock + r) * D + e) = all;
-                if (e == 0) {
-                    *reinterpret_cast<float2 *>(args.ends + ((int64_t)slot * L::kBlock + r) * 2) = float2{t, s};
-                }
-            }
-        };
-        if constexpr (L::kKeyWaves == 1) {
-#pragma unroll
-            for (int j = 0; j < kDims; ++j) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    put(rowWave * kRows + col, 32 * j + 2 * i + 4 * half,
-                        f32x4_t{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]}, top, sum);
-                }
-            }
-        } else {
-            // The groups' results together.
-            constexpr int kPitch = D + 4;
-            if (half == 0) {
-                tops[keyWave][rowWave * kRows + col] = top;
-                sums[keyWave][rowWave * kRows + col] = sum;
-            }
-            float *out = reinterpret_cast<float *>(lds) + (keyWave * L::kBlock + rowWave * kRows + col) * kPitch;
-            __syncthreads();  // (the tiles are read)
-#pragma unroll
-            for (int j = 0; j < kDims; ++j) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    *reinterpret_cast<f32x4_t *>(out + 32 * j + 2 * i + 4 * half) =
-                        f32x4_t{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]};
-                }
-            }
+        if constexpr (L::kKeyWaves > 1) {
+            // The groups' results together, in the first one's registers: the others leave theirs,
+            // as they lie, in the buffers that are read.
+            const auto left = [&](int k, int x) {
+                const int region = L::kRowWaves == 1 ? k : rowWave;
+                return (__attribute__((address_space(3))) f32x4_t *)(uintptr_t)(
+                    (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (2 * region + buffer) * L::kBuffer +
+                    (x * kWave + lane) * 16);
+            };
             __syncthreads();
-            for (int at = (int)threadIdx.x; at < L::kBlock * (D / 4); at += L::kThreads) {
-                const int r = at / (D / 4), e = at % (D / 4) * 4;
-                float most = -INFINITY;
+            if (half == 0) {
+                ends[keyWave][rowWave * kRows + col] = float2{top, sum};
+            }
+            if (keyWave > 0) {
 #pragma unroll
-                for (int x = 0; x < L::kKeyWaves; ++x) {
-                    most = fmaxf(most, tops[x][r]);
-                }
-                const float zero = most == -INFINITY ? 0.f : most;
-                float total = 0.f;
-                f32x4_t all = {0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < kDims; ++j) {
 #pragma unroll
-                for (int x = 0; x < L::kKeyWaves; ++x) {
-                    const float f = __builtin_amdgcn_exp2f(tops[x][r] - zero);
-                    total += f * sums[x][r];
-                    const f32x4_t v = *reinterpret_cast<const f32x4_t *>(
-                        reinterpret_cast<const float *>(lds) + (x * L::kBlock + r) * kPitch + e);
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        all[y] += scaled(v[y], f);
+                    for (int i = 0; i < 16; i += 4) {
+                        *left(keyWave, 4 * j + i / 4) = f32x4_t{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]};
                     }
                 }
-                put(r, e, all, most, total);
             }
             __syncthreads();
-        }
-
-        unit += tiles;
-        if (unit < end) {
-            place.start += place.keys.units;
-            place.tile = 0;
-            if (++place.block == args.blocks) {
-                place.block = 0;
-                if (++place.kv == a.kvHeads) {
-                    place.kv = 0;
-                    ++place.b;
+            if (keyWave == 0) {
+                float2 end_[L::kKeyWaves];
+                float most = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < L::kKeyWaves; ++k) {
+                    end_[k] = ends[k][rowWave * kRows + col];
+                    most = fmaxf(most, end_[k].x);
+                }
+                const float zero = most == -INFINITY ? 0.f : most;
+                top = most;
+                sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < L::kKeyWaves; ++k) {
+                    const float f = __builtin_amdgcn_exp2f(end_[k].x - zero);
+                    sum += f * end_[k].y;
+#pragma unroll
+                    for (int j = 0; j < kDims; ++j) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            if (k == 0) {
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) {
+                                    o[j][i + y] = scaled(o[j][i + y], f);
+                                }
+                            } else {
+                                const f32x4_t v = *left(k, 4 * j + i / 4);
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) {
+                                    o[j][i + y] += scaled(v[y], f);
+                                }
+                            }
+                        }
+                    }
                 }
             }
-            place.keys = Sequence(a, place.b).keys(args, place.block);
         }
+        const bool all = firstTile == 0 && here.tile + 1 == here.keys.tiles;
+        const int slot = 2 * w + (wholeStretch ? 0 : 1);
+        if (threadIdx.x == 0 && firstTile == 0 && !all) {
+            args.open[w] = Open{here.b, here.kv, here.block, here.start, here.start + here.keys.tiles - 1, line.all, slot, 0};
+        }
+        if (keyWave == 0) {
+            const int r = rowWave * kRows + col, x = here.block * L::kBlock + r;
+            const int head = x % args.group;
+            if (node < a.S) {
+#pragma unroll
+                for (int j = 0; j < kDims; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const int e = 32 * j + 2 * i + 4 * half;
+                        const f32x4_t value = {o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]};
+                        if (all) {
+                            finish<kBf16>(args, here, node, head, e, value, top, sum);
+                        } else {
+                            *reinterpret_cast<f32x4_t *>(args.outs + ((int64_t)slot * L::kBlock + r) * D + e) = value;
+                        }
+                    }
+                }
+                if (!all && half == 0) {
+                    *reinterpret_cast<float2 *>(args.ends + ((int64_t)slot * L::kBlock + r) * 2) = float2{top, sum};
+                }
+            }
+        }
+        if (!more) {
+            break;
+        }
+        if constexpr (L::kKeyWaves > 1) {
+            __syncthreads();  // (what the groups left is read)
+        }
+        here = next;
+        firstTile = 0;
+        fresh = true;
+        wholeStretch = false;
+        clear();
     }
+    dev::wait_vm<0>();  // (the rows of zeros, before the LDS is another workgroup's)
 }
 
 // Joins the parts of the (sequence, kv head, block)s that no stretch finished: a workgroup
@@ -843,7 +966,7 @@ __global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
 {
     const DraftAttentionArgs &a = args.a;
     const Open open = args.open[blockIdx.x];
-    if (open.units == 0) {
+    if (open.last < 0) {
         return;
     }
     const int r = (int)blockIdx.y * (kJoinThreads / (D / 4)) + (int)threadIdx.x / (D / 4);
@@ -853,13 +976,12 @@ __global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
     p.b = open.b;
     p.kv = open.kv;
     p.block = open.block;
-    const int base = open.start, first = (int)blockIdx.x, last = shares.owner(open.start + open.units - 1);
+    const int first = (int)blockIdx.x, last = shares.owner(open.last);
     const int64_t row = (int64_t)p.block * args.rows + r;
     const int node = (int)(row / args.group), head = (int)(row % args.group);
     if (r >= args.rows || node >= a.S || (int)threadIdx.x >= kJoinThreads / (D / 4) * (D / 4)) {
         return;
     }
-    const int firstSlot = 2 * first + (shares.start(first) == base ? 0 : 1);
     float top = -INFINITY, total = 0.f;
     f32x4_t all = {0.f, 0.f, 0.f, 0.f};
     for (int x0 = first; x0 <= last; x0 += kJoinBatch) {
@@ -868,7 +990,7 @@ __global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
 #pragma unroll
         for (int m = 0; m < kJoinBatch; ++m) {
             const int x = x0 + m <= last ? x0 + m : last;
-            const int64_t slot = x == first ? firstSlot : 2 * x;
+            const int64_t slot = x == first ? open.slot : 2 * x;
             ends[m] = *reinterpret_cast<const float2 *>(args.ends + (slot * args.rows + r) * 2);
             outs[m] = *reinterpret_cast<const f32x4_t *>(args.outs + (slot * args.rows + r) * D + e);
         }
