@@ -58,6 +58,14 @@ __device__ __forceinline__ void load_to_lds(const void *from, __attribute__((add
                  : "s"((uint32_t)(uintptr_t)to), "v"(from)
                  : "memory");
 }
+// The same from `base`, which all lanes share, and an offset of the lane's.
+__device__ __forceinline__ void load_to_lds(uint64_t base, uint32_t offset, __attribute__((address_space(3))) char *to)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"((uint32_t)(uintptr_t)to), "v"(offset), "s"(base)
+                 : "memory");
+}
 
 // How a workgroup's waves are laid out: kRowWaves share a tile, each with rows of its
 // own, and kKeyWaves such groups have tiles of their own.  Tiles come from memory
@@ -79,6 +87,10 @@ struct Layout {
     static_assert(kLoads * kRowWaves * 1024 == kSide && kLds + kMore <= 160 * 1024);
     // A wave's output fits a buffer (the groups of key waves leave theirs there to be joined).
     static_assert(kKeyWaves == 1 || (kRows * D * 4 <= kBuffer && (kRowWaves == 1 || kRowWaves <= kKeyWaves)));
+
+    // Rows that whole loads of 64 chunks cover together: in a page of a multiple of these the
+    // loads of such a group have one page.
+    static constexpr int kGroupRows = kChunks % 16 == 0 ? 64 / kChunks : kChunks % 8 == 0 ? 8 : 16;
 
     // Where chunk c of row r lies among its row's chunks: turned so that what 16 lanes read at
     // a time lies in different banks, of K the same chunk of 16 rows, of V 64 bytes of 4 rows.
@@ -113,6 +125,7 @@ struct Args {
     int rows;    // of a block
     int unit;    // keys of a unit
     int most;    // workgroups of the launch
+    bool grouped;  // pages of whole groups of rows (Layout::kGroupRows), the caches' strides alike
     float *outs, *ends;  // the parts: [2 * most][rows][D], [2 * most][rows][2]
     Open *open;          // [most]
 };
@@ -181,9 +194,12 @@ __device__ __forceinline__ f32x16_t mfma(u32x4_t a, u32x4_t b, f32x16_t c)
     }
 }
 
-// log2 of what the probabilities are multiplied by.
+// Weights are relative to a reference near the maximum, which follows it only where it
+// has grown by more than 2^kSlack: a weight may be that large, and in fp16 with what all of
+// them are multiplied by (2^kLiftBits, for the type ends at 2^-24) 2^15.
+constexpr float kSlack = 5.f;
 template <bool kBf16>
-constexpr float kLiftBits = kBf16 ? 0.f : 15.f;
+constexpr float kLiftBits = kBf16 ? 0.f : 15.f - kSlack;
 
 template <bool kBf16>
 __device__ __forceinline__ bool infinite(uint32_t bits)
@@ -446,50 +462,80 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     // The lane's key (lane % kTile) of the tile at `ahead`: its page and slot.
     Place ahead = here;
     const int32_t *table = a.table + (int64_t)here.b * a.width;
-    int page = -1, slot = 0, foundKv = here.kv;
-    bool key = false;
+    uint32_t page = 0, t = 0, column = 0, slot = 0;
+    int foundKv = here.kv;
+    bool key = false, enters = true;  // enters: `ahead` is the first tile of its block here
+    const uint32_t pageSize = (uint32_t)a.pageSize, stepColumns = L::kUnit / pageSize, stepSlots = L::kUnit % pageSize;
     const auto find_page = [&]() {
-        uint32_t t = 0;
         key = false;
         if (ahead.inside(args, end)) {
-            t = (uint32_t)(ahead.keys.first + ahead.tile) * L::kUnit + keyWave * kTile + lane % kTile;
+            if (enters) {
+                t = (uint32_t)(ahead.keys.first + ahead.tile) * L::kUnit + keyWave * kTile + lane % kTile;
+                column = t / pageSize;
+                slot = t - column * pageSize;
+                table = a.table + (int64_t)ahead.b * a.width;
+                foundKv = ahead.kv;
+            } else {
+                t += L::kUnit;
+                slot += stepSlots;
+                const bool over_ = slot >= pageSize;
+                column += stepColumns + (over_ ? 1u : 0u);
+                slot -= over_ ? pageSize : 0u;
+            }
             key = t >= (uint32_t)ahead.keys.low && t < (uint32_t)ahead.keys.high;
-            table = a.table + (int64_t)ahead.b * a.width;
-            foundKv = ahead.kv;
             ahead.advance(args);
+            enters = ahead.tile == 0;
         }
         // (Always a load, of the row's first entry where there is no key: under a branch it would
         // be waited for at once.)
-        const uint32_t at = (key ? t : 0u) / (uint32_t)a.pageSize;
-        page = table[at];
-        slot = (int)(t - at * (uint32_t)a.pageSize);
+        page = (uint32_t)table[key ? column : 0u];
     };
     uint64_t loaded = 0;  // keys of the tile on its way
     const auto load = [&](int buffer) {
-        const bool seen = key && page >= 0 && page < a.pages;
+        const bool seen = key && page < (uint64_t)a.pages;
         loaded = __ballot(seen);
         if constexpr (kTile == 32) {
             loaded &= 0xFFFFFFFFull;
         }
-        const char *zeros = reinterpret_cast<const char *>(kZeros);
-        const char *kRow = seen ? static_cast<const char *>(a.kCache.data) +
-                                      2 * (foundKv * a.kCache.head + page * a.kCache.page + slot * a.kCache.slot)
-                                : zeros;
-        const char *vRow = seen ? static_cast<const char *>(a.vCache.data) +
-                                      2 * (foundKv * a.vCache.head + page * a.vCache.page + slot * a.vCache.slot)
-                                : zeros;
+        const uint64_t kAt = 2 * (page * (uint64_t)a.kCache.page + slot * (uint64_t)a.kCache.slot);
+        const uint64_t kFirst = (uint64_t)a.kCache.data + 2 * foundKv * a.kCache.head;
+        const uint64_t vFirst = (uint64_t)a.vCache.data + 2 * foundKv * a.vCache.head;
         auto *const to = mine + buffer * L::kBuffer;
+        if (args.grouped && loaded == (kTile == 64 ? ~0ull : 0xFFFFFFFFull)) {
+            // The row where a group of rows begins is found by one lane for all, and the others lie
+            // behind it: no address is a lane's own.
+            const uint32_t slotBytes = 2 * (uint32_t)a.kCache.slot;
+#pragma unroll
+            for (int n = 0; n < L::kLoads; ++n) {
+                const int first = (n * L::kRowWaves + rowWave) * kWave, at = first + lane;
+                const int r = at / L::kChunks, ch = at % L::kChunks ^ L::turn(r), group = first / L::kChunks & -L::kGroupRows;
+                const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(kAt >> 32), group) << 32 |
+                                     (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)kAt, group);
+                const uint32_t offset = (uint32_t)(r - group) * slotBytes + ch * 16;
+                load_to_lds(kFirst + row, offset, to + first * 16);
+                load_to_lds(vFirst + row, offset, to + L::kSide + first * 16);
+            }
+            return;
+        }
+        const uint64_t vAt = 2 * (page * (uint64_t)a.vCache.page + slot * (uint64_t)a.vCache.slot);
+        const uint64_t zeros = (uint64_t)kZeros;
+        const int64_t kRow = (int64_t)(seen ? kFirst + kAt : zeros), vRow = (int64_t)(seen ? vFirst + vAt : zeros);
+        uint64_t k[L::kLoads], v[L::kLoads];
 #pragma unroll
         for (int n = 0; n < L::kLoads; ++n) {
-            const int first = (n * L::kRowWaves + rowWave) * kWave, at = first + lane;
+            const int at = (n * L::kRowWaves + rowWave) * kWave + lane;
             const int r = at / L::kChunks, ch = at % L::kChunks ^ L::turn(r);
-            const char *k = reinterpret_cast<const char *>(shfl64(reinterpret_cast<int64_t>(kRow), r)) + ch * 16;
-            const char *v = reinterpret_cast<const char *>(shfl64(reinterpret_cast<int64_t>(vRow), r)) + ch * 16;
+            k[n] = (uint64_t)shfl64(kRow, r) + ch * 16;
+            v[n] = (uint64_t)shfl64(vRow, r) + ch * 16;
             if (ch * 8 >= a.d) {
-                k = v = zeros;
+                k[n] = v[n] = zeros;
             }
-            load_to_lds(k, to + first * 16);
-            load_to_lds(v, to + L::kSide + first * 16);
+        }
+#pragma unroll
+        for (int n = 0; n < L::kLoads; ++n) {
+            const int first = (n * L::kRowWaves + rowWave) * kWave;
+            load_to_lds((const void *)k[n], to + first * 16);
+            load_to_lds((const void *)v[n], to + L::kSide + first * 16);
         }
     };
     // The operand of the rows of a place's block.  (It is turned where it is used first: what a
@@ -607,7 +653,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                 const uint32_t bits = (uint32_t)(seen >> (32 * kt)) >> (4 * half);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    s[kt][i] = (bits >> (8 * (i / 4) + i % 4) & 1u) != 0u ? s[kt][i] : -INFINITY;
+                    s[kt][i] = (int)(bits << (31 - (8 * (i / 4) + i % 4))) < 0 ? s[kt][i] : -INFINITY;
                 }
             }
         }
@@ -620,10 +666,10 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
             }
         }
         most = fmaxf(most, __shfl_xor(most, 32));
-        const float next = fmaxf(top, most * factor);
-        const float zero = next == -INFINITY ? 0.f : next;
-        if (__any((int)(next > top))) {  // (else the sums are on the right scale)
-            const float keep = __builtin_amdgcn_exp2f(top - zero);
+        most *= factor;
+        if (__any((int)(most > top + kSlack))) {
+            const float next = most > top + kSlack ? most : top;
+            const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.f : next));
             top = next;
             sum *= keep;
 #pragma unroll
@@ -634,7 +680,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                 }
             }
         }
-        const float shift = kLiftBits<kBf16> - zero;
+        const float shift = kLiftBits<kBf16> - (top == -INFINITY ? 0.f : top);
         // The weights of 16 keys, two at a time, between the products of the 16 before, whose
         // values of V are read ahead.
         constexpr int kGroups = kTile / 16, kProducts = kGroups * kDims, kAhead = kProducts < 4 ? kProducts : 4;
@@ -729,6 +775,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         load_q(here);
         ahead = here;
         ahead.tile = firstTile;
+        enters = true;
         for (int tile = firstTile; tile <= lastTile; ++tile) {
             find_page();
             __syncthreads();  // (the tile before is done)
@@ -835,6 +882,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
             again(firstTile);
             // The next one anew.
             ahead = next;
+            enters = true;
             find_page();
             load(buffer ^ 1);
             find_page();

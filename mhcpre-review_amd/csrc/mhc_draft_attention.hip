@@ -21,6 +21,11 @@ void plan_kind(Args &p, int cus)
         p.rows = L::kBlock;
         p.unit = L::kUnit;
         p.most = cus * L::kPerCu;
+        // (A page's rows by 32-bit offsets from a group's first one; d as wide as the layout, for
+        // what lies behind a narrower row is not read.)
+        const DraftAttentionArgs &a = p.a;
+        p.grouped = a.pageSize % L::kGroupRows == 0 && a.d == L::D && a.kCache.page == a.vCache.page &&
+                    a.kCache.slot == a.vCache.slot && a.kCache.slot < (1 << 24);
         return 0;
     });
 }
