@@ -85,8 +85,9 @@ struct Layout {
     // Workgroups of a CU: what its registers (two waves a SIMD up to D = 128) and LDS hold.
     static constexpr int kPerCu = kThreads == 256 && D <= 128 && 2 * (kLds + kMore) <= 160 * 1024 ? 2 : 1;
     static_assert(kLoads * kRowWaves * 1024 == kSide && kLds + kMore <= 160 * 1024);
-    // A wave's output fits a buffer (the groups of key waves leave theirs there to be joined).
-    static_assert(kKeyWaves == 1 || (kRows * D * 4 <= kBuffer && (kRowWaves == 1 || kRowWaves <= kKeyWaves)));
+    // What a group's waves leave to be joined fits a buffer.
+    static_assert(kKeyWaves == 1 || (kRowWaves == 1 && kRows * D * 4 <= kBuffer) ||
+                  kRowWaves * kRows * D * 4 / kKeyWaves <= kBuffer);
 
     // Rows that whole loads of 64 chunks cover together: in a page of a multiple of these the
     // loads of such a group have one page.
@@ -139,6 +140,7 @@ struct Keys {
 struct Sequence {
     int c, n;  // tokens in front of the new ones, new ones
 
+    __device__ Sequence(int c_, int n_) : c(c_), n(n_) {}
     __device__ Sequence(const DraftAttentionArgs &a, int L, int m)
     {
         const int most = a.width * a.pageSize;
@@ -157,9 +159,11 @@ struct Sequence {
     }
     __device__ Keys keys(const Args &args, int block) const
     {
-        const int i0 = (int)((int64_t)block * args.rows / args.group);
-        const int64_t last = ((int64_t)(block + 1) * args.rows + args.group - 1) / args.group;
-        const int i1 = last < n ? (int)last : n;
+        // (rows of a kv head stay below 2^30)
+        const uint32_t group = (uint32_t)args.group, row0 = (uint32_t)(block * args.rows);
+        const int i0 = args.blocks == 1 ? 0 : (int)(row0 / group);
+        const int last = args.blocks == 1 ? n : (int)((row0 + (uint32_t)args.rows + group - 1) / group);
+        const int i1 = last < n ? last : n;
         Keys k{0, 0, 0, 1};
         if (i0 < n) {
             // A chain's token i is at position c + i, a tree's at c or later.
@@ -252,34 +256,52 @@ struct Place {
     }
 };
 
-// The line of all tiles.
+// The line of all tiles, 64 sequences at a time: a lane has one's context, new tokens and
+// units, and the units up to it.
 struct Line {
     int all;  // all units
+    int c, n, units, upto;  // of sequences 0 to 63
 
-    // Finds the first tile at unit `at` of the line or behind it.
-    __device__ static Place find(const Args &args, int at)
+    __device__ explicit Line(const Args &args) : all(0)
+    {
+        for (int b0 = 0; b0 < args.a.B; b0 += kWave) {
+            Line part;
+            part.read(args, b0);
+            all += __builtin_amdgcn_readlane(part.upto, kWave - 1);
+            if (b0 == 0) {
+                c = part.c;
+                n = part.n;
+                units = part.units;
+                upto = part.upto;
+            }
+        }
+    }
+    // The first tile at unit `at` of the line or behind it.
+    __device__ Place find(const Args &args, int at) const
     {
         const DraftAttentionArgs &a = args.a;
-        const int lane = (int)threadIdx.x % kWave;
         int base = 0;
-        for (int b0 = 0;; b0 += kWave) {
-            const int x = b0 + lane;
-            const int units = x < a.B ? Sequence::of(a, x).units(args) * a.kvHeads : 0;
-            const int upto = dev::wave_scan(units);
-            const uint64_t past = __ballot(base + upto > at);
+        Line part = *this;
+        for (int b0 = 0;;) {
+            const uint64_t past = __ballot(base + part.upto > at);
             if (past == 0 && b0 + kWave < a.B) {
-                base += __builtin_amdgcn_readlane(upto, kWave - 1);
+                base += __builtin_amdgcn_readlane(part.upto, kWave - 1);
+                b0 += kWave;
+                part.read(args, b0);
                 continue;
             }
             const int hit = __ffsll((unsigned long long)past) - 1;
             Place p;
             p.b = b0 + hit;
-            const int all = __builtin_amdgcn_readlane(units, hit) / a.kvHeads;
-            base += __builtin_amdgcn_readlane(upto, hit) - all * a.kvHeads;
-            p.kv = (at - base) / all;
-            base += p.kv * all;
+            p.c = __builtin_amdgcn_readlane(part.c, hit);
+            p.n = __builtin_amdgcn_readlane(part.n, hit);
+            const int row = __builtin_amdgcn_readlane(part.units, hit);
+            base += __builtin_amdgcn_readlane(part.upto, hit) - row;
+            const uint32_t one = (uint32_t)row / (uint32_t)a.kvHeads;
+            p.kv = (int)((uint32_t)(at - base) / one);
+            base += p.kv * (int)one;
             for (p.block = 0;; ++p.block) {
-                p.enter(args);
+                p.keys = Sequence(p.c, p.n).keys(args, p.block);
                 if (at < base + kItemUnits + p.keys.tiles) {
                     break;
                 }
@@ -290,14 +312,17 @@ struct Line {
             return p;
         }
     }
-    __device__ explicit Line(const Args &args) : all(0)
+
+private:
+    Line() = default;
+    __device__ void read(const Args &args, int b0)
     {
-        const int lane = (int)threadIdx.x % kWave;
-        for (int b0 = 0; b0 < args.a.B; b0 += kWave) {
-            const int x = b0 + lane;
-            all += __builtin_amdgcn_readlane(
-                dev::wave_scan(x < args.a.B ? Sequence::of(args.a, x).units(args) * args.a.kvHeads : 0), kWave - 1);
-        }
+        const int x = b0 + (int)threadIdx.x % kWave;
+        const Sequence s = Sequence::of(args.a, x < args.a.B ? x : 0);
+        c = s.c;
+        n = s.n;
+        units = x < args.a.B ? s.units(args) * args.a.kvHeads : 0;
+        upto = dev::wave_scan(units);
     }
 };
 
@@ -454,7 +479,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         return;
     }
     const int begin = shares.start(w), end = shares.start(w + 1);
-    Place here = Line::find(args, begin);
+    Place here = line.find(args, begin);
     if (!here.inside(args, end)) {
         return;
     }
@@ -825,7 +850,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     load_q(here);
     clear();
     int firstTile = here.tile;  // of the block, in this stretch
-    bool fresh = true, wholeStretch = true;
+    bool fresh = true, firstBlock = true;
     for (int buffer = 0;; buffer ^= 1) {
         const uint64_t valid = loaded;
         dev::wait_vm<0>();  // (the tile is there, the next one's pages are known, and so is q)
@@ -849,21 +874,17 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         }
 
         // The block's end, or the stretch's.
-        bool finite = true;
+        float none = 0.f;  // 0 times a value that is not finite is no number
 #pragma unroll
         for (int j = 0; j < kDims; ++j) {
-            float none = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                none += o[j][i] * 0.f;
+                none = __builtin_fmaf(o[j][i], 0.f, none);
             }
-            finite = finite && none == 0.f;
         }
+        const bool finite = __all((int)(none == 0.f));
         if (lane == 0) {
-            odd[wave] = false;
-        }
-        if (!finite) {
-            odd[wave] = true;
+            odd[wave] = !finite;
         }
         Place next = here;
         next.advance(args);
@@ -903,90 +924,97 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                 }
             }
         }
-        if constexpr (L::kKeyWaves > 1) {
-            // The groups' results together, in the first one's registers: the others leave theirs,
-            // as they lie, in the buffers that are read.
-            const auto left = [&](int k, int x) {
-                const int region = L::kRowWaves == 1 ? k : rowWave;
-                return (__attribute__((address_space(3))) f32x4_t *)(uintptr_t)(
-                    (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (2 * region + buffer) * L::kBuffer +
-                    (x * kWave + lane) * 16);
-            };
-            __syncthreads();
-            if (half == 0) {
-                ends[keyWave][rowWave * kRows + col] = float2{top, sum};
-            }
-            if (keyWave > 0) {
-#pragma unroll
-                for (int j = 0; j < kDims; ++j) {
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        *left(keyWave, 4 * j + i / 4) = f32x4_t{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]};
-                    }
-                }
-            }
-            __syncthreads();
-            if (keyWave == 0) {
-                float2 end_[L::kKeyWaves];
-                float most = -INFINITY;
-#pragma unroll
-                for (int k = 0; k < L::kKeyWaves; ++k) {
-                    end_[k] = ends[k][rowWave * kRows + col];
-                    most = fmaxf(most, end_[k].x);
-                }
-                const float zero = most == -INFINITY ? 0.f : most;
-                top = most;
-                sum = 0.f;
-#pragma unroll
-                for (int k = 0; k < L::kKeyWaves; ++k) {
-                    const float f = __builtin_amdgcn_exp2f(end_[k].x - zero);
-                    sum += f * end_[k].y;
-#pragma unroll
-                    for (int j = 0; j < kDims; ++j) {
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            if (k == 0) {
-#pragma unroll
-                                for (int y = 0; y < 4; ++y) {
-                                    o[j][i + y] = scaled(o[j][i + y], f);
-                                }
-                            } else {
-                                const f32x4_t v = *left(k, 4 * j + i / 4);
-#pragma unroll
-                                for (int y = 0; y < 4; ++y) {
-                                    o[j][i + y] += scaled(v[y], f);
-                                }
-                            }
-                        }
-                    }
-                }
-            }
-        }
         const bool all = firstTile == 0 && here.tile + 1 == here.keys.tiles;
-        const int slot = 2 * w + (wholeStretch ? 0 : 1);
+        const int slot = 2 * w + (firstBlock ? 0 : 1);
         if (threadIdx.x == 0 && firstTile == 0 && !all) {
             args.open[w] = Open{here.b, here.kv, here.block, here.start, here.start + here.keys.tiles - 1, line.all, slot, 0};
         }
-        if (keyWave == 0) {
-            const int r = rowWave * kRows + col, x = here.block * L::kBlock + r;
-            const int head = x % args.group;
-            if (node < a.S) {
+        // 4 values of the lane's row, from e on.
+        const int r = rowWave * kRows + col;
+        const int head = here.block * L::kBlock + r - node * args.group;
+        const auto put = [&](int e, f32x4_t value, float t, float total) {
+            if (node >= a.S) {
+            } else if (all) {
+                finish<kBf16>(args, here, node, head, e, value, t, total);
+            } else {
+                *reinterpret_cast<f32x4_t *>(args.outs + ((int64_t)slot * L::kBlock + r) * D + e) = value;
+                if (e == 0) {
+                    *reinterpret_cast<float2 *>(args.ends + ((int64_t)slot * L::kBlock + r) * 2) = float2{t, total};
+                }
+            }
+        };
+        if constexpr (L::kKeyWaves == 1) {
 #pragma unroll
-                for (int j = 0; j < kDims; ++j) {
+            for (int j = 0; j < kDims; ++j) {
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const int e = 32 * j + 2 * i + 4 * half;
-                        const f32x4_t value = {o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]};
-                        if (all) {
-                            finish<kBf16>(args, here, node, head, e, value, top, sum);
-                        } else {
-                            *reinterpret_cast<f32x4_t *>(args.outs + ((int64_t)slot * L::kBlock + r) * D + e) = value;
+                for (int i = 0; i < 16; i += 4) {
+                    put(32 * j + 2 * i + 4 * half, f32x4_t{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]}, top, sum);
+                }
+            }
+        } else {
+            // The groups' results together: each has a share of the values and leaves the others',
+            // as they lie in its registers, in the buffer that it has read.
+            constexpr int kShare = kDims * 4 / L::kKeyWaves;  // fours of values
+            const auto left = [&](int k, int x) {
+                return (__attribute__((address_space(3))) f32x4_t *)(uintptr_t)(
+                    (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (2 * k + buffer) * L::kBuffer +
+                    ((L::kRowWaves == 1 ? x : rowWave * kShare + x % kShare) * kWave + lane) * 16);
+            };
+            __syncthreads();  // (the tiles are read)
+            if (half == 0) {
+                ends[keyWave][r] = float2{top, sum};
+            }
+#pragma unroll
+            for (int share = 0; share < L::kKeyWaves; ++share) {
+                if (share != keyWave) {
+#pragma unroll
+                    for (int x = share * kShare; x < (share + 1) * kShare; ++x) {
+                        const f32x16_t &from_ = o[x / 4];
+                        const int i = x % 4 * 4;
+                        *left(keyWave, x) = f32x4_t{from_[i], from_[i + 1], from_[i + 2], from_[i + 3]};
+                    }
+                }
+            }
+            __syncthreads();
+            float f[L::kKeyWaves], total = 0.f, most = -INFINITY;
+            float2 end_[L::kKeyWaves];
+#pragma unroll
+            for (int k = 0; k < L::kKeyWaves; ++k) {
+                end_[k] = ends[k][r];
+                most = fmaxf(most, end_[k].x);
+            }
+#pragma unroll
+            for (int k = 0; k < L::kKeyWaves; ++k) {
+                f[k] = __builtin_amdgcn_exp2f(end_[k].x - (most == -INFINITY ? 0.f : most));
+                total += f[k] * end_[k].y;
+            }
+            const auto join = [&](auto kInfinite) {
+#pragma unroll
+                for (int share = 0; share < L::kKeyWaves; ++share) {
+                    if (share == keyWave) {
+#pragma unroll
+                        for (int x = share * kShare; x < (share + 1) * kShare; ++x) {
+                            f32x4_t value = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int k = 0; k < L::kKeyWaves; ++k) {
+                                const f32x16_t &own = o[x / 4];
+                                const int i = x % 4 * 4;
+                                const f32x4_t v = k == share ? f32x4_t{own[i], own[i + 1], own[i + 2], own[i + 3]}
+                                                             : *left(k, x);
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) {
+                                    value[y] += decltype(kInfinite)::value ? scaled(v[y], f[k]) : v[y] * f[k];
+                                }
+                            }
+                            put(x / 4 * 32 + x % 4 * 8 + 4 * half, value, most, total);
                         }
                     }
                 }
-                if (!all && half == 0) {
-                    *reinterpret_cast<float2 *>(args.ends + ((int64_t)slot * L::kBlock + r) * 2) = float2{top, sum};
-                }
+            };
+            if (redo) {
+                join(std::true_type{});
+            } else {
+                join(std::false_type{});
             }
         }
         if (!more) {
@@ -998,7 +1026,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         here = next;
         firstTile = 0;
         fresh = true;
-        wholeStretch = false;
+        firstBlock = false;
         clear();
     }
     dev::wait_vm<0>();  // (the rows of zeros, before the LDS is another workgroup's)
@@ -1007,7 +1035,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
 // Joins the parts of the (sequence, kv head, block)s that no stretch finished: a workgroup
 // for some rows of the one that stretch blockIdx.x began.
 constexpr int kJoinThreads = 256;
-constexpr int kJoinBatch = 8;
+constexpr int kJoinBatch = 16;
 
 template <bool kBf16, int D>
 __global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
@@ -1037,10 +1065,13 @@ __global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
         f32x4_t outs[kJoinBatch];
 #pragma unroll
         for (int m = 0; m < kJoinBatch; ++m) {
-            const int x = x0 + m <= last ? x0 + m : last;
-            const int64_t slot = x == first ? open.slot : 2 * x;
-            ends[m] = *reinterpret_cast<const float2 *>(args.ends + (slot * args.rows + r) * 2);
-            outs[m] = *reinterpret_cast<const f32x4_t *>(args.outs + (slot * args.rows + r) * D + e);
+            ends[m] = float2{-INFINITY, 0.f};
+            outs[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (x0 + m <= last) {
+                const int64_t slot = x0 + m == first ? open.slot : 2 * (x0 + m);
+                ends[m] = *reinterpret_cast<const float2 *>(args.ends + (slot * args.rows + r) * 2);
+                outs[m] = *reinterpret_cast<const f32x4_t *>(args.outs + (slot * args.rows + r) * D + e);
+            }
         }
         float next = top;
 #pragma unroll

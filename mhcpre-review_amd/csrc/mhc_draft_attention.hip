@@ -54,7 +54,7 @@ bool draft_attention_units_fit(const DraftAttentionArgs &a)
     const int64_t blocks = ((int64_t)a.S * (a.heads / a.kvHeads) + draft::kRows - 1) / draft::kRows;
     const int64_t units = (int64_t)a.width * a.pageSize / 32 + 2 + draft::kItemUnits;
     int64_t all;
-    return !__builtin_mul_overflow(units, blocks, &all) && !__builtin_mul_overflow(all, (int64_t)a.B * a.kvHeads, &all) &&
+    return blocks <= (1 << 25) && !__builtin_mul_overflow(units, blocks, &all) && !__builtin_mul_overflow(all, (int64_t)a.B * a.kvHeads, &all) &&
            all < INT32_MAX;
 }
 

@@ -232,18 +232,23 @@ struct Range {
     }
 };
 
-// A workgroup does a page of a row and 16 pieces of 16 bytes (of the page's heads and
-// dimensions): a thread a piece, every 16th token.
-constexpr int kBoundsThreads = 256, kPieces = 16, kSplit = kBoundsThreads / kPieces, kBoundsBatch = 4;
-constexpr int64_t kBoundsMost = 1 << 20;  // workgroups of a launch
+// kLanes lanes do 16 bytes (of a head's dimensions) of a page of a row, each every
+// kLanes-th token; neighbouring groups have neighbouring pieces.  A lane has kBoundsBatch
+// tokens on their way at once.
+constexpr int kBoundsThreads = 256, kBoundsBatch = 8;
 
-template <bool kBf16>
+template <bool kBf16, int kLanes>
 __global__ __launch_bounds__(kBoundsThreads) void bounds_pages(CacheBoundsArgs a)
 {
-    __shared__ Range others[kBoundsThreads / kWave - 1][kPieces];
+    constexpr int kPieces = kBoundsThreads / kLanes;  // of a workgroup
+    // Lanes of a piece lie kStride lanes apart in a wave.
+    constexpr int kStride = kWave / kLanes;
+    const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
+    const int split = lane / kStride, inGroup = wave * kStride + lane % kStride;
     for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
-        const int64_t b = item / ((int64_t)a.columns * a.pieceGroups);
-        const int inRow = (int)(item % ((int64_t)a.columns * a.pieceGroups));
+        const int64_t perRow = (int64_t)a.columns * a.pieceGroups;
+        const int64_t b = a.B == 1 ? 0 : item / perRow;
+        const int inRow = (int)(item - b * perRow);
         const int L = clamped(a.lengths[b], a.width * a.pageSize);
         const int wanted = clamped(a.counts[b], a.tokens), count = wanted < L ? wanted : L, begin = L - count;
         const int64_t column = (int64_t)(begin / a.pageSize) + inRow / a.pieceGroups;
@@ -255,8 +260,7 @@ __global__ __launch_bounds__(kBoundsThreads) void bounds_pages(CacheBoundsArgs a
         if (page < 0 || page >= a.pages) {
             continue;
         }
-        const int chunks = a.d / 8, piece = inRow % a.pieceGroups * kPieces + (int)threadIdx.x % kPieces;
-        const int split = (int)threadIdx.x / kPieces;
+        const int chunks = a.d / 8, piece = inRow % a.pieceGroups * kPieces + inGroup;
         const bool on = piece < a.kvHeads * chunks;
         const int head = on ? piece / chunks : 0, e = on ? piece % chunks * 8 : 0;
         const uint32_t first = begin > start ? (uint32_t)(begin - start) : 0u;
@@ -266,15 +270,17 @@ __global__ __launch_bounds__(kBoundsThreads) void bounds_pages(CacheBoundsArgs a
         uint16_t *hi = static_cast<uint16_t *>(a.hi.data) + page * a.hi.row + head * a.hi.head + e;
         Range range;
         range.clear();
-        if (split == 0 && first > 0) {
-            range.add(*reinterpret_cast<const u32x4_t *>(lo), *reinterpret_cast<const u32x4_t *>(hi));
-            range.mark<kBf16>();
+        const bool old = split == 0 && first > 0;
+        u32x4_t oldLow = {0, 0, 0, 0}, oldHigh = oldLow;
+        if (old) {
+            oldLow = *reinterpret_cast<const u32x4_t *>(lo);
+            oldHigh = *reinterpret_cast<const u32x4_t *>(hi);
         }
-        for (uint32_t t0 = first + split; t0 < end; t0 += kSplit * kBoundsBatch) {
+        for (uint32_t t0 = first + split; t0 < end; t0 += kLanes * kBoundsBatch) {
             u32x4_t k[kBoundsBatch];
 #pragma unroll
             for (int x = 0; x < kBoundsBatch; ++x) {
-                const uint32_t t = t0 + x * kSplit < end ? t0 + x * kSplit : t0;
+                const uint32_t t = t0 + x * kLanes < end ? t0 + x * kLanes : t0;
                 k[x] = *reinterpret_cast<const u32x4_t *>(from + t * a.k.slot);
             }
 #pragma unroll
@@ -282,20 +288,19 @@ __global__ __launch_bounds__(kBoundsThreads) void bounds_pages(CacheBoundsArgs a
                 range.add(k[x], k[x]);
             }
         }
-        range.add(range.shuffled(16));
-        range.add(range.shuffled(32));
-        const int wave = (int)threadIdx.x / kWave;
-        __syncthreads();  // (the page before is done)
-        if (wave > 0 && (int)threadIdx.x % kWave < kPieces) {
-            others[wave - 1][threadIdx.x % kPieces] = range;
-        }
-        __syncthreads();
-        if (split != 0 || !on) {
-            continue;
+        if (old) {
+            Range before;
+            before.clear();
+            before.add(oldLow, oldHigh);
+            before.mark<kBf16>();
+            range.add(before);
         }
 #pragma unroll
-        for (int x = 0; x < kBoundsThreads / kWave - 1; ++x) {
-            range.add(others[x][threadIdx.x]);
+        for (int mask = kStride; mask < kWave; mask *= 2) {
+            range.add(range.shuffled(mask));
+        }
+        if (split != 0 || !on) {
+            continue;
         }
         range.mark<kBf16>();
         constexpr uint32_t kNan = kBf16 ? 0x7FC0 : 0x7E00;
@@ -355,20 +360,38 @@ hipError_t launch_cache_keep(const CacheKeepArgs &a, hipStream_t stream)
     return a.elemBytes == 4 ? launch_keep<uint32_t>(a, stream) : launch_keep<uint16_t>(a, stream);
 }
 
-hipError_t launch_cache_bounds(const CacheBoundsArgs &given, hipStream_t stream)
+namespace {
+
+// Workgroups of a launch: what is on the CUs at once, a few times over.
+constexpr int64_t kBoundsMost = 8192;
+
+template <bool kBf16, int kLanes>
+hipError_t launch_bounds(CacheBoundsArgs a, hipStream_t stream)
 {
-    CacheBoundsArgs a = given;
+    constexpr int kPieces = kBoundsThreads / kLanes;
     const int64_t columns = ((int64_t)a.tokens + a.pageSize - 2) / a.pageSize + 1;
     a.columns = (int)(columns < a.width ? columns : (int64_t)a.width);
     a.pieceGroups = (a.kvHeads * (a.d / 8) + kPieces - 1) / kPieces;
     a.items = (int64_t)a.B * a.columns * a.pieceGroups;
-    const dim3 grid((unsigned)(a.items < kBoundsMost ? a.items : kBoundsMost));
-    if (a.isBf16) {
-        hipLaunchKernelGGL((bounds_pages<true>), grid, dim3(kBoundsThreads), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((bounds_pages<false>), grid, dim3(kBoundsThreads), 0, stream, a);
-    }
+    hipLaunchKernelGGL((bounds_pages<kBf16, kLanes>), dim3((unsigned)(a.items < kBoundsMost ? a.items : kBoundsMost)),
+                       dim3(kBoundsThreads), 0, stream, a);
     return hipGetLastError();
+}
+
+template <bool kBf16>
+hipError_t launch_bounds_type(const CacheBoundsArgs &a, hipStream_t stream)
+{
+    // Tokens of a page that a call may bring: several lanes to a piece where they are many.
+    const int64_t tokens = a.tokens < a.pageSize ? a.tokens : a.pageSize;
+    return tokens <= 16 ? launch_bounds<kBf16, 1>(a, stream)
+           : tokens <= 64 ? launch_bounds<kBf16, 4>(a, stream) : launch_bounds<kBf16, 16>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_cache_bounds(const CacheBoundsArgs &a, hipStream_t stream)
+{
+    return a.isBf16 ? launch_bounds_type<true>(a, stream) : launch_bounds_type<false>(a, stream);
 }
 
 }  // namespace mhc

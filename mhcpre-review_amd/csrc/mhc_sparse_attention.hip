@@ -20,7 +20,7 @@ using dev::kWave;
 using dev::u32x4_t;
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kColumns = 256;  // columns of a workgroup's item
+constexpr int kColumns = 64;  // columns of a workgroup's item
 
 // Scores as ordered integers; what cannot be taken is 0.
 constexpr uint64_t kAlways = ~0ull, kNotANumber = ~0ull - 1;
