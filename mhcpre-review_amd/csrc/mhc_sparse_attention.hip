@@ -20,7 +20,7 @@ using dev::kWave;
 using dev::u32x4_t;
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kColumns = 64;  // columns of a workgroup's item
+constexpr int kBatch = 4;  // pages of a group of lanes on their way at once
 
 // Scores as ordered integers; what cannot be taken is 0.
 constexpr uint64_t kAlways = ~0ull, kNotANumber = ~0ull - 1;
@@ -30,6 +30,7 @@ struct Args {
     uint64_t *keys;     // [B * kvHeads, width]
     int32_t *table;     // [B * kvHeads, top]: the pages taken
     int32_t *lengths;   // [B * kvHeads]: their tokens
+    int columns;        // of a workgroup's item
 };
 
 // Columns that row b of the batch holds, and its tokens.
@@ -58,55 +59,73 @@ __global__ __launch_bounds__(kThreads) void score_pages(Args args)
     const SparseAttentionArgs &s = args.a;
     const PagedAttentionArgs &a = s.attention;
     constexpr int kPages = kWave / kLanes;  // of a wave at a time
-    constexpr int kBatch = 2;
     const int lane = (int)threadIdx.x % kWave, wave = (int)threadIdx.x / kWave;
     const int sub = lane % kLanes, e = 8 * sub;
     const bool on = e < a.d;
-    const int group = a.heads / a.kvHeads, chunks = (a.width + kColumns - 1) / kColumns;
+    const int group = a.heads / a.kvHeads, chunks = (a.width + args.columns - 1) / args.columns;
     const int64_t items = (int64_t)a.B * a.kvHeads * chunks;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int64_t row = item / chunks;
-        const int b = (int)(row / a.kvHeads), kv = (int)(row % a.kvHeads), column0 = (int)(item % chunks) * kColumns;
+        const int b = (int)(row / a.kvHeads), kv = (int)(row % a.kvHeads), column0 = (int)(item % chunks) * args.columns;
         const Row r(a, b);
         if (column0 >= r.held) {
             continue;
         }
+        const int end = r.held - column0 < args.columns ? r.held : column0 + args.columns;
+        const int32_t *table = a.table + (int64_t)b * a.width;
+        // The pages of a step are known a step ahead.
+        int c0 = column0 + wave * kPages + lane / kLanes;
+        int page[kBatch], next[kBatch];
+        const auto find = [&](int from) {
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x) {
+                const int c = from + x * kWaves * kPages;
+                next[x] = table[c < end ? c : column0];
+            }
+        };
+        find(c0);
         double up[8], down[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
             up[x] = down[x] = 0;
         }
-        const uint16_t *q = static_cast<const uint16_t *>(a.q.data) + b * a.q.row + (int64_t)kv * group * a.q.head + e;
-        for (int h = 0; h < group && on; ++h) {
-            float f[8];
-            dev::unpack8<kBf16>(*reinterpret_cast<const u32x4_t *>(q + h * a.q.head), f);
+        const uint16_t *q = static_cast<const uint16_t *>(a.q.data) + b * a.q.row + (int64_t)kv * group * a.q.head +
+                            (on ? e : 0);
+        for (int h0 = 0; h0 < group; h0 += 4) {
+            u32x4_t heads[4];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {  // (NaN goes to both)
-                up[x] += f[x] < 0.f ? 0.0 : (double)f[x];
-                down[x] += f[x] > 0.f ? 0.0 : (double)f[x];
+            for (int y = 0; y < 4; ++y) {
+                heads[y] = *reinterpret_cast<const u32x4_t *>(q + (h0 + y < group ? h0 + y : h0) * a.q.head);
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                if (h0 + y < group) {
+                    float f[8];
+                    dev::unpack8<kBf16>(heads[y], f);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {  // (NaN goes to both)
+                        up[x] += f[x] < 0.f ? 0.0 : (double)f[x];
+                        down[x] += f[x] > 0.f ? 0.0 : (double)f[x];
+                    }
+                }
             }
         }
-        const int end = r.held - column0 < kColumns ? r.held : column0 + kColumns;
-        for (int c0 = column0 + wave * kPages + lane / kLanes; c0 - lane / kLanes < end; c0 += kBatch * kWaves * kPages) {
-            int page[kBatch];
+        const uint16_t *loBase = static_cast<const uint16_t *>(s.lo.data) + kv * s.lo.head + (on ? e : 0);
+        const uint16_t *hiBase = static_cast<const uint16_t *>(s.hi.data) + kv * s.hi.head + (on ? e : 0);
+        for (; c0 - lane / kLanes < end; c0 += kBatch * kWaves * kPages) {
             u32x4_t lo[kBatch], hi[kBatch];
 #pragma unroll
             for (int x = 0; x < kBatch; ++x) {
-                const int c = c0 + x * kWaves * kPages;
-                page[x] = c < end ? a.table[(int64_t)b * a.width + c] : -1;
-            }
-#pragma unroll
-            for (int x = 0; x < kBatch; ++x) {
-                const bool good = page[x] >= 0 && page[x] < a.pages;
-                page[x] = good ? page[x] : -1;
-                lo[x] = hi[x] = u32x4_t{0, 0, 0, 0};
-                if (good && on) {
-                    lo[x] = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(s.lo.data) +
-                                                               page[x] * s.lo.row + kv * s.lo.head + e);
-                    hi[x] = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(s.hi.data) +
-                                                               page[x] * s.hi.row + kv * s.hi.head + e);
+                const bool good = next[x] >= 0 && next[x] < a.pages && c0 + x * kWaves * kPages < end;
+                page[x] = good ? next[x] : -1;
+                const int64_t from = good ? next[x] : 0;  // (no page: the first one is read, and not used)
+                lo[x] = *reinterpret_cast<const u32x4_t *>(loBase + from * s.lo.row);
+                hi[x] = *reinterpret_cast<const u32x4_t *>(hiBase + from * s.hi.row);
+                if (!on) {
+                    lo[x] = hi[x] = u32x4_t{0, 0, 0, 0};
                 }
             }
+            find(c0 + kBatch * kWaves * kPages);
 #pragma unroll
             for (int x = 0; x < kBatch; ++x) {
                 float l[8], h[8];
@@ -136,30 +155,31 @@ __global__ __launch_bounds__(kThreads) void score_pages(Args args)
     }
 }
 
-// The highest `top` keys of a (sequence, kv head), in order.
-constexpr int kSelectThreads = 512, kSelectWaves = kSelectThreads / kWave, kBins = 256;
+// The highest `top` keys of a (sequence, kv head), in order.  A thread has kHeld columns
+// that follow each other (in registers; where the table is wider, segment by segment, read
+// anew in each round).
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave, kBins = 256;
+constexpr int kHeld = 8, kSegment = kSelectThreads * kHeld;
 
-template <typename T, typename F>
-__device__ __forceinline__ T reduced(T v, F &&f)
+template <typename F>
+__device__ __forceinline__ uint64_t reduced(uint64_t v, F &&f)
 {
 #pragma unroll
     for (int mask = 1; mask < kWave; mask *= 2) {
-        const uint64_t bits = (uint64_t)v;
-        const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)bits, mask),
-                       hi = (uint32_t)__shfl_xor((int)(bits >> 32), mask);
-        v = f(v, (T)((uint64_t)hi << 32 | lo));
+        const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, mask), hi = (uint32_t)__shfl_xor((int)(v >> 32), mask);
+        v = f(v, (uint64_t)hi << 32 | lo);
     }
     return v;
 }
 
+template <bool kOneSegment>
 __global__ __launch_bounds__(kSelectThreads) void select_pages(Args args)
 {
-    __shared__ uint64_t least[kSelectWaves], greatest[kSelectWaves];
-    __shared__ int there[kSelectWaves], always[kSelectWaves];
+    __shared__ uint64_t least[kSelectWaves], greatest[kSelectWaves], counts[kSelectWaves];
     __shared__ int bins[kBins];
     __shared__ uint64_t rangeLow;
     __shared__ int rangeNeed, rangeIn;
-    __shared__ int before[2][kSelectWaves];
+    __shared__ int before[kSelectWaves], tiesBefore[kSelectWaves];
     __shared__ int lastTaken;
     const SparseAttentionArgs &s = args.a;
     const PagedAttentionArgs &a = s.attention;
@@ -167,47 +187,67 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages(Args args)
     const int64_t row = blockIdx.x;
     const int b = (int)(row / a.kvHeads);
     const Row r(a, b);
-    const uint64_t *keys = args.keys + row * a.width;
+    const uint64_t *all = args.keys + row * a.width;
+    uint64_t keys[kHeld];
+    const int segments = kOneSegment ? 1 : (r.held + kSegment - 1) / kSegment;
+    const auto read = [&](int segment) {
+#pragma unroll
+        for (int x = 0; x < kHeld; ++x) {
+            const int c = segment * kSegment + (int)threadIdx.x * kHeld + x;
+            keys[x] = c < r.held ? all[c] : 0;
+        }
+    };
+    const auto each_segment = [&](auto &&f) {
+        for (int segment = 0; segment < segments; ++segment) {
+            if (!kOneSegment) {
+                read(segment);
+            }
+            f(segment);
+        }
+    };
+    if (kOneSegment) {
+        read(0);
+    }
 
     // How many can be taken, how many are in any case, and the others' range.
-    uint64_t low = kAlways, high = 0;
-    int some = 0, sure = 0;
-    for (int c = (int)threadIdx.x; c < r.held; c += kSelectThreads) {
-        const uint64_t key = keys[c];
-        some += key != 0 ? 1 : 0;
-        sure += key == kAlways ? 1 : 0;
-        if (key != 0 && key != kAlways) {
-            low = key < low ? key : low;
-            high = key > high ? key : high;
+    uint64_t low = kAlways, high = 0, count = 0;  // count: of the first in the lower half, of the second in the upper
+    each_segment([&](int) {
+#pragma unroll
+        for (int x = 0; x < kHeld; ++x) {
+            const uint64_t key = keys[x];
+            count += (key != 0 ? 1ull : 0ull) + (key == kAlways ? 1ull << 32 : 0ull);
+            const bool ranked = key != 0 && key != kAlways;
+            low = ranked && key < low ? key : low;
+            high = ranked && key > high ? key : high;
         }
-    }
+    });
     low = reduced(low, [](uint64_t x, uint64_t y) { return x < y ? x : y; });
     high = reduced(high, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
-    some = reduced(some, [](int x, int y) { return x + y; });
-    sure = reduced(sure, [](int x, int y) { return x + y; });
+    count = reduced(count, [](uint64_t x, uint64_t y) { return x + y; });
     if (threadIdx.x == 0) {
         lastTaken = 0;
     }
     if (lane == 0) {
         least[wave] = low;
         greatest[wave] = high;
-        there[wave] = some;
-        always[wave] = sure;
+        counts[wave] = count;
+    }
+    if ((int)threadIdx.x < kBins) {
+        bins[threadIdx.x] = 0;
     }
     __syncthreads();
-    some = sure = 0;
+    count = 0;
 #pragma unroll
     for (int x = 0; x < kSelectWaves; ++x) {
         low = least[x] < low ? least[x] : low;
         high = greatest[x] > high ? greatest[x] : high;
-        some += there[x];
-        sure += always[x];
+        count += counts[x];
     }
     // Taken: keys above `floor`, and the first `ties` of those that equal it.
     uint64_t floor = 0;
     int ties = 0;
-    if (some > s.top) {
-        int need = s.top - sure;  // of the keys in [low, high]
+    if ((int)(uint32_t)count > s.top) {
+        int need = s.top - (int)(count >> 32);  // of the keys in [low, high]
         if (need == 0) {
             floor = kAlways - 1;
         }
@@ -216,35 +256,34 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages(Args args)
             if ((high - low) / kBins != 0) {
                 shift = 64 - __clzll((long long)((high - low) / kBins));
             }
-            __syncthreads();
-            for (int x = (int)threadIdx.x; x < kBins; x += kSelectThreads) {
-                bins[x] = 0;
-            }
-            __syncthreads();
-            for (int c = (int)threadIdx.x; c < r.held; c += kSelectThreads) {
-                const uint64_t key = keys[c];
-                if (key >= low && key <= high) {
-                    atomicAdd(&bins[(key - low) >> shift], 1);
+            each_segment([&](int) {
+#pragma unroll
+                for (int x = 0; x < kHeld; ++x) {
+                    if (keys[x] >= low && keys[x] <= high) {
+                        atomicAdd(&bins[(keys[x] - low) >> shift], 1);
+                    }
                 }
-            }
+            });
             __syncthreads();
             if (wave == 0) {
                 // From the top: the bin at which `need` is reached.
-                int mine[kBins / kWave], all = 0;
+                int mine[kBins / kWave], sum = 0;
 #pragma unroll
                 for (int x = 0; x < kBins / kWave; ++x) {
                     mine[x] = bins[kBins - 1 - (lane * (kBins / kWave) + x)];
-                    all += mine[x];
+                    sum += mine[x];
                 }
-                int above = dev::wave_scan(all) - all;
+                int above = dev::wave_scan(sum) - sum;
 #pragma unroll
                 for (int x = 0; x < kBins / kWave; ++x) {
+                    const int bin = kBins - 1 - (lane * (kBins / kWave) + x);
                     if (above < need && above + mine[x] >= need) {
-                        rangeLow = low + ((uint64_t)(kBins - 1 - (lane * (kBins / kWave) + x)) << shift);
+                        rangeLow = low + ((uint64_t)bin << shift);
                         rangeNeed = need - above;
                         rangeIn = mine[x];
                     }
                     above += mine[x];
+                    bins[bin] = 0;
                 }
             }
             __syncthreads();
@@ -260,54 +299,80 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages(Args args)
                 ties = need;
                 need = 0;
             }
+            __syncthreads();  // (rangeLow and the others are read)
         }
     }
     // In the columns' order.
     int taken = 0, equal = 0;
     int32_t *columns = s.columns + row * s.top, *table = args.table + row * s.top;
-    for (int c0 = 0; c0 < r.held; c0 += kSelectThreads) {
-        const int c = c0 + (int)threadIdx.x;
-        const uint64_t key = c < r.held ? keys[c] : 0;
-        const bool tie = ties > 0 && key == floor;
-        const uint64_t tied = __ballot(tie);
-        __syncthreads();
-        if (lane == 0) {
-            before[0][wave] = __popcll(tied);
-        }
-        __syncthreads();
-        int rank = equal + __popcll(tied & ((1ull << lane) - 1));
+    each_segment([&](int segment) {
+        int tied = 0, takes = 0;
 #pragma unroll
-        for (int x = 0; x < kSelectWaves; ++x) {
-            rank += x < wave ? before[0][x] : 0;
-            equal += before[0][x];
+        for (int x = 0; x < kHeld; ++x) {
+            tied += ties > 0 && keys[x] == floor ? 1 : 0;
         }
-        const bool take = key > floor || (tie && rank < ties);
-        const uint64_t takes = __ballot(take);
-        if (lane == 0) {
-            before[1][wave] = __popcll(takes);
-        }
-        __syncthreads();
-        int at = taken + __popcll(takes & ((1ull << lane) - 1));
+        int rank = 0;  // of the thread's first tie
+        if (ties > 0) {
+            const int upto = dev::wave_scan(tied);
+            if (lane == kWave - 1) {
+                tiesBefore[wave] = upto;
+            }
+            __syncthreads();
+            rank = equal + upto - tied;
 #pragma unroll
-        for (int x = 0; x < kSelectWaves; ++x) {
-            at += x < wave ? before[1][x] : 0;
-            taken += before[1][x];
-        }
-        if (take) {
-            columns[at] = c;
-            table[at] = a.table[(int64_t)b * a.width + c];
-            if (c == r.held - 1) {
-                lastTaken = 1;
+            for (int x = 0; x < kSelectWaves; ++x) {
+                rank += x < wave ? tiesBefore[x] : 0;
+                equal += tiesBefore[x];
             }
         }
-    }
+        uint32_t mine = 0;
+#pragma unroll
+        for (int x = 0; x < kHeld; ++x) {
+            const bool tie = ties > 0 && keys[x] == floor;
+            const bool take = keys[x] > floor || (tie && rank < ties);
+            rank += tie ? 1 : 0;
+            mine |= take ? 1u << x : 0u;
+        }
+        takes = __popc(mine);
+        const int upto = dev::wave_scan(takes);
+        if (lane == kWave - 1) {
+            before[wave] = upto;
+        }
+        __syncthreads();
+        int at = taken + upto - takes;
+#pragma unroll
+        for (int x = 0; x < kSelectWaves; ++x) {
+            at += x < wave ? before[x] : 0;
+            taken += before[x];
+        }
+#pragma unroll
+        for (int x = 0; x < kHeld; ++x) {
+            if ((mine >> x & 1u) != 0u) {
+                const int c = segment * kSegment + (int)threadIdx.x * kHeld + x;
+                columns[at] = c;
+                table[at] = a.table[(int64_t)b * a.width + c];
+                ++at;
+                if (c == r.held - 1) {
+                    lastTaken = 1;
+                }
+            }
+        }
+        __syncthreads();
+    });
     for (int x = taken + (int)threadIdx.x; x < s.top; x += kSelectThreads) {
         columns[x] = table[x] = -1;
     }
-    __syncthreads();
     if (threadIdx.x == 0) {  // (the last column may be filled in part)
         args.lengths[row] = taken * a.pageSize - (lastTaken != 0 ? r.held * a.pageSize - r.length : 0);
     }
+}
+
+// Columns of a workgroup's item: enough items for all CUs, and beyond that long ones, whose
+// start (lengths, query heads) costs as much as some dozens of columns.
+int columns_of(const PagedAttentionArgs &a)
+{
+    const int64_t all = (int64_t)a.B * a.kvHeads * a.width;
+    return all <= (int64_t)32 * 2048 ? 32 : all <= (int64_t)128 * 2048 ? 128 : 512;
 }
 
 // The attention's call: a row for each kv head of a sequence.
@@ -372,9 +437,9 @@ hipError_t launch_sparse_attention(const SparseAttentionArgs &s, void *workspace
     const sparse::Workspace at(s, cus);
     char *base = static_cast<char *>(workspace);
     const sparse::Args args{s, reinterpret_cast<uint64_t *>(base + at.keys), reinterpret_cast<int32_t *>(base + at.table),
-                            reinterpret_cast<int32_t *>(base + at.lengths)};
+                            reinterpret_cast<int32_t *>(base + at.lengths), sparse::columns_of(s.attention)};
     const PagedAttentionArgs &a = s.attention;
-    const int64_t items = (int64_t)a.B * a.kvHeads * ((a.width + sparse::kColumns - 1) / sparse::kColumns);
+    const int64_t items = (int64_t)a.B * a.kvHeads * ((a.width + args.columns - 1) / args.columns);
     const unsigned grid = (unsigned)(items < (1 << 20) ? items : (1 << 20));
     if (a.isBf16) {
         sparse::launch_scores<true>(args, grid, stream);
@@ -385,8 +450,12 @@ hipError_t launch_sparse_attention(const SparseAttentionArgs &s, void *workspace
     if (err != hipSuccess) {
         return err;
     }
-    hipLaunchKernelGGL(sparse::select_pages, dim3((unsigned)(a.B * a.kvHeads)), dim3(sparse::kSelectThreads), 0, stream,
-                       args);
+    const dim3 rowsGrid((unsigned)(a.B * a.kvHeads)), threads(sparse::kSelectThreads);
+    if (a.width <= sparse::kSegment) {
+        hipLaunchKernelGGL((sparse::select_pages<true>), rowsGrid, threads, 0, stream, args);
+    } else {
+        hipLaunchKernelGGL((sparse::select_pages<false>), rowsGrid, threads, 0, stream, args);
+    }
     if ((err = hipGetLastError()) != hipSuccess) {
         return err;
     }
