@@ -1117,7 +1117,7 @@ hipError_t launch_layout(const Args &args, hipStream_t stream)
 }
 
 // The layouts by rows of a (sequence, kv head).
-enum class Kind { kOne, kTwo, kFour };
+enum class Kind { kOne, kTwo, kFour, kEight };
 
 template <int D, Kind kKind>
 struct LayoutOf;
@@ -1127,6 +1127,9 @@ template <int D>
 struct LayoutOf<D, Kind::kTwo> : Layout<D, 2, 2, 32> {};
 template <int D>
 struct LayoutOf<D, Kind::kFour> : Layout<D, 4, 1, 64> {};
+
+template <int D>
+struct LayoutOf<D, Kind::kEight> : Layout<D, (D == 64 || D == 128 ? 8 : 4), 1, 64> {};
 
 // Calls f(layout) for a kind and (padded) head size.
 template <Kind kKind, typename F>
@@ -1153,6 +1156,10 @@ template <>
 hipError_t launch_kind<true, Kind::kTwo>(const Args &args, hipStream_t stream);
 template <>
 hipError_t launch_kind<true, Kind::kFour>(const Args &args, hipStream_t stream);
+template <>
+hipError_t launch_kind<true, Kind::kEight>(const Args &args, hipStream_t stream);
+template <>
+hipError_t launch_kind<false, Kind::kEight>(const Args &args, hipStream_t stream);
 template <>
 hipError_t launch_kind<false, Kind::kOne>(const Args &args, hipStream_t stream);
 template <>

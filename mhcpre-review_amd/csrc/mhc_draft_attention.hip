@@ -6,11 +6,14 @@ namespace mhc {
 namespace draft {
 namespace {
 
-// The layout for rows of a (sequence, kv head).
+// The layout for rows of a (sequence, kv head).  Blocks of 256 rows read the cache half as
+// often as blocks of 128 but have one workgroup a CU; us, 128 / 256 rows a block, d = 128: 512
+// rows, 2 sequences of 65536 322 / 297, 32 of up to 8192 321 / 317; 256 rows, 2 of 65536 178 /
+// 167, 32 of up to 8192 with trees of different sizes 196 / 207.
 Kind kind_of(const DraftAttentionArgs &a)
 {
     const int64_t rows = (int64_t)a.S * (a.heads / a.kvHeads);
-    return rows <= 32 ? Kind::kOne : rows <= 64 ? Kind::kTwo : Kind::kFour;
+    return rows <= 32 ? Kind::kOne : rows <= 64 ? Kind::kTwo : rows <= 256 || a.d > 128 ? Kind::kFour : Kind::kEight;
 }
 
 template <Kind kKind>
@@ -39,6 +42,7 @@ Args plan(const DraftAttentionArgs &a, int cus)
     case Kind::kOne: plan_kind<Kind::kOne>(p, cus); break;
     case Kind::kTwo: plan_kind<Kind::kTwo>(p, cus); break;
     case Kind::kFour: plan_kind<Kind::kFour>(p, cus); break;
+    case Kind::kEight: plan_kind<Kind::kEight>(p, cus); break;
     }
     p.blocks = (int)(((int64_t)a.S * p.group + p.rows - 1) / p.rows);
     return p;
@@ -77,9 +81,12 @@ hipError_t launch_draft_attention(const DraftAttentionArgs &a, void *workspace, 
     case draft::Kind::kTwo:
         return a.isBf16 ? draft::launch_kind<true, draft::Kind::kTwo>(p, stream)
                         : draft::launch_kind<false, draft::Kind::kTwo>(p, stream);
-    default:
+    case draft::Kind::kFour:
         return a.isBf16 ? draft::launch_kind<true, draft::Kind::kFour>(p, stream)
                         : draft::launch_kind<false, draft::Kind::kFour>(p, stream);
+    default:
+        return a.isBf16 ? draft::launch_kind<true, draft::Kind::kEight>(p, stream)
+                        : draft::launch_kind<false, draft::Kind::kEight>(p, stream);
     }
 }
 

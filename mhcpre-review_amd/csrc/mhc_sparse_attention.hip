@@ -20,7 +20,7 @@ using dev::kWave;
 using dev::u32x4_t;
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kBatch = 4;  // pages of a group of lanes on their way at once
+constexpr int kBatch = 4;  // pages that a group of lanes scores at once
 
 // Scores as ordered integers; what cannot be taken is 0.
 constexpr uint64_t kAlways = ~0ull, kNotANumber = ~0ull - 1;
@@ -31,6 +31,7 @@ struct Args {
     int32_t *table;     // [B * kvHeads, top]: the pages taken
     int32_t *lengths;   // [B * kvHeads]: their tokens
     int columns;        // of a workgroup's item
+    int heads;          // kv heads of a workgroup's item: 4, 2 or 1, of its waves each does one's
 };
 
 // Columns that row b of the batch holds, and its tokens.
@@ -63,23 +64,26 @@ __global__ __launch_bounds__(kThreads) void score_pages(Args args)
     const int sub = lane % kLanes, e = 8 * sub;
     const bool on = e < a.d;
     const int group = a.heads / a.kvHeads, chunks = (a.width + args.columns - 1) / args.columns;
-    const int64_t items = (int64_t)a.B * a.kvHeads * chunks;
+    const int headGroups = (a.kvHeads + args.heads - 1) / args.heads, perHead = kWaves / args.heads;
+    const int64_t items = (int64_t)a.B * headGroups * chunks;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t row = item / chunks;
-        const int b = (int)(row / a.kvHeads), kv = (int)(row % a.kvHeads), column0 = (int)(item % chunks) * args.columns;
+        const int chunk = (int)(item % chunks), b = (int)(item / chunks / headGroups);
+        const int kv = (int)(item / chunks % headGroups) * args.heads + wave / perHead, column0 = chunk * args.columns;
+        const int64_t row = (int64_t)b * a.kvHeads + kv;
         const Row r(a, b);
-        if (column0 >= r.held) {
+        if (column0 >= r.held || kv >= a.kvHeads) {
             continue;
         }
         const int end = r.held - column0 < args.columns ? r.held : column0 + args.columns;
         const int32_t *table = a.table + (int64_t)b * a.width;
         // The pages of a step are known a step ahead.
-        int c0 = column0 + wave * kPages + lane / kLanes;
-        int page[kBatch], next[kBatch];
+        const int step = perHead * kPages;
+        int c0 = column0 + wave % perHead * kPages + lane / kLanes;
+        int next[kBatch];
         const auto find = [&](int from) {
 #pragma unroll
             for (int x = 0; x < kBatch; ++x) {
-                const int c = from + x * kWaves * kPages;
+                const int c = from + x * step;
                 next[x] = table[c < end ? c : column0];
             }
         };
@@ -112,45 +116,68 @@ __global__ __launch_bounds__(kThreads) void score_pages(Args args)
         }
         const uint16_t *loBase = static_cast<const uint16_t *>(s.lo.data) + kv * s.lo.head + (on ? e : 0);
         const uint16_t *hiBase = static_cast<const uint16_t *>(s.hi.data) + kv * s.hi.head + (on ? e : 0);
-        for (; c0 - lane / kLanes < end; c0 += kBatch * kWaves * kPages) {
+        struct Bounds {
             u32x4_t lo[kBatch], hi[kBatch];
+            uint32_t good;  // pages there are, a bit each
+        };
+        const auto load = [&](Bounds &p, int from) {
+            p.good = 0;
 #pragma unroll
             for (int x = 0; x < kBatch; ++x) {
-                const bool good = next[x] >= 0 && next[x] < a.pages && c0 + x * kWaves * kPages < end;
-                page[x] = good ? next[x] : -1;
-                const int64_t from = good ? next[x] : 0;  // (no page: the first one is read, and not used)
-                lo[x] = *reinterpret_cast<const u32x4_t *>(loBase + from * s.lo.row);
-                hi[x] = *reinterpret_cast<const u32x4_t *>(hiBase + from * s.hi.row);
-                if (!on) {
-                    lo[x] = hi[x] = u32x4_t{0, 0, 0, 0};
-                }
+                const bool good = next[x] >= 0 && next[x] < a.pages && from + x * step < end;
+                p.good |= good ? 1u << x : 0u;
+                const int64_t page = good ? next[x] : 0;  // (no page: the first one is read, and not used)
+                p.lo[x] = *reinterpret_cast<const u32x4_t *>(loBase + page * s.lo.row);
+                p.hi[x] = *reinterpret_cast<const u32x4_t *>(hiBase + page * s.hi.row);
             }
-            find(c0 + kBatch * kWaves * kPages);
+            find(from + kBatch * step);
+        };
+        const auto score = [&](const Bounds &p, int from) {
+            double sum[kBatch];
 #pragma unroll
             for (int x = 0; x < kBatch; ++x) {
                 float l[8], h[8];
-                dev::unpack8<kBf16>(lo[x], l);
-                dev::unpack8<kBf16>(hi[x], h);
-                double sum = 0;
+                dev::unpack8<kBf16>(p.lo[x], l);
+                dev::unpack8<kBf16>(p.hi[x], h);
+                sum[x] = 0;
 #pragma unroll
                 for (int y = 0; y < 8; ++y) {
-                    sum = __builtin_fma(up[y], (double)h[y], sum);
-                    sum = __builtin_fma(down[y], (double)l[y], sum);
+                    sum[x] = __builtin_fma(up[y], (double)h[y], sum[x]);
+                    sum[x] = __builtin_fma(down[y], (double)l[y], sum[x]);
                 }
-#pragma unroll
-                for (int mask = 1; mask < kLanes; mask *= 2) {
-                    sum += shuffled(sum, mask);
-                }
-                sum += 0.0;  // (-0 is 0)
-                const uint64_t bits = (uint64_t)__double_as_longlong(sum);
-                uint64_t key = bits >> 63 != 0 ? ~bits : bits | 1ull << 63;
-                key = sum != sum ? kNotANumber : key;
-                const int c = c0 + x * kWaves * kPages;
-                key = c < s.first || c >= r.held - s.last ? kAlways : key;
-                if (sub == 0 && c < end) {
-                    args.keys[row * a.width + c] = page[x] >= 0 ? key : 0;
-                }
+                sum[x] = on ? sum[x] : 0;  // (whatever lies behind a head's dimensions)
             }
+            // Over the lanes: in the first two steps a lane gives its neighbour the sums of half of
+            // the pages and goes on with the others', so that one is left, page sub % 4's.
+            const bool odd = (sub & 1) != 0, second = (sub & 2) != 0;
+            double two[2], one;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                two[x] = (odd ? sum[2 * x + 1] : sum[2 * x]) + shuffled(odd ? sum[2 * x] : sum[2 * x + 1], 1);
+            }
+            one = (second ? two[1] : two[0]) + shuffled(second ? two[0] : two[1], 2);
+#pragma unroll
+            for (int mask = 4; mask < kLanes; mask *= 2) {
+                one += shuffled(one, mask);
+            }
+            one += 0.0;  // (-0 is 0)
+            const uint64_t bits = (uint64_t)__double_as_longlong(one);
+            uint64_t key = bits >> 63 != 0 ? ~bits : bits | 1ull << 63;
+            key = one != one ? kNotANumber : key;
+            const int c = from + sub * step;
+            key = c < s.first || c >= r.held - s.last ? kAlways : key;
+            if (sub < kBatch && c < end) {
+                args.keys[row * a.width + c] = (p.good >> sub & 1u) != 0u ? key : 0;
+            }
+        };
+        // The next pages' bounds are on their way while these are scored.
+        Bounds here, ahead;
+        load(here, c0);
+        for (; c0 - lane / kLanes < end; c0 += 2 * kBatch * step) {
+            load(ahead, c0 + kBatch * step);
+            score(here, c0);
+            load(here, c0 + 2 * kBatch * step);
+            score(ahead, c0 + kBatch * step);
         }
     }
 }
@@ -367,12 +394,15 @@ __global__ __launch_bounds__(kSelectThreads) void select_pages(Args args)
     }
 }
 
-// Columns of a workgroup's item: enough items for all CUs, and beyond that long ones, whose
-// start (lengths, query heads) costs as much as some dozens of columns.
+// kv heads of a workgroup's item: those of a page lie together in memory.
+int heads_of(const PagedAttentionArgs &a) { return a.kvHeads >= 4 ? 4 : a.kvHeads >= 2 ? 2 : 1; }
+
+// Columns of an item: enough items for all CUs, and beyond that long ones, whose start
+// (lengths, query heads) costs as much as some dozens of columns.
 int columns_of(const PagedAttentionArgs &a)
 {
-    const int64_t all = (int64_t)a.B * a.kvHeads * a.width;
-    return all <= (int64_t)32 * 2048 ? 32 : all <= (int64_t)128 * 2048 ? 128 : 512;
+    const int64_t all = (int64_t)a.B * a.kvHeads / heads_of(a) * a.width;
+    return all <= (int64_t)16 * 2048 ? 16 : 64;
 }
 
 // The attention's call: a row for each kv head of a sequence.
@@ -437,9 +467,11 @@ hipError_t launch_sparse_attention(const SparseAttentionArgs &s, void *workspace
     const sparse::Workspace at(s, cus);
     char *base = static_cast<char *>(workspace);
     const sparse::Args args{s, reinterpret_cast<uint64_t *>(base + at.keys), reinterpret_cast<int32_t *>(base + at.table),
-                            reinterpret_cast<int32_t *>(base + at.lengths), sparse::columns_of(s.attention)};
+                            reinterpret_cast<int32_t *>(base + at.lengths), sparse::columns_of(s.attention),
+                            sparse::heads_of(s.attention)};
     const PagedAttentionArgs &a = s.attention;
-    const int64_t items = (int64_t)a.B * a.kvHeads * ((a.width + args.columns - 1) / args.columns);
+    const int64_t items = (int64_t)a.B * ((a.kvHeads + args.heads - 1) / args.heads) *
+                          ((a.width + args.columns - 1) / args.columns);
     const unsigned grid = (unsigned)(items < (1 << 20) ? items : (1 << 20));
     if (a.isBf16) {
         sparse::launch_scores<true>(args, grid, stream);
