@@ -131,6 +131,18 @@ struct Args {
     Open *open;          // [most]
 };
 
+// The kernel's arguments, and the lane's number, for what is done once a block: read and
+// derived there.  (Derived from what is known at the kernel's start, all of it would be
+// computed in front of the loop and held over it, and registers be spilled in it, whose
+// reloads wait for the tile on its way.)
+__device__ __forceinline__ const Args &late() { return *(const Args *)dev::late_args<Args>(); }
+__device__ __forceinline__ int late_lane()
+{
+    int lane = (int)threadIdx.x % kWave;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 // The keys of a block of a sequence with c + n tokens, n of them new: [low, high), in
 // `tiles` (units of the launch, one at least) from `first` on.
 struct Keys {
@@ -235,12 +247,14 @@ struct Place {
         n = s.n;
         keys = s.keys(args, block);
     }
-    __device__ bool inside(const Args &args, int end) const { return b < args.a.B && start + tile < end; }
-    __device__ void advance(const Args &args)
+    __device__ bool inside(int end) const { return start + tile < end; }
+    // (Behind the last sequence: at the line's end, which is inside of no stretch.)
+    __device__ void advance()
     {
         if (++tile < keys.tiles) {
             return;
         }
+        const Args &args = late();
         tile = 0;
         start += keys.tiles + kItemUnits;
         if (++block == args.blocks) {
@@ -252,6 +266,9 @@ struct Place {
         }
         if (b < args.a.B) {
             enter(args);
+        } else {
+            start = INT32_MAX;
+            keys.tiles = INT32_MAX;
         }
     }
 };
@@ -423,16 +440,13 @@ __device__ __forceinline__ uint64_t seen_keys(bool tree, int c, int node, uint32
     return seen;
 }
 
-// What one of two packed 16-bit values leaves of x.
+// What the first of a weight's two terms leaves: x without its upper 8 (bf16) or 11 (fp16)
+// bits.  (An fp16 below 2^-14 holds fewer: then up to 2^-24 is lost, 2^-34 of the largest
+// weight.)
 template <bool kBf16>
-__device__ __forceinline__ float rest(float x, uint32_t two, int which)
+__device__ __forceinline__ float rest(float x)
 {
-    if constexpr (kBf16) {  // (cut: the upper half of x itself)
-        return x - __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-    } else {
-        const _Float16 h = __builtin_bit_cast(_Float16, (uint16_t)(which == 0 ? two : two >> 16));
-        return __builtin_fmaf(-(float)h, 1.f, x);
-    }
+    return x - __uint_as_float(__float_as_uint(x) & (kBf16 ? 0xFFFF0000u : 0xFFFFE000u));
 }
 
 // 4 values at the same column of 4 rows of LDS (the lane's column of 16).
@@ -480,7 +494,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     }
     const int begin = shares.start(w), end = shares.start(w + 1);
     Place here = line.find(args, begin);
-    if (!here.inside(args, end)) {
+    if (!here.inside(end)) {
         return;
     }
 
@@ -493,7 +507,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     const uint32_t pageSize = (uint32_t)a.pageSize, stepColumns = L::kUnit / pageSize, stepSlots = L::kUnit % pageSize;
     const auto find_page = [&]() {
         key = false;
-        if (ahead.inside(args, end)) {
+        if (ahead.inside(end)) {
             if (enters) {
                 t = (uint32_t)(ahead.keys.first + ahead.tile) * L::kUnit + keyWave * kTile + lane % kTile;
                 column = t / pageSize;
@@ -508,7 +522,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                 slot -= over_ ? pageSize : 0u;
             }
             key = t >= (uint32_t)ahead.keys.low && t < (uint32_t)ahead.keys.high;
-            ahead.advance(args);
+            ahead.advance();
             enters = ahead.tile == 0;
         }
         // (Always a load, of the row's first entry where there is no key: under a branch it would
@@ -567,19 +581,21 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     // load brings must not be touched before the wait at the loop's head.)
     u32x4_t q[kSteps];
     const auto load_q = [&](const Place &p) {
-        const int row = p.block * L::kBlock + rowWave * kRows + col;
-        const int node = row / args.group, head = row % args.group;
-        const uint16_t *from = static_cast<const uint16_t *>(a.q.data) + p.b * a.q.row + node * a.q.token +
-                               (int64_t)(p.kv * args.group + head) * a.q.head + 8 * half;
-        const bool on = node < p.n && a.scale != 0.f;
+        const Args &l = late();
+        const int ln = late_lane();
+        const int row = p.block * L::kBlock + rowWave * kRows + ln % 32;
+        const int node = row / l.group, head = row - node * l.group;
+        const uint16_t *from = static_cast<const uint16_t *>(l.a.q.data) + p.b * l.a.q.row + node * l.a.q.token +
+                               (int64_t)(p.kv * l.group + head) * l.a.q.head + ln / 32 * 8;
+        const bool on = node < p.n && l.a.scale != 0.f;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            q[s] = *reinterpret_cast<const u32x4_t *>(on && 16 * s < a.d ? from + 16 * s
-                                                                         : reinterpret_cast<const uint16_t *>(kZeros));
+            q[s] = *reinterpret_cast<const u32x4_t *>(on && 16 * s < l.a.d ? from + 16 * s
+                                                                           : reinterpret_cast<const uint16_t *>(kZeros));
         }
     };
     const auto turn_q = [&]() {
-        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+        const uint32_t flip = late().a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             q[s] ^= u32x4_t{flip, flip, flip, flip};
@@ -605,21 +621,22 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     int node = 0, over = 0, maskedRow = -1;
     bool there = false;
     uint32_t from = 0;
-    int64_t wholeFrom = 0, wholeTo = 0;
+    int wholeFrom = 0, wholeTo = 0;  // (a chain's last block may say one more than there are)
     const auto enter = [&]() {
+        const Args &l = late();
         const int row0 = here.block * L::kBlock + rowWave * kRows;
-        node = (row0 + col) / args.group;
+        node = (row0 + late_lane() % 32) / l.group;
         there = node < here.n;
         int depth = node;
         const int lastTile = end - 1 - here.start < here.keys.tiles - 1 ? end - 1 - here.start : here.keys.tiles - 1;
         if (tree && here.n > 0 &&
-            (a.window > 0 || (int64_t)(here.keys.first + lastTile + 1) * L::kUnit > here.c)) {
+            (l.a.window > 0 || (int64_t)(here.keys.first + lastTile + 1) * L::kUnit > here.c)) {
             if (maskedRow != here.b) {
                 __syncthreads();  // (the ones before are read)
-                find_ancestors<L::kThreads>(a, here.b, here.n, known, farthest);
+                find_ancestors<L::kThreads>(l.a, here.b, here.n, known, farthest);
                 maskedRow = here.b;
             }
-            if (a.window > 0) {
+            if (l.a.window > 0) {
                 depth = -1;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -627,12 +644,13 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                 }
             }
         }
-        over = a.window > 0 && a.window < depth + 1 ? depth + 1 - (int)a.window : 0;
+        over = l.a.window > 0 && l.a.window < depth + 1 ? depth + 1 - (int)l.a.window : 0;
         // (The context that the row sees: [from, c); a chain's row: [from, c + node].)
-        const int64_t from64 = (int64_t)here.c + depth + 1 - a.window;
-        from = a.window > 0 && from64 > 0 ? (uint32_t)from64 : 0u;
-        wholeTo = tree ? here.c : (int64_t)here.c + row0 / args.group + 1;
-        wholeFrom = a.window > 0 ? (int64_t)here.c + here.n - a.window : 0;
+        const int64_t from64 = (int64_t)here.c + depth + 1 - l.a.window;
+        from = l.a.window > 0 && from64 > 0 ? (uint32_t)from64 : 0u;
+        wholeTo = tree ? here.c : here.c + row0 / l.group + 1;
+        const int64_t all = (int64_t)here.c + here.n - l.a.window;
+        wholeFrom = l.a.window > 0 && all > 0 ? (int)all : 0;
     };
 
     // A tile: its keys from t0 on, of which `valid` are in the cache.  kChecked: with infinite and
@@ -710,14 +728,16 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         // values of V are read ahead.
         constexpr int kGroups = kTile / 16, kProducts = kGroups * kDims, kAhead = kProducts < 4 ? kProducts : 4;
         u32x4_t p[kGroups][2], v[kAhead];
-        const auto weigh = [&](int t, int x) {  // (keys 2 x and 2 x + 1 of the lane's 8)
-            const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x], factor, shift));
-            const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x + 1], factor, shift));
+        float x0 = 0.f, x1 = 0.f;
+        const auto raise = [&](int t, int x) {  // (keys 2 x and 2 x + 1 of the lane's 8)
+            x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x], factor, shift));
+            x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][t % 2 * 8 + 2 * x + 1], factor, shift));
+        };
+        const auto split = [&](int t, int x) {
             sum += x0;
             sum += x1;
-            const uint32_t first = attention::cut2<kBf16>(x0, x1);
-            p[t][0][x] = first;
-            p[t][1][x] = dev::pack2_x<kBf16>(rest<kBf16>(x0, first, 0), rest<kBf16>(x1, first, 1));
+            p[t][0][x] = attention::cut2<kBf16>(x0, x1);
+            p[t][1][x] = dev::pack2_x<kBf16>(rest<kBf16>(x0), rest<kBf16>(x1));
         };
         const auto read = [&](int x) {  // (rows r and r + 8 of the tile, the lane's 4 columns of 32)
             const uint32_t rows = x / kDims * 16 * L::kChunks * 16;
@@ -731,22 +751,30 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            weigh(0, x);
+            raise(0, x);
+            split(0, x);
         }
         in_order();
 #pragma unroll
         for (int x = 0; x < kProducts; ++x) {
             const int t = x / kDims, j = x % kDims;
+            // (This product's share of the next 16 keys' four pairs.)
+            const int y0 = t + 1 < kGroups ? j * 4 / kDims : 0, y1 = t + 1 < kGroups ? (j + 1) * 4 / kDims : 0;
             o[j] = mfma<kBf16>(v[x % kAhead], p[t][0], o[j]);
+            if (y0 < y1) {
+                raise(t + 1, y0);
+            }
+            in_order();
             o[j] = mfma<kBf16>(v[x % kAhead], p[t][1], o[j]);
             if (x + kAhead < kProducts) {
                 v[x % kAhead] = read(x + kAhead);
             }
-            if (t + 1 < kGroups) {
 #pragma unroll
-                for (int y = j * 4 / kDims; y < (j + 1) * 4 / kDims; ++y) {
-                    weigh(t + 1, y);
+            for (int y = y0; y < y1; ++y) {
+                if (y > y0) {
+                    raise(t + 1, y);
                 }
+                split(t + 1, y);
             }
             in_order();
         }
@@ -772,16 +800,17 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                 const bool on = (seen >> at & 1u) != 0u;
                 // (a weight that is 0 in 32 bits is above 0 all the same)
                 weight = weight == 0.f ? 1e-30f : weight;
-                const uint32_t t = (uint32_t)t0 + at, column = t / (uint32_t)a.pageSize;
-                const uint16_t *value = static_cast<const uint16_t *>(a.vCache.data) + here.kv * a.vCache.head +
-                                        a.table[(int64_t)here.b * a.width + column] * a.vCache.page +
-                                        (t - column * (uint32_t)a.pageSize) * a.vCache.slot;
+                const DraftAttentionArgs &l = late().a;
+                const uint32_t t = (uint32_t)t0 + at, column = t / (uint32_t)l.pageSize;
+                const uint16_t *value = static_cast<const uint16_t *>(l.vCache.data) + here.kv * l.vCache.head +
+                                        l.table[(int64_t)here.b * l.width + column] * l.vCache.page +
+                                        (t - column * (uint32_t)l.pageSize) * l.vCache.slot;
 #pragma unroll
                 for (int j = 0; j < kDims; ++j) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int e = 32 * j + 8 * (i / 4) + 4 * half + i % 4;
-                        if (32 * j + i / 8 * 16 < a.d) {  // (e < d, for d % 16 is 0)
+                        const int e = 32 * j + 8 * (i / 4) + 4 * (late_lane() / 32) + i % 4;
+                        if (32 * j + i / 8 * 16 < l.d) {  // (e < d, for d % 16 is 0)
                             const uint32_t bits = value[e];
                             if (on && infinite<kBf16>(bits)) {
                                 o[j][i] += weight * dev::x_to_f32<kBf16>(bits);
@@ -887,8 +916,8 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
             odd[wave] = !finite;
         }
         Place next = here;
-        next.advance(args);
-        const bool more = next.inside(args, end);
+        next.advance();
+        const bool more = next.inside(end);
         if (more) {
             load_q(next);
         }
@@ -927,19 +956,21 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         const bool all = firstTile == 0 && here.tile + 1 == here.keys.tiles;
         const int slot = 2 * w + (firstBlock ? 0 : 1);
         if (threadIdx.x == 0 && firstTile == 0 && !all) {
-            args.open[w] = Open{here.b, here.kv, here.block, here.start, here.start + here.keys.tiles - 1, line.all, slot, 0};
+            late().open[w] = Open{here.b, here.kv, here.block, here.start, here.start + here.keys.tiles - 1, shares.units, slot, 0};
         }
         // 4 values of the lane's row, from e on.
-        const int r = rowWave * kRows + col;
-        const int head = here.block * L::kBlock + r - node * args.group;
+        const Args &l = late();
+        const int ln = late_lane(), r = rowWave * kRows + ln % 32, upper = ln / 32;
+        const int head = here.block * L::kBlock + r - node * l.group;
+        float *const parts = l.outs + ((int64_t)slot * L::kBlock + r) * D;
         const auto put = [&](int e, f32x4_t value, float t, float total) {
-            if (node >= a.S) {
+            if (node >= l.a.S) {
             } else if (all) {
-                finish<kBf16>(args, here, node, head, e, value, t, total);
+                finish<kBf16>(l, here, node, head, e, value, t, total);
             } else {
-                *reinterpret_cast<f32x4_t *>(args.outs + ((int64_t)slot * L::kBlock + r) * D + e) = value;
+                *reinterpret_cast<f32x4_t *>(parts + e) = value;
                 if (e == 0) {
-                    *reinterpret_cast<float2 *>(args.ends + ((int64_t)slot * L::kBlock + r) * 2) = float2{t, total};
+                    *reinterpret_cast<float2 *>(l.ends + ((int64_t)slot * L::kBlock + r) * 2) = float2{t, total};
                 }
             }
         };
@@ -948,7 +979,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
             for (int j = 0; j < kDims; ++j) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    put(32 * j + 2 * i + 4 * half, f32x4_t{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]}, top, sum);
+                    put(32 * j + 2 * i + 4 * upper, f32x4_t{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]}, top, sum);
                 }
             }
         } else {
@@ -958,10 +989,10 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
             const auto left = [&](int k, int x) {
                 return (__attribute__((address_space(3))) f32x4_t *)(uintptr_t)(
                     (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (2 * k + buffer) * L::kBuffer +
-                    ((L::kRowWaves == 1 ? x : rowWave * kShare + x % kShare) * kWave + lane) * 16);
+                    ((L::kRowWaves == 1 ? x : rowWave * kShare + x % kShare) * kWave + ln) * 16);
             };
             __syncthreads();  // (the tiles are read)
-            if (half == 0) {
+            if (upper == 0) {
                 ends[keyWave][r] = float2{top, sum};
             }
 #pragma unroll
@@ -1006,7 +1037,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                                     value[y] += decltype(kInfinite)::value ? scaled(v[y], f[k]) : v[y] * f[k];
                                 }
                             }
-                            put(x / 4 * 32 + x % 4 * 8 + 4 * half, value, most, total);
+                            put(x / 4 * 32 + x % 4 * 8 + 4 * upper, value, most, total);
                         }
                     }
                 }
