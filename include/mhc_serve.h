@@ -190,7 +190,7 @@ MHC_API int mhcPagedAttention(void *workspace, uint64_t workspaceSize, mhcServeE
  *
  * with query head h reading kv head h / (heads / kvHeads), in fp32, out rounded
  * once.  (The weights are held in 16 bits in bf16 and in 22 in fp16, there small
- * ones to 2^-39 of the largest.)  Nodes i >= n, and nodes that see no key, have out
+ * ones to 2^-34 of the largest.)  Nodes i >= n, and nodes that see no key, have out
  * 0 and lse -inf.  What a node does not see may be infinite or NaN; an infinite
  * value that it sees is infinite in its output.
  *
@@ -295,8 +295,8 @@ MHC_API int mhcCacheBounds(void *workspace, uint64_t workspaceSize, mhcServeExec
 /*
  * Attention of one new token per sequence over `top` pages for each of its kv heads.
  * Row b holds its table's first ceil(L / pageSize) columns (L: lengths[b] clamped to
- * the table); holes are left out.  kv head g takes the first `first` and the last
- * `last` of these columns that are no holes of their own, and of the others those with
+ * the table); holes are left out.  Of these columns kv head g takes those among the
+ * first `first` and the last `last` that are no holes, and of the others those with
  * the highest scores, until it has `top` (or all); of equal scores the lower column.
  * With the query heads h that share g
  *
@@ -304,7 +304,8 @@ MHC_API int mhcCacheBounds(void *workspace, uint64_t workspaceSize, mhcServeExec
  *         = sum_i (sum_h max(q_hi, 0)) hi_i + (sum_h min(q_hi, 0)) lo_i,
  *
  * the largest value that the sum of the heads' products with a key between the bounds
- * lo and hi can have, in 64 bits; a score that is NaN is above all others.  Over the
+ * lo and hi can have, in 64 bits as the second line has it (with bounds that are
+ * infinite a sum of 0 makes NaN); a score that is NaN is above all others.  Over the
  * tokens of these pages
  *
  *   s_t = scale * q . k_t,  out = sum_t exp(s_t - lse) v_t,  lse = log sum_t exp(s_t)

@@ -6,10 +6,13 @@ namespace mhc {
 namespace draft {
 namespace {
 
-// The layout for rows of a (sequence, kv head).  Blocks of 256 rows read the cache half as
-// often as blocks of 128 but have one workgroup a CU; us, 128 / 256 rows a block, d = 128: 512
-// rows, 2 sequences of 65536 322 / 297, 32 of up to 8192 321 / 317; 256 rows, 2 of 65536 178 /
-// 167, 32 of up to 8192 with trees of different sizes 196 / 207.
+// The layout for rows of a (sequence, kv head): blocks that hold them, for smaller ones read the
+// cache again and larger ones multiply rows that are not there.  us, 32 / 64 / 128 rows a block,
+// 8 kv heads of 128: 32 rows, 32 sequences of 8192 212 / 219 / 274, 2 of 65536 82 / 86 / 92; 64
+// rows, the same 355 / 222 / 259 and 124 / 90 / 95; 128 rows, 32 of 8192 608 / 349 / 287.  Blocks
+// of 256 rows have one workgroup a CU; 128 / 256: 512 rows, 2 of 65536 322 / 297, 32 of up to 8192
+// 321 / 317; 256 rows, 2 of 65536 178 / 167, 32 of up to 8192 with trees of different sizes 196 /
+// 207.
 Kind kind_of(const DraftAttentionArgs &a)
 {
     const int64_t rows = (int64_t)a.S * (a.heads / a.kvHeads);
