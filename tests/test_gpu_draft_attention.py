@@ -307,3 +307,44 @@ def test_offsets_beyond_31_bits(ops, device):
     want = ops.draft_attention(*[a[k] for k in ("q", "k_cache", "v_cache", "page_table", "lengths", "drafted", "parents")])
     got = ops.draft_attention(a["q"], a["k_cache_big"], a["v_cache_big"], moved, a["lengths"], a["drafted"], a["parents"])
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d,S,heads,kv_heads", [(64, 130, 8, 2), (128, 90, 4, 1), (80, 150, 2, 1), (256, 70, 4, 1),
+                                                (128, 5, 7, 1), (96, 40, 14, 2), (64, 6, 96, 2)])
+@pytest.mark.parametrize("window", [0, 45])
+def test_many_rows_and_odd_groups(ops, device, dtype, d, S, heads, kv_heads, window):
+    """More than 256 rows of a kv head, with masks of trees and windows; 7 and 48 heads of one."""
+    check(ops, make(device, 3, S, heads, kv_heads, d, 16, 260, dtype, seed=d), window=window)
+
+
+@pytest.mark.parametrize("S", [4, 12, 40, 100])
+@pytest.mark.parametrize("page", [4, 32])
+def test_caches_of_different_layouts(ops, device, S, page):
+    """Keys by slots, values by heads, or spread out: the same bits as from caches that are laid out alike."""
+    a = make(device, 3, S, 8, 2, 128, page, 300, BF16)
+    want = check(ops, a)
+    by_slot = torch.empty(a["k_cache"].shape, dtype=BF16, device=device)
+    by_slot.copy_(a["k_cache"])
+    room = torch.empty(*a["v_cache"].shape[:3], 136, dtype=BF16, device=device)
+    room.fill_(math.nan)
+    room[..., :128] = a["v_cache"]
+    for k, v in ((by_slot, a["v_cache"]), (a["k_cache"], room[..., :128]), (by_slot, room[..., :128])):
+        got = ops.draft_attention(a["q"], k, v, a["page_table"], a["lengths"], a["drafted"], a["parents"])
+        assert torch.equal(got[0].cpu().double(), want[0]) and torch.equal(got[1].cpu().double(), want[1])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("S,heads", [(6, 4), (20, 4), (40, 4), (100, 8)])
+def test_a_query_that_is_no_number(ops, device, dtype, S, heads):
+    """It reaches its own outputs only, and what lies behind a row's nodes reaches none."""
+    a = make(device, 2, S, heads, 2, 64, 16, 300, dtype, drafted=[S, S - 2])
+    want, want_lse = check(ops, a)
+    a["q"][0, S // 2, 1, 3] = math.nan
+    a["q"][0, 1, 0] = math.inf
+    a["q"][1, S - 2:] = math.nan
+    out, lse = (t.cpu().double() for t in ops.draft_attention(*a.values()))
+    own = torch.zeros_like(lse, dtype=torch.bool)
+    own[0, S // 2, 1] = own[0, 1, 0] = True
+    assert torch.isnan(out[own]).all() and torch.isnan(lse[own]).all()
+    assert torch.equal(out[~own], want[~own]) and torch.equal(lse[~own], want_lse[~own])
