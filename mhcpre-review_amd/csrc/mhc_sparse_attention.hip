@@ -13,7 +13,7 @@
 // 16 sequences of 131072 tokens at most, 64 heads to 8 of 128, 256 pages of 16 for each: scores
 // 60 us (196 MB at 3.3 TB/s, bound by the 64-bit arithmetic and the loads together: alone these
 // take 40 and 47), selection 13.5 (one workgroup a kv head: its rounds follow each other),
-// attention 56 (244 MB at 4.4 TB/s).  One sequence, 64 pages of 64: 7.8, 11.6 and 12.2 us, all
+// attention 56 (244 MB at 4.4 TB/s).  One sequence, 64 pages of 64: 7.8, 9.0 and 12.2 us, all
 // of them chains of loads.
 
 #include "mhc_paged_attention.h"
@@ -190,9 +190,10 @@ __global__ __launch_bounds__(kThreads) void score_pages(Args args)
 
 // The highest `top` keys of a (sequence, kv head), in order.  A thread has kHeld columns
 // that follow each other (in registers; where the table is wider, segment by segment, read
-// anew in each round).
+// anew in each round).  Up to 2048 columns a thread has 2, which come sooner than 8: 64 of 2048
+// 9.0 us, with 8 11.6.
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / kWave, kBins = 256;
-constexpr int kHeld = 8, kSegment = kSelectThreads * kHeld;
+constexpr int kMostHeld = 8;
 
 template <typename F>
 __device__ __forceinline__ uint64_t reduced(uint64_t v, F &&f)
@@ -205,9 +206,10 @@ __device__ __forceinline__ uint64_t reduced(uint64_t v, F &&f)
     return v;
 }
 
-template <bool kOneSegment>
+template <int kHeld, bool kOneSegment>
 __global__ __launch_bounds__(kSelectThreads) void select_pages(Args args)
 {
+    constexpr int kSegment = kSelectThreads * kHeld;
     __shared__ uint64_t least[kSelectWaves], greatest[kSelectWaves], counts[kSelectWaves];
     __shared__ int bins[kBins];
     __shared__ uint64_t rangeLow;
@@ -492,10 +494,12 @@ hipError_t launch_sparse_attention(const SparseAttentionArgs &s, void *workspace
         return err;
     }
     const dim3 rowsGrid((unsigned)(a.B * a.kvHeads)), threads(sparse::kSelectThreads);
-    if (a.width <= sparse::kSegment) {
-        hipLaunchKernelGGL((sparse::select_pages<true>), rowsGrid, threads, 0, stream, args);
+    if (a.width <= 2 * sparse::kSelectThreads) {
+        hipLaunchKernelGGL((sparse::select_pages<2, true>), rowsGrid, threads, 0, stream, args);
+    } else if (a.width <= sparse::kMostHeld * sparse::kSelectThreads) {
+        hipLaunchKernelGGL((sparse::select_pages<sparse::kMostHeld, true>), rowsGrid, threads, 0, stream, args);
     } else {
-        hipLaunchKernelGGL((sparse::select_pages<false>), rowsGrid, threads, 0, stream, args);
+        hipLaunchKernelGGL((sparse::select_pages<sparse::kMostHeld, false>), rowsGrid, threads, 0, stream, args);
     }
     if ((err = hipGetLastError()) != hipSuccess) {
         return err;

@@ -245,3 +245,47 @@ def test_other_streams(ops, device):
             got += [ops.sparse_attention(*a.values(), 9) for _ in range(4)]
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for run in got for x, y in zip(run, want))
+
+
+@pytest.mark.parametrize("longest,top", [(2049, 40), (8192, 7), (8193, 500), (20000, 9000)])
+def test_tables_of_several_segments(ops, device, longest, top):
+    """Columns in registers, and read anew in each round; holes among them."""
+    a = make(device, 2, 4, 1, 32, 1, longest, F16, lengths=[longest, longest - 1000])
+    a["table"][0, 5::97] = -1
+    check(ops, a, top, 2, 3)
+
+
+def test_ties_over_segments(ops, device):
+    a = make(device, 1, 2, 1, 32, 1, 20000, F16, lengths=[20000])
+    a["lo"].fill_(0.5)
+    a["hi"].fill_(0.5)
+    better = int(a["table"][0, 15000])
+    a["lo"][better], a["hi"][better] = -8.0, 8.0
+    columns = check(ops, a, 9000, 0, 1)[2]
+    assert columns[0, 0].tolist() == list(range(8998)) + [15000, 19999]
+
+
+def test_offsets_beyond_31_bits(ops, device):
+    """Bounds and caches of more than 2^31 elements, of which the pages in use lie at both ends: kept, bounded, selected."""
+    page, kv_heads, d = 1, 16, 64
+    pages = 2 ** 31 // (kv_heads * d) + 50
+    a = make(device, 1, 16, kv_heads, d, page, 61, BF16)
+    small = a["k_cache"].shape[0]
+    to = torch.cat((torch.arange(small // 2), torch.arange(pages - (small - small // 2), pages))).to(device)
+    big = {}
+    for key in ("k_cache", "v_cache", "lo", "hi"):
+        big[key] = torch.zeros(pages, *a[key].shape[1:], dtype=BF16, device=device)
+        big[key][to] = a[key]
+    table = torch.where(a["table"] >= 0, to[a["table"].long().clamp(min=0)], -1).int()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=device)  # noqa: E731
+    path = i32([[0, 3, 5, 8, -1, -1, -1, -1, -1, -1]])
+    lengths, drafted, accepted, after = a["lengths"], i32([10]), i32([4]), a["lengths"] - 6
+    results = []
+    for at, tab in ((a, a["table"]), (big, table)):
+        ops.cache_keep(at["k_cache"], at["v_cache"], tab, lengths, drafted, path)
+        ops.cache_bounds(at["k_cache"], tab, after, accepted, at["lo"], at["hi"], 10)
+        results.append(ops.sparse_attention(a["q"], at["k_cache"], at["v_cache"], at["lo"], at["hi"], tab, after, 20))
+    for key in big:
+        there = a["table"][0, :int(after)].long()
+        assert torch.equal(big[key][table[0, :int(after)].long()], a[key][there])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
