@@ -31,7 +31,7 @@
 // with trees of 64 of 8 heads each 297 us, 493 TFLOP/s of the formulas' operations, 740 with
 // the second term's.  There a tile's exponentials, splits and LDS reads stand between its
 // products: they are written among each other, and half of the time is the products' own.  A
-// single small sequence costs two launches, one chain of loads and the join: 18 us.
+// single small sequence costs two launches, one chain of loads and the join: 17 us.
 #pragma once
 
 #include "mhc_paged_attention.h"
@@ -136,7 +136,7 @@ struct Args {
     int unit;    // keys of a unit
     int most;    // workgroups of the launch
     bool grouped;  // pages of whole groups of rows (Layout::kGroupRows), the caches' strides alike
-    float *outs, *ends;  // the parts: [2 * most][rows][D], [2 * most][rows][2]
+    float *outs, *ends;  // the parts: [2 * most][rows / 32][D / 8][64][4], [2 * most][rows][2]
     Open *open;          // [most]
 };
 
@@ -967,17 +967,19 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         if (threadIdx.x == 0 && firstTile == 0 && !all) {
             late().open[w] = Open{here.b, here.kv, here.block, here.start, here.start + here.keys.tiles - 1, shares.units, slot, 0};
         }
-        // 4 values of the lane's row, from e on.
+        // The lane's four x of values: of a row's dimension 32 (x / 4) + 8 (x % 4) + 4 upper on.
+        // A part lies in the workspace as in the registers, so that a wave writes 1 KB at a time.
         const Args &l = late();
         const int ln = late_lane(), r = rowWave * kRows + ln % 32, upper = ln / 32;
         const int head = here.block * L::kBlock + r - node * l.group;
-        float *const parts = l.outs + ((int64_t)slot * L::kBlock + r) * D;
-        const auto put = [&](int e, f32x4_t value, float t, float total) {
+        float *const parts = l.outs + (int64_t)slot * L::kBlock * D + rowWave * kRows * D + ln * 4;
+        const auto put = [&](int x, f32x4_t value, float t, float total) {
+            const int e = x / 4 * 32 + x % 4 * 8 + 4 * upper;
             if (node >= l.a.S) {
             } else if (all) {
                 finish<kBf16>(l, here, node, head, e, value, t, total);
             } else {
-                *reinterpret_cast<f32x4_t *>(parts + e) = value;
+                *reinterpret_cast<f32x4_t *>(parts + x * kWave * 4) = value;
                 if (e == 0) {
                     *reinterpret_cast<float2 *>(l.ends + ((int64_t)slot * L::kBlock + r) * 2) = float2{t, total};
                 }
@@ -988,7 +990,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
             for (int j = 0; j < kDims; ++j) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
-                    put(32 * j + 2 * i + 4 * upper, f32x4_t{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]}, top, sum);
+                    put(4 * j + i / 4, f32x4_t{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]}, top, sum);
                 }
             }
         } else {
@@ -1046,7 +1048,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                                     value[y] += decltype(kInfinite)::value ? scaled(v[y], f[k]) : v[y] * f[k];
                                 }
                             }
-                            put(x / 4 * 32 + x % 4 * 8 + 4 * upper, value, most, total);
+                            put(x, value, most, total);
                         }
                     }
                 }
@@ -1073,9 +1075,9 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
 }
 
 // Joins the parts of the (sequence, kv head, block)s that no stretch finished: a workgroup
-// for some rows of the one that stretch blockIdx.x began.  Bound by its chain of loads (what
-// there is to join, then up to 16 parts at once): 5 us for one small sequence, 13 to 22 with
-// 70 MB of parts.
+// for some rows of the one that stretch `first` began.  Bound by its chain of loads (what
+// there is to join, then up to 16 parts at once) for one small sequence, 4.0 us, and by memory
+// for many, 11.8 to 13.2 with 40 to 50 MB of parts.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBatch = 16;
 
@@ -1083,21 +1085,25 @@ template <bool kBf16, int D>
 __global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
 {
     const DraftAttentionArgs &a = args.a;
-    const Open open = args.open[blockIdx.x];
+    // (Turned by blockIdx.y: the stretches that begin parts may lie 8 apart, and so all on one XCD.
+    // 32 blocks of 8 parts each: 21.8 us not turned, 12.4 so.)
+    const int first = (int)((blockIdx.x + blockIdx.y) % gridDim.x);
+    const Open open = args.open[first];
     if (open.last < 0) {
         return;
     }
-    const int r = (int)blockIdx.y * (kJoinThreads / (D / 4)) + (int)threadIdx.x / (D / 4);
-    const int e = (int)threadIdx.x % (D / 4) * 4;
+    // (32 rows, four x of each, of each lane of a wave.)
+    const int at = (int)blockIdx.y * kJoinThreads + (int)threadIdx.x, lane = at % kWave, x = at / kWave % (D / 8);
+    const int r = at / (kRows * D / 4) * kRows + lane % 32, e = x / 4 * 32 + x % 4 * 8 + lane / 32 * 4;
     const attention::Shares shares(open.all, args.most);
     Place p{};
     p.b = open.b;
     p.kv = open.kv;
     p.block = open.block;
-    const int first = (int)blockIdx.x, last = shares.owner(open.last);
+    const int last = shares.owner(open.last);
     const int64_t row = (int64_t)p.block * args.rows + r;
     const int node = (int)(row / args.group), head = (int)(row % args.group);
-    if (r >= args.rows || node >= a.S || (int)threadIdx.x >= kJoinThreads / (D / 4) * (D / 4)) {
+    if (node >= a.S) {
         return;
     }
     float top = -INFINITY, total = 0.f;
@@ -1112,7 +1118,7 @@ __global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
             if (x0 + m <= last) {
                 const int64_t slot = x0 + m == first ? open.slot : 2 * (x0 + m);
                 ends[m] = *reinterpret_cast<const float2 *>(args.ends + (slot * args.rows + r) * 2);
-                outs[m] = *reinterpret_cast<const f32x4_t *>(args.outs + (slot * args.rows + r) * D + e);
+                outs[m] = *reinterpret_cast<const f32x4_t *>(args.outs + slot * args.rows * D + at * 4);
             }
         }
         float next = top;
@@ -1151,10 +1157,11 @@ hipError_t launch_layout(const Args &args, hipStream_t stream)
     if (err != hipSuccess) {
         return err;
     }
-    constexpr int kPer = kJoinThreads / (L::D / 4);
+    static_assert(kRows * (L::D / 4) % kJoinThreads == 0);
     const int64_t rows = (int64_t)args.a.S * args.group < args.rows ? (int64_t)args.a.S * args.group : args.rows;
     hipLaunchKernelGGL((draft_join<kBf16, L::D>),
-                       dim3((unsigned)args.most, (unsigned)((rows + kPer - 1) / kPer)), dim3(kJoinThreads), 0, stream, args);
+                       dim3((unsigned)args.most, (unsigned)((rows + kRows - 1) / kRows) * (kRows * (L::D / 4) / kJoinThreads)),
+                       dim3(kJoinThreads), 0, stream, args);
     return hipGetLastError();
 }
 
