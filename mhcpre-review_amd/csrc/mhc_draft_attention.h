@@ -371,13 +371,13 @@ __device__ __forceinline__ void finish(const Args &args, const Place &p, int nod
     }
 }
 
-// The ancestors of every node of row b, 256 bits each (itself among them).  A node's
-// farthest known ancestor's are its own too: each round doubles how far.
-template <int kThreads>
-__device__ __forceinline__ void find_ancestors(const DraftAttentionArgs &a, int b, int n,
-                                               uint64_t (&known)[kDraftNodes][4], int (&farthest)[kDraftNodes])
+// The ancestors of every node of a row, 256 bits each (itself among them), from the parents
+// of a thread's nodes.  A node's farthest known ancestor's are its own too: each round doubles
+// how far.
+template <int kThreads, int kNodes>
+__device__ __forceinline__ void find_ancestors(const int (&parents)[kNodes], int n, uint64_t (&known)[kDraftNodes][4],
+                                               int (&farthest)[kDraftNodes])
 {
-    constexpr int kNodes = kDraftNodes / kThreads > 0 ? kDraftNodes / kThreads : 1;  // of a thread
     uint64_t own[kNodes][4];
     int far[kNodes];
 #pragma unroll
@@ -385,7 +385,7 @@ __device__ __forceinline__ void find_ancestors(const DraftAttentionArgs &a, int 
         const int i = k * kThreads + (int)threadIdx.x;
         far[k] = -1;
         if (i < n) {
-            const int p = a.parents[(int64_t)b * a.S + i];
+            const int p = parents[k];
             far[k] = p >= 0 && p < i ? p : -1;
         }
 #pragma unroll
@@ -589,6 +589,8 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     // The operand of the rows of a place's block.  (It is turned where it is used first: what a
     // load brings must not be touched before the wait at the loop's head.)
     u32x4_t q[kSteps];
+    constexpr int kNodes = kDraftNodes / L::kThreads > 0 ? kDraftNodes / L::kThreads : 1;  // of a thread
+    int parents[kNodes];
     const auto load_q = [&](const Place &p) {
         const Args &l = late();
         const int ln = late_lane();
@@ -601,6 +603,14 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         for (int s = 0; s < kSteps; ++s) {
             q[s] = *reinterpret_cast<const u32x4_t *>(on && 16 * s < l.a.d ? from + 16 * s
                                                                            : reinterpret_cast<const uint16_t *>(kZeros));
+        }
+        // (and the parents, which are asked for where the block is entered)
+        const int32_t *const row_ = l.a.parents != nullptr ? l.a.parents + (int64_t)p.b * l.a.S
+                                                           : reinterpret_cast<const int32_t *>(kZeros);
+#pragma unroll
+        for (int k = 0; k < kNodes; ++k) {
+            const int i = k * L::kThreads + (int)threadIdx.x;
+            parents[k] = row_[l.a.parents != nullptr && i < l.a.S ? i : 0];
         }
     };
     const auto turn_q = [&]() {
@@ -642,7 +652,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
             (l.a.window > 0 || (int64_t)(here.keys.first + lastTile + 1) * L::kUnit > here.c)) {
             if (maskedRow != here.b) {
                 __syncthreads();  // (the ones before are read)
-                find_ancestors<L::kThreads>(l.a, here.b, here.n, known, farthest);
+                find_ancestors<L::kThreads>(parents, here.n, known, farthest);
                 maskedRow = here.b;
             }
             if (l.a.window > 0) {
