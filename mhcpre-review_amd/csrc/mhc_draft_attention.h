@@ -121,11 +121,10 @@ struct Layout {
 // trees of 8: 206 us if it stands for nothing, 99 so.)
 constexpr int kItemUnits = 3;
 
-// What a stretch begins and does not finish: a (sequence, kv head, block), the line's units
-// of its first and its last tile, the units of the line, and the slot of its part.  last
-// < 0: nothing.
+// What a stretch begins and does not finish: a (sequence, kv head, block), the stretch that
+// finishes it, and the slot of its first part.  last < 0: nothing.
 struct Open {
-    int b, kv, block, first, last, all, slot, none;
+    int last, b, kv, block, slot, none[3];
 };
 
 struct Args {
@@ -975,7 +974,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         const bool all = firstTile == 0 && here.tile + 1 == here.keys.tiles;
         const int slot = 2 * w + (firstBlock ? 0 : 1);
         if (threadIdx.x == 0 && firstTile == 0 && !all) {
-            late().open[w] = Open{here.b, here.kv, here.block, here.start, here.start + here.keys.tiles - 1, shares.units, slot, 0};
+            late().open[w] = Open{shares.owner(here.start + here.keys.tiles - 1), here.b, here.kv, here.block, slot, {}};
         }
         // The lane's four x of values: of a row's dimension 32 (x / 4) + 8 (x % 4) + 4 upper on.
         // A part lies in the workspace as in the registers, so that a wave writes 1 KB at a time.
@@ -1085,78 +1084,128 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
 }
 
 // Joins the parts of the (sequence, kv head, block)s that no stretch finished: a workgroup
-// for some rows of the one that stretch `first` began.  Bound by its chain of loads (what
-// there is to join, then up to 16 parts at once) for one small sequence, 4.0 us, and by memory
-// for many, 11.8 to 13.2 with 40 to 50 MB of parts.
-constexpr int kJoinThreads = 256;
+// for some rows of the one that stretch `first` began.  Where one has more than kJoinBatch
+// parts, the workgroups of the next three stretches, which begin none, help: each has a quarter of
+// the values, and its waves a quarter of the parts each (256 parts, one sequence of 131072 tokens
+// with 16 heads to one of 128, a chain of 4: the call 90.8 us without them, 48.8 so; 47 parts of one
+// row 28.3 and 19.2).  Bound by its chain of loads (what there is to join, then up to 16 parts at
+// once) for one small sequence, 4.0 us, and by memory for many, 12 to 14 with 40 to 50 MB of parts.
+constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / kWave;
 constexpr int kJoinBatch = 16;
 
-template <bool kBf16, int D>
-__global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
-{
-    const DraftAttentionArgs &a = args.a;
-    // (Turned by blockIdx.y: the stretches that begin parts may lie 8 apart, and so all on one XCD.
-    // 32 blocks of 8 parts each: 21.8 us not turned, 12.4 so.)
-    const int first = (int)((blockIdx.x + blockIdx.y) % gridDim.x);
-    const Open open = args.open[first];
-    if (open.last < 0) {
-        return;
-    }
-    // (32 rows, four x of each, of each lane of a wave.)
-    const int at = (int)blockIdx.y * kJoinThreads + (int)threadIdx.x, lane = at % kWave, x = at / kWave % (D / 8);
-    const int r = at / (kRows * D / 4) * kRows + lane % 32, e = x / 4 * 32 + x % 4 * 8 + lane / 32 * 4;
-    const attention::Shares shares(open.all, args.most);
-    Place p{};
-    p.b = open.b;
-    p.kv = open.kv;
-    p.block = open.block;
-    const int last = shares.owner(open.last);
-    const int64_t row = (int64_t)p.block * args.rows + r;
-    const int node = (int)(row / args.group), head = (int)(row % args.group);
-    if (node >= a.S) {
-        return;
-    }
-    float top = -INFINITY, total = 0.f;
-    f32x4_t all = {0.f, 0.f, 0.f, 0.f};
-    for (int x0 = first; x0 <= last; x0 += kJoinBatch) {
-        float2 ends[kJoinBatch];
-        f32x4_t outs[kJoinBatch];
-#pragma unroll
-        for (int m = 0; m < kJoinBatch; ++m) {
-            ends[m] = float2{-INFINITY, 0.f};
-            outs[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            if (x0 + m <= last) {
-                const int64_t slot = x0 + m == first ? open.slot : 2 * (x0 + m);
-                ends[m] = *reinterpret_cast<const float2 *>(args.ends + (slot * args.rows + r) * 2);
-                outs[m] = *reinterpret_cast<const f32x4_t *>(args.outs + slot * args.rows * D + at * 4);
-            }
-        }
-        float next = top;
-#pragma unroll
-        for (int m = 0; m < kJoinBatch; ++m) {
-            next = fmaxf(next, ends[m].x);
-        }
-        const float zero = next == -INFINITY ? 0.f : next;
-        const float keep = __builtin_amdgcn_exp2f(top - zero);
+// What some parts amount to, of four values of a row.
+struct Joined {
+    float top, total;
+    f32x4_t all;
+
+    // To a reference of `next` (which is 0 where nothing is seen).
+    __device__ void turn(float next)
+    {
+        const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.f : next));
         top = next;
         total *= keep;
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
             all[y] = scaled(all[y], keep);
         }
+    }
+    __device__ void add(float factor, float weights, f32x4_t values)
+    {
+        total += factor * weights;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            all[y] += scaled(values[y], factor);
+        }
+    }
+};
+
+template <bool kBf16, int D>
+__global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
+{
+    __shared__ Joined shared[kJoinWaves][kWave];
+    const DraftAttentionArgs &a = args.a;
+    // (Turned by blockIdx.y: the stretches that begin parts may lie 8 apart, and so all on one XCD.
+    // 32 blocks of 8 parts each: 21.8 us not turned, 12.4 so.)
+    const int own = (int)((blockIdx.x + blockIdx.y) % gridDim.x);
+    // The one to join: begun by this stretch, or one of many parts begun by a stretch just before.
+    // (Its stretches begin nothing else, so there is one at most.)
+    int first = -1, last = -1;
+#pragma unroll
+    for (int k = 0; k < kJoinWaves; ++k) {
+        const int begun = own >= k ? own - k : 0, to = args.open[begun].last;
+        if (k == 0 ? to >= 0 : to - begun >= kJoinBatch) {
+            first = begun;
+            last = to;
+        }
+    }
+    if (first < 0) {
+        return;
+    }
+    const Open open = args.open[first];
+    const bool shares = last - first >= kJoinBatch;
+    const int wave = (int)threadIdx.x / kWave;
+    // (32 rows, four x of each, of each lane of a wave.)
+    const int at = (int)blockIdx.y * kJoinThreads + (shares ? own - first : wave) * kWave + (int)threadIdx.x % kWave;
+    const int lane = at % kWave, x = at / kWave % (D / 8);
+    const int r = at / (kRows * D / 4) * kRows + lane % 32, e = x / 4 * 32 + x % 4 * 8 + lane / 32 * 4;
+    Place p{};
+    p.b = open.b;
+    p.kv = open.kv;
+    p.block = open.block;
+    const uint32_t row = (uint32_t)p.block * args.rows + r, group = (uint32_t)args.group;  // (below 2^30)
+    const int node = (int)(row / group), head = (int)(row % group);
+    const bool there = node < a.S;
+    const int quarter = (last - first) / kJoinWaves + 1;
+    const int from = shares ? first + wave * quarter : first;
+    const int to = !there ? from - 1 : shares && from + quarter - 1 < last ? from + quarter - 1 : last;
+    Joined sum{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+    for (int x0 = from; x0 <= to; x0 += kJoinBatch) {
+        float2 ends[kJoinBatch];
+        f32x4_t outs[kJoinBatch];
 #pragma unroll
         for (int m = 0; m < kJoinBatch; ++m) {
-            if (x0 + m <= last) {
-                const float f = __builtin_amdgcn_exp2f(ends[m].x - zero);
-                total += f * ends[m].y;
+            ends[m] = float2{-INFINITY, 0.f};
+            outs[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (x0 + m <= to) {
+                const int64_t slot = x0 + m == first ? open.slot : 2 * (x0 + m);
+                ends[m] = *reinterpret_cast<const float2 *>(args.ends + (slot * args.rows + r) * 2);
+                outs[m] = *reinterpret_cast<const f32x4_t *>(args.outs + slot * args.rows * D + at * 4);
+            }
+        }
+        float next = sum.top;
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    all[y] += scaled(outs[m][y], f);
-                }
+        for (int m = 0; m < kJoinBatch; ++m) {
+            next = fmaxf(next, ends[m].x);
+        }
+        sum.turn(next);
+#pragma unroll
+        for (int m = 0; m < kJoinBatch; ++m) {
+            if (x0 + m <= to) {
+                sum.add(__builtin_amdgcn_exp2f(ends[m].x - (next == -INFINITY ? 0.f : next)), ends[m].y, outs[m]);
             }
         }
     }
-    finish<kBf16>(args, p, node, head, e, all, top, total);
+    if (shares) {
+        shared[wave][lane] = sum;
+        __syncthreads();
+        if (wave != 0) {
+            return;
+        }
+        float next = sum.top;
+#pragma unroll
+        for (int k = 1; k < kJoinWaves; ++k) {
+            next = fmaxf(next, shared[k][lane].top);
+        }
+        sum.turn(next);
+#pragma unroll
+        for (int k = 1; k < kJoinWaves; ++k) {
+            const Joined other = shared[k][lane];
+            sum.add(__builtin_amdgcn_exp2f(other.top - (next == -INFINITY ? 0.f : next)), other.total, other.all);
+        }
+    }
+    if (there) {
+        finish<kBf16>(args, p, node, head, e, sum.all, sum.top, sum.total);
+    }
 }
 
 template <bool kBf16, typename L>

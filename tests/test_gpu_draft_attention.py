@@ -348,3 +348,20 @@ def test_a_query_that_is_no_number(ops, device, dtype, S, heads):
     own[0, S // 2, 1] = own[0, 1, 0] = True
     assert torch.isnan(out[own]).all() and torch.isnan(lse[own]).all()
     assert torch.equal(out[~own], want[~own]) and torch.equal(lse[~own], want_lse[~own])
+
+
+@pytest.mark.parametrize("S,heads,d", [(3, 4, 128), (9, 2, 64), (30, 2, 32), (70, 1, 64), (290, 1, 64)])
+def test_rows_of_very_many_parts(ops, device, S, heads, d):
+    """One sequence over all workgroups: more parts than one round of the join takes, and infinite values among them."""
+    a = make(device, 1, S, heads, 1, d, 64, 33000, BF16, lengths=[33000], drafted=[S], tree=S <= 256)
+    plain, _ = check(ops, a)
+    again = ops.draft_attention(*a.values())
+    assert torch.equal(again[0].cpu().double(), plain)
+    for t, e, value in ((7, 3, math.inf), (20000, 9, -math.inf)):
+        a["v_cache"][int(a["page_table"][0, t // 64]), t % 64, 0, e] = value
+    out = ops.draft_attention(*a.values())[0].cpu().double()
+    assert (out[..., 3] == math.inf).all() and (out[..., 9] == -math.inf).all()
+    other = torch.ones(d, dtype=torch.bool)
+    other[[3, 9]] = False
+    # (in a pass that sets such values apart a part's sums are the same)
+    assert ((out - plain)[..., other].abs() <= 2.0 ** -8 * plain[..., other].abs() + 2.0 ** -12).all()
