@@ -147,7 +147,8 @@ MHC_API int mhcRotaryFrequencies(int32_t rot, double base, int32_t kind, double 
  * once.  (In fp16 the weights are held in 21 bits, small ones to 2^-39 of the
  * largest.)  A row that sees no key (L = 0, holes only) has out 0 and lse -inf.
  * What a row does not see may be infinite or NaN; an infinite value that it sees
- * is infinite in out.
+ * is infinite in out.  (So may finite ones in bf16 be whose sum, weighted by exp(s_t -
+ * max s), is 2^128 or more.)
  *
  *   q          fp16 | bf16   [B, heads, d]
  *   kCache, vCache  same     [pages, pageSize, kvHeads, d]
@@ -192,7 +193,7 @@ MHC_API int mhcPagedAttention(void *workspace, uint64_t workspaceSize, mhcServeE
  * once.  (The weights are held in 16 bits in bf16 and in 22 in fp16, there small
  * ones to 2^-34 of the largest.)  Nodes i >= n, and nodes that see no key, have out
  * 0 and lse -inf.  What a node does not see may be infinite or NaN; an infinite
- * value that it sees is infinite in its output.
+ * value that it sees is infinite in its output, and finite ones are never.
  *
  *   q          fp16 | bf16   [B, S, heads, d]
  *   kCache, vCache  same     [pages, pageSize, kvHeads, d]

@@ -22,8 +22,9 @@
 // doubling (the ancestors of my farthest known ancestor are mine), 256 bits a token.
 // Tiles that all rows see whole have no masks.  The loop takes V as finite: an
 // infinite or NaN value times a weight of zero would reach rows that do not see
-// it.  Where a block's output is not finite, the block is done again with such
-// values taken out of the products and added to the rows that see them alone.
+// it.  Where a block's output is not finite (or near the end of fp32), the block is done
+// again with such values taken out of the products and added to the rows that see them
+// alone.
 //
 // What bounds it, and what it reaches (8 kv heads of 128; a copy reaches 4.9 TB/s, a
 // product of 8192^3 1140 TFLOP/s): memory for few rows, 32 sequences of 8192 tokens with
@@ -224,6 +225,20 @@ __device__ __forceinline__ f32x16_t mfma(u32x4_t a, u32x4_t b, f32x16_t c)
 constexpr float kSlack = 5.f;
 template <bool kBf16>
 constexpr float kLiftBits = kBf16 ? 0.f : 15.f - kSlack;
+
+// bf16 values end where fp32 does, so that sums of finite ones may pass its end before they
+// are divided.  Below 2^116 at a block's end they do not later: up to 4 waves' and 512
+// workgroups' are added.  Where one is not, the block is done again, and the reference is then
+// kRaised + log2 n bits above the scores of the values that are large: n of them below 2^128, with
+// weights of at most 2^(kSlack - kRaised) / n, and n others of weights up to 2^kSlack, sum up to
+// less than 2^116.  (Weights of less than 2^-108 n of a large value's may then count as 0:
+// whatever their values, n of them are not n^3 2^-90 of that value's product.)  fp16's have room.
+template <bool kBf16>
+constexpr float kFar = kBf16 ? 8192.f : 1.f;  // (2^116 times this takes any finite sum beyond the end)
+constexpr float kRaised = 18.f;
+// log2 n, rounded up, and the exponent bits of a large value, 2^110 / n.
+__device__ __forceinline__ int bits_of(int n) { return 32 - __clz(n); }
+__device__ __forceinline__ uint32_t large_from(int n) { return (uint32_t)(127 + 110 - bits_of(n)) << 7; }
 
 template <bool kBf16>
 __device__ __forceinline__ bool infinite(uint32_t bits)
@@ -475,7 +490,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     __shared__ __align__(256) char lds[L::kLds];
     __shared__ uint64_t known[kDraftNodes][4];  // the new tokens' ancestors
     __shared__ int farthest[kDraftNodes];
-    __shared__ uint64_t badKeys[L::kKeyWaves][2];
+    __shared__ uint64_t setApart[L::kKeyWaves][2];  // keys of a tile with infinite and NaN values, and with large ones
     __shared__ float2 ends[L::kKeyWaves][L::kBlock];
     __shared__ bool odd[L::kWaves];
     const DraftAttentionArgs &a = args.a;
@@ -672,8 +687,8 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
     };
 
     // A tile: its keys from t0 on, of which `valid` are in the cache.  kChecked: with infinite and
-    // NaN values of V set apart.
-    const auto attend = [&](auto kChecked, uint32_t buffer, int64_t t0, uint64_t valid, const uint64_t &badHere) {
+    // NaN values of V set apart, at the keys set[0], and large ones at the keys set[1].
+    const auto attend = [&](auto kChecked, uint32_t buffer, int64_t t0, uint64_t valid, const uint64_t *set) {
         constexpr bool checked = decltype(kChecked)::value;
         const uint32_t kFrom = buffer + kPlace, vFrom = buffer + L::kSide + vPlace;
         constexpr uint64_t kAll = kTile == 64 ? ~0ull : 0xFFFFFFFFull;
@@ -728,6 +743,21 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         }
         most = fmaxf(most, __shfl_xor(most, 32));
         most *= factor;
+        if constexpr (checked && kBf16) {
+            if (set[1] != 0) {
+                float high = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < kKt; ++kt) {
+                    const uint32_t bits = (uint32_t)(set[1] >> (32 * kt)) >> (late_lane() / 32 * 4);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        high = (int)(bits << (31 - (8 * (i / 4) + i % 4))) < 0 ? fmaxf(high, s[kt][i]) : high;
+                    }
+                }
+                high = fmaxf(high, __shfl_xor(high, 32)) * factor;
+                most = fmaxf(most, high + (kRaised + (float)bits_of(here.keys.high - here.keys.low)));
+            }
+        }
         if (__any((int)(most > top + kSlack))) {
             const float next = most > top + kSlack ? most : top;
             const float keep = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.f : next));
@@ -798,7 +828,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         }
         if constexpr (checked) {
             // The infinite and NaN values of the rows that see them.
-            uint64_t bad = badHere;
+            uint64_t bad = set[0];
             while (bad != 0) {
                 const int at = __ffsll((unsigned long long)bad) - 1;
                 bad &= bad - 1;
@@ -854,8 +884,12 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
             load(0);
             const uint64_t valid = loaded;
             if (rowWave == 0 && lane == 0) {
-                badKeys[keyWave][0] = 0;
+                setApart[keyWave][0] = 0;
+                if (kBf16) {
+                    setApart[keyWave][1] = 0;
+                }
             }
+            const uint32_t least = large_from(here.keys.high - here.keys.low);
             dev::wait_vm<0>();
             if (tile == firstTile) {
                 turn_q();
@@ -867,9 +901,11 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                 const int at = (n * L::kRowWaves + rowWave) * kWave + lane;
                 auto *const place16 = (__attribute__((address_space(3))) u32x4_t *)(uintptr_t)(buffer + L::kSide + at * 16);
                 u32x4_t v = *place16;
-                bool bad = false;
+                bool bad = false, large = false;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
+                    const uint32_t low = v[e] & 0x7FFFu, high = v[e] >> 16 & 0x7FFFu;
+                    large = large || (low >= least && low < 0x7F80u) || (high >= least && high < 0x7F80u);
                     if (infinite<kBf16>(v[e])) {
                         v[e] &= 0xFFFF0000u;
                         bad = true;
@@ -879,14 +915,17 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
                         bad = true;
                     }
                 }
-                if (bad) {
+                if (__builtin_expect(bad, 0)) {
                     *place16 = v;
-                    atomicOr(reinterpret_cast<unsigned long long *>(&badKeys[keyWave][0]), 1ull << (at / L::kChunks));
+                    atomicOr(reinterpret_cast<unsigned long long *>(&setApart[keyWave][0]), 1ull << (at / L::kChunks));
+                }
+                if (kBf16 && large) {
+                    atomicOr(reinterpret_cast<unsigned long long *>(&setApart[keyWave][1]), 1ull << (at / L::kChunks));
                 }
             }
             __syncthreads();
             attend(std::true_type{}, buffer, (int64_t)(here.keys.first + tile) * L::kUnit + keyWave * kTile, valid,
-                   badKeys[keyWave][0]);
+                   setApart[keyWave]);
         }
         __syncthreads();
     };
@@ -914,22 +953,22 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         load(buffer ^ 1);
         find_page();
         attend(std::false_type{}, (uint32_t)(uintptr_t)mine + buffer * L::kBuffer,
-               (int64_t)(here.keys.first + here.tile) * L::kUnit + keyWave * kTile, valid, 0ull);
+               (int64_t)(here.keys.first + here.tile) * L::kUnit + keyWave * kTile, valid, nullptr);
         if (here.tile + 1 < here.keys.tiles && here.start + here.tile + 1 < end) {
             ++here.tile;
             continue;
         }
 
         // The block's end, or the stretch's.
-        float none = 0.f;  // 0 times a value that is not finite is no number
+        float far = 0.f;  // (not finite where one of the sums is not, or is 2^116 or more)
 #pragma unroll
         for (int j = 0; j < kDims; ++j) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                none = __builtin_fmaf(o[j][i], 0.f, none);
+                far = __builtin_fmaf(o[j][i], kFar<kBf16>, far);
             }
         }
-        const bool finite = __all((int)(none == 0.f));
+        const bool finite = __all((int)__builtin_isfinite(far));
         if (lane == 0) {
             odd[wave] = !finite;
         }
@@ -945,7 +984,7 @@ __global__ __launch_bounds__(L::kThreads, (L::kThreads * L::kPerCu + 255) / 256)
         for (int x = 0; x < L::kWaves; ++x) {
             redo = redo || odd[x];
         }
-        if (redo) {
+        if (__builtin_expect(redo, 0)) {
             dev::wait_vm<0>();  // (the tile on its way)
             again(firstTile);
             // The next one anew.
