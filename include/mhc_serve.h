@@ -320,7 +320,8 @@ MHC_API int mhcCacheBounds(void *workspace, uint64_t workspaceSize, mhcServeExec
  *   out        type of q     [B, heads, d]   lse      fp32  [B, heads], or NULL
  *   columns    int32         [B, kvHeads, top]: the columns taken, ascending, then -1
  *
- * 0 <= first, last; first + last <= top; top >= 1; top * pageSize below 2^31.
+ * 0 <= first, last; first + last <= top; top >= 1; top * pageSize below 2^31; width at
+ * most 2^30; B * kvHeads at most 2^20.
  */
 MHC_API int mhcSparseAttentionGetWorkspaceSize(
     const mhcStridedTensor *q, const mhcStridedTensor *kCache, const mhcStridedTensor *vCache,

@@ -467,7 +467,9 @@ void launch_scores(const Args &args, unsigned grid, hipStream_t stream)
 bool sparse_attention_fits(const SparseAttentionArgs &s)
 {
     const PagedAttentionArgs &a = s.attention;
-    return (int64_t)a.B * a.kvHeads <= (1 << 20) && paged_attention_units_fit(sparse::rows_of(s, nullptr, nullptr));
+    // (Columns are counted in steps that end behind the last one, in 32 bits.)
+    return a.width <= (1 << 30) && (int64_t)a.B * a.kvHeads <= (1 << 20) &&
+           paged_attention_units_fit(sparse::rows_of(s, nullptr, nullptr));
 }
 
 size_t sparse_attention_workspace(const SparseAttentionArgs &s, int cus) { return sparse::Workspace(s, cus).bytes; }
