@@ -252,10 +252,13 @@ __global__ __launch_bounds__(kBoundsThreads) void bounds_pages(CacheBoundsArgs a
     for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
         const int64_t perRow = (int64_t)a.columns * a.pieceGroups;
         const int64_t b = a.B == 1 ? 0 : item / perRow;
-        const int inRow = (int)(item - b * perRow);
+        // (A row's items may be more than 2^31.  A 64-bit division where they need it only.)
+        const int64_t inRow = item - b * perRow;
+        const int64_t ofRow = inRow <= INT32_MAX ? (int)inRow / a.pieceGroups : inRow / a.pieceGroups;
+        const int pieceGroup = (int)(inRow - ofRow * a.pieceGroups);
         const int L = clamped(a.lengths[b], a.width * a.pageSize);
         const int wanted = clamped(a.counts[b], a.tokens), count = wanted < L ? wanted : L, begin = L - count;
-        const int64_t column = (int64_t)(begin / a.pageSize) + inRow / a.pieceGroups;
+        const int64_t column = begin / a.pageSize + ofRow;
         const int64_t start = column * a.pageSize;
         if (count == 0 || start >= L) {
             continue;
@@ -264,7 +267,7 @@ __global__ __launch_bounds__(kBoundsThreads) void bounds_pages(CacheBoundsArgs a
         if (page < 0 || page >= a.pages) {
             continue;
         }
-        const int chunks = a.d / 8, piece = inRow % a.pieceGroups * kPieces + inGroup;
+        const int chunks = a.d / 8, piece = pieceGroup * kPieces + inGroup;
         const bool on = piece < a.kvHeads * chunks;
         const int head = on ? piece / chunks : 0, e = on ? piece % chunks * 8 : 0;
         const uint32_t first = begin > start ? (uint32_t)(begin - start) : 0u;
