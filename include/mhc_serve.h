@@ -254,7 +254,7 @@ MHC_API int mhcDraftAccept(void *workspace, uint64_t workspaceSize, mhcServeExec
  * that for rows that append).
  *
  *   kCache, vCache  fp16 | bf16 | fp32 [pages, pageSize, kvHeads, d]
- *   pageTable int32 [B, width]   lengths, drafted int32 [B]   path int32 [B, S]
+ *   pageTable int32 [B, width]   lengths, drafted int32 [B]   path int32 [B, S], S <= 2^30
  */
 MHC_API int mhcCacheKeepGetWorkspaceSize(
     const mhcStridedTensor *kCache, const mhcStridedTensor *vCache, const mhcTensor *pageTable,

@@ -891,7 +891,7 @@ int mhcCacheKeepGetWorkspaceSize(const mhcStridedTensor *kCache, const mhcStride
     }
     const int64_t B = pageTable->dims[0], S = path->dims[1];
     const int size = elem_bytes(kCache->dtype);
-    if (S > kMaxCount || d > (1 << 16) || kvHeads > 65536 || kvHeads * d > kMaxCount) {
+    if (S > (1 << 30) || d > (1 << 16) || kvHeads > 65536 || kvHeads * d > kMaxCount) {
         return MHC_STATUS_UNSUPPORTED_SHAPE;
     }
     st = first_of({check_strided(kCache, kCache->dtype, {pages, pageSize, kvHeads, d}, size > 0 ? size : 2),
