@@ -251,7 +251,7 @@ MHC_API int mhcDraftAccept(void *workspace, uint64_t workspaceSize, mhcServeExec
  * path[b, k] < n) above path[b, k - 1].  Where either place is in a hole nothing is
  * moved.  lengths is the one that mhcDraftAttention and mhcDraftAccept were given.
  * Pages that the moves touch must be held by one row only (mhcCacheUpdate sees to
- * that for rows that append).
+ * that for rows that append).  vCache may be kCache; else they share no element.
  *
  *   kCache, vCache  fp16 | bf16 | fp32 [pages, pageSize, kvHeads, d]
  *   pageTable int32 [B, width]   lengths, drafted int32 [B]   path int32 [B, S], S <= 2^30

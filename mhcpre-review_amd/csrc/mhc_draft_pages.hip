@@ -87,7 +87,8 @@ __global__ __launch_bounds__(kAcceptWaves *kWave) void accept_rows(DraftAcceptAr
 // ---- keep --------------------------------------------------------------------
 
 // A workgroup does a row of the batch and some columns (bytes of a slot, of both
-// caches).  Its path goes through LDS in pieces as pairs of offsets.  A node moves
+// caches, or of the one that is both: two threads at one place would not keep the
+// order).  Its path goes through LDS in pieces as pairs of offsets.  A node moves
 // towards the front only and paths ascend, so a thread that goes along the path with
 // loads before stores never reads what it has written.  Bound by its chain (lengths,
 // path, table, values): 6.0 us for 32 rows with 5 nodes of 32 (8 kv heads of 128), 13.3
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(kKeepThreads) void keep_rows(CacheKeepArgs a)
         toSlot[threadIdx.x] = slots[1];
         __syncthreads();
         const int count = broken;
-        for (uint64_t at = (uint64_t)blockIdx.y * kKeepThreads + threadIdx.x; at < 2ull * half;
+        for (uint64_t at = (uint64_t)blockIdx.y * kKeepThreads + threadIdx.x; at < (uint64_t)a.caches * half;
              at += (uint64_t)gridDim.y * kKeepThreads) {
             const CacheRows &cache = at < half ? a.k : a.v;
             const uint32_t in = (uint32_t)(at < half ? at : at - half);
@@ -350,7 +351,8 @@ bool divides(const CacheRows &c, int elemBytes, uintptr_t by)
 template <typename Piece>
 hipError_t launch_keep(const CacheKeepArgs &a, hipStream_t stream)
 {
-    const int64_t groups = (2 * (int64_t)a.kvHeads * (a.rowBytes / (int)sizeof(Piece)) + kKeepThreads - 1) / kKeepThreads;
+    const int64_t pieces = (int64_t)a.caches * a.kvHeads * (a.rowBytes / (int)sizeof(Piece));
+    const int64_t groups = (pieces + kKeepThreads - 1) / kKeepThreads;
     hipLaunchKernelGGL((keep_rows<Piece>), dim3((unsigned)a.B, (unsigned)(groups < 256 ? groups : 256)),
                        dim3(kKeepThreads), 0, stream, a);
     return hipGetLastError();

@@ -906,8 +906,11 @@ int mhcCacheKeepGetWorkspaceSize(const mhcStridedTensor *kCache, const mhcStride
     }
     ex->op = Op::kKeep;
     ex->empty = B == 0 || S == 0;
-    ex->keep = {cache_rows(kCache),
-                cache_rows(vCache),
+    const mhc::CacheRows k = cache_rows(kCache), v = cache_rows(vCache);
+    const bool one = k.data == v.data && k.page == v.page && k.slot == v.slot && k.head == v.head;
+    ex->keep = {k,
+                v,
+                one ? 1 : 2,
                 pages,
                 static_cast<int>(pageSize),
                 static_cast<int>(pageTable->dims[1]),

@@ -82,6 +82,7 @@ struct DraftAcceptArgs {
 
 struct CacheKeepArgs {
     CacheRows k, v;
+    int caches;  // 1: v is k
     int64_t pages;
     int pageSize, width, kvHeads, rowBytes, elemBytes;
     int B, S;

@@ -4,6 +4,9 @@ from __future__ import annotations
 import pytest
 import torch
 
+import draft_ref as ref
+from test_gpu_draft_pages import caches
+
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
 
@@ -28,3 +31,20 @@ def test_bounds_of_the_widest_rows(ops, device):
     others = [0, 2, 4, 6, 8]
     for bound in (lo, hi):
         assert torch.equal(bound[held], k[held, 0]) and (bound[others] == 9.0).all()
+
+
+@pytest.mark.parametrize("slot_major", [False, True])
+@pytest.mark.parametrize("d,dtype", [(64, BF16), (6, torch.float16), (33, torch.float32)])
+def test_keep_where_values_are_the_keys(ops, device, d, dtype, slot_major):
+    """One tensor as both caches, and a view of it that only has other strides where there is one head: every node
+    moves once, in the path's order."""
+    for kv_heads in (1, 8):
+        (made,), table = caches(device, 3, 4, kv_heads, d, 400, dtype, slot_major, count=1)
+        i32 = dict(dtype=torch.int32, device=device)
+        paths = [list(range(1, 300)) + [-1], [0] + list(range(2, 300, 2)) + [-1] * 150, list(range(7, 300)) + [-1] * 7]
+        args = table, torch.tensor([400, 377, 310], **i32), torch.tensor([300] * 3, **i32), torch.tensor(
+            [(p + [-1] * 300)[:300] for p in paths], **i32)
+        want, _ = ref.cache_keep(made, made, *(x.cpu() for x in args))
+        same = made if kv_heads > 1 else made.as_strided(made.shape, (*made.stride()[:2], 5, 1))
+        ops.cache_keep(made, same, *args)
+        assert torch.equal(made.cpu(), want)
