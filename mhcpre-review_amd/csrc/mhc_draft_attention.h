@@ -1274,23 +1274,33 @@ template <int D>
 struct LayoutOf<D, Kind::kTwo> : Layout<D, 2, 2, 32> {};
 template <int D>
 struct LayoutOf<D, Kind::kFour> : Layout<D, 4, 1, 64> {};
-// (Above 128 kFour is taken, and the other sizes' tiles do not split into 8 waves' whole loads.)
+// (For heads of 64 and 128 only: other sizes' tiles do not split into 8 waves' whole loads, and
+// larger ones' registers do not hold it.)
 template <int D>
-struct LayoutOf<D, Kind::kEight> : Layout<D, (D == 64 || D == 128 ? 8 : 4), 1, 64> {};
+struct LayoutOf<D, Kind::kEight> : Layout<D, 8, 1, 64> {};
 
-// Calls f(layout) for a kind and (padded) head size.
+// The sizes that there are layouts for.
+inline int padded(int d)
+{
+    return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 160 ? 160 : d <= 192 ? 192 : 256;
+}
+
+// Calls f(layout) for a kind and head size.
 template <Kind kKind, typename F>
 auto with_size(int d, F &&f)
 {
-    const int padded = d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 160 ? 160 : d <= 192 ? 192 : 256;
-    switch (padded) {
-    case 32: return f(LayoutOf<32, kKind>{});
-    case 64: return f(LayoutOf<64, kKind>{});
-    case 96: return f(LayoutOf<96, kKind>{});
-    case 128: return f(LayoutOf<128, kKind>{});
-    case 160: return f(LayoutOf<160, kKind>{});
-    case 192: return f(LayoutOf<192, kKind>{});
-    default: return f(LayoutOf<256, kKind>{});
+    if constexpr (kKind == Kind::kEight) {
+        return padded(d) == 64 ? f(LayoutOf<64, kKind>{}) : f(LayoutOf<128, kKind>{});
+    } else {
+        switch (padded(d)) {
+        case 32: return f(LayoutOf<32, kKind>{});
+        case 64: return f(LayoutOf<64, kKind>{});
+        case 96: return f(LayoutOf<96, kKind>{});
+        case 128: return f(LayoutOf<128, kKind>{});
+        case 160: return f(LayoutOf<160, kKind>{});
+        case 192: return f(LayoutOf<192, kKind>{});
+        default: return f(LayoutOf<256, kKind>{});
+        }
     }
 }
 

@@ -16,7 +16,8 @@ namespace {
 Kind kind_of(const DraftAttentionArgs &a)
 {
     const int64_t rows = (int64_t)a.S * (a.heads / a.kvHeads);
-    return rows <= 32 ? Kind::kOne : rows <= 64 ? Kind::kTwo : rows <= 256 || a.d > 128 ? Kind::kFour : Kind::kEight;
+    const bool eight = rows > 256 && (padded(a.d) == 64 || padded(a.d) == 128);
+    return rows <= 32 ? Kind::kOne : rows <= 64 ? Kind::kTwo : eight ? Kind::kEight : Kind::kFour;
 }
 
 template <Kind kKind>
@@ -50,8 +51,6 @@ Args plan(const DraftAttentionArgs &a, int cus)
     p.blocks = (int)(((int64_t)a.S * p.group + p.rows - 1) / p.rows);
     return p;
 }
-
-int padded(int d) { return with_size<Kind::kOne>(d, [](auto l) { return decltype(l)::D; }); }
 
 }  // namespace
 }  // namespace draft
