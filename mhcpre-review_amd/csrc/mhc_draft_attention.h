@@ -151,6 +151,12 @@ __device__ __forceinline__ int late_lane()
     asm volatile("" : "+v"(lane));
     return lane;
 }
+__device__ __forceinline__ int late_thread()
+{
+    int thread = (int)threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    return thread;
+}
 
 // The keys of a block of a sequence with c + n tokens, n of them new: [low, high), in
 // `tiles` (units of the launch, one at least) from `first` on.
@@ -392,11 +398,12 @@ template <int kThreads, int kNodes>
 __device__ __forceinline__ void find_ancestors(const int (&parents)[kNodes], int n, uint64_t (&known)[kDraftNodes][4],
                                                int (&farthest)[kDraftNodes])
 {
+    const int thread = late_thread();
     uint64_t own[kNodes][4];
     int far[kNodes];
 #pragma unroll
     for (int k = 0; k < kNodes; ++k) {
-        const int i = k * kThreads + (int)threadIdx.x;
+        const int i = k * kThreads + thread;
         far[k] = -1;
         if (i < n) {
             const int p = parents[k];
@@ -410,7 +417,7 @@ __device__ __forceinline__ void find_ancestors(const int (&parents)[kNodes], int
     for (int reach = 1;; reach *= 2) {
 #pragma unroll
         for (int k = 0; k < kNodes; ++k) {
-            const int i = k * kThreads + (int)threadIdx.x;
+            const int i = k * kThreads + thread;
             if (i < n) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
