@@ -15,7 +15,7 @@
 // is read transposed (ds_read_b64_tr_b16).  A probability is the sum of two 16-bit
 // terms, the first one cut, the second rounded: bf16 holds 16 bits, fp16 (lifted, for
 // its range ends at 2^-24) 22.  One term alone would add an error of the size of the
-// output's own rounding; it would take 237 us where two take 297 (below).
+// output's own rounding; it took 237 us where two took 297 (2 of 65536, below).
 //
 // What a row sees is all of the context in front of the new tokens (but for a
 // window), and of the new tokens its ancestors, found from the parents by
@@ -28,11 +28,19 @@
 //
 // What bounds it, and what it reaches (8 kv heads of 128; a copy reaches 4.9 TB/s, a
 // product of 8192^3 1140 TFLOP/s): memory for few rows, 32 sequences of 8192 tokens with
-// trees of 8 nodes of 4 heads each 212 us, 5.1 TB/s; the matrix cores for many, 2 of 65536
-// with trees of 64 of 8 heads each 297 us, 493 TFLOP/s of the formulas' operations, 740 with
-// the second term's.  There a tile's exponentials, splits and LDS reads stand between its
-// products: they are written among each other, and half of the time is the products' own.  A
+// trees of 8 nodes of 4 heads each 202 to 212 us, 5.1 to 5.3 TB/s; the matrix cores for many,
+// 2 of up to 65536 with trees of 64 of 8 heads each 265 us, and 285 to 300 where calls follow each
+// other without a pause (the clock falls): 490 to 550 TFLOP/s of the formulas' operations, half
+// as many again with the second term's.  There a tile's exponentials, splits and LDS reads
+// stand between its products: they are written among each other, and half of the time is
+// the products' own.  A chunk of 2048 tokens behind 6144, 4 heads each, 370 us, 650 TFLOP/s.  A
 // single small sequence costs two launches, one chain of loads and the join: 17 us.
+//
+// What is not used, and could be: a wave without rows that are there does all products
+// (a block is 256 rows for a tree of 64 of 8 heads, of which 52 nodes may be there), a window's
+// whole tiles are taken to begin where the last new token's window does, and every workgroup
+// counts all blocks of a sequence before its first tile (a call for 2048 tokens of 16 heads to
+// one of which one is there 70 us, for 8192 242).
 #pragma once
 
 #include "mhc_paged_attention.h"
