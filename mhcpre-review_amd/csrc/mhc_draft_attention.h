@@ -1265,6 +1265,9 @@ __global__ __launch_bounds__(kJoinThreads) void draft_join(Args args)
 template <bool kBf16, typename L>
 hipError_t launch_layout(const Args &args, hipStream_t stream)
 {
+    if (args.rows != L::kBlock || args.unit != L::kUnit || args.a.d > L::D) {
+        return hipErrorInvalidValue;  // (planned for another layout, and so is the workspace)
+    }
     hipLaunchKernelGGL((draft_units<kBf16, L>), dim3((unsigned)args.most), dim3(L::kThreads), 0, stream, args);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) {
